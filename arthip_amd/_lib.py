@@ -49,6 +49,47 @@ class VsModelInfo(ctypes.Structure):
                 ("scale_h", ctypes.c_int)]
 
 
+_I64x3 = ctypes.c_int64 * 3
+_I64x2 = ctypes.c_int64 * 2
+
+
+class RopeArgs(ctypes.Structure):
+    """arthip_rope_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "pos", "packed")]
+                + [(n, _I64x3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride",
+                                         "pos_stride")]
+                + [(n, ctypes.c_int32) for n in ("n_freq", "dtype", "pairs", "inverse", "batch",
+                                                 "tokens", "q_heads", "k_heads", "head_dim")])
+
+
+class AttentionArgs(ctypes.Structure):
+    """arthip_attention_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "q_start", "kv_len",
+                                                "prefix", "doc_q", "doc_k", "code_q", "code_k",
+                                                "slopes", "table", "workspace")]
+                + [("workspace_bytes", ctypes.c_uint64)]
+                + [(n, _I64x3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+                + [(n, ctypes.c_int64) for n in ("doc_q_stride", "doc_k_stride", "code_q_stride",
+                                                 "code_k_stride")]
+                + [("scale", ctypes.c_float), ("cap", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("left", "right", "table_len", "table_zero", "dtype",
+                                                 "batch", "q_tokens", "k_tokens", "q_heads",
+                                                 "k_heads", "head_dim")])
+
+
+class NormArgs(ctypes.Structure):
+    """arthip_norm_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("residual", "y", "residual_out", "h", "gate",
+                                                "mod_scale", "mod_shift", "post_weight", "post_bias",
+                                                "pre_weight", "pre_bias")]
+                + [(n, _I64x2) for n in ("residual_stride", "y_stride", "residual_out_stride",
+                                         "h_stride", "gate_stride", "mod_scale_stride",
+                                         "mod_shift_stride")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "residual_dtype", "post", "pre", "gate_act",
+                                                 "batch", "tokens", "channels")]
+                + [(n, ctypes.c_float) for n in ("eps", "residual_scale", "branch_scale")])
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     c_int, c_size, c_void, c_char = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
     i32p = ctypes.POINTER(ctypes.c_int)
@@ -120,6 +161,13 @@ def _declare(lib: ctypes.CDLL) -> None:
         c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_void)
     sig("arthip_conv3x3_limits", c_int, i32p, i32p)
     sig("arthip_padded_dims", c_int, c_int, c_int, i32p, i32p)
+    sig("arthip_rope_packed_bytes", c_size, c_int)
+    sig("arthip_rope_pack", c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int32),
+        c_int, c_int, c_void, c_size)
+    sig("arthip_rope_axes", c_int, ctypes.POINTER(RopeArgs), c_void)
+    sig("arthip_attention_workspace", c_size, ctypes.POINTER(AttentionArgs))
+    sig("arthip_attention", c_int, ctypes.POINTER(AttentionArgs), c_void)
+    sig("arthip_gated_norm", c_int, ctypes.POINTER(NormArgs), c_void)
     sig("arthip_f32_to_f16", ctypes.c_uint16, ctypes.c_float)
     sig("arthip_f16_to_f32", ctypes.c_float, ctypes.c_uint16)
     sig("arthip_f32_to_f16_no_subnormals", ctypes.c_uint16, ctypes.c_float)
@@ -141,7 +189,9 @@ EXPORTED_SYMBOLS = (
     "arthip_vs_model_create", "arthip_vs_model_get_frame", "arthip_vs_model_destroy",
     "arthip_vs_version", "arthip_vs_device_properties",
     "arthip_conv3x3_packed_halfs", "arthip_conv3x3_bias_len", "arthip_conv3x3_pack",
-    "arthip_conv3x3_f16_nhwc", "arthip_conv3x3_block_f16_nhwc", "arthip_conv3x3_limits", "arthip_padded_dims", "arthip_f32_to_f16",
+    "arthip_conv3x3_f16_nhwc", "arthip_conv3x3_block_f16_nhwc", "arthip_conv3x3_limits", "arthip_padded_dims",
+    "arthip_rope_packed_bytes", "arthip_rope_pack", "arthip_rope_axes", "arthip_attention_workspace",
+    "arthip_attention", "arthip_gated_norm", "arthip_f32_to_f16",
     "arthip_f16_to_f32", "arthip_f32_to_f16_no_subnormals", "arthip_last_error", "arthip_version",
 )
 

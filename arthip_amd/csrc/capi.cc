@@ -1,6 +1,7 @@
 // extern "C" surface of libarthip.so (include/arthip.h).
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstring>
 #include <exception>
 #include <memory>
@@ -15,6 +16,7 @@
 #include "half.h"
 #include "launch.h"
 #include "pack.h"
+#include "transformer.h"
 
 static_assert(ARTHIP_DEBUG_POISON == arthip::kDebugPoison &&
                   ARTHIP_DEBUG_SYNC_EACH == arthip::kDebugSyncEach &&
@@ -71,6 +73,12 @@ int guard(int code, char* err, int errlen, const char* prefix, F&& body) {
   } catch (...) {
     return report(std::string(prefix) + "internal error", code, err, errlen);
   }
+}
+
+// The return of an entry point that has launched.
+int launched(const char* name, hipError_t e) {
+  if (e == hipSuccess) return ARTHIP_OK;
+  return fail(std::string(name) + " launch failed: " + hipGetErrorString(e), ARTHIP_ERR_RUN);
 }
 
 constexpr int kMaxRank = 8;
@@ -736,6 +744,70 @@ int arthip_conv3x3_block_f16_nhwc(const void* in, const void* packed1, const flo
     return fail(std::string("conv3x3 block launch failed: ") + hipGetErrorString(err),
                 ARTHIP_ERR_RUN);
   return ARTHIP_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Transformer operators
+// ---------------------------------------------------------------------------
+
+size_t arthip_rope_packed_bytes(int n) {
+  return n <= 0 ? 0 : static_cast<size_t>(n) * sizeof(arthip::RopeFreq);
+}
+
+int arthip_rope_pack(const double* freq, const int32_t* axis, int n, int n_axes, void* packed,
+                     size_t packed_bytes) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (freq == nullptr || axis == nullptr || packed == nullptr || n < 1)
+      return fail("arthip_rope_pack: null buffer or no frequencies", ARTHIP_ERR_BUILD);
+    if (packed_bytes < arthip_rope_packed_bytes(n))
+      return fail("arthip_rope_pack: output buffer too small", ARTHIP_ERR_BUILD);
+    for (int i = 0; i < n; ++i) {
+      if (axis[i] < 0 || axis[i] >= n_axes)
+        return fail("arthip_rope_pack: axis out of range", ARTHIP_ERR_BUILD);
+      if (!std::isfinite(freq[i]))
+        return fail("arthip_rope_pack: frequency is not finite", ARTHIP_ERR_BUILD);
+    }
+    for (int i = 0; i < n; ++i) {
+      const arthip::RopeFreq f{freq[i] / 6.283185307179586476925, axis[i], 0};
+      std::memcpy(static_cast<char*>(packed) + i * sizeof(f), &f, sizeof(f));
+    }
+    return ARTHIP_OK;
+  });
+}
+
+int arthip_rope_axes(const arthip_rope_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_rope_axes: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_rope(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_rope_axes", arthip::launch_rope(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+size_t arthip_attention_workspace(const arthip_attention_args* args) {
+  if (args == nullptr || args->batch < 0 || args->q_tokens < 0 || args->k_tokens < 0 ||
+      args->k_heads < 1 || args->q_heads < 0 || args->head_dim < 1)
+    return 0;
+  return arthip::attention_plan(*args).workspace;
+}
+
+int arthip_attention(const arthip_attention_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_attention: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_attention(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_attention",
+                    arthip::launch_attention(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+int arthip_gated_norm(const arthip_norm_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_gated_norm: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_norm(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_gated_norm", arthip::launch_norm(*args, static_cast<hipStream_t>(stream)));
+  });
 }
 
 }  // extern "C"

@@ -1,0 +1,174 @@
+// Rotary positions with several axes (arthip_rope_axes): queries and keys of a token
+// in one launch.
+//
+// A thread owns one unit of a head, V frequencies and their 2 V values, at one token:
+// it computes the V angles once and turns that unit of every head of its group. Units
+// are contiguous (pairs (2f, 2f + 1)) or two runs half a head apart (pairs (f, f + n)),
+// so that neighbouring threads read neighbouring memory either way. Values past the
+// turned ones are units without angles, copied.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "launch.h"
+#include "token_dev.h"
+#include "transformer.h"
+
+namespace arthip {
+
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+  arthip_rope_args c;
+  int units;      // of a head: the turned ones first, then copies
+  int turned;     // units that turn
+  int groups;     // threads of a token and unit, heads dealt out in turn
+  int per_token;  // units * groups
+  int per_block;  // tokens of a workgroup
+};
+
+// sin and cos of 2 pi x, |x| <= 1/2. The nearest quarter turn comes off exactly, the
+// rest, |y| <= 1/8, goes through the Taylor polynomials of degree 9 and 10, whose
+// next terms are below 2e-9 there; the quarter picks and signs the results.
+__device__ __forceinline__ void sincos_turns(float x, float& s, float& c) {
+  const float quarter = __builtin_rintf(4.0f * x);
+  const float y = __builtin_fmaf(-0.25f, quarter, x);
+  const int k = static_cast<int>(quarter);
+  const float z = y * y;
+  float ps = 42.058693944897655f;  // (2 pi)^9 / 9!
+  ps = __builtin_fmaf(ps, z, -76.70585975306136f);
+  ps = __builtin_fmaf(ps, z, 81.60524927607504f);
+  ps = __builtin_fmaf(ps, z, -41.341702240399755f);
+  ps = __builtin_fmaf(ps, z, 6.283185307179586f);
+  ps *= y;
+  float pc = -26.42625678337438f;  // (2 pi)^10 / 10!
+  pc = __builtin_fmaf(pc, z, 60.24464137187666f);
+  pc = __builtin_fmaf(pc, z, -85.45681720669373f);
+  pc = __builtin_fmaf(pc, z, 64.93939402266829f);
+  pc = __builtin_fmaf(pc, z, -19.739208802178716f);
+  pc = __builtin_fmaf(pc, z, 1.0f);
+  const float a = (k & 1) ? pc : ps;
+  const float b = (k & 1) ? ps : pc;
+  s = (k & 2) ? -a : a;
+  c = ((k + 1) & 2) ? -b : b;
+}
+
+template <class T, int V, bool PAIRS>
+__global__ void __launch_bounds__(kRopeThreads) rope_axes(RopeArgs a) {
+  const int tid = threadIdx.x;
+  const int slot = tid / a.per_token;
+  const int rest = tid - slot * a.per_token;
+  const int group = rest / a.units;
+  const int unit = rest - group * a.units;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * a.per_block + slot;
+  if (slot >= a.per_block || token >= static_cast<int64_t>(a.c.batch) * a.c.tokens) return;
+  const uint32_t b = static_cast<uint32_t>(token) / static_cast<uint32_t>(a.c.tokens);
+  const uint32_t t = static_cast<uint32_t>(token) - b * static_cast<uint32_t>(a.c.tokens);
+
+  const bool turn = unit < a.turned;
+  // The two runs of V values of this unit.
+  const int first = PAIRS || !turn ? 2 * V * unit : V * unit;
+  const int second = PAIRS || !turn ? first + V : first + a.c.n_freq;
+
+  float sn[V], cs[V];
+  if (turn) {
+    const RopeFreq* const fr = static_cast<const RopeFreq*>(a.c.packed) + unit * V;
+    const int32_t* const pos = a.c.pos + b * a.c.pos_stride[1] + t * a.c.pos_stride[2];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const double turns = static_cast<double>(pos[fr[i].axis * a.c.pos_stride[0]]) * fr[i].turns;
+      sincos_turns(static_cast<float>(turns - __builtin_rint(turns)), sn[i], cs[i]);
+      if (a.c.inverse) sn[i] = -sn[i];
+    }
+  }
+
+  const T* const q = static_cast<const T*>(a.c.q) + b * a.c.q_stride[0] + t * a.c.q_stride[1];
+  const T* const k = static_cast<const T*>(a.c.k) + b * a.c.k_stride[0] + t * a.c.k_stride[1];
+  T* const qo = static_cast<T*>(a.c.q_out) + b * a.c.q_out_stride[0] + t * a.c.q_out_stride[1];
+  T* const ko = static_cast<T*>(a.c.k_out) + b * a.c.k_out_stride[0] + t * a.c.k_out_stride[1];
+  const int heads = a.c.q_heads + a.c.k_heads;
+  for (int head = group; head < heads; head += a.groups) {
+    const bool is_q = head < a.c.q_heads;
+    const int h = is_q ? head : head - a.c.q_heads;
+    const T* const in = is_q ? q + h * a.c.q_stride[2] : k + h * a.c.k_stride[2];
+    T* const out = is_q ? qo + h * a.c.q_out_stride[2] : ko + h * a.c.k_out_stride[2];
+    float x[V], y[V];
+    load_chunk<T, V>(in + first, x);
+    load_chunk<T, V>(in + second, y);
+    if (turn) {
+      if constexpr (PAIRS) {
+        // x and y are the first and second half of the unit's pairs.
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float* const half = i < (V + 1) / 2 ? x : y;
+          if constexpr (V == 1) {
+            const float u = x[0], w = y[0];
+            x[0] = u * cs[0] - w * sn[0];
+            y[0] = w * cs[0] + u * sn[0];
+          } else {
+            const int j = 2 * i % V;
+            const float u = half[j], w = half[j + 1];
+            half[j] = u * cs[i] - w * sn[i];
+            half[j + 1] = w * cs[i] + u * sn[i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float u = x[i], w = y[i];
+          x[i] = u * cs[i] - w * sn[i];
+          y[i] = w * cs[i] + u * sn[i];
+        }
+      }
+    }
+    store_chunk<T, V>(out + first, x);
+    store_chunk<T, V>(out + second, y);
+  }
+}
+
+template <class T, int V>
+void (*rope_kernel(bool pairs))(RopeArgs) {
+  return pairs ? rope_axes<T, V, true> : rope_axes<T, V, false>;
+}
+
+template <class T>
+void (*rope_kernel(int v, bool pairs))(RopeArgs) {
+  switch (v) {
+    case 8: return rope_kernel<T, 8>(pairs);
+    case 4: return rope_kernel<T, 4>(pairs);
+    case 2: return rope_kernel<T, 2>(pairs);
+    default: return rope_kernel<T, 1>(pairs);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_rope(const arthip_rope_args& c, hipStream_t s) {
+  const int heads = c.q_heads + c.k_heads;
+  if (c.batch == 0 || c.tokens == 0 || heads == 0) return hipSuccess;
+  RopeArgs a{};
+  a.c = c;
+  // In place, values that do not turn stay where they are.
+  const bool in_place = (c.q_heads == 0 || c.q == c.q_out) && (c.k_heads == 0 || c.k == c.k_out);
+  const int copied = in_place ? 0 : c.head_dim - 2 * c.n_freq;
+  int v = c.dtype == ARTHIP_TYPE_F32 ? 4 : 8;
+  while (c.n_freq % v != 0 || copied % (2 * v) != 0) v /= 2;
+  a.turned = c.n_freq / v;
+  a.units = a.turned + copied / (2 * v);
+  const int64_t tokens = static_cast<int64_t>(c.batch) * c.tokens;
+  a.groups = std::min(heads, kRopeThreads / a.units);
+  a.per_token = a.units * a.groups;
+  a.per_block = kRopeThreads / a.per_token;
+  const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;
+  void (*fn)(RopeArgs) = c.dtype == ARTHIP_TYPE_F16    ? rope_kernel<_Float16>(v, c.pairs != 0)
+                         : c.dtype == ARTHIP_TYPE_BF16 ? rope_kernel<__bf16>(v, c.pairs != 0)
+                                                       : rope_kernel<float>(v, c.pairs != 0);
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(kRopeThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace arthip

@@ -1,0 +1,350 @@
+"""Transformer operators over libarthip.so: the block of an image or video network.
+
+``rope_axes`` (rotary positions with several axes), ``attention`` (capped scores,
+distance bias, windows, prefixes, documents, ragged caches) and ``gated_norm`` (the
+norms around a gated residual) mirror the C entry points of the same names, which
+include/arthip.h describes. Inference only.
+
+Tensors are torch tensors on one GPU (torch is used only as device-memory plumbing)
+and keep their strides: only the innermost dimension has to be contiguous. Work goes
+to torch's current stream, or to ``stream`` (a raw handle); results that a call makes
+itself belong to that stream. Arguments that do not fit raise :class:`EngineError`
+before anything is launched.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .engine import EngineError
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
+_GATES = {None: 0, "none": 0, "sigmoid": 1, "tanh": 2, "silu": 3}
+
+
+def _need(ok: bool, text: str) -> None:
+    if not ok:
+        raise EngineError(text)
+
+
+def _call(fn, args, stream: int) -> None:
+    if fn(ctypes.byref(args), stream) != 0:
+        raise EngineError(_lib.last_error() or f"{fn.__name__} failed")
+
+
+class _On:
+    """The device and stream of a call: the tensors' device is made current, and
+    tensors made inside belong to the stream."""
+
+    def __init__(self, device, stream):
+        self.stream = stream
+        self._guards = []
+        if device.index != torch.cuda.current_device():
+            self._guards.append(torch.cuda.device(device))
+        if stream is not None:
+            self._guards.append(torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)))
+        self._device = device
+
+    def __enter__(self):
+        for g in self._guards:
+            g.__enter__()
+        if self.stream is None:
+            self.stream = torch._C._cuda_getCurrentRawStream(self._device.index)
+        return self.stream
+
+    def __exit__(self, *exc):
+        for g in reversed(self._guards):
+            g.__exit__(*exc)
+
+
+def _check(name: str, t, device, dtype, dim: int | None = None) -> None:
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a tensor on a GPU")
+    _need(t.device == device, f"{name} is on another device")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
+    _need(dim is None or t.dim() == dim, f"{name} must have {dim} dimensions")
+
+
+def _inner(name: str, t) -> None:
+    _need(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name}: the innermost dimension must be contiguous")
+
+
+# -- rotary positions ---------------------------------------------------------------
+
+class RopePlan:
+    """The frequencies of a rotary embedding, packed for the kernel and kept on the GPU.
+
+    ``sections`` gives the turned pairs of each axis (time, height, width, ...); their
+    sum n turns 2 n values of a head. Pair f turns by position * theta ** (-f / n), f
+    counted over all axes, or with ``per_axis`` over its own axis' pairs. ``order``
+    "blocks" gives an axis its pairs in a row, "cycle" deals them out one axis after
+    the other. ``scale`` multiplies an axis' positions. ``pairs`` turns neighbours (2f,
+    2f + 1) rather than (f, f + n). ``freqs`` (radians a position) replaces theta."""
+
+    def __init__(self, sections, *, theta: float = 10000.0, per_axis: bool = False,
+                 pairs: bool = False, order: str = "blocks", scale=None, freqs=None,
+                 device="cuda"):
+        sections = [int(s) for s in sections]
+        _need(len(sections) > 0 and min(sections) >= 0 and sum(sections) > 0,
+              "RopePlan: sections must be counts of pairs")
+        _need(order in ("blocks", "cycle"), "RopePlan: order is 'blocks' or 'cycle'")
+        _need(theta > 0, "RopePlan: theta must be positive")
+        n = sum(sections)
+        scale = [1.0] * len(sections) if scale is None else [float(s) for s in scale]
+        _need(len(scale) == len(sections), "RopePlan: one scale an axis")
+        if order == "blocks":
+            axis = [a for a, s in enumerate(sections) for _ in range(s)]
+        else:
+            axis = [a for turn in range(max(sections)) for a, s in enumerate(sections) if turn < s]
+        if freqs is None:
+            freqs, seen = [], [0] * len(sections)
+            for f, a in enumerate(axis):
+                freqs.append(theta ** (-(seen[a] / sections[a] if per_axis else f / n)))
+                seen[a] += 1
+        _need(len(freqs) == n, "RopePlan: one frequency a pair")
+        self.n, self.n_axes, self.pairs = n, len(sections), bool(pairs)
+        self.axis = tuple(axis)
+        self.freqs = tuple(float(f) * scale[a] for f, a in zip(freqs, axis))
+        lib = _lib.lib()
+        host = torch.empty(lib.arthip_rope_packed_bytes(n), dtype=torch.uint8)
+        rc = lib.arthip_rope_pack((ctypes.c_double * n)(*self.freqs), (ctypes.c_int32 * n)(*axis), n,
+                                  self.n_axes, host.data_ptr(), host.numel())
+        if rc != 0:
+            raise EngineError(_lib.last_error() or "arthip_rope_pack failed")
+        self.packed = host.to(device)
+
+
+def rope_axes(q, k, pos, plan: RopePlan, *, q_out=None, k_out=None, inverse: bool = False,
+              stream=None):
+    """Queries [B, L, Hq, D] and keys [B, L, Hk, D] (either may be None) turned by int32
+    positions [axes, B, L] (or [axes, L], the same for every batch item). Returns
+    (q_out, k_out), new contiguous tensors unless given; q_out=q turns in place."""
+    x = q if q is not None else k
+    _need(isinstance(x, torch.Tensor) and x.is_cuda, "rope_axes: q or k must be a tensor on a GPU")
+    _need(x.dtype in _TYPES, f"rope_axes: unsupported type {x.dtype}")
+    _need(x.dim() == 4, "rope_axes: q and k must have 4 dimensions")
+    batch, tokens, _, dim = x.shape
+    _check("pos", pos, x.device, torch.int32)
+    _need(tuple(pos.shape) in ((plan.n_axes, batch, tokens), (plan.n_axes, tokens)),
+          "rope_axes: pos must be [axes, B, L] or [axes, L]")
+    _need(plan.packed.device == x.device, "rope_axes: the plan is on another device")
+    lib = _lib.lib()
+    a = _lib.RopeArgs()
+    with _On(x.device, stream) as s:
+        outs = []
+        for name, t, out in (("q", q, q_out), ("k", k, k_out)):
+            if t is None:
+                outs.append(None)
+                continue
+            _check(name, t, x.device, x.dtype, 4)
+            _need(t.shape[0] == batch and t.shape[1] == tokens and t.shape[3] == dim,
+                  "rope_axes: q and k must agree in batch, tokens and head_dim")
+            _inner(name, t)
+            if out is None:
+                out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            else:
+                _check(name + "_out", out, x.device, x.dtype, 4)
+                _need(out.shape == t.shape, f"rope_axes: {name}_out must have {name}'s shape")
+                _inner(name + "_out", out)
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_out", out.data_ptr())
+            setattr(a, name + "_heads", t.shape[2])
+            setattr(a, name + "_stride", t.stride()[:3])
+            setattr(a, name + "_out_stride", out.stride()[:3])
+            outs.append(out)
+        a.pos = pos.data_ptr()
+        st = pos.stride()
+        a.pos_stride = st if pos.dim() == 3 else (st[0], 0, st[1])
+        a.packed = plan.packed.data_ptr()
+        a.n_freq, a.dtype, a.pairs, a.inverse = plan.n, _TYPES[x.dtype], plan.pairs, bool(inverse)
+        a.batch, a.tokens, a.head_dim = batch, tokens, dim
+        _call(lib.arthip_rope_axes, a, s)
+    return tuple(outs)
+
+
+# -- attention ------------------------------------------------------------------------
+
+def _per_token(name: str, t, device, batch: int, tokens: int):
+    """(pointer, batch stride) of int32 values [B, L] or [L]."""
+    _check(name, t, device, torch.int32)
+    _need(tuple(t.shape) in ((batch, tokens), (tokens,)), f"attention: {name} must be [B, L] or [L]")
+    _inner(name, t)
+    return t.data_ptr(), t.stride(0) if t.dim() == 2 else 0
+
+
+def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: bool = False,
+              window=(None, None), q_start=None, kv_len=None, prefix=None, docs=None, codes=None,
+              slopes=None, table=None, table_zero: int = 0, out=None, return_lse: bool = False,
+              workspace=None, stream=None):
+    """softmax(score + mask) V of queries [B, Lq, Hq, D] over keys and values
+    [B, Lk, Hk, D]; see arthip_attention. ``causal`` is window[1] = 0; ``window`` counts
+    the keys to the left and right of a query's own position (None: no limit).
+    q_start, kv_len and prefix are int32 [B]; docs and codes are pairs of int32 tensors
+    (queries', keys'), [B, L] or [L]; slopes is fp32 [Hq], table fp32 [Hq, n]. Returns
+    out, or (out, lse) with lse fp32 [B, Hq, Lq]. Without ``workspace`` (uint8) a call
+    that needs one makes it."""
+    _need(isinstance(q, torch.Tensor) and q.is_cuda, "attention: q must be a tensor on a GPU")
+    _need(q.dtype in (torch.float16, torch.bfloat16), f"attention: unsupported type {q.dtype}")
+    device = q.device
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(name, t, device, q.dtype, 4)
+        _inner(name, t)
+    batch, q_tokens, q_heads, dim = q.shape
+    k_tokens, k_heads = k.shape[1], k.shape[2]
+    _need(tuple(k.shape) == (batch, k_tokens, k_heads, dim) and k.shape == v.shape,
+          "attention: k and v must be [B, Lk, Hk, D] of q's batch and head_dim")
+    a = _lib.AttentionArgs()
+    for name, t in (("q_start", q_start), ("kv_len", kv_len), ("prefix", prefix)):
+        if t is not None:
+            _check(name, t, device, torch.int32)
+            _need(tuple(t.shape) == (batch,) and t.is_contiguous(),
+                  f"attention: {name} must be contiguous [B]")
+            setattr(a, name, t.data_ptr())
+    for name, pair in (("doc", docs), ("code", codes)):
+        if pair is not None:
+            _need(len(pair) == 2, f"attention: {name}s is a pair of tensors (queries', keys')")
+            for side, t, tokens in (("q", pair[0], q_tokens), ("k", pair[1], k_tokens)):
+                ptr, stride = _per_token(f"{name}_{side}", t, device, batch, tokens)
+                setattr(a, f"{name}_{side}", ptr)
+                setattr(a, f"{name}_{side}_stride", stride)
+    if slopes is not None:
+        _check("slopes", slopes, device, torch.float32)
+        _need(tuple(slopes.shape) == (q_heads,) and slopes.is_contiguous(),
+              "attention: slopes must be contiguous [Hq]")
+        a.slopes = slopes.data_ptr()
+    if table is not None:
+        _check("table", table, device, torch.float32, 2)
+        _need(table.shape[0] == q_heads and table.is_contiguous(),
+              "attention: table must be contiguous [Hq, n]")
+        _need(table.shape[1] > 0, "attention: table without entries")
+        a.table, a.table_len, a.table_zero = table.data_ptr(), table.shape[1], int(table_zero)
+    left, right = window
+    _need(not causal or right in (None, 0), "attention: causal and a window to the right")
+    for side in (left, right):
+        _need(side is None or side >= 0, "attention: a window counts keys")
+    a.left = -1 if left is None else int(left)
+    a.right = 0 if causal else -1 if right is None else int(right)
+    a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    a.cap = float(cap)
+    a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.dtype, a.batch, a.q_tokens, a.k_tokens = _TYPES[q.dtype], batch, q_tokens, k_tokens
+    a.q_heads, a.k_heads, a.head_dim = q_heads, k_heads, dim
+    lib = _lib.lib()
+    with _On(device, stream) as s:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        else:
+            _check("out", out, device, q.dtype, 4)
+            _need(out.shape == q.shape, "attention: out must have q's shape")
+            _inner("out", out)
+        a.out, a.out_stride = out.data_ptr(), out.stride()[:3]
+        lse = None
+        if return_lse:
+            lse = torch.empty((batch, q_heads, q_tokens), dtype=torch.float32, device=device)
+            a.lse = lse.data_ptr()
+        need = lib.arthip_attention_workspace(ctypes.byref(a))
+        if need > 0 and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        if workspace is not None:
+            _check("workspace", workspace, device, torch.uint8, 1)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        _call(lib.arthip_attention, a, s)
+    return (out, lse) if return_lse else out
+
+
+# -- norms around a block ----------------------------------------------------------------
+
+def _spread(name: str, t, shape, device, dtype):
+    """(pointer, batch and token stride) of a tensor that broadcasts to [B, L, C]."""
+    _check(name, t, device, dtype)
+    dims = tuple(t.shape)
+    _need(1 <= len(dims) <= 3 and dims[-1] == shape[-1]
+          and all(n in (1, m) for n, m in zip(dims[::-1], shape[::-1])),
+          f"gated_norm: {name} must broadcast to [B, L, C]")
+    _inner(name, t)
+    strides = (0,) * (3 - len(dims)) + tuple(st if n > 1 else 0 for n, st in zip(dims, t.stride()))
+    return t.data_ptr(), strides[:2]
+
+
+def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None, gate=None,
+               gate_act="none", residual_scale: float = 1.0, branch_scale: float = 1.0, pre=None,
+               pre_weight=None, pre_bias=None, mod_scale=None, mod_shift=None, eps: float = 1e-6,
+               residual_out=None, h=None, dtype=None, stream=None):
+    """The norms before and after a block with its gate and residual scale, on tokens
+    [B, L, C]; see arthip_gated_norm. ``post`` and ``pre`` are "rms", "layer" or None,
+    ``gate_act`` is "none", "sigmoid", "tanh" or "silu"; gate, mod_scale and mod_shift
+    broadcast to [B, L, C], weights and biases are fp32 [C]. The residual has y's type or
+    fp32. Returns (new residual, h); residual_out=residual updates in place, and without y
+    and with a residual_scale of 1 the residual is returned as it is. h has y's type, or
+    ``dtype`` where there is no y."""
+    _need(isinstance(residual, torch.Tensor) and residual.is_cuda,
+          "gated_norm: residual must be a tensor on a GPU")
+    _need(residual.dtype in _TYPES, f"gated_norm: unsupported type {residual.dtype}")
+    _need(residual.dim() == 3, "gated_norm: residual must have 3 dimensions")
+    _need(post in _NORMS and pre in _NORMS, "gated_norm: a norm is 'rms', 'layer' or None")
+    _need(gate_act in _GATES, "gated_norm: unknown gate activation")
+    _need(y is not None or (gate is None and post in (None, "none")),
+          "gated_norm: gate or post norm without y")
+    device, shape = residual.device, tuple(residual.shape)
+    if y is not None:
+        _need(isinstance(y, torch.Tensor) and y.dtype in _TYPES, "gated_norm: unsupported type of y")
+        _need(dtype in (None, y.dtype), "gated_norm: h has y's type")
+        dtype = y.dtype
+    elif dtype is None:
+        dtype = residual.dtype if h is None else h.dtype
+    _need(dtype in _TYPES, f"gated_norm: unsupported type {dtype}")
+    a = _lib.NormArgs()
+    _inner("residual", residual)
+    a.residual, a.residual_stride = residual.data_ptr(), residual.stride()[:2]
+    if y is not None:
+        _check("y", y, device, dtype, 3)
+        _need(tuple(y.shape) == shape, "gated_norm: y must have the residual's shape")
+        _inner("y", y)
+        a.y, a.y_stride = y.data_ptr(), y.stride()[:2]
+    if gate is not None:
+        a.gate, a.gate_stride = _spread("gate", gate, shape, device, dtype)
+    if mod_scale is not None:
+        a.mod_scale, a.mod_scale_stride = _spread("mod_scale", mod_scale, shape, device, dtype)
+    if mod_shift is not None:
+        a.mod_shift, a.mod_shift_stride = _spread("mod_shift", mod_shift, shape, device, dtype)
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias),
+                    ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
+        if t is not None:
+            _check(name, t, device, torch.float32, 1)
+            _need(t.shape[0] == shape[2] and t.is_contiguous(),
+                  f"gated_norm: {name} must be contiguous [C]")
+            setattr(a, name, t.data_ptr())
+    a.dtype, a.residual_dtype = _TYPES[dtype], _TYPES[residual.dtype]
+    a.post, a.pre, a.gate_act = _NORMS[post], _NORMS[pre], _GATES[gate_act]
+    a.batch, a.tokens, a.channels = shape
+    a.eps, a.residual_scale, a.branch_scale = float(eps), float(residual_scale), float(branch_scale)
+    lib = _lib.lib()
+    with _On(device, stream) as s:
+        if residual_out is None:
+            if y is None and residual_scale == 1.0:
+                new = residual
+            else:
+                new = torch.empty(shape, dtype=residual.dtype, device=device)
+        else:
+            new = residual_out
+            _check("residual_out", new, device, residual.dtype, 3)
+            _need(tuple(new.shape) == shape, "gated_norm: residual_out must have the residual's shape")
+            _inner("residual_out", new)
+        if new is not residual or residual_out is not None:
+            a.residual_out, a.residual_out_stride = new.data_ptr(), new.stride()[:2]
+        if pre not in (None, "none") or mod_scale is not None or mod_shift is not None or h is not None:
+            if h is None:
+                h = torch.empty(shape, dtype=dtype, device=device)
+            else:
+                _check("h", h, device, dtype, 3)
+                _need(tuple(h.shape) == shape, "gated_norm: h must have the residual's shape")
+                _inner("h", h)
+            a.h, a.h_stride = h.data_ptr(), h.stride()[:2]
+        if a.residual_out or a.h:
+            _call(lib.arthip_gated_norm, a, s)
+    return new, h

@@ -407,6 +407,161 @@ int arthip_conv3x3_block_f16_nhwc(const void* in, const void* packed1, const flo
 int arthip_conv3x3_limits(int* max_c, int* max_m);
 
 /* ------------------------------------------------------------------------ */
+/* Transformer operators (device buffers of tokens)                          */
+/*                                                                           */
+/* The block of an image or video network over patches: rotary positions    */
+/* with several axes, attention, and the norms around a gated residual.     */
+/* Inference only. The tensors are strided: the innermost dimension (the    */
+/* values of a head, the channels of a token) is contiguous, every other    */
+/* one has a stride in elements, which may be 0 (a broadcast input) or      */
+/* negative. Every call validates its arguments on the host (return code 1, */
+/* text in arthip_last_error), enqueues on `stream` (NULL: the default      */
+/* stream) of the calling thread's current device and returns; it allocates */
+/* nothing, never synchronizes and may be captured into a graph. A call     */
+/* with no tokens does nothing and succeeds. The same inputs give the same  */
+/* bits, on whatever stream. Sums, softmax and norm statistics are held in  */
+/* fp32, results are rounded once. Outputs must not overlap inputs unless a */
+/* field says so.                                                            */
+/* ------------------------------------------------------------------------ */
+
+#define ARTHIP_TYPE_F16 0
+#define ARTHIP_TYPE_BF16 1
+#define ARTHIP_TYPE_F32 2
+
+/* Rotary frequencies, packed on the host once per model: pair f of a head turns
+ * by pos[axis[f]] * freq[f] radians. `packed` takes 16 bytes a frequency and is
+ * copied to the device by the caller; its layout belongs to this version of the
+ * library. Returns 1 for a NULL buffer, n < 1, an axis outside [0, n_axes), a
+ * frequency that is not finite, or a short buffer. */
+size_t arthip_rope_packed_bytes(int n);
+int arthip_rope_pack(const double* freq, const int32_t* axis, int n, int n_axes, void* packed,
+                     size_t packed_bytes);
+
+/* Queries [B][L][q_heads][D] and keys [B][L][k_heads][D] turned by the positions
+ * of their token. A turned pair is (f, f + n) or, with `pairs`, (2f, 2f + 1) for
+ * n frequencies; values from 2n on are copied. Angles are reduced in fp64, so
+ * that large positions keep their phase. */
+typedef struct arthip_rope_args {
+  const void* q;            /* may be NULL when q_heads = 0 */
+  const void* k;            /* may be NULL when k_heads = 0 */
+  void* q_out;              /* may be q with q's strides (in place) */
+  void* k_out;              /* may be k with k's strides */
+  const int32_t* pos;       /* [axis][batch][token] */
+  const void* packed;       /* device copy of arthip_rope_pack's buffer */
+  int64_t q_stride[3];      /* batch, token, head */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  int64_t pos_stride[3];    /* axis, batch, token */
+  int32_t n_freq;           /* 2 n_freq <= D */
+  int32_t dtype;            /* ARTHIP_TYPE_* of q, k and the outputs */
+  int32_t pairs;            /* 0: (f, f + n_freq); 1: (2f, 2f + 1) */
+  int32_t inverse;          /* 1: turns back (the transpose) */
+  int32_t batch, tokens, q_heads, k_heads;
+  int32_t head_dim;         /* even, up to 512 */
+} arthip_rope_args;
+
+int arthip_rope_axes(const arthip_rope_args* args, void* stream);
+
+/* out = softmax(score + mask) V for queries [B][Lq][q_heads][D], keys and values
+ * [B][Lk][k_heads][D]; q_heads is a multiple of k_heads, and each run of
+ * q_heads / k_heads query heads shares a key head.
+ *   score(i, j) = scale * q_i . k_j, then cap * tanh(score / cap) if cap > 0,
+ *                 then - slopes[h] * |cq_i - ck_j| and + table[h][clamp(cq_i - ck_j + table_zero)]
+ *   j is visible to i when j < kv_len[b], doc_q[i] == doc_k[j], and either
+ *   j < prefix[b] or p_i - left <= j <= p_i + right, with p_i = q_start[b] + i.
+ * cq and ck are code_q and code_k, or p_i and j without them. (A two-dimensional
+ * table needs one number a token: y * (2 W - 1) + x names every offset inside a
+ * window W wide.) A table entry of -inf hides its offset. A query that sees
+ * nothing gives zeros, and -inf as its log-sum. Keys that a query does not see
+ * add nothing to it, whatever their K and V hold, NaN and infinities among
+ * them. fp16 or bf16. */
+typedef struct arthip_attention_args {
+  const void* q;
+  const void* k;            /* may be NULL when k_tokens = 0 */
+  const void* v;
+  void* out;                /* [B][Lq][q_heads][D] */
+  float* lse;               /* [B][q_heads][Lq] contiguous, natural log; or NULL */
+  const int32_t* q_start;   /* [B], or NULL: Lk - Lq */
+  const int32_t* kv_len;    /* [B], or NULL: Lk; clamped to [0, Lk] */
+  const int32_t* prefix;    /* [B], or NULL: no prefix */
+  const int32_t* doc_q;     /* [B][Lq] with doc_k, or NULL */
+  const int32_t* doc_k;     /* [B][Lk] */
+  const int32_t* code_q;    /* [B][Lq] with code_k, or NULL */
+  const int32_t* code_k;    /* [B][Lk] */
+  const float* slopes;      /* [q_heads], or NULL */
+  const float* table;       /* [q_heads][table_len], or NULL */
+  void* workspace;          /* arthip_attention_workspace bytes, for this call's time on its stream */
+  uint64_t workspace_bytes;
+  int64_t q_stride[3];      /* batch, token, head: multiples of 8, as all data is 16-byte aligned */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t out_stride[3];
+  int64_t doc_q_stride;     /* of a batch item; tokens are contiguous */
+  int64_t doc_k_stride;
+  int64_t code_q_stride;
+  int64_t code_k_stride;
+  float scale;
+  float cap;                /* 0: none */
+  int32_t left, right;      /* -1: no limit; right = 0: causal */
+  int32_t table_len, table_zero;
+  int32_t dtype;            /* ARTHIP_TYPE_F16 or ARTHIP_TYPE_BF16 */
+  int32_t batch, q_tokens, k_tokens, q_heads, k_heads;
+  int32_t head_dim;         /* a multiple of 8 up to 256 */
+} arthip_attention_args;
+
+/* Bytes of workspace that arthip_attention needs for these arguments (0 when the
+ * keys are not split; pointers are not read). */
+size_t arthip_attention_workspace(const arthip_attention_args* args);
+int arthip_attention(const arthip_attention_args* args, void* stream);
+
+/* The norms before and after a block, with its gate and residual scale, on tokens
+ * [B][L][C]:
+ *   r' = residual_scale * residual + branch_scale * act(gate) * post_norm(y)
+ *   h  = pre_norm(r') * (1 + mod_scale) + mod_shift
+ * y is a block's output, h the next block's input. Norms: rms x / sqrt(mean x^2 +
+ * eps) * weight + bias, layer the same of x - mean x. Without y the first line
+ * only scales the residual; without h or residual_out that output is not
+ * written. r' goes into the second line unrounded. */
+#define ARTHIP_NORM_NONE 0
+#define ARTHIP_NORM_RMS 1
+#define ARTHIP_NORM_LAYER 2
+#define ARTHIP_GATE_NONE 0
+#define ARTHIP_GATE_SIGMOID 1
+#define ARTHIP_GATE_TANH 2
+#define ARTHIP_GATE_SILU 3
+
+typedef struct arthip_norm_args {
+  const void* residual;
+  const void* y;               /* or NULL */
+  void* residual_out;          /* may be residual with its strides (in place); or NULL */
+  void* h;                     /* or NULL */
+  const void* gate;            /* or NULL: 1 */
+  const void* mod_scale;       /* or NULL: 0 */
+  const void* mod_shift;       /* or NULL: 0 */
+  const float* post_weight;    /* [C], or NULL: 1 */
+  const float* post_bias;      /* [C], or NULL: 0 */
+  const float* pre_weight;
+  const float* pre_bias;
+  int64_t residual_stride[2];  /* batch, token */
+  int64_t y_stride[2];
+  int64_t residual_out_stride[2];
+  int64_t h_stride[2];
+  int64_t gate_stride[2];
+  int64_t mod_scale_stride[2];
+  int64_t mod_shift_stride[2];
+  int32_t dtype;               /* of y, h, gate and the modulation: ARTHIP_TYPE_* */
+  int32_t residual_dtype;      /* dtype, or ARTHIP_TYPE_F32 */
+  int32_t post, pre;           /* ARTHIP_NORM_* */
+  int32_t gate_act;            /* ARTHIP_GATE_* */
+  int32_t batch, tokens;
+  int32_t channels;            /* up to 32768 */
+  float eps, residual_scale, branch_scale;
+} arthip_norm_args;
+
+int arthip_gated_norm(const arthip_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Helpers                                                                   */
 /* ------------------------------------------------------------------------ */
 

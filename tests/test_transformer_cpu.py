@@ -1,0 +1,184 @@
+"""The transformer operators' host side, without a GPU: the C entry points refuse
+arguments that would read or write out of range before any launch, frequencies are
+packed in fp64, calls without tokens succeed."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from arthip_amd import _lib
+from arthip_amd import transformer as tr
+from arthip_amd.engine import EngineError
+
+BUF = 1 << 20  # stands for a device buffer; never read here
+
+
+def _refused(fn, args, text):
+    assert fn(ctypes.byref(args), None) == 1
+    assert text in _lib.last_error(), _lib.last_error()
+
+
+def _set(args, **fields):
+    for name, value in fields.items():
+        setattr(args, name, value)
+    return args
+
+
+def _attention(**change):
+    a = _lib.AttentionArgs()
+    _set(a, q=BUF, k=BUF * 2, v=BUF * 3, out=BUF * 4, scale=0.1, left=-1, right=-1, dtype=0, batch=2,
+         q_tokens=5, k_tokens=7, q_heads=4, k_heads=2, head_dim=64, q_stride=(1280, 256, 64),
+         k_stride=(896, 128, 64), v_stride=(896, 128, 64), out_stride=(1280, 256, 64))
+    return _set(a, **change)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), "type"), (dict(dtype=-1), "type"), (dict(batch=-1), "negative"),
+    (dict(q_tokens=-1), "negative"), (dict(k_tokens=-4), "negative"), (dict(k_heads=0), "multiple of k_heads"),
+    (dict(q_heads=3), "multiple of k_heads"), (dict(head_dim=0), "head_dim"), (dict(head_dim=60), "head_dim"),
+    (dict(head_dim=264), "head_dim"), (dict(q_tokens=2 ** 30 + 1), "too many tokens"),
+    (dict(q_heads=2 ** 20, k_heads=1, q_tokens=2 ** 12), "too many tokens"),
+    (dict(batch=2 ** 24, q_tokens=64), "too large"), (dict(scale=math.nan), "scale"),
+    (dict(scale=math.inf), "scale"), (dict(cap=-0.5), "cap"), (dict(cap=math.inf), "cap"),
+    (dict(left=-2), "window"), (dict(right=2 ** 30 + 1), "window"), (dict(doc_q=BUF), "come together"),
+    (dict(code_k=BUF), "come together"), (dict(table=BUF, table_len=0), "without entries"),
+    (dict(table=BUF, table_len=5, table_zero=2 ** 30 + 1), "table_zero"), (dict(q=None), "null"),
+    (dict(out=None), "null"), (dict(v=None), "null"), (dict(k=BUF + 8), "aligned"),
+    (dict(out=BUF + 2), "aligned"), (dict(q_stride=(1280, 260, 64)), "strides"),
+    (dict(v_stride=(896, 128, 4)), "strides"), (dict(lse=BUF + 2), "misaligned"),
+    (dict(kv_len=BUF + 1), "misaligned"), (dict(out=BUF), "overlap"), (dict(out=BUF * 3), "overlap"),
+    (dict(out_stride=(0, 256, 64)), "zero stride"), (dict(out_stride=(1280, 256, 0)), "zero stride"),
+])
+def test_attention_refusals(change, text):
+    _refused(_lib.lib().arthip_attention, _attention(**change), text)
+
+
+def test_attention_workspace():
+    """Few rows over many keys need one, and a call without it is refused; many rows, or
+    few keys, need none."""
+    lib = _lib.lib()
+    size = lambda a: lib.arthip_attention_workspace(ctypes.byref(a))  # noqa: E731
+    assert size(_attention()) == 0
+    assert size(_attention(batch=64, q_tokens=4096, k_tokens=4096, q_heads=32, k_heads=8)) == 0
+    long = _attention(q_tokens=1, k_tokens=100000)
+    need = size(long)
+    assert need > 0
+    _refused(lib.arthip_attention, long, f"{need} bytes")
+    _refused(lib.arthip_attention, _set(long, workspace=BUF * 8, workspace_bytes=need - 1), "workspace")
+    _refused(lib.arthip_attention, _set(long, workspace=BUF * 8 + 4, workspace_bytes=need), "misaligned")
+    for a in (_attention(k_heads=0), _attention(batch=0), _attention(q_tokens=0), _attention(q_heads=0),
+              _attention(batch=-1)):
+        assert size(a) == 0
+    assert lib.arthip_attention_workspace(None) == 0
+
+
+def test_calls_without_tokens():
+    lib = _lib.lib()
+    for change in (dict(batch=0), dict(q_tokens=0), dict(q_heads=0)):
+        a = _attention(q=None, k=None, v=None, out=None, **change)
+        assert lib.arthip_attention(ctypes.byref(a), None) == 0
+    for change in (dict(batch=0), dict(tokens=0)):
+        assert lib.arthip_rope_axes(ctypes.byref(_rope(q=None, k=None, **change)), None) == 0
+        n = _norm(residual=None, **change)
+        assert lib.arthip_gated_norm(ctypes.byref(n), None) == 0
+    assert lib.arthip_attention(None, None) == 1 and "null" in _lib.last_error()
+    assert lib.arthip_rope_axes(None, None) == 1 and "null" in _lib.last_error()
+    assert lib.arthip_gated_norm(None, None) == 1 and "null" in _lib.last_error()
+
+
+def _rope(**change):
+    a = _lib.RopeArgs()
+    _set(a, q=BUF, k=BUF * 2, q_out=BUF * 3, k_out=BUF * 4, pos=BUF * 5, packed=BUF * 6, batch=2, tokens=3,
+         q_heads=4, k_heads=2, head_dim=64, n_freq=32, dtype=0, q_stride=(768, 256, 64),
+         k_stride=(384, 128, 64), q_out_stride=(768, 256, 64), k_out_stride=(384, 128, 64),
+         pos_stride=(6, 3, 1))
+    return _set(a, **change)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=3), "type"), (dict(tokens=-1), "negative"), (dict(k_heads=-1), "negative"),
+    (dict(batch=2 ** 16, tokens=2 ** 16), "too many tokens"), (dict(q_heads=65536, k_heads=1), "too many heads"),
+    (dict(head_dim=63), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(head_dim=514), "head_dim"),
+    (dict(n_freq=0), "n_freq"), (dict(n_freq=33), "n_freq"), (dict(pairs=2), "0 or 1"),
+    (dict(inverse=-1), "0 or 1"), (dict(q=None), "null query"), (dict(k_out=None), "null key"),
+    (dict(pos=None), "null positions"), (dict(packed=None), "null positions"), (dict(q=BUF + 1), "misaligned"),
+    (dict(packed=BUF + 8), "misaligned"), (dict(pos=BUF + 2), "misaligned"),
+    (dict(q_out_stride=(768, 0, 64)), "zero stride"), (dict(k_out_stride=(0, 128, 64)), "zero stride"),
+    (dict(q_out=BUF, q_out_stride=(768, 64, 192)), "in place"),
+])
+def test_rope_refusals(change, text):
+    _refused(_lib.lib().arthip_rope_axes, _rope(**change), text)
+
+
+def test_rope_pack():
+    lib = _lib.lib()
+    freqs, axis = [1.0, 0.25, 1e-4], [0, 2, 1]
+    f, x = (ctypes.c_double * 3)(*freqs), (ctypes.c_int32 * 3)(*axis)
+    size = lib.arthip_rope_packed_bytes(3)
+    assert size == 48 and lib.arthip_rope_packed_bytes(0) == 0 and lib.arthip_rope_packed_bytes(-1) == 0
+    buf = ctypes.create_string_buffer(size)
+    assert lib.arthip_rope_pack(f, x, 3, 3, buf, size) == 0
+    got = np.frombuffer(buf.raw, dtype=np.dtype([("turns", "<f8"), ("axis", "<i4"), ("pad", "<i4")]))
+    np.testing.assert_array_equal(got["turns"], np.array(freqs) / (2 * math.pi))
+    np.testing.assert_array_equal(got["axis"], axis)
+    for args, text in [((None, x, 3, 3, buf, size), "null"), ((f, x, 0, 3, buf, size), "null"),
+                       ((f, x, 3, 3, buf, size - 1), "small"), ((f, x, 3, 2, buf, size), "axis"),
+                       (((ctypes.c_double * 3)(1.0, math.nan, 1.0), x, 3, 3, buf, size), "finite")]:
+        assert lib.arthip_rope_pack(*args) == 1 and text in _lib.last_error()
+
+
+def test_rope_plan_frequencies():
+    """The plan's frequencies and axes (host logic; the packed copy stays on the CPU)."""
+    plan = tr.RopePlan((2, 1, 1), theta=100.0, device="cpu")
+    assert plan.axis == (0, 0, 1, 2)
+    np.testing.assert_allclose(plan.freqs, [100.0 ** (-f / 4) for f in range(4)], rtol=1e-15)
+    plan = tr.RopePlan((2, 1, 1), theta=100.0, order="cycle", per_axis=True, scale=(1, 2, 0.5), device="cpu")
+    assert plan.axis == (0, 1, 2, 0)
+    np.testing.assert_allclose(plan.freqs, [1, 2, 0.5, 0.1], rtol=1e-15)
+    assert tr.RopePlan((1, 1), freqs=(3.0, 4.0), device="cpu").freqs == (3.0, 4.0)
+    for kw in (dict(sections=()), dict(sections=(0,)), dict(sections=(-1, 2)), dict(sections=(2,), order="x"),
+               dict(sections=(2,), theta=0.0), dict(sections=(2,), scale=(1, 2)), dict(sections=(2,), freqs=(1.0,)),
+               dict(sections=(1,), freqs=(math.inf,))):
+        with pytest.raises(EngineError):
+            tr.RopePlan(kw.pop("sections"), device="cpu", **kw)
+
+
+def _norm(**change):
+    a = _lib.NormArgs()
+    _set(a, residual=BUF, y=BUF * 2, residual_out=BUF * 3, h=BUF * 4, batch=2, tokens=3, channels=64, dtype=0,
+         residual_dtype=0, post=1, pre=2, gate_act=0, eps=1e-6, residual_scale=1.0, branch_scale=1.0,
+         residual_stride=(192, 64), y_stride=(192, 64), residual_out_stride=(192, 64), h_stride=(192, 64))
+    return _set(a, **change)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=3), "type"), (dict(dtype=0, residual_dtype=1), "residual type"),
+    (dict(dtype=2, residual_dtype=0), "residual type"), (dict(post=3), "unknown norm"),
+    (dict(pre=-1), "unknown norm"), (dict(gate_act=4), "activation"), (dict(tokens=-1), "negative"),
+    (dict(batch=2 ** 16, tokens=2 ** 15), "too many"), (dict(channels=0), "channels"),
+    (dict(channels=32769), "channels"), (dict(eps=-1e-6), "eps"), (dict(eps=math.nan), "eps"),
+    (dict(branch_scale=math.inf), "scale"), (dict(residual_scale=math.nan), "scale"),
+    (dict(residual=None), "null residual"), (dict(residual_out=None, h=None, pre=0), "no output"),
+    (dict(y=None), "without y"), (dict(h=None), "without h"), (dict(h=None, pre=0, mod_shift=BUF), "without h"),
+    (dict(residual=BUF + 1), "misaligned"), (dict(y=BUF + 1), "misaligned"), (dict(pre_weight=BUF + 2), "misaligned"),
+    (dict(residual_out_stride=(0, 64)), "zero stride"), (dict(h_stride=(192, 0)), "zero stride"),
+    (dict(residual_out=BUF, residual_out_stride=(384, 128)), "in place"), (dict(h=BUF), "overlap"),
+    (dict(h=BUF * 2), "overlap"), (dict(h=BUF * 3), "overlap"), (dict(residual_out=BUF * 2), "overlap"),
+])
+def test_norm_refusals(change, text):
+    _refused(_lib.lib().arthip_gated_norm, _norm(**change), text)
+
+
+def test_tensors_must_be_on_a_gpu():
+    x = torch.zeros(1, 2, 2, 32, dtype=torch.float16)
+    with pytest.raises(EngineError, match="on a GPU"):
+        tr.attention(x, x, x)
+    with pytest.raises(EngineError, match="on a GPU"):
+        tr.rope_axes(x, x, torch.zeros(1, 1, 2, dtype=torch.int32), tr.RopePlan((16,), device="cpu"))
+    with pytest.raises(EngineError, match="on a GPU"):
+        tr.gated_norm(torch.zeros(1, 2, 64), pre="rms")

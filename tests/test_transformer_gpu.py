@@ -1,0 +1,585 @@
+"""The transformer operators on the GPU against their definitions in float64
+(tests/transformer_reference.py, whose tolerances are derived there): types, head
+layouts, lengths, masks, strides, streams, graphs and values that are not finite."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from arthip_amd import transformer as tr
+from arthip_amd.engine import EngineError
+from tests import transformer_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _normal(g, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, generator=g) * std).to(dtype).cuda()
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32).cuda()
+
+
+# -- rotary positions ------------------------------------------------------------------
+
+ROPE = [
+    # dtype, B, L, Hq, Hk, D, sections, pairs, per_axis, order
+    (BF16, 1, 1, 4, 2, 128, (16, 24, 24), False, False, "blocks"),
+    (F16, 2, 5, 3, 3, 64, (8, 12, 12), True, True, "blocks"),
+    (F16, 1, 33, 32, 8, 128, (16, 24, 24), False, False, "cycle"),
+    (BF16, 3, 7, 5, 1, 72, (36,), True, False, "blocks"),
+    (F16, 1, 9, 2, 2, 72, (9, 9), False, True, "blocks"),      # half of a head turned
+    (F32, 2, 11, 3, 1, 80, (10, 20, 10), False, True, "cycle"),
+    (F32, 1, 3, 1, 1, 32, (16,), True, False, "blocks"),
+    (BF16, 1, 300, 1, 1, 6, (1, 1), True, True, "blocks"),      # odd counts: single values
+    (F16, 1, 4, 2, 1, 2, (1,), False, False, "blocks"),
+    (F16, 1, 4, 70, 3, 512, (100, 28), False, False, "blocks"),
+    (BF16, 5, 257, 6, 2, 96, (2, 46), True, True, "blocks"),
+]
+
+
+def _rope_case(dtype, b, l, hq, hk, d, sections, seed=0, top=9000):
+    g = _gen(seed)
+    q, k = _normal(g, b, l, hq, d, dtype=dtype), _normal(g, b, l, hk, d, dtype=dtype)
+    pos = torch.randint(-top, top, (len(sections), b, l), generator=g, dtype=torch.int32).cuda()
+    return q, k, pos
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("dtype,b,l,hq,hk,d,sections,pairs,per_axis,order", ROPE)
+def test_rope(dtype, b, l, hq, hk, d, sections, pairs, per_axis, order, inverse):
+    q, k, pos = _rope_case(dtype, b, l, hq, hk, d, sections)
+    plan = tr.RopePlan(sections, per_axis=per_axis, pairs=pairs, order=order)
+    qo, ko = tr.rope_axes(q, k, pos, plan, inverse=inverse)
+    for name, x, got in (("q", q, qo), ("k", k, ko)):
+        ref.check(got, ref.rope(x, pos, plan.axis, plan.freqs, pairs, inverse), name)
+
+
+def test_rope_large_positions_keep_their_phase():
+    q, k, pos = _rope_case(F32, 1, 64, 2, 1, 64, (16, 16), top=2 ** 31 - 1)
+    plan = tr.RopePlan((16, 16))
+    qo, _ = tr.rope_axes(q, k, pos, plan)
+    ref.check(qo, ref.rope(q, pos, plan.axis, plan.freqs), "q")
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+def test_rope_in_place_strides_and_one_side(pairs):
+    """q and k as views of one projection, turned in place; values past the turned ones
+    and the rest of the buffer stay."""
+    g = _gen(3)
+    qkv = _normal(g, 2, 6, 8, 80, dtype=F16)
+    want = qkv.clone()
+    pos = torch.randint(0, 500, (2, 6), generator=g, dtype=torch.int32).cuda()  # for every batch item
+    plan = tr.RopePlan((5, 15), pairs=pairs)
+    q, k = qkv[:, :, :4], qkv[:, :, 4:6]
+    fresh_q, fresh_k = tr.rope_axes(q, k, pos, plan)
+    full = pos[:, None].expand(2, 2, 6)
+    ref.check(fresh_q, ref.rope(q, full, plan.axis, plan.freqs, pairs), "q")
+    assert torch.equal(qkv, want)
+    out = tr.rope_axes(q, None, pos, plan, q_out=q)
+    assert out[1] is None and torch.equal(q, fresh_q) and torch.equal(k, want[:, :, 4:6])
+    tr.rope_axes(None, k, pos, plan, k_out=k)
+    assert torch.equal(k, fresh_k) and torch.equal(qkv[:, :, 6:], want[:, :, 6:])
+    # heads first, and an odd element offset
+    flat = _normal(g, 2 * 3 * 6 * 40 + 1, dtype=F16)[1:]
+    q = flat.view(2, 3, 6, 40).permute(0, 2, 1, 3)
+    got, _ = tr.rope_axes(q, None, pos, plan)
+    ref.check(got, ref.rope(q, full, plan.axis, plan.freqs, pairs), "permuted")
+
+
+def test_rope_inverse_is_the_transpose():
+    q, k, pos = _rope_case(F32, 1, 40, 2, 2, 64, (16, 16))
+    plan = tr.RopePlan((16, 16), theta=500.0)
+    qo, _ = tr.rope_axes(q, k, pos, plan)
+    _, kb = tr.rope_axes(q, k, pos, plan, inverse=True)
+    back, _ = tr.rope_axes(qo, None, pos, plan, inverse=True)
+    assert (back - q).abs().max() < 4e-6 * q.abs().max()
+    a, b = (qo.double() * k.double()).sum(), (q.double() * kb.double()).sum()
+    assert (a - b).abs() < 1e-6 * (q.double().norm() * k.double().norm())
+
+
+# -- attention -------------------------------------------------------------------------
+
+def _qkv(seed, dtype, b, lq, lk, hq, hk, d, std=1.0):
+    g = _gen(seed)
+    return (_normal(g, b, lq, hq, d, dtype=dtype, std=std), _normal(g, b, lk, hk, d, dtype=dtype, std=std),
+            _normal(g, b, lk, hk, d, dtype=dtype))
+
+
+def _attend(q, k, v, name="", **kw):
+    out, lse = tr.attention(q, k, v, return_lse=True, **kw)
+    want = ref.attention(q, k, v, **kw)
+    ref.check(out, want[0], name + " out")
+    ref.check(lse, want[1], name + " lse")
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [8, 32, 40, 64, 80, 96, 128, 136, 256])
+def test_attention_head_dims(dtype, d):
+    for lq, lk, hq, hk in ((1, 70, 2, 2), (45, 130, 4, 2), (300, 65, 3, 1)):
+        _attend(*_qkv(d, dtype, 1, lq, lk, hq, hk, d), name=f"{lq}x{lk}")
+
+
+@pytest.mark.parametrize("lk", [0, 1, 31, 32, 33, 63, 64, 65, 127, 200])
+def test_attention_lengths(lk):
+    for lq in (1, 2, 33, 129):
+        _attend(*_qkv(lk, F16, 2, lq, lk, 2, 1, 64), name=f"{lq}x{lk}")
+
+
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 65), (2, 64), (17, 17), (64, 64), (65, 130), (130, 65),
+                                   (257, 257), (40, 300)])
+@pytest.mark.parametrize("heads", [(4, 4), (4, 1), (6, 2)])
+def test_attention_causal(lq, lk, heads):
+    """Also more queries than keys: the first rows see nothing."""
+    out, lse = _attend(*_qkv(lq + lk, BF16, 2, lq, lk, *heads, 64), causal=True)
+    empty = max(lq - lk, 0)
+    assert not out[:, :empty].any() and torch.isneginf(lse[:, :, :empty]).all()
+    assert torch.isfinite(lse[:, :, empty:]).all()
+
+
+@pytest.mark.parametrize("window", [(0, 0), (7, 3), (64, 0), (None, 5), (100, None), (1000, 1000)])
+def test_attention_window(window):
+    q, k, v = _qkv(5, F16, 1, 150, 210, 2, 2, 32)
+    _attend(q, k, v, window=window)
+    _attend(q, k, v, window=window, q_start=_ints([-40]))
+    _attend(q, k, v, window=window, q_start=_ints([500]))
+
+
+@pytest.mark.parametrize("lq", [1, 5, 140])
+def test_attention_prefix_and_lengths(lq):
+    q, k, v = _qkv(6, BF16, 4, lq, 190, 4, 2, 64)
+    kv_len = _ints([190, 0, 1, 100])
+    q_start = _ints([190 - lq, 0, 0, 60])
+    prefix = _ints([0, 50, 190, 33])
+    _attend(q, k, v, kv_len=kv_len)
+    _attend(q, k, v, causal=True, kv_len=kv_len, q_start=q_start)
+    _attend(q, k, v, causal=True, prefix=prefix)
+    _attend(q, k, v, window=(20, 0), prefix=prefix, kv_len=kv_len, q_start=q_start)
+    # lengths and prefixes outside the cache are taken to its ends
+    far = _ints([1000, -5, 191, 100])
+    a = tr.attention(q, k, v, causal=True, kv_len=far, prefix=far)
+    b = tr.attention(q, k, v, causal=True, kv_len=_ints([190, 0, 190, 100]), prefix=_ints([190, 0, 190, 100]))
+    assert torch.equal(a, b)
+
+
+def test_attention_documents():
+    g = _gen(7)
+    q, k, v = _qkv(7, F16, 2, 330, 330, 2, 1, 64)
+    packed = torch.repeat_interleave(torch.arange(6), torch.tensor([1, 100, 63, 65, 40, 61])).int().cuda()
+    _attend(q, k, v, docs=(packed, packed))
+    _attend(q, k, v, docs=(packed, packed), causal=True)
+    mixed = torch.randint(-3, 3, (2, 330), generator=g, dtype=torch.int32).cuda()  # in no order
+    _attend(q, k, v, docs=(mixed, mixed))
+    _attend(q, k, v, docs=(mixed, mixed), window=(50, 20), prefix=_ints([9, 70]))
+    other = packed + 4  # some queries' documents hold no key
+    out, lse = _attend(q, k, v, docs=(other, packed))
+    gone = (other > 5).cpu()
+    assert not out[:, gone].any() and torch.isneginf(lse[:, :, gone]).all()
+
+
+def test_attention_documents_long():
+    """More tiles than one look over the documents covers."""
+    n = 140000
+    q, k, v = _qkv(8, BF16, 1, 3, n, 1, 1, 32)
+    doc_k = (torch.arange(n) // 1000).int().cuda()
+    doc_q = _ints([0, 139, 70])
+    _attend(q, k, v, docs=(doc_q, doc_k))
+
+
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("lq,lk", [(1, 100), (81, 81), (200, 70)])
+def test_attention_bias(lq, lk, cap):
+    g = _gen(9)
+    q, k, v = _qkv(9, F16, 2, lq, lk, 6, 2, 32)
+    slopes = torch.rand(6, generator=g).cuda()
+    _attend(q, k, v, slopes=slopes, cap=cap)
+    _attend(q, k, v, slopes=slopes, cap=cap, causal=True, q_start=_ints([3, lk - lq]))
+    table = _normal(g, 6, 41)
+    _attend(q, k, v, table=table, table_zero=20, cap=cap)
+    codes = (torch.randint(-40, 40, (2, lq), generator=g, dtype=torch.int32).cuda(),
+             torch.randint(-40, 40, (lk,), generator=g, dtype=torch.int32).cuda())
+    _attend(q, k, v, table=table, table_zero=20, codes=codes, cap=cap)
+    _attend(q, k, v, table=table, table_zero=20, slopes=slopes, codes=codes, cap=cap, window=(30, 5))
+    big = _normal(g, 6, 9000)  # more entries than a workgroup keeps on the chip
+    _attend(q, k, v, table=big, table_zero=4500, cap=cap)
+
+
+def test_attention_window_table_in_two_dimensions():
+    g = _gen(10)
+    n, d = 7, 32
+    q, k, v = _qkv(10, F16, 3, n * n, n * n, 2, 2, d)
+    y, x = torch.arange(n * n) // n, torch.arange(n * n) % n
+    codes = (y * (2 * n - 1) + x).int().cuda()
+    zero = (n - 1) * (2 * n - 1) + n - 1
+    table = _normal(g, 2, (2 * n - 1) ** 2)
+    _attend(q, k, v, table=table, table_zero=zero, codes=(codes, codes))
+    hidden = table.clone()
+    hidden[:, zero + 1:] = -math.inf  # entries that hide: only offsets of zero or less are seen
+    _attend(q, k, v, table=hidden, table_zero=zero, codes=(codes, codes))
+    hidden[1] = -math.inf
+    out, lse = _attend(q, k, v, table=hidden, table_zero=zero, codes=(codes, codes))
+    assert not out[:, :, 1].any() and torch.isneginf(lse[:, 1]).all()
+
+
+@pytest.mark.parametrize("scale,std", [(0.0, 1.0), (-0.3, 1.0), (3.0, 3.0), (1e-4, 1.0)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_attention_scale(scale, std, cap):
+    """Peaked, flat and reversed scores; a running maximum that keeps growing."""
+    q, k, v = _qkv(11, BF16, 1, 70, 300, 2, 1, 64, std=std)
+    k = k * torch.linspace(0.1, 2, 300, device="cuda")[None, :, None, None].to(BF16)
+    _attend(q, k, v, scale=scale, cap=cap)
+
+
+@pytest.mark.parametrize("lq", [1, 100])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_hidden_values(lq, dtype):
+    """NaN, infinities and the type's ends in places that no query, or not every query,
+    sees."""
+    q, k, v = _qkv(12, dtype, 2, lq, 200, 4, 2, 64)
+    top = torch.finfo(dtype).max
+    for bad in (math.nan, math.inf, -math.inf, top, -top):
+        kb, vb = k.clone(), v.clone()
+        kb[:, 150:], vb[:, 150:] = bad, bad
+        _attend(q, kb, vb, f"{bad} past the length", kv_len=_ints([150, 149]))
+        docs = (torch.zeros(lq).int().cuda(), (torch.arange(200) >= 150).int().cuda())
+        _attend(q, kb, vb, f"{bad} in another document", docs=docs)
+        table = torch.zeros(4, 2)
+        table[:, 1] = -math.inf
+        codes = (torch.zeros(lq).int().cuda(), -(torch.arange(200) >= 150).int().cuda())
+        _attend(q, kb, vb, f"{bad} behind the table", table=table.cuda(), codes=codes)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_hidden_from_some(bad):
+    """A key that is not finite reaches the rows that see it and no other."""
+    q, k, v = _qkv(13, F16, 1, 100, 100, 2, 1, 64)
+    vb = v.clone()
+    vb[0, 70, 0, 5] = bad
+    vb[0, 80, 0, 6] = -bad
+    out, _ = _attend(q, k, vb, causal=True)
+    assert torch.isfinite(out[:, :70]).all() and not torch.isfinite(out[0, 70:, :, 5]).any()
+    kb = k.clone()
+    kb[0, 70] = math.nan
+    out = tr.attention(q, kb, v, causal=True)
+    assert torch.isfinite(out[:, :70]).all() and torch.isnan(out[:, 70:]).all()
+
+
+def test_attention_layouts():
+    """Heads before tokens, one projection's views, a broadcast key, gaps between tokens."""
+    g = _gen(14)
+    qkv = _normal(g, 2, 75, 12, 64, dtype=F16)
+    q, k, v = qkv[:, :, :6], qkv[:, :, 6:9], qkv[:, :, 9:]
+    plain, _ = _attend(q, k, v, causal=True)
+    heads = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    out = torch.empty(2, 6, 75, 64, dtype=F16, device="cuda").transpose(1, 2)
+    got = tr.attention(*heads, causal=True, out=out)
+    assert got is out and torch.equal(out, plain)
+    one = [t[:1].expand(2, -1, -1, -1) for t in (k, v)]
+    _attend(q, *one)
+    wide = torch.full((2, 75, 6, 96), math.nan, dtype=F16, device="cuda")
+    wide[..., 16:80] = q
+    assert torch.equal(tr.attention(wide[..., 16:80], k, v, causal=True), plain)
+    assert torch.equal(tr.attention(q[:1], k[:1], v[:1], causal=True), plain[:1])
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_attention_long_strides(lq):
+    """Keys whose offsets pass 32 bits."""
+    n, step = 70, 2 ** 25
+    store = torch.zeros(n * step + 64, dtype=F16, device="cuda")
+    k = store.as_strided((1, n, 1, 64), (0, step, 64, 1))
+    q, kd, vd = _qkv(15, F16, 1, lq, n, 2, 1, 64)
+    k.copy_(kd)
+    want = tr.attention(q, kd, vd)
+    assert torch.equal(tr.attention(q, k, vd), want)
+    k.copy_(vd)
+    assert torch.equal(tr.attention(q, kd, k), want)
+
+
+@pytest.mark.parametrize("lq,lk,hq,hk,b", [(1, 5000, 4, 1, 2), (3, 3000, 8, 2, 1), (100, 2500, 2, 1, 1),
+                                           (300, 4000, 2, 2, 1), (1, 20000, 32, 8, 1), (40, 700, 1, 1, 1)])
+def test_attention_split_keys(lq, lk, hq, hk, b):
+    """Few rows over many keys, which are divided over workgroups and joined."""
+    q, k, v = _qkv(16, BF16, b, lq, lk, hq, hk, 32)
+    _attend(q, k, v)
+    _attend(q, k, v, causal=True, kv_len=_ints([lk - 7 * i - 1 for i in range(b)]),
+            q_start=_ints([lk - lq - 7 * i - 1 for i in range(b)]))
+    _attend(q, k, v, window=(1000, 0), prefix=_ints([37] * b))
+    none = _ints([0] * b)
+    out, lse = _attend(q, k, v, kv_len=none)
+    assert not out.any() and torch.isneginf(lse).all()
+
+
+def test_attention_nothing_to_do():
+    q, k, v = _qkv(17, F16, 2, 4, 9, 2, 2, 32)
+    assert tr.attention(q[:0], k[:0], v[:0]).shape == (0, 4, 2, 32)
+    assert tr.attention(q[:, :0], k, v).shape == (2, 0, 2, 32)
+    out, lse = tr.attention(q, k[:, :0], v[:, :0], return_lse=True)
+    assert not out.any() and torch.isneginf(lse).all()
+
+
+def test_attention_masks_by_differences():
+    """Moving a hidden key or value changes no bit; moving a seen one moves the output
+    by its weight (a central difference of the value against the softmax's weight)."""
+    q, k, v = _qkv(18, F16, 1, 50, 50, 1, 1, 32)
+    base, lse = tr.attention(q, k, v, causal=True, return_lse=True)
+    kb, vb = k.clone(), v.clone()
+    kb[:, 30:], vb[:, 30:] = -kb[:, 30:], 5 * vb[:, 30:]
+    moved = tr.attention(q, kb, vb, causal=True)
+    assert torch.equal(moved[:, :30], base[:, :30])
+    up, down = v.clone(), v.clone()
+    up[0, 10, 0], down[0, 10, 0] = 64.0, -64.0
+    diff = (tr.attention(q, k, up, causal=True).double() - tr.attention(q, k, down, causal=True).double()) / 128
+    s = (q[0, :, 0].double() @ k[0, 10, 0].double()) / math.sqrt(32)
+    weight = torch.exp(s - lse[0, 0].double())
+    weight[:10] = 0
+    # rounding of the weight (2^-11) and of the two results (2^-11 of at most 64 + max |v|)
+    assert (diff[0, :, 0] - weight[:, None]).abs().max() < 2 ** -11 + 2 * 2 ** -11 * 68 / 128 + 1e-5
+
+
+# -- norms around a gated residual ---------------------------------------------------------
+
+NORM = [
+    # dtype, residual, B, L, C, post, pre, gate shape, act, modulation, biases
+    (BF16, BF16, 4, 1, 4096, "rms", "rms", "channel", "none", False, False),
+    (F16, F16, 2, 37, 1024, "layer", "layer", "batch", "tanh", True, True),
+    (BF16, F32, 3, 19, 975, "rms", "rms", "token", "sigmoid", False, False),
+    (F16, F32, 1, 5, 1, "rms", "layer", "channel", "silu", False, True),
+    (F16, F16, 1, 9, 7, "layer", "rms", "token", "none", True, False),
+    (F32, F32, 2, 3, 513, "layer", "layer", "batch", "tanh", True, True),
+    (F16, F16, 1, 3, 5120, "rms", None, None, "none", False, True),
+    (BF16, BF16, 1, 3, 8200, None, "layer", "token", "silu", True, True),
+    (BF16, F32, 1, 2, 32768, "layer", "rms", "channel", "sigmoid", True, True),
+    (F32, F32, 1, 130, 64, None, None, "batch", "none", True, False),
+    (F16, F16, 5, 41, 72, "rms", "rms", "channel", "none", False, False),
+    (BF16, BF16, 1, 7, 2047, "layer", "layer", "token", "tanh", True, True),
+]
+
+
+def _norm_case(dtype, res, b, l, c, post, pre, gate, act, mod, bias, seed=0):
+    g = _gen(seed + c)
+    shapes = {"channel": (c,), "batch": (b, 1, c), "token": (b, l, c)}
+    kw = {"post": post, "pre": pre, "gate_act": act, "branch_scale": 0.7, "residual_scale": 1.1}
+    for side, kind in (("post", post), ("pre", pre)):
+        if kind is not None:
+            kw[side + "_weight"] = 1 + _normal(g, c, std=0.2)
+            if bias:
+                kw[side + "_bias"] = _normal(g, c, std=0.2)
+    if gate is not None:
+        kw["gate"] = _normal(g, *shapes[gate], dtype=dtype)
+    if mod:
+        kw["mod_scale"], kw["mod_shift"] = (_normal(g, b, 1, c, dtype=dtype, std=0.3) for _ in range(2))
+    return _normal(g, b, l, c, dtype=res, std=2.0), _normal(g, b, l, c, dtype=dtype) + 0.5, kw
+
+
+@pytest.mark.parametrize("dtype,res,b,l,c,post,pre,gate,act,mod,bias", NORM)
+def test_gated_norm(dtype, res, b, l, c, post, pre, gate, act, mod, bias):
+    r, y, kw = _norm_case(dtype, res, b, l, c, post, pre, gate, act, mod, bias)
+    want = ref.gated_norm(r, y, **kw)
+    new, h = tr.gated_norm(r, y, **kw)
+    ref.check(new, want[0], "residual")
+    if h is not None:
+        ref.check(h, want[1], "h")
+    again = tr.gated_norm(r, y, **kw)
+    assert torch.equal(again[0], new) and (h is None or torch.equal(again[1], h))
+    place = r.clone()
+    out, _ = tr.gated_norm(place, y, residual_out=place, **kw)
+    assert out is place and torch.equal(place, new)
+
+
+def test_gated_norm_parts_alone():
+    """The first norm of a network (no branch), the last residual (no norm after it)."""
+    g = _gen(20)
+    r, y = _normal(g, 2, 5, 136, dtype=BF16), _normal(g, 2, 5, 136, dtype=BF16)
+    w = 1 + _normal(g, 136, std=0.1)
+    same, h = tr.gated_norm(r, pre="rms", pre_weight=w)
+    assert same is r
+    ref.check(h, ref.gated_norm(r, pre="rms", pre_weight=w)[1], "h")
+    new, h = tr.gated_norm(r, y, post="rms", post_weight=w)
+    assert h is None
+    ref.check(new, ref.gated_norm(r, y, post="rms", post_weight=w)[0], "residual")
+    scaled, none = tr.gated_norm(r, residual_scale=0.5)
+    assert none is None and torch.equal(scaled, r * 0.5)
+    wide, h = tr.gated_norm(r.float(), pre="layer", dtype=F16)
+    assert h.dtype == F16
+    ref.check(h, ref.gated_norm(r.float(), pre="layer", dtype=F16)[1], "h of an fp32 residual")
+
+
+def test_gated_norm_strides():
+    """Views of wider tensors, misaligned rows, a broadcast residual, tokens of an image's
+    interior."""
+    g = _gen(21)
+    big = _normal(g, 2, 9, 301, dtype=F16)
+    y = _normal(g, 2, 9, 77, dtype=F16)
+    for lo in (0, 1, 3, 8, 200):
+        r = big[..., lo:lo + 77]
+        want = ref.gated_norm(r, y, post="rms", pre="layer")
+        new, h = tr.gated_norm(r, y, post="rms", pre="layer")
+        ref.check(new, want[0], "residual")
+        ref.check(h, want[1], "h")
+        place = big.clone()
+        tr.gated_norm(r, y, post="rms", pre="layer", residual_out=place[..., lo:lo + 77])
+        assert torch.equal(place[..., lo:lo + 77], new)
+        place[..., lo:lo + 77] = big[..., lo:lo + 77]
+        assert torch.equal(place, big)
+    one = big[:1, :1, :77].expand(2, 9, 77)
+    ref.check(tr.gated_norm(one, y)[0], ref.gated_norm(one, y)[0], "broadcast residual")
+    padded = _normal(g, 6, 10, 64, dtype=F16)  # rows of an image with a border
+    inner = padded[1:5, 1:9]
+    ref.check(tr.gated_norm(inner, pre="rms")[1], ref.gated_norm(inner, pre="rms")[1], "interior")
+
+
+def test_gated_norm_large_mean_and_zeros():
+    """A mean a thousand times the spread; rows of zeros; eps = 0 on them."""
+    g = _gen(22)
+    r = 1000 + _normal(g, 1, 4, 640)
+    ref.check(tr.gated_norm(r, pre="layer")[1], ref.gated_norm(r, pre="layer")[1], "large mean")
+    zero = torch.zeros(1, 3, 100, dtype=F16, device="cuda")
+    assert not tr.gated_norm(zero, pre="rms")[1].any() and not tr.gated_norm(zero, pre="layer")[1].any()
+    assert torch.isnan(tr.gated_norm(zero, pre="rms", eps=0.0)[1]).all()
+
+
+def test_gated_norm_rows_do_not_mix():
+    """A row of NaN stays one row, also where rows share a workgroup."""
+    for c in (64, 72, 700, 1024):
+        r = _normal(_gen(c), 1, 11, c, dtype=F16)
+        clean = tr.gated_norm(r, pre="layer")[1]
+        r[0, 5, c // 2] = math.nan
+        h = tr.gated_norm(r, pre="layer")[1]
+        assert torch.isnan(h[0, 5]).all()
+        keep = [i for i in range(11) if i != 5]
+        assert torch.equal(h[0, keep], clean[0, keep])
+
+
+# -- streams and graphs ------------------------------------------------------------------------
+
+def _block_case():
+    q, k, v = _qkv(30, F16, 1, 3, 3000, 4, 2, 64)
+    kq = k[:, -3:].contiguous()
+    g = _gen(30)
+    res = _normal(g, 1, 3, 256, dtype=F16)
+    pos = torch.randint(0, 99, (2, 1, 3), generator=g, dtype=torch.int32).cuda()
+    return q, kq, k, v, pos, tr.RopePlan((16, 16)), res, {"post": "rms", "pre": "layer"}
+
+
+def _run(case):
+    q, kq, k, v, pos, plan, res, kw = case
+    qr, kr = tr.rope_axes(q, kq, pos, plan)
+    o, lse = tr.attention(qr, k, v, causal=True, return_lse=True)
+    new, h = tr.gated_norm(res, o.flatten(2), **kw)
+    return qr, kr, o, lse, new, h
+
+
+def test_streams():
+    """On a stream of their own, chosen as the current one or by its handle, the operators
+    give the same bits, with inputs that the stream itself made just before."""
+    case = _block_case()
+    want = _run(case)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    q, k, v = case[0], case[2], case[3]
+    with torch.cuda.stream(s):
+        late = q + 0
+        got = _run((late,) + case[1:])
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.cuda.stream(s):
+        late = want[0] + 0
+    o = tr.attention(late, k, v, causal=True, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(o, want[2])
+
+
+def test_graph_replays():
+    case = _block_case()
+    want = _run(case)
+    q = case[0]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            _run(case)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _run(case)
+    other = -q
+    first = q.clone()
+    for turn in range(4):
+        for t in got:
+            t.zero_()
+        q.copy_(other if turn % 2 else first)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = _run(case)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)), turn
+        if turn % 2 == 0:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# -- refusals that need tensors on the GPU ---------------------------------------------------------
+
+def test_refusals():
+    q, k, v = _qkv(40, F16, 2, 4, 9, 4, 2, 32)
+    bad = [
+        (dict(q=q.float()), "unsupported type"),
+        (dict(k=k.bfloat16()), "k must be"),
+        (dict(v=v[:, :8]), "k and v"),
+        (dict(k=k[:, :, :1], v=v[:, :, :1].expand(-1, -1, 3, -1)), "k and v"),
+        (dict(q=q[:, :, :3]), "multiple of k_heads"),
+        (dict(q=q[..., ::2], k=k[..., ::2], v=v[..., ::2]), "contiguous"),
+        (dict(q=q[..., :12], k=k[..., :12], v=v[..., :12]), "multiple of 8"),
+        (dict(q=q[..., 4:28], k=k[..., 4:28], v=v[..., 4:28]), "aligned"),
+        (dict(kv_len=torch.ones(2, dtype=torch.int64, device="cuda")), "kv_len must be"),
+        (dict(prefix=_ints([1])), "prefix must be"),
+        (dict(docs=(_ints([0] * 4), _ints([0] * 8))), "doc_k must be"),
+        (dict(slopes=torch.ones(2, device="cuda")), "slopes must be"),
+        (dict(table=torch.ones(4, 0, device="cuda")), "table without entries"),
+        (dict(cap=-1.0), "cap"),
+        (dict(cap=math.nan), "cap"),
+        (dict(scale=math.inf), "scale"),
+        (dict(window=(-2, 0)), "window"),
+        (dict(causal=True, window=(None, 3)), "causal"),
+        (dict(out=q), "overlap"),
+        (dict(out=torch.empty_like(q[:1]).expand(2, -1, -1, -1)), "zero stride"),
+    ]
+    for change, text in bad:
+        args = {"q": q, "k": k, "v": v, **change}
+        with pytest.raises(EngineError, match=text):
+            tr.attention(args.pop("q"), args.pop("k"), args.pop("v"), **args)
+    big_k = k[:, :1].expand(2, 5000, 2, 32)
+    with pytest.raises(EngineError, match="workspace too small"):
+        tr.attention(q, big_k, big_k, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    plan = tr.RopePlan((8, 8))
+    pos = torch.zeros(2, 2, 4, dtype=torch.int32, device="cuda")
+    for change, text in [(dict(pos=pos[:1]), "pos must be"), (dict(pos=pos.long()), "pos must be"),
+                         (dict(plan=tr.RopePlan((8, 9))), "n_freq"), (dict(q=q.transpose(2, 3)), "must agree|contiguous|n_freq"),
+                         (dict(q_out=q.transpose(0, 1)), "q_out"), (dict(k=k[:1]), "agree")]:
+        args = {"q": q, "k": k[:, :4], "pos": pos, "plan": plan, **change}
+        with pytest.raises(EngineError, match=text):
+            tr.rope_axes(args.pop("q"), args.pop("k"), args.pop("pos"), args.pop("plan"), **args)
+    r = _normal(_gen(1), 2, 3, 64, dtype=F16)
+    w = torch.ones(64, device="cuda")
+    for change, text in [(dict(y=r[:, :2]), "shape"), (dict(post="max"), "norm is"),
+                         (dict(pre_weight=w.half()), "pre_weight"), (dict(gate=r[:, :, :32]), "broadcast"),
+                         (dict(gate_act="relu"), "activation"), (dict(eps=-1.0), "eps"),
+                         (dict(y=r.bfloat16()), "residual type"), (dict(y=None, gate=r), "without y"),
+                         (dict(residual_out=r[:1].expand(2, -1, -1)), "zero stride"),
+                         (dict(h=r, pre="rms"), "overlap")]:
+        args = {"y": r.clone(), **change}
+        with pytest.raises(EngineError, match=text):
+            tr.gated_norm(r, args.pop("y"), **args)
+    assert torch.isfinite(tr.attention(q, k, v)).all()  # nothing was left behind
