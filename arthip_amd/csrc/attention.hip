@@ -19,6 +19,8 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
+#include <type_traits>
 
 #include "launch.h"
 #include "token_dev.h"
@@ -42,6 +44,8 @@ struct AttnArgs {
   int row_tiles;  // workgroups along the rows
   int splits;     // workgroups along the keys
   int items;      // batch * k_heads * row_tiles * splits
+  int table_lds;  // the tables of a key head's rows are kept in LDS
+  int wide;       // keys further apart than 32-bit offsets reach
   float* part;    // [splits][batch * k_heads * rows][D] unscaled sums, if splits > 1
   float* stat;    // [splits][batch * k_heads * rows][2] maximum (base 2) and sum
 };
@@ -51,7 +55,6 @@ struct Elem;
 template <>
 struct Elem<_Float16> {
   typedef h8 frag;
-  static constexpr uint32_t kExp = 0x7c007c00u;
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -59,18 +62,10 @@ struct Elem<_Float16> {
 template <>
 struct Elem<__bf16> {
   typedef b8 frag;
-  static constexpr uint32_t kExp = 0x7f807f80u;
   static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
-
-// Whether a half-word of x is an infinity or NaN of T.
-template <class T>
-__device__ __forceinline__ bool nonfinite(uint32_t x) {
-  constexpr uint32_t lo = Elem<T>::kExp & 0xffffu, hi = Elem<T>::kExp & 0xffff0000u;
-  return (x & lo) == lo || (x & hi) == hi;
-}
 
 // The two halves' values of a lane's x. (The results are copied before they are cast:
 // a bit cast of a vector's element takes element 0, whichever is named.)
@@ -92,33 +87,89 @@ __device__ __forceinline__ float halves_sum(float x) {
   return a + b;
 }
 
-// LDS of a workgroup. Rows of K are padded by 16 bytes, rows of V to 64 bytes modulo
-// 256: the 32 rows of a K operand, and the four rows of a transposed V read, start on
-// different banks, and every address is a lane's base plus a constant.
+// LDS of a workgroup: two buffers of K tiles and of V tiles, written by loads that go
+// to LDS without passing registers. Such a load puts a wave's 64 x 16 bytes in a row,
+// so rows cannot be padded; their 16-byte chunks are permuted instead, by an exclusive
+// or with bits of the row, so that the 16 rows of a K operand, and the four rows of a
+// transposed V read, lie on different banks. The permutation is in the addresses that
+// the lanes load from.
 template <int DP>
 struct TileL {
   static constexpr int KT = DP > 128 ? 32 : 64;  // keys of a tile
-  static constexpr int KS = DP * 2 + 16;
-  static constexpr int VS = DP == 64 ? 192 : DP >= 128 ? DP * 2 + 64 : DP * 2;
+  static constexpr int RB = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row
+  static constexpr int kTile = KT * RB;
+  static constexpr int kV = 2 * kTile;
   static constexpr int kChunk = 2048;            // tiles whose documents are looked over at once
-  static constexpr int kV = 2 * KT * KS;
-  static constexpr int kDoc = kV + 2 * KT * VS;  // int32 [2][KT]
-  static constexpr int kCode = kDoc + 2 * KT * 4;
-  static constexpr int kAny = kCode + 2 * KT * 4;     // bit a tile: some key of a row's document
-  static constexpr int kWhole = kAny + kChunk / 8;    // bit a tile: all keys, all rows of one
-  static constexpr int kMisc = kWhole + kChunk / 8;   // int32 [2] bad tile, [2][16] documents' range
-  static constexpr int kBytes = kMisc + (2 + 32) * 4;
+  static constexpr int kDoc = kV + 2 * kTile;    // int32 [2][64]
+  static constexpr int kCode = kDoc + 2 * 64 * 4;
+  static constexpr int kAny = kCode + 2 * 64 * 4;   // bit a tile: some key of a row's document
+  static constexpr int kWhole = kAny + kChunk / 8;  // bit a tile: all keys, all rows of one
+  static constexpr int kRange = kWhole + kChunk / 8;  // int32 [2][16] documents of the waves
+  static constexpr int kTable = kRange + 2 * 16 * 4;  // fp32 [group][table_len], if it fits
+  static constexpr int kBytes = kTable;
+  static __device__ __forceinline__ int k_swizzle(int row) {
+    return RB == 64 ? (row >> 2) & 3 : RB == 128 ? (row >> 1) & 7 : RB == 256 ? row & 15 : row & 7;
+  }
+  static __device__ __forceinline__ int v_swizzle(int row) {
+    return RB == 64 ? 0 : RB == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+  }
 };
 
-template <class T, int DP, int NW>
+constexpr int kTableBytes = 16384;  // of the tables that a workgroup keeps in LDS
+
+typedef uint32_t rsrc_t __attribute__((ext_vector_type(4)));
+
+// A buffer of up to `bytes` bytes from p (uniform).
+__device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return rsrc_t{lo, hi & 0xffffu, bytes, 0x00020000u};
+}
+
+// 16 (4) bytes a lane from the buffer to LDS, lane after lane from `to`. Offsets past
+// the buffer bring zeros. The compiler does not see these loads (its own would make
+// every later LDS read wait for them): vm_wait() stands between them and their use.
+__device__ __forceinline__ void load_lds16(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(to), "v"(at), "s"(from), "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void load_lds4(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :
+               : "s"(to), "v"(at), "s"(from), "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The order of a block of N products with R LDS reads each: the reads run four products
+// ahead, so that their latency (some 64 to 128 clocks) passes behind the matrix unit.
+// Left to itself the compiler reads an operand right before its product.
+template <int N, int R>
+__device__ __forceinline__ void ahead() {
+  constexpr int A = N < 4 ? N : 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - A; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+}
+
+template <class T, int DP, int NW, bool SHAPED>
 __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(AttnArgs a) {
   using L = TileL<DP>;
   using E = Elem<T>;
   using frag = typename E::frag;
-  constexpr int KT = L::KT, NT = NW * 64, KB = KT / 32, KS = DP / 16, DB = DP / 32;
-  constexpr int CH = DP / 8;                          // 16-byte chunks of a key
-  constexpr int LOADS = (KT * CH + NT - 1) / NT;      // chunks of a tile a thread moves
+  constexpr int KT = L::KT, RB = L::RB, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+  constexpr int SEG = L::kTile / 1024;                // loads of a tile, 1 KiB each
+  constexpr int LOADS = (SEG + NW - 1) / NW;          // of a wave
+  constexpr uint32_t kOob = 0x80000000u;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   const int per = (int)gridDim.x >> 3;
   int item = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);  // one XCD: neighbours share K, V
@@ -137,16 +188,18 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int half = lane >> 5;  // which keys and values of it
 
   // -- rows ------------------------------------------------------------------------
-  const int kv_len = a.c.kv_len ? min(max(a.c.kv_len[b], 0), a.c.k_tokens) : a.c.k_tokens;
-  const int q_start = a.c.q_start ? min(max(a.c.q_start[b], -kFar), kFar) : a.c.k_tokens - a.c.q_tokens;
-  const int pre = a.c.prefix ? min(max(a.c.prefix[b], 0), kv_len) : 0;
+  auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int kv_len = scalar(a.c.kv_len ? min(max(a.c.kv_len[b], 0), a.c.k_tokens) : a.c.k_tokens);
+  const int q_start =
+      scalar(a.c.q_start ? min(max(a.c.q_start[b], -kFar), kFar) : a.c.k_tokens - a.c.q_tokens);
+  const int pre = scalar(a.c.prefix ? min(max(a.c.prefix[b], 0), kv_len) : 0);
   // Keys [lo, hi) that a window leaves to a token (and those below pre).
-  auto low = [&](int token) -> int {
+  auto low = [&](int token) __attribute__((always_inline)) -> int {
     if (a.c.left < 0) return 0;
     const int64_t p = (int64_t)q_start + token - a.c.left;
     return p < 0 ? 0 : p > kv_len ? kv_len : (int)p;
   };
-  auto high = [&](int token) -> int {
+  auto high = [&](int token) __attribute__((always_inline)) -> int {
     if (a.c.right < 0) return kv_len;
     const int64_t p = (int64_t)q_start + token + a.c.right + 1;
     return p < 0 ? 0 : p > kv_len ? kv_len : (int)p;
@@ -156,7 +209,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int row = first_row + wave * 32 + n;
   const bool real = row <= last_row;
   const int token = min(row, last_row) / a.group;
-  const int head = kh * a.group + min(row, last_row) - token * a.group;
+  const int g_head = min(row, last_row) - token * a.group;
+  const int head = kh * a.group + g_head;
   const int lo = low(token), hi = high(token);
   // The wave's and the workgroup's rows together: all see [lo_max, hi_min), some see
   // [lo_min, hi_max). Positions grow with the row.
@@ -164,8 +218,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int w_lo_min = low(wr0 / a.group), w_lo_max = low(wr1 / a.group);
   const int w_hi_min = high(wr0 / a.group), w_hi_max = high(wr1 / a.group);
   const bool w_real = first_row + wave * 32 <= last_row;
-  const int g_lo_min = low(first_row / a.group), g_lo_max = low(last_row / a.group);
-  const int g_hi_min = high(first_row / a.group), g_hi_max = high(last_row / a.group);
+  const int g_lo_min = low(first_row / a.group), g_hi_max = high(last_row / a.group);
 
   frag q[KS];
   {
@@ -180,14 +233,31 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
 
   // -- score transforms --------------------------------------------------------------
   // Without cap and bias the scale goes into the exponent's multiply-add.
-  const bool shaped = a.c.cap > 0 || a.c.slopes || a.c.table || !(a.c.scale > 0);
-  const float mul = shaped ? 1.0f : a.c.scale * kLog2e;
-  const float slope = a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
-  const int cq = a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
-  const float* const table = a.c.table ? a.c.table + (int64_t)head * a.c.table_len : nullptr;
+  const float mul = SHAPED ? 1.0f : a.c.scale * kLog2e;
+  const float slope = SHAPED && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
+  const int cq = SHAPED && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
+  const float* const table = SHAPED && a.c.table ? a.c.table : nullptr;
+  const int32_t* const code_k = SHAPED && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
   const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
   const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
-  const int32_t* const code_k = a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
+  bool hides = false;  // the table has an entry of -inf
+  if (table) {
+    float* const t = reinterpret_cast<float*>(lds + L::kTable);
+    const int len = a.group * a.c.table_len;
+    const float* const from = table + (int64_t)kh * len;
+    bool h = false;
+    for (int i = tid; i < len; i += NW * 64) {
+      const float e = from[i];
+      if (a.table_lds) t[i] = e * kLog2e;
+      h = h || e == -__builtin_inff();
+    }
+    int* const flag = reinterpret_cast<int*>(lds + L::kRange);
+    if (__any(h) && lane == 0) flag[wave] = 1;
+    if (!__any(h) && lane == 0) flag[wave] = 0;
+    lds_sync();
+    for (int i = 0; i < NW; ++i) hides = hides || flag[i] != 0;
+    hides = __builtin_amdgcn_readfirstlane(hides);
+  }
 
   // -- the tiles: those of the prefix, then those of the windows ----------------------
   const int pre_tiles = (pre + KT - 1) / KT;
@@ -196,21 +266,20 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int count = pre_tiles + max(win_end - win_first, 0);
   const int begin = (int)((int64_t)count * split / a.splits);
   const int end = (int)((int64_t)count * (split + 1) / a.splits);
-  auto tile_of = [&](int i) { return i < pre_tiles ? i : i - pre_tiles + win_first; };
+  auto tile_of = [&](int i) __attribute__((always_inline)) { return i < pre_tiles ? i : i - pre_tiles + win_first; };
 
   uint32_t* const any = reinterpret_cast<uint32_t*>(lds + L::kAny);
   uint32_t* const whole = reinterpret_cast<uint32_t*>(lds + L::kWhole);
-  int* const bad = reinterpret_cast<int*>(lds + L::kMisc);
-  int* const range = bad + 2;
   int dmin = 0, dmax = 0;
-  if (tid < 2) bad[tid] = -1;
   if (doc_k) {
+    int* const range = reinterpret_cast<int*>(lds + L::kRange);
     int lo_d = dq, hi_d = dq;  // a lane past the last row repeats it
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       lo_d = min(lo_d, __shfl_xor(lo_d, o));
       hi_d = max(hi_d, __shfl_xor(hi_d, o));
     }
+    lds_sync();
     if (lane == 0) {
       range[wave] = lo_d;
       range[16 + wave] = hi_d;
@@ -230,78 +299,130 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   float m = -__builtin_inff(), l = 0.0f;
 
   // -- staging -------------------------------------------------------------------------
+  // A wave's loads of a tile are NW KiB apart, whole periods of the permutation, so
+  // that one offset a lane serves them all.
   const T* const kp = static_cast<const T*>(a.c.k) + b * a.c.k_stride[0] + kh * a.c.k_stride[2];
   const T* const vp = static_cast<const T*>(a.c.v) + b * a.c.v_stride[0] + kh * a.c.v_stride[2];
-  u4 kr[LOADS], vr[LOADS];
-  int doc_r = 0, code_r = 0;
-  auto fetch = [&](int tile) {
+  const int s_row = (wave * 1024 + lane * 16) / RB;
+  const int s_chunk = lane * 16 % RB / 16;
+  const int k_chunk = s_chunk ^ L::k_swizzle(s_row), v_chunk = s_chunk ^ L::v_swizzle(s_row);
+  const bool k_in = k_chunk * 8 < a.c.head_dim, v_in = v_chunk * 8 < a.c.head_dim;
+  const int64_t ks2 = a.c.k_stride[1] * 2, vs2 = a.c.v_stride[1] * 2;  // bytes
+  auto stage = [&](const T* from, int64_t stride, int chunk, bool in, int tile, uint32_t to) __attribute__((always_inline)) {
+    const char* const p = reinterpret_cast<const char*>(from) + (int64_t)tile * KT * stride;
+    const int left = kv_len - tile * KT;  // keys past the length come as zeros
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int c = tid + i * NT;
-      const int64_t key = (int64_t)tile * KT + c / CH;
-      const int d = c % CH * 8;
-      // Keys past the length and values past the head read nothing and are zeros.
-      const bool in = c < KT * CH && key < kv_len && d < a.c.head_dim;
-      kr[i] = in ? *reinterpret_cast<const u4*>(kp + key * a.c.k_stride[1] + d) : u4{};
-      vr[i] = in ? *reinterpret_cast<const u4*>(vp + key * a.c.v_stride[1] + d) : u4{};
-    }
-    if (tid < KT) {
-      const int64_t key = (int64_t)tile * KT + tid;
-      if (doc_k) doc_r = key < kv_len ? doc_k[key] : 0;
-      if (code_k) code_r = key < kv_len ? code_k[key] : 0;
+      if (SEG % NW != 0 && wave + i * NW >= SEG) break;
+      const int row = s_row + i * NW * 1024 / RB;
+      if (a.wide) {
+        // 32-bit offsets would wrap: a buffer of its own for every key of the load.
+        constexpr int keys = RB < 1024 ? 1024 / RB : 1;
+#pragma unroll 1
+        for (int r = 0; r < keys; ++r) {
+          const int first = (wave * 1024 + i * NW * 1024) / RB + r;
+          const rsrc_t one = buffer_of(p + first * stride, 0x7fffffffu);
+          if (row == first)
+            load_lds16(one, in && row < left ? chunk * 16u : kOob, 0, to + (wave + i * NW) * 1024);
+        }
+      } else {
+        const uint32_t at = (uint32_t)(row * (int)stride + chunk * 16);
+        load_lds16(buffer_of(p, 0x7fffffffu), in && row < left ? at : kOob, 0, to + (wave + i * NW) * 1024);
+      }
     }
   };
-  auto stage = [&](int buf, int tile, bool partial) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int c = tid + i * NT;
-      if (KT * CH % NT != 0 && c >= KT * CH) break;
-      *reinterpret_cast<u4*>(lds + buf * KT * L::KS + c / CH * L::KS + c % CH * 16) = kr[i];
-      *reinterpret_cast<u4*>(lds + L::kV + buf * KT * L::VS + c / CH * L::VS + c % CH * 16) = vr[i];
-      // A value that is not finite, in a tile that some row does not see whole: the
-      // products below would carry it into rows that do not see it.
-      if (partial && (nonfinite<T>(vr[i][0]) || nonfinite<T>(vr[i][1]) || nonfinite<T>(vr[i][2]) ||
-                      nonfinite<T>(vr[i][3])))
-        bad[buf] = tile;
-    }
-    if (tid < KT) {
-      if (doc_k) reinterpret_cast<int*>(lds + L::kDoc)[buf * KT + tid] = doc_r;
-      if (code_k) reinterpret_cast<int*>(lds + L::kCode)[buf * KT + tid] = code_r;
-    }
+  auto stage_k = [&](int buf, int tile) __attribute__((always_inline)) {
+    stage(kp, ks2, k_chunk, k_in, tile, lds_base + buf * L::kTile);
+    if (doc_k && wave == 0)
+      load_lds4(buffer_of(doc_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, lds_base + L::kDoc + buf * 256);
+    if (code_k && wave == NW - 1)
+      load_lds4(buffer_of(code_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, lds_base + L::kCode + buf * 256);
+  };
+  auto stage_v = [&](int buf, int tile) __attribute__((always_inline)) {
+    stage(vp, vs2, v_chunk, v_in, tile, lds_base + L::kV + buf * L::kTile);
   };
 
-  // -- one tile ------------------------------------------------------------------------
-  const unsigned char* const k_lane = lds + n * L::KS + half * 16;
-  const unsigned char* const v_lane =
-      lds + L::kV + (4 * half + (lane & 15) / 4) * L::VS + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-  auto v_frag = [&](int buf, int db, int kk) -> frag {  // 32 values (block db) of 16 keys (block kk)
-    typedef __attribute__((address_space(3))) s4 lds_s4;
-    const unsigned char* const p = v_lane + buf * KT * L::VS + kk * 16 * L::VS + db * 64;
-    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p));
-    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * L::VS));
+  // -- the products --------------------------------------------------------------------
+  // Operands come from a lane's base plus constants; the permutation, an exclusive or
+  // with the lane's bits, leaves one base for each K step and each block of V values.
+  typedef __attribute__((address_space(3))) unsigned char lds_byte;
+  typedef __attribute__((address_space(3))) const frag lds_frag;
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  lds_byte* const lds0 = (lds_byte*)lds;
+  const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
+  const int v_row = 4 * half + (lane & 15) / 4;
+  const uint32_t v_lane =
+      v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+
+  f16v s[KB];        // scores of the current tile, key block by key block
+  frag p[KT / 16];   // weights of the previous tile
+  auto scores = [&](int buf) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + buf * L::kTile;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      lds_byte* const k = at + (k_lane ^ (ks * 32));
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[kb] = E::mma(*(lds_frag*)(k + kb * 32 * RB), q[ks], ks == 0 ? f16v{} : s[kb]);
+    }
+    ahead<KS * KB, 1>();
+  };
+  auto v_frag = [&](lds_byte* at, int kk) __attribute__((always_inline)) -> frag {  // 32 values of 16 keys (block kk)
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + kk * 16 * RB));
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + kk * 16 * RB + 8 * RB));
     return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto compute = [&](int buf, int tile, bool one_doc) {
-    const int k0 = tile * KT;
-    const int k1 = k0 + KT;
-    const bool seen = k0 < pre || (k0 < w_hi_max && k1 > w_lo_min);
-    if (!w_real || !seen) return;
-    const bool inside = k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min);
-    const bool partial = !inside || !one_doc;
-
-    f16v s[KB];
+  bool odd = false;  // a tile that a row does not see whole holds an infinity or NaN in V
+  auto values = [&](int buf, bool look) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + L::kV + buf * L::kTile;
+    lds_byte* v[DB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = f16v{};
+    for (int db = 0; db < DB; ++db) v[db] = at + (v_lane ^ (db * 64));
+    if (look) {
+      // Rows that do not see all of this tile weigh some of V by 0, which infinities and
+      // NaN survive: 0 times the tile tells whether it has any.
+      f16v z = f16v{};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const frag k = *reinterpret_cast<const frag*>(k_lane + buf * KT * L::KS + kb * 32 * L::KS + ks * 32);
-        s[kb] = E::mma(k, q[ks], s[kb]);
+        for (int db = 0; db < DB; ++db) z = E::mma(v_frag(v[db], kk), frag{}, z);
+      float t = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t += z[r];
+      odd = odd || t != 0.0f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
+    ahead<KT / 16 * DB, 2>();
+  };
+  // The same key by key, each added only to the rows that weigh it.
+  auto values_apart = [&](int buf) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + L::kV + buf * L::kTile;
+#pragma unroll
+    for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll 1
+      for (int key = 0; key < 16; ++key) {
+        const int of = (key >> 2) & 1, j = (key & 3) | ((key >> 1) & 4);  // its half and element
+        u4 keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keep[e] = half != of || j >> 1 != e ? 0u : j & 1 ? 0xffff0000u : 0x0000ffffu;
+        const u4 one = __builtin_bit_cast(u4, p[kk]) & keep;
+        const float sees = halves_max(((one[0] | one[1] | one[2] | one[3]) & 0x7fff7fffu) != 0 ? 1.0f : 0.0f);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u4 x = __builtin_bit_cast(u4, v_frag(at + (v_lane ^ (db * 64)), kk)) & keep;
+          const f16v c = E::mma(__builtin_bit_cast(frag, x), __builtin_bit_cast(frag, one), f16v{});
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[db][r] += sees != 0.0f ? c[r] : 0.0f;
+        }
       }
+  };
 
-    const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
-    if (shaped) {
+  // -- scores to weights -----------------------------------------------------------------
+  auto weights = [&](int buf, int tile, bool partial) __attribute__((always_inline)) {
+    const int key0 = tile * KT + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
+    if constexpr (SHAPED) {
       if (a.c.cap > 0) {
         // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2
         const float in = 2.0f * kLog2e * a.c.scale / a.c.cap, out = kLog2e * a.c.cap;
@@ -319,7 +440,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
           for (int r = 0; r < 16; ++r) s[kb][r] *= a.c.scale * kLog2e;
       }
       if (a.c.slopes || table) {
-        const int* const codes = reinterpret_cast<const int*>(lds + L::kCode) + buf * KT + 4 * half;
+        const int* const codes = reinterpret_cast<const int*>(lds + L::kCode) + buf * 64 + 4 * half;
+        const float* const t_lds = reinterpret_cast<const float*>(lds + L::kTable) + g_head * a.c.table_len;
+        const float* const t_far = table + (int64_t)head * a.c.table_len;
+        const int t_last = a.c.table_len - 1, t_zero = a.c.table_zero;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -328,16 +452,16 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
             const int diff = cq - (code_k ? codes[off] : key0 + off);
             if (a.c.slopes) s[kb][r] = __builtin_fmaf(-slope, fabsf((float)diff), s[kb][r]);
             if (table) {
-              const int64_t e = (int64_t)diff + a.c.table_zero;
-              const int at = e < 0 ? 0 : e >= a.c.table_len ? a.c.table_len - 1 : (int)e;
-              const float entry = table[at];
-              s[kb][r] = entry == -__builtin_inff() ? entry : __builtin_fmaf(entry, kLog2e, s[kb][r]);
+              const int at = min(max(diff + t_zero, 0), t_last);
+              const float entry = a.table_lds ? t_lds[at] : t_far[at] * kLog2e;
+              const float sum = s[kb][r] + entry;
+              s[kb][r] = hides && entry == -__builtin_inff() ? entry : sum;
             }
           }
       }
     }
     if (partial) {
-      const int* const docs = reinterpret_cast<const int*>(lds + L::kDoc) + buf * KT + 4 * half;
+      const int* const docs = reinterpret_cast<const int*>(lds + L::kDoc) + buf * 64 + 4 * half;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -350,16 +474,26 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
         }
     }
 
-    float top = m;
+    float top = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
     top = halves_max(top);
-    // A row that has seen nothing yet keeps -inf; its exponents are taken about 0.
-    const float base = top == -__builtin_inff() ? 0.0f : top * mul;
-    const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m, mul, -base));
-    m = top;
+    // The base of a row's exponents follows its largest score only where that has grown
+    // by more than 2^8: until then weights are at most 256, and nothing is rescaled.
+    if (__any((top - m) * mul > 8.0f)) {
+      const float next = fmaxf(m, top);
+      // A row that has seen nothing yet has no sums to keep (next may be -inf as well).
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= f;
+    }
+    const float base = m == -__builtin_inff() ? 0.0f : m * mul;
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -368,113 +502,104 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
         s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], mul, -base));
         sum += s[kb][r];
       }
-    l = __builtin_fmaf(l, keep, sum);  // this half's keys; the halves are added at the end
-    if (__any(keep != 1.0f)) {
-#pragma unroll
-      for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] *= keep;
-    }
-
-    auto p_frag = [&](int kk) -> frag {
-      const f16v x = s[kk / 2];
-      return kk & 1 ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
-                    : __builtin_convertvector(__builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7), frag);
-    };
-    if ((partial || table) && __builtin_amdgcn_readfirstlane(bad[buf]) == tile) {
-      // Infinities and NaN of V apart from its finite values: how many of each sign
-      // the row weighs, NaN as both.
-#pragma unroll 1
-      for (int kk = 0; kk < KT / 16; ++kk) {
-        frag p = frag{}, one = frag{};
-#pragma unroll
-        for (int e = 0; e < KT / 16; ++e)
-          if (e == kk) {
-            p = p_frag(e);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) one[j] = to_elem<T>(s[e / 2][8 * (e & 1) + j] != 0.0f ? 1.0f : 0.0f);
-          }
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const frag v = v_frag(buf, db, kk);
-          frag fin, up, down;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float x = static_cast<float>(v[j]);
-            const bool ok = __builtin_isfinite(x);
-            fin[j] = ok ? v[j] : to_elem<T>(0.0f);
-            up[j] = to_elem<T>(!ok && !(x < 0.0f) ? 1.0f : 0.0f);
-            down[j] = to_elem<T>(!ok && !(x > 0.0f) ? 1.0f : 0.0f);
-          }
-          o[db] = E::mma(fin, p, o[db]);
-          const f16v nu = E::mma(up, one, f16v{}), nd = E::mma(down, one, f16v{});
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (nu[r] > 0.0f) o[db][r] += __builtin_inff();
-            if (nd[r] > 0.0f) o[db][r] -= __builtin_inff();
-          }
-        }
-      }
-      return;
-    }
+    l += sum;  // this half's keys; the halves are added at the end
 #pragma unroll
     for (int kk = 0; kk < KT / 16; ++kk) {
-      const frag p = p_frag(kk);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(buf, db, kk), p, o[db]);
+      const f16v x = s[kk / 2];
+      p[kk] = kk & 1
+                  ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
+                  : __builtin_convertvector(__builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7), frag);
     }
   };
 
   // -- the walk ------------------------------------------------------------------------
-  // Two buffers and one barrier a tile: a wave writes a buffer only after the barrier
-  // that follows every wave's last use of it.
-  const int chunk = doc_k ? L::kChunk : max(end - begin, 1);
-  for (int c0 = begin; c0 < end; c0 += chunk) {
-    const int c1 = min(end, c0 + chunk);
-    if (doc_k) {
-      // Tiles whose documents cannot be a row's are not read. A wave looks over 64 / KT
-      // .. one tile at a time; a word of the bit sets has one writer.
-      lds_sync();
-      for (int w = wave; w < (c1 - c0 + 31) / 32; w += NW) {
-        uint32_t some = 0, all = 0;
-        for (int i = 0; i < 32 && c0 + w * 32 + i < c1; ++i) {
-          const int64_t key = (int64_t)tile_of(c0 + w * 32 + i) * KT + (lane & (KT - 1));
-          const bool in = key < kv_len;
-          const int d = in ? doc_k[key] : 0;
-          if (__any(in && d >= dmin && d <= dmax)) some |= 1u << i;
-          if (__all(in && d == dmin && d == dmax)) all |= 1u << i;
+  // One barrier a tile. While tile t's scores and the previous tile's values are
+  // multiplied, K of the next tile and V of this one are on their way to the buffers
+  // that the last barrier freed.
+  auto walk = [&](auto apart) __attribute__((always_inline)) {
+    const int chunk = doc_k ? L::kChunk : max(end - begin, 1);
+    for (int c0 = begin; c0 < end; c0 += chunk) {
+      const int c1 = min(end, c0 + chunk);
+      lds_sync();  // the last chunk's tiles and bits have been used
+      if (doc_k) {
+        // Tiles whose documents cannot be a row's are not read. A word of the bit sets has
+        // one writer.
+        for (int w = wave; w < (c1 - c0 + 31) / 32; w += NW) {
+          uint32_t some = 0, all = 0;
+          for (int i = 0; i < 32 && c0 + w * 32 + i < c1; ++i) {
+            const int64_t key = (int64_t)tile_of(c0 + w * 32 + i) * KT + (lane & (KT - 1));
+            const bool in = key < kv_len;
+            const int d = in ? doc_k[key] : 0;
+            if (__any(in && d >= dmin && d <= dmax)) some |= 1u << i;
+            if (__all(in && d == dmin && d == dmax)) all |= 1u << i;
+          }
+          if (lane == 0) {
+            any[w] = some;
+            whole[w] = all;
+          }
         }
-        if (lane == 0) {
-          any[w] = some;
-          whole[w] = all;
-        }
+        lds_sync();
       }
+      auto next = [&](int i) __attribute__((always_inline)) {
+        if (doc_k)
+          while (i < c1 && !(any[(i - c0) >> 5] >> ((i - c0) & 31) & 1)) ++i;
+        return __builtin_amdgcn_readfirstlane(i);
+      };
+      int i = next(c0);
+      int buf = 0;
+      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
+      if (i >= c1) continue;
+      stage_k(0, tile_of(i));
+      vm_wait();
       lds_sync();
+      while (true) {
+        const bool more = i < c1;
+        const int tile = tile_of(i), k0 = tile * KT, k1 = k0 + KT;
+        bool seen = false, partial = false;
+        int following = i;
+        if (more) {
+          const bool one_doc =
+              !doc_k || __builtin_amdgcn_readfirstlane(whole[(i - c0) >> 5] >> ((i - c0) & 31) & 1) != 0;
+          following = next(i + 1);
+          if (following < c1) stage_k(buf ^ 1, tile_of(following));
+          stage_v(buf, tile);
+          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min));
+          partial = !(k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min)) || !one_doc;
+        }
+        if (seen) scores(buf);
+        if (has) {
+          if constexpr (decltype(apart)::value)
+            values_apart(buf ^ 1);
+          else
+            values(buf ^ 1, look);
+        }
+        if (!more) break;
+        if (seen) weights(buf, tile, partial);
+        has = seen;
+        look = partial || hides;
+        vm_wait();
+        lds_sync();
+        i = following;
+        buf ^= 1;
+      }
     }
-    auto next = [&](int i) {
-      if (doc_k)
-        while (i < c1 && !(any[(i - c0) >> 5] >> ((i - c0) & 31) & 1)) ++i;
-      return __builtin_amdgcn_readfirstlane(i);
-    };
-    auto one_doc = [&](int i) {
-      return !doc_k || __builtin_amdgcn_readfirstlane(whole[(i - c0) >> 5] >> ((i - c0) & 31) & 1) != 0;
-    };
-    int i = next(c0);
-    int buf = 0;
-    if (i < c1) fetch(tile_of(i));
-    lds_sync();  // the last chunk's tiles have been used
-    while (i < c1) {
-      const int tile = tile_of(i);
-      const bool od = one_doc(i);
-      const int k0 = tile * KT;
-      const bool inside = k0 + KT <= pre || (k0 >= g_lo_max && k0 + KT <= g_hi_min);
-      stage(buf, tile, !inside || !od || table != nullptr);
-      const int following = next(i + 1);
-      lds_sync();
-      if (following < c1) fetch(tile_of(following));
-      compute(buf, tile, od);
-      i = following;
-      buf ^= 1;
+  };
+  walk(std::false_type{});
+  // A workgroup that met such a tile starts over and takes the keys one by one.
+  {
+    int* const flag = reinterpret_cast<int*>(lds + L::kRange);
+    lds_sync();
+    if (lane == 0) flag[wave] = 0;
+    if (odd) flag[wave] = 1;
+    lds_sync();
+    int again = 0;
+    for (int i = 0; i < NW; ++i) again |= flag[i];
+    if (__builtin_amdgcn_readfirstlane(again) != 0) {
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i] = f16v{};
+      m = -__builtin_inff();
+      l = 0.0f;
+      walk(std::true_type{});
     }
   }
 
@@ -568,23 +693,20 @@ struct TilePick {
 };
 
 template <class T, int DP, int NW>
-TilePick pick() {
-  return {attention_tile<T, DP, NW>, TileL<DP>::kBytes};
+TilePick pick(bool shaped) {
+  return {shaped ? attention_tile<T, DP, NW, true> : attention_tile<T, DP, NW, false>, TileL<DP>::kBytes};
 }
 
-template <class T, int NW>
-TilePick pick_dim(int d) {
-  if (d <= 32) return pick<T, 32, NW>();
-  if (d <= 64) return pick<T, 64, NW>();
-  if (d <= 96) return pick<T, 96, NW>();
-  if (d <= 128) return pick<T, 128, NW>();
-  return pick<T, 256, 4>();
+template <class T>
+TilePick pick(int d, bool shaped) {
+  if (d <= 32) return pick<T, 32, 4>(shaped);
+  if (d <= 64) return pick<T, 64, 4>(shaped);
+  if (d <= 96) return pick<T, 96, 4>(shaped);
+  if (d <= 128) return pick<T, 128, 4>(shaped);
+  return pick<T, 256, 4>(shaped);
 }
 
-int waves_of(const arthip_attention_args& c) {
-  const int64_t rows = (int64_t)c.q_tokens * (c.q_heads / c.k_heads);
-  return rows > 128 && c.head_dim <= 128 ? 8 : 4;
-}
+int waves_of(const arthip_attention_args&) { return 4; }
 
 }  // namespace
 
@@ -615,8 +737,15 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.part = static_cast<float*>(c.workspace);
   if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
   const bool f16 = c.dtype == ARTHIP_TYPE_F16;
-  const TilePick k = nw == 8 ? (f16 ? pick_dim<_Float16, 8>(c.head_dim) : pick_dim<__bf16, 8>(c.head_dim))
-                             : (f16 ? pick_dim<_Float16, 4>(c.head_dim) : pick_dim<__bf16, 4>(c.head_dim));
+  // Cap and bias take the scores through more steps; so does a scale that turns their order.
+  const bool shaped = c.cap > 0 || c.slopes != nullptr || c.table != nullptr || !(c.scale > 0);
+  TilePick k = f16 ? pick<_Float16>(c.head_dim, shaped) : pick<__bf16>(c.head_dim, shaped);
+  const int64_t table = c.table == nullptr ? 0 : (int64_t)a.group * c.table_len * 4;
+  a.table_lds = table <= kTableBytes;
+  if (a.table_lds) k.bytes += (int)table;
+  // Offsets of a tile's keys from its first one have 31 bits.
+  const int64_t far = std::max(std::abs(c.k_stride[1]), std::abs(c.v_stride[1]));
+  a.wide = c.k_stride[1] < 0 || c.v_stride[1] < 0 || far * 2 * 64 + 512 > INT32_MAX;
   hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, k.bytes);
   if (e != hipSuccess) return e;
