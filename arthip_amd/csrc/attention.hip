@@ -18,8 +18,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
-#include <cstdlib>
 #include <type_traits>
 
 #include "launch.h"
@@ -46,6 +46,11 @@ struct AttnArgs {
   int items;      // batch * k_heads * row_tiles * splits
   int table_lds;  // the tables of a key head's rows are kept in LDS
   int wide;       // keys further apart than 32-bit offsets reach
+  FastDiv by_group, by_k_heads, by_row_tiles, by_splits;
+  float cap_reach;  // |q.k| up to which the polynomial holds
+  float cap_fit[5];
+  const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
+  int doc_tiles, doc_tile;  // tiles of a sequence, keys of a tile
   float* part;    // [splits][batch * k_heads * rows][D] unscaled sums, if splits > 1
   float* stat;    // [splits][batch * k_heads * rows][2] maximum (base 2) and sum
 };
@@ -99,12 +104,12 @@ struct TileL {
   static constexpr int RB = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row
   static constexpr int kTile = KT * RB;
   static constexpr int kV = 2 * kTile;
-  static constexpr int kChunk = 2048;            // tiles whose documents are looked over at once
+  static constexpr int kChunk = 1024;            // tiles whose documents are looked over at once
   static constexpr int kDoc = kV + 2 * kTile;    // int32 [2][64]
   static constexpr int kCode = kDoc + 2 * 64 * 4;
-  static constexpr int kAny = kCode + 2 * 64 * 4;   // bit a tile: some key of a row's document
-  static constexpr int kWhole = kAny + kChunk / 8;  // bit a tile: all keys, all rows of one
-  static constexpr int kRange = kWhole + kChunk / 8;  // int32 [2][16] documents of the waves
+  static constexpr int kTileDocs = kCode + 2 * 64 * 4;   // int2 a tile: its documents' range
+  static constexpr int kAny = kTileDocs + kChunk * 8;    // bit a tile: some key of a row's document
+  static constexpr int kRange = kAny + kChunk / 8;       // int32 [2][16] documents of the waves
   static constexpr int kTable = kRange + 2 * 16 * 4;  // fp32 [group][table_len], if it fits
   static constexpr int kBytes = kTable;
   static __device__ __forceinline__ int k_swizzle(int row) {
@@ -159,8 +164,12 @@ __device__ __forceinline__ void ahead() {
   __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
 }
 
-template <class T, int DP, int NW, bool SHAPED>
-__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(AttnArgs a) {
+// What the scores go through: nothing (the scale is in the exponent), the cap, or any
+// of cap, slopes, table and a scale that turns their order.
+enum Shape { kPlain, kCap, kAny };
+
+template <class T, int DP, int NW, Shape SHAPE>
+__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kAny ? 2 : 3) attention_tile(AttnArgs a) {
   using L = TileL<DP>;
   using E = Elem<T>;
   using frag = typename E::frag;
@@ -174,11 +183,11 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int per = (int)gridDim.x >> 3;
   int item = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);  // one XCD: neighbours share K, V
   if (item >= a.items) return;
-  const int split = item % a.splits;
-  item /= a.splits;
-  const int row_tile = a.row_tiles - 1 - item % a.row_tiles;  // causal: the longest first
-  const int bh = item / a.row_tiles;
-  const int b = bh / a.c.k_heads;
+  const int ranges = (int)fdiv((uint32_t)item, a.by_splits);
+  const int split = item - ranges * a.splits;
+  const int bh = (int)fdiv((uint32_t)ranges, a.by_row_tiles);
+  const int row_tile = a.row_tiles - 1 - (ranges - bh * a.row_tiles);  // causal: the longest first
+  const int b = (int)fdiv((uint32_t)bh, a.by_k_heads);
   const int kh = bh - b * a.c.k_heads;
 
   const int tid = threadIdx.x;
@@ -188,6 +197,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int half = lane >> 5;  // which keys and values of it
 
   // -- rows ------------------------------------------------------------------------
+  auto token_of = [&](int row) __attribute__((always_inline)) { return (int)fdiv((uint32_t)row, a.by_group); };
   auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int kv_len = scalar(a.c.kv_len ? min(max(a.c.kv_len[b], 0), a.c.k_tokens) : a.c.k_tokens);
   const int q_start =
@@ -208,17 +218,17 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int last_row = min(first_row + 32 * NW, a.rows) - 1;
   const int row = first_row + wave * 32 + n;
   const bool real = row <= last_row;
-  const int token = min(row, last_row) / a.group;
+  const int token = token_of(min(row, last_row));
   const int g_head = min(row, last_row) - token * a.group;
   const int head = kh * a.group + g_head;
   const int lo = low(token), hi = high(token);
   // The wave's and the workgroup's rows together: all see [lo_max, hi_min), some see
   // [lo_min, hi_max). Positions grow with the row.
   const int wr0 = min(first_row + wave * 32, last_row), wr1 = min(wr0 + 31, last_row);
-  const int w_lo_min = low(wr0 / a.group), w_lo_max = low(wr1 / a.group);
-  const int w_hi_min = high(wr0 / a.group), w_hi_max = high(wr1 / a.group);
+  const int w_lo_min = low(token_of(wr0)), w_lo_max = low(token_of(wr1));
+  const int w_hi_min = high(token_of(wr0)), w_hi_max = high(token_of(wr1));
   const bool w_real = first_row + wave * 32 <= last_row;
-  const int g_lo_min = low(first_row / a.group), g_hi_max = high(last_row / a.group);
+  const int g_lo_min = low(token_of(first_row)), g_hi_max = high(token_of(last_row));
 
   frag q[KS];
   {
@@ -233,11 +243,11 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
 
   // -- score transforms --------------------------------------------------------------
   // Without cap and bias the scale goes into the exponent's multiply-add.
-  const float mul = SHAPED ? 1.0f : a.c.scale * kLog2e;
-  const float slope = SHAPED && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
-  const int cq = SHAPED && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
-  const float* const table = SHAPED && a.c.table ? a.c.table : nullptr;
-  const int32_t* const code_k = SHAPED && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
+  const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
+  const float slope = SHAPE == kAny && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
+  const int cq = SHAPE == kAny && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
+  const float* const table = SHAPE == kAny && a.c.table ? a.c.table : nullptr;
+  const int32_t* const code_k = SHAPE == kAny && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
   const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
   const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
   bool hides = false;  // the table has an entry of -inf
@@ -268,21 +278,25 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   const int end = (int)((int64_t)count * (split + 1) / a.splits);
   auto tile_of = [&](int i) __attribute__((always_inline)) { return i < pre_tiles ? i : i - pre_tiles + win_first; };
 
-  uint32_t* const any = reinterpret_cast<uint32_t*>(lds + L::kAny);
-  uint32_t* const whole = reinterpret_cast<uint32_t*>(lds + L::kWhole);
-  int dmin = 0, dmax = 0;
+  // Documents: the range of a wave's rows, and of the workgroup's.
+  uint64_t* const any = reinterpret_cast<uint64_t*>(lds + L::kAny);
+  int2* const tile_docs = reinterpret_cast<int2*>(lds + L::kTileDocs);
+  const int2* const doc_ranges =
+      doc_k ? a.doc_ranges + (a.c.doc_k_stride == 0 ? 0 : (int64_t)b * a.doc_tiles) : nullptr;
+  int w_dmin = dq, w_dmax = dq, dmin = 0, dmax = 0;
   if (doc_k) {
     int* const range = reinterpret_cast<int*>(lds + L::kRange);
-    int lo_d = dq, hi_d = dq;  // a lane past the last row repeats it
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      lo_d = min(lo_d, __shfl_xor(lo_d, o));
-      hi_d = max(hi_d, __shfl_xor(hi_d, o));
+    for (int o = 32; o > 0; o >>= 1) {  // a lane past the last row repeats it
+      w_dmin = min(w_dmin, __shfl_xor(w_dmin, o));
+      w_dmax = max(w_dmax, __shfl_xor(w_dmax, o));
     }
+    w_dmin = scalar(w_dmin);
+    w_dmax = scalar(w_dmax);
     lds_sync();
     if (lane == 0) {
-      range[wave] = lo_d;
-      range[16 + wave] = hi_d;
+      range[wave] = w_dmin;
+      range[16 + wave] = w_dmax;
     }
     lds_sync();
     dmin = range[0];
@@ -420,10 +434,31 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
   };
 
   // -- scores to weights -----------------------------------------------------------------
-  auto weights = [&](int buf, int tile, bool partial) __attribute__((always_inline)) {
+  auto weights = [&](int buf, int tile, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
     const int key0 = tile * KT + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
-    if constexpr (SHAPED) {
-      if (a.c.cap > 0) {
+    const float unit = a.c.cap > 0 ? 1.0f : a.c.scale * kLog2e;  // what scores are still to be scaled by
+    if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
+      float far = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
+      if (SHAPE == kCap && !__any(!(far <= a.cap_reach))) {
+        // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
+        // less than 8e-8), six plain operations where the exponential and the reciprocal
+        // take a quarter of the rate each.
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float x = s[kb][r], z = x * x;
+            float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
+            t = __builtin_fmaf(t, z, a.cap_fit[2]);
+            t = __builtin_fmaf(t, z, a.cap_fit[1]);
+            t = __builtin_fmaf(t, z, a.cap_fit[0]);
+            s[kb][r] = x * t;
+          }
+      } else {
         // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2
         const float in = 2.0f * kLog2e * a.c.scale / a.c.cap, out = kLog2e * a.c.cap;
 #pragma unroll
@@ -433,45 +468,106 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
             const float e = __builtin_amdgcn_exp2f(s[kb][r] * in);
             s[kb][r] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
           }
-      } else {
+      }
+    }
+    if constexpr (SHAPE == kAny) {
+      // The loops below are whole loops a branch: a uniform branch inside would be taken
+      // for every score.
+      const int4* const codes = reinterpret_cast<const int4*>(lds + L::kCode + buf * 256) + half;
+      auto bias = [&](auto coded, auto add) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] *= a.c.scale * kLog2e;
+          for (int g = 0; g < 4; ++g) {
+            int4 c{};
+            if constexpr (decltype(coded)::value) c = codes[8 * kb + 2 * g];
+            const int ck[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[kb][4 * g + e] =
+                  add(s[kb][4 * g + e], decltype(coded)::value ? cq - ck[e] : cq - key0 - (32 * kb + 8 * g + e));
+          }
+      };
+      if (a.c.slopes) {
+        auto add = [&](float x, int diff) __attribute__((always_inline)) {
+          return __builtin_fmaf(x, unit, -slope * fabsf((float)diff));
+        };
+        if (code_k)
+          bias(std::true_type{}, add);
+        else {
+          const float first = (float)(cq - key0);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[kb][r] = __builtin_fmaf(s[kb][r], unit, -slope * fabsf(first - (float)(32 * kb + 8 * (r / 4) + r % 4)));
+        }
       }
-      if (a.c.slopes || table) {
-        const int* const codes = reinterpret_cast<const int*>(lds + L::kCode) + buf * 64 + 4 * half;
-        const float* const t_lds = reinterpret_cast<const float*>(lds + L::kTable) + g_head * a.c.table_len;
-        const float* const t_far = table + (int64_t)head * a.c.table_len;
-        const int t_last = a.c.table_len - 1, t_zero = a.c.table_zero;
+      if (table) {
+        const float by = a.c.slopes ? 1.0f : unit;
+        const int last = a.c.table_len - 1, zero = a.c.table_zero;
+        if (a.table_lds) {
+          // Entries in the base of 2.
+          const float* const t = reinterpret_cast<const float*>(lds + L::kTable) + g_head * a.c.table_len;
+          auto add = [&](float x, int diff) __attribute__((always_inline)) {
+            return __builtin_fmaf(x, by, t[min(max(diff + zero, 0), last)]);
+          };
+          auto add_hidden = [&](float x, int diff) __attribute__((always_inline)) {
+            const float entry = t[min(max(diff + zero, 0), last)];
+            const float sum = __builtin_fmaf(x, by, entry);
+            return entry == -__builtin_inff() ? entry : sum;
+          };
+          if (hides)
+            code_k ? bias(std::true_type{}, add_hidden) : bias(std::false_type{}, add_hidden);
+          else
+            code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+        } else {
+          const float* const t = table + (int64_t)head * a.c.table_len;
+          auto add = [&](float x, int diff) __attribute__((always_inline)) {
+            const float entry = t[min(max(diff + zero, 0), last)] * kLog2e;
+            const float sum = __builtin_fmaf(x, by, entry);
+            return entry == -__builtin_inff() ? entry : sum;
+          };
+          code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+        }
+      }
+      if (!a.c.slopes && !table && unit != 1.0f) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] *= unit;
+      }
+    }
+    if (partial) {
+      const bool whole = tile * KT + KT <= pre || (tile * KT >= w_lo_max && tile * KT + KT <= w_hi_min);
+      if (!whole) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int off = 32 * kb + 8 * (r / 4) + r % 4;
-            const int diff = cq - (code_k ? codes[off] : key0 + off);
-            if (a.c.slopes) s[kb][r] = __builtin_fmaf(-slope, fabsf((float)diff), s[kb][r]);
-            if (table) {
-              const int at = min(max(diff + t_zero, 0), t_last);
-              const float entry = a.table_lds ? t_lds[at] : t_far[at] * kLog2e;
-              const float sum = s[kb][r] + entry;
-              s[kb][r] = hides && entry == -__builtin_inff() ? entry : sum;
-            }
+            const int key = key0 + 32 * kb + 8 * (r / 4) + r % 4;
+            s[kb][r] = (key >= lo && key < hi) || key < pre ? s[kb][r] : -__builtin_inff();
           }
       }
-    }
-    if (partial) {
-      const int* const docs = reinterpret_cast<const int*>(lds + L::kDoc) + buf * 64 + 4 * half;
+      if (doc_k && t_dmin == t_dmax) {
+        const float away = t_dmin == dq ? 0.0f : 1.0f;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int off = 32 * kb + 8 * (r / 4) + r % 4;
-          const int key = key0 + off;
-          bool sees = (key >= lo && key < hi) || key < pre;
-          if (doc_k) sees = sees && docs[off] == dq;
-          s[kb][r] = sees ? s[kb][r] : -__builtin_inff();
-        }
+          for (int r = 0; r < 16; ++r) s[kb][r] = away != 0.0f ? -__builtin_inff() : s[kb][r];
+      } else if (doc_k) {
+        const int4* const docs = reinterpret_cast<const int4*>(lds + L::kDoc + buf * 256) + half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 d = docs[8 * kb + 2 * g];
+            s[kb][4 * g] = d.x == dq ? s[kb][4 * g] : -__builtin_inff();
+            s[kb][4 * g + 1] = d.y == dq ? s[kb][4 * g + 1] : -__builtin_inff();
+            s[kb][4 * g + 2] = d.z == dq ? s[kb][4 * g + 2] : -__builtin_inff();
+            s[kb][4 * g + 3] = d.w == dq ? s[kb][4 * g + 3] : -__builtin_inff();
+          }
+      }
     }
 
     float top = s[0][0];
@@ -522,28 +618,28 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
       const int c1 = min(end, c0 + chunk);
       lds_sync();  // the last chunk's tiles and bits have been used
       if (doc_k) {
-        // Tiles whose documents cannot be a row's are not read. A word of the bit sets has
-        // one writer.
-        for (int w = wave; w < (c1 - c0 + 31) / 32; w += NW) {
-          uint32_t some = 0, all = 0;
-          for (int i = 0; i < 32 && c0 + w * 32 + i < c1; ++i) {
-            const int64_t key = (int64_t)tile_of(c0 + w * 32 + i) * KT + (lane & (KT - 1));
-            const bool in = key < kv_len;
-            const int d = in ? doc_k[key] : 0;
-            if (__any(in && d >= dmin && d <= dmax)) some |= 1u << i;
-            if (__all(in && d == dmin && d == dmax)) all |= 1u << i;
-          }
-          if (lane == 0) {
-            any[w] = some;
-            whole[w] = all;
-          }
+        // Tiles whose documents cannot be a row's are not read: a lane looks at the range
+        // of one tile, a wave at 64.
+        for (int w = wave; w < (c1 - c0 + 63) / 64; w += NW) {
+          const int at = c0 + w * 64 + lane;
+          const int2 r = at < c1 ? doc_ranges[tile_of(at)] : int2{INT32_MAX, INT32_MIN};
+          tile_docs[w * 64 + lane] = r;
+          const uint64_t in = __ballot(r.y >= dmin && r.x <= dmax);
+          if (lane == 0) any[w] = in;
         }
         lds_sync();
       }
       auto next = [&](int i) __attribute__((always_inline)) {
         if (doc_k)
-          while (i < c1 && !(any[(i - c0) >> 5] >> ((i - c0) & 31) & 1)) ++i;
-        return __builtin_amdgcn_readfirstlane(i);
+          while (i < c1) {
+            const uint64_t left = any[(i - c0) >> 6] >> ((i - c0) & 63);
+            if (left != 0) {
+              i += __builtin_ctzll(left);
+              break;
+            }
+            i = c0 + (((i - c0) >> 6) + 1) * 64;
+          }
+        return scalar(min(i, c1));
       };
       int i = next(c0);
       int buf = 0;
@@ -556,15 +652,20 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
         const bool more = i < c1;
         const int tile = tile_of(i), k0 = tile * KT, k1 = k0 + KT;
         bool seen = false, partial = false;
+        int t_dmin = w_dmin, t_dmax = w_dmin;
         int following = i;
         if (more) {
-          const bool one_doc =
-              !doc_k || __builtin_amdgcn_readfirstlane(whole[(i - c0) >> 5] >> ((i - c0) & 31) & 1) != 0;
+          if (doc_k) {
+            const int2 r = tile_docs[i - c0];
+            t_dmin = scalar(r.x);
+            t_dmax = scalar(r.y);
+          }
           following = next(i + 1);
           if (following < c1) stage_k(buf ^ 1, tile_of(following));
           stage_v(buf, tile);
-          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min));
-          partial = !(k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min)) || !one_doc;
+          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min)) && (!doc_k || (t_dmax >= w_dmin && t_dmin <= w_dmax));
+          partial = !(k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min)) ||
+                    (doc_k && !(t_dmin == t_dmax && w_dmin == w_dmax));
         }
         if (seen) scores(buf);
         if (has) {
@@ -574,7 +675,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
             values(buf ^ 1, look);
         }
         if (!more) break;
-        if (seen) weights(buf, tile, partial);
+        if (seen) weights(buf, tile, partial, t_dmin, t_dmax);
         has = seen;
         look = partial || hides;
         vm_wait();
@@ -652,6 +753,24 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) attention_tile(Attn
         (m * mul + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// Smallest and largest document of each tile of keys: a wave a tile. (Looked over by
+// every workgroup instead, the documents of 16384 keys took each some 30 us.)
+__global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int64_t total) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= total) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t b = at / a.doc_tiles, first = (at - b * a.doc_tiles) * a.doc_tile;
+  int lo = INT32_MAX, hi = INT32_MIN;
+  if (lane < a.doc_tile && first + lane < a.c.k_tokens)
+    lo = hi = a.c.doc_k[b * a.c.doc_k_stride + first + lane];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  if (lane == 0) out[at] = int2{lo, hi};
+}
+
 // Joins the ranges of the keys: a wave a row.
 template <class T>
 __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
@@ -674,8 +793,8 @@ __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
   }
   const int64_t bh = at / a.rows;
   const int row = (int)(at - bh * a.rows);
-  const int b = (int)(bh / a.c.k_heads), kh = (int)(bh - (int64_t)b * a.c.k_heads);
-  const int token = row / a.group, head = kh * a.group + row % a.group;
+  const int b = (int)fdiv((uint32_t)bh, a.by_k_heads), kh = (int)(bh - (int64_t)b * a.c.k_heads);
+  const int token = (int)fdiv((uint32_t)row, a.by_group), head = kh * a.group + row - token * a.group;
   const float scale = l == 0.0f ? 0.0f : 1.0f / l;
   T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
                 head * a.c.out_stride[2];
@@ -693,18 +812,24 @@ struct TilePick {
 };
 
 template <class T, int DP, int NW>
-TilePick pick(bool shaped) {
-  return {shaped ? attention_tile<T, DP, NW, true> : attention_tile<T, DP, NW, false>, TileL<DP>::kBytes};
+TilePick pick(Shape shape) {
+  return {shape == kPlain ? attention_tile<T, DP, NW, kPlain>
+          : shape == kCap ? attention_tile<T, DP, NW, kCap>
+                          : attention_tile<T, DP, NW, kAny>,
+          TileL<DP>::kBytes};
 }
 
 template <class T>
-TilePick pick(int d, bool shaped) {
-  if (d <= 32) return pick<T, 32, 4>(shaped);
-  if (d <= 64) return pick<T, 64, 4>(shaped);
-  if (d <= 96) return pick<T, 96, 4>(shaped);
-  if (d <= 128) return pick<T, 128, 4>(shaped);
-  return pick<T, 256, 4>(shaped);
+TilePick pick(int d, Shape shape) {
+  if (d <= 32) return pick<T, 32, 4>(shape);
+  if (d <= 64) return pick<T, 64, 4>(shape);
+  if (d <= 96) return pick<T, 96, 4>(shape);
+  if (d <= 128) return pick<T, 128, 4>(shape);
+  return pick<T, 256, 4>(shape);
 }
+
+// Keys of a tile (TileL::KT).
+int tile_keys(int d) { return d > 128 ? 32 : 64; }
 
 int waves_of(const arthip_attention_args&) { return 4; }
 
@@ -720,6 +845,10 @@ AttnPlan attention_plan(const arthip_attention_args& c) {
   if (items < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, tiles / 4, 64}));
   if (p.splits > 1)
     p.workspace = (size_t)p.splits * c.batch * c.k_heads * rows * (c.head_dim + 2) * sizeof(float);
+  if (c.doc_k != nullptr) {
+    const int64_t n = (c.k_tokens + tile_keys(c.head_dim) - 1) / tile_keys(c.head_dim);
+    p.workspace += (size_t)(c.doc_k_stride == 0 ? 1 : c.batch) * n * sizeof(int2);
+  }
   return p;
 }
 
@@ -733,13 +862,32 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.row_tiles = (a.rows + 32 * nw - 1) / (32 * nw);
   a.splits = attention_plan(c).splits;
   a.items = c.batch * c.k_heads * a.row_tiles * a.splits;
+  a.by_group = make_fastdiv((uint32_t)a.group);
+  a.by_k_heads = make_fastdiv((uint32_t)c.k_heads);
+  a.by_row_tiles = make_fastdiv((uint32_t)a.row_tiles);
+  a.by_splits = make_fastdiv((uint32_t)a.splits);
   const int64_t total = (int64_t)c.batch * c.k_heads * a.rows;
   a.part = static_cast<float*>(c.workspace);
   if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
   const bool f16 = c.dtype == ARTHIP_TYPE_F16;
-  // Cap and bias take the scores through more steps; so does a scale that turns their order.
-  const bool shaped = c.cap > 0 || c.slopes != nullptr || c.table != nullptr || !(c.scale > 0);
-  TilePick k = f16 ? pick<_Float16>(c.head_dim, shaped) : pick<__bf16>(c.head_dim, shaped);
+  const Shape shape = c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
+  TilePick k = f16 ? pick<_Float16>(c.head_dim, shape) : pick<__bf16>(c.head_dim, shape);
+  if (shape == kCap) {
+    static constexpr double fit[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825, 0.015486690367999443};
+    const double r = (double)c.scale / c.cap;
+    a.cap_reach = (float)(0.6 / r);
+    for (int i = 0; i < 5; ++i) a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
+  }
+  if (c.doc_k != nullptr && c.k_tokens > 0) {
+    a.doc_tile = tile_keys(c.head_dim);
+    a.doc_tiles = (c.k_tokens + a.doc_tile - 1) / a.doc_tile;
+    int2* const ranges = reinterpret_cast<int2*>(a.splits > 1 ? a.stat + 2 * a.splits * total : a.part);
+    const int64_t n = (int64_t)(c.doc_k_stride == 0 ? 1 : c.batch) * a.doc_tiles;
+    a.doc_ranges = ranges;
+    hipLaunchKernelGGL(attention_docs, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a, ranges, n);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   const int64_t table = c.table == nullptr ? 0 : (int64_t)a.group * c.table_len * 4;
   a.table_lds = table <= kTableBytes;
   if (a.table_lds) k.bytes += (int)table;
