@@ -1,0 +1,1067 @@
+// Attention over strided tokens (arthip_attention): softmax(score + mask) V in one
+// pass over the keys, with capped scores, a bias over the distance, windows,
+// prefixes, documents and ragged lengths.
+//
+// The query heads that share a key head are rows of one matrix: row r of a key head
+// is token r / G, head r % G of its G heads. A workgroup takes 32 rows a wave and
+// walks the keys in tiles that it stages in LDS for all its waves. Both products are
+// v_mfma_f32_32x32x16 with the keys of the first as rows, S^T = K Q^T: a lane then
+// holds 16 keys of ONE query in its accumulator, so that the running maximum and sum
+// need one exchange between the wave's halves a tile, the rescale of the output is
+// one factor a lane, and the accumulator, packed to the element type, already is the
+// right operand of O^T += V^T P^T. (The order of the keys inside a product is free:
+// V's rows are fetched in the accumulator's order, by transposing LDS reads.)
+//
+// Statistics are fp32 in the base of 2. P is rounded to the element type for the
+// second product (it lies in [0, 1]); its sum is taken before the rounding.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+#include <cstdint>
+#include <type_traits>
+
+#include "launch.h"
+#include "token_dev.h"
+#include "transformer.h"
+
+namespace arthip {
+
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kFar = 1 << 30;
+
+struct AttnArgs {
+  arthip_attention_args c;
+  int group;      // query heads of a key head
+  int rows;       // rows of a key head: q_tokens * group
+  int row_tiles;  // workgroups along the rows
+  int splits;     // workgroups along the keys
+  int range;      // tiles of each but the last
+  int buffers;    // of K and of V tiles, 2 or 3
+  int items;      // batch * k_heads * row_tiles * splits
+  int table_lds;  // the tables of a key head's rows are kept in LDS
+  int table_bytes;  // and take these
+  int wide;       // keys further apart than 32-bit offsets reach
+  FastDiv by_group, by_k_heads, by_row_tiles, by_splits;
+  float cap_reach;  // |q.k| up to which the polynomial holds
+  float cap_fit[5];
+  const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
+  int doc_tiles, doc_tile;  // tiles of a sequence, keys of a tile
+  float* part;    // [splits][batch * k_heads * rows][D] unscaled sums, if splits > 1
+  float* stat;    // [splits][batch * k_heads * rows][2] maximum (base 2) and sum
+};
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+  typedef h8 frag;
+  static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Elem<__bf16> {
+  typedef b8 frag;
+  static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// The two halves' values of a lane's x. (The results are copied before they are cast:
+// a bit cast of a vector's element takes element 0, whichever is named.)
+__device__ __forceinline__ void halves(float x, float& low, float& high) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
+  const u2 r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  low = __builtin_bit_cast(float, r0);
+  high = __builtin_bit_cast(float, r1);
+}
+__device__ __forceinline__ float halves_max(float x) {
+  float a, b;
+  halves(x, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  float a, b;
+  halves(x, a, b);
+  return a + b;
+}
+
+// LDS of a workgroup: two or three buffers of K tiles and of V tiles, written by loads that go
+// to LDS without passing registers. Such a load puts a wave's 64 x 16 bytes in a row,
+// so rows cannot be padded; their 16-byte chunks are permuted instead, by an exclusive
+// or with bits of the row, so that the 16 rows of a K operand, and the four rows of a
+// transposed V read, lie on different banks. The permutation is in the addresses that
+// the lanes load from.
+template <int DP, int KT>  // values of a head, padded; keys of a tile
+struct TileL {
+  static constexpr int RB = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row
+  static constexpr int kTile = KT * RB;
+  static constexpr int kChunk = 1024;  // tiles whose documents are looked over at once
+  // After `buffers` K tiles and as many V tiles:
+  static constexpr int kRange = 0;                   // int32 [2][16] documents of the waves
+  static constexpr int kDoc = kRange + 2 * 16 * 4;   // int32 [3][64]
+  static constexpr int kCode = kDoc + 3 * 64 * 4;    // int32 [3][64]
+  static constexpr int kAny = kCode + 3 * 64 * 4;    // bit a tile: some key of a row's document
+  static constexpr int kTable = kAny + kChunk / 8;   // fp32 [group][table_len], if it fits
+  // and after that, with documents, int2 a tile: its range of them
+  static constexpr int bytes(int buffers) { return 2 * buffers * kTile + kTable; }
+  static __device__ __forceinline__ int k_swizzle(int row) {
+    return RB == 64 ? (row >> 2) & 3 : RB == 128 ? (row >> 1) & 7 : RB == 256 ? row & 15 : row & 7;
+  }
+  static __device__ __forceinline__ int v_swizzle(int row) {
+    return RB == 64 ? 0 : RB == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+  }
+};
+
+constexpr int kTableBytes = 16384;  // of the tables that a workgroup keeps in LDS
+
+typedef uint32_t rsrc_t __attribute__((ext_vector_type(4)));
+
+// A buffer of up to `bytes` bytes from p (uniform).
+__device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return rsrc_t{lo, hi & 0xffffu, bytes, 0x00020000u};
+}
+
+// 16 (4) bytes a lane from the buffer to LDS, lane after lane from `to`. Offsets past
+// the buffer bring zeros. The compiler does not see these loads (its own would make
+// every later LDS read wait for them): vm_wait() stands between them and their use.
+__device__ __forceinline__ void load_lds16(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(to), "v"(at), "s"(from), "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void load_lds4(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :
+               : "s"(to), "v"(at), "s"(from), "s"(base)
+               : "memory");
+}
+// Waits until at most `groups` groups of N loads, the latest, are on their way.
+template <int N>
+__device__ __forceinline__ void vm_wait(int groups) {
+  static_assert(2 * N < 64, "the counter has six bits");
+  if (groups >= 2)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * N) : "memory");
+  else if (groups == 1)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// The order of a block of N products with R LDS reads each: the reads run four products
+// ahead, so that their latency (some 64 to 128 clocks) passes behind the matrix unit.
+// Left to itself the compiler reads an operand right before its product.
+template <int N, int R>
+__device__ __forceinline__ void ahead() {
+  constexpr int A = N < 4 ? N : 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - A; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+}
+
+// What the scores go through: nothing (the scale is in the exponent), the cap, or any
+// of cap, slopes, table and a scale that turns their order.
+enum Shape { kPlain, kCap, kAny };
+
+// SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
+// tile's keys; otherwise each holds 32 rows of its own and takes all keys.
+template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
+__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kAny ? 2 : 3) attention_tile(AttnArgs a) {
+  using L = TileL<DP, KT>;
+  using E = Elem<T>;
+  using frag = typename E::frag;
+  constexpr int RB = L::RB, KW = SHARED ? KT / NW : KT, KB = KW / 32, KS = DP / 16, DB = DP / 32;
+  constexpr int ROWS = SHARED ? 32 : 32 * NW;
+  constexpr int SEG = L::kTile / 1024;                // loads of a tile, 1 KiB each
+  constexpr int LOADS = (SEG + NW - 1) / NW;          // of a wave
+  constexpr uint32_t kOob = 0x80000000u;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  const int v_at = a.buffers * L::kTile;  // V's buffers
+  unsigned char* const more = lds + 2 * v_at;  // what follows them
+  const uint32_t more_base = lds_base + 2 * v_at;
+
+  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
+  // stay on one XCD. A single row tile shares nothing, and sequences of different
+  // lengths are then spread over all.
+  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
+  // stay on one XCD. A single row tile shares nothing: its items go round as they come,
+  // one further each round, so that no XCD gets all the first (long) ranges.
+  const int bid = (int)blockIdx.x, per = (int)gridDim.x >> 3;
+  const int item = a.row_tiles == 1 ? (bid & ~7) + ((bid + (bid >> 3)) & 7) : (bid & 7) * per + (bid >> 3);
+  if (item >= a.items) return;
+  const int ranges = (int)fdiv((uint32_t)item, a.by_splits);
+  const int split = item - ranges * a.splits;
+  const int bh = (int)fdiv((uint32_t)ranges, a.by_row_tiles);
+  const int row_tile = a.row_tiles - 1 - (ranges - bh * a.row_tiles);  // causal: the longest first
+  const int b = (int)fdiv((uint32_t)bh, a.by_k_heads);
+  const int kh = bh - b * a.c.k_heads;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int n = lane & 31;     // the lane's row of the wave's 32
+  const int half = lane >> 5;  // which keys and values of it
+
+  // -- rows ------------------------------------------------------------------------
+  auto token_of = [&](int row) __attribute__((always_inline)) { return (int)fdiv((uint32_t)row, a.by_group); };
+  auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int kv_len = scalar(a.c.kv_len ? min(max(a.c.kv_len[b], 0), a.c.k_tokens) : a.c.k_tokens);
+  const int q_start =
+      scalar(a.c.q_start ? min(max(a.c.q_start[b], -kFar), kFar) : a.c.k_tokens - a.c.q_tokens);
+  const int pre = scalar(a.c.prefix ? min(max(a.c.prefix[b], 0), kv_len) : 0);
+  // Keys [lo, hi) that a window leaves to a token (and those below pre).
+  auto low = [&](int token) __attribute__((always_inline)) -> int {
+    if (a.c.left < 0) return 0;
+    const int64_t p = (int64_t)q_start + token - a.c.left;
+    return p < 0 ? 0 : p > kv_len ? kv_len : (int)p;
+  };
+  auto high = [&](int token) __attribute__((always_inline)) -> int {
+    if (a.c.right < 0) return kv_len;
+    const int64_t p = (int64_t)q_start + token + a.c.right + 1;
+    return p < 0 ? 0 : p > kv_len ? kv_len : (int)p;
+  };
+  const int first_row = row_tile * ROWS;
+  const int last_row = min(first_row + ROWS, a.rows) - 1;
+  const int w_row = first_row + (SHARED ? 0 : wave * 32);  // the wave's first
+  const int wk = SHARED ? wave * KW : 0;                   // and its first key of a tile
+  const int row = w_row + n;
+  const bool real = row <= last_row;
+  const int token = token_of(min(row, last_row));
+  const int g_head = min(row, last_row) - token * a.group;
+  const int head = kh * a.group + g_head;
+  const int lo = low(token), hi = high(token);
+  // The wave's and the workgroup's rows together: all see [lo_max, hi_min), some see
+  // [lo_min, hi_max). Positions grow with the row.
+  const int wr0 = min(w_row, last_row), wr1 = min(wr0 + 31, last_row);
+  const int w_lo_min = low(token_of(wr0)), w_lo_max = low(token_of(wr1));
+  const int w_hi_min = high(token_of(wr0)), w_hi_max = high(token_of(wr1));
+  const bool w_real = w_row <= last_row;
+  const int g_lo_min = low(token_of(first_row)), g_hi_max = high(token_of(last_row));
+
+  frag q[KS];
+  {
+    const T* const qp = static_cast<const T*>(a.c.q) + b * a.c.q_stride[0] + token * a.c.q_stride[1] +
+                        head * a.c.q_stride[2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = s * 16 + half * 8;
+      q[s] = real && d < a.c.head_dim ? *reinterpret_cast<const frag*>(qp + d) : frag{};
+    }
+  }
+
+  // -- score transforms --------------------------------------------------------------
+  // Without cap and bias the scale goes into the exponent's multiply-add.
+  const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
+  const float slope = SHAPE == kAny && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
+  const int cq = SHAPE == kAny && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
+  const float* const table = SHAPE == kAny && a.c.table ? a.c.table : nullptr;
+  const int32_t* const code_k = SHAPE == kAny && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
+  const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
+  const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
+  bool hides = false;  // the table has an entry of -inf
+  auto load_table = [&]() __attribute__((always_inline)) {
+    float* const t = reinterpret_cast<float*>(more + L::kTable);
+    const int len = a.group * a.c.table_len;
+    const float* const from = table + (int64_t)kh * len;
+    bool h = false;
+    for (int i = tid; i < len; i += NW * 64) {
+      const float e = from[i];
+      if (a.table_lds) t[i] = e * kLog2e;
+      h = h || e == -__builtin_inff();
+    }
+    int* const flag = reinterpret_cast<int*>(more + L::kRange);
+    const int found = __any(h);
+    if (lane == 0) flag[wave] = found;
+    lds_sync();
+    int all = 0;
+    for (int i = 0; i < NW; ++i) all |= flag[i];
+    hides = scalar(all) != 0;
+  };
+
+  // -- the tiles: those of the prefix, then those of the windows ----------------------
+  const int pre_tiles = (pre + KT - 1) / KT;
+  const int win_first = max(g_lo_min / KT, pre_tiles);
+  const int win_end = g_hi_max > g_lo_min ? (g_hi_max + KT - 1) / KT : 0;
+  const int count = pre_tiles + max(win_end - win_first, 0);
+  const int begin = min(split * a.range, count);
+  const int end = split == a.splits - 1 ? count : min(begin + a.range, count);
+  auto tile_of = [&](int i) __attribute__((always_inline)) { return i < pre_tiles ? i : i - pre_tiles + win_first; };
+
+  // Documents: the range of a wave's rows, and of the workgroup's.
+  uint64_t* const any = reinterpret_cast<uint64_t*>(more + L::kAny);
+  int2* const tile_docs = reinterpret_cast<int2*>(more + L::kTable + a.table_bytes);
+  const int2* const doc_ranges =
+      doc_k ? a.doc_ranges + (a.c.doc_k_stride == 0 ? 0 : (int64_t)b * a.doc_tiles) : nullptr;
+  int w_dmin = dq, w_dmax = dq, dmin = 0, dmax = 0;
+  if (doc_k) {
+    int* const range = reinterpret_cast<int*>(more + L::kRange);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {  // a lane past the last row repeats it
+      w_dmin = min(w_dmin, __shfl_xor(w_dmin, o));
+      w_dmax = max(w_dmax, __shfl_xor(w_dmax, o));
+    }
+    w_dmin = scalar(w_dmin);
+    w_dmax = scalar(w_dmax);
+    lds_sync();
+    if (lane == 0) {
+      range[wave] = w_dmin;
+      range[16 + wave] = w_dmax;
+    }
+    lds_sync();
+    dmin = range[0];
+    dmax = range[16];
+    for (int i = 1; i < NW; ++i) {
+      dmin = min(dmin, range[i]);
+      dmax = max(dmax, range[16 + i]);
+    }
+  }
+
+  f16v o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = f16v{};
+  float m = -__builtin_inff(), l = 0.0f;
+
+  // -- staging -------------------------------------------------------------------------
+  const T* const kp = static_cast<const T*>(a.c.k) + b * a.c.k_stride[0] + kh * a.c.k_stride[2];
+  const T* const vp = static_cast<const T*>(a.c.v) + b * a.c.v_stride[0] + kh * a.c.v_stride[2];
+  const int s_row = (wave * 1024 + lane * 16) / RB;  // of the wave's first load; the others' follow
+  const int s_chunk = lane * 16 % RB / 16;
+  const int64_t ks2 = a.c.k_stride[1] * 2, vs2 = a.c.v_stride[1] * 2;  // bytes
+  constexpr int STEP = NW * 1024 / RB;  // rows from one load of a wave to the next
+  // K's permutation comes round after 16 rows (8 of 512 bytes), V's after 4.
+  constexpr int KP = (RB == 512 ? 8 : 16) / STEP > 1 ? (RB == 512 ? 8 : 16) / STEP : 1;
+  static_assert(STEP % 4 == 0, "V's permutation is the same for all loads of a lane");
+  uint32_t k_off[KP], v_off;  // a lane's offsets, but for the rows between its loads
+#pragma unroll
+  for (int i = 0; i < KP; ++i) {
+    const int chunk = s_chunk ^ L::k_swizzle(s_row + i * STEP);
+    k_off[i] = chunk * 8 < a.c.head_dim ? (uint32_t)(s_row * (int)ks2 + chunk * 16) : kOob;
+  }
+  {
+    const int chunk = s_chunk ^ L::v_swizzle(s_row);
+    v_off = chunk * 8 < a.c.head_dim ? (uint32_t)(s_row * (int)vs2 + chunk * 16) : kOob;
+  }
+  auto stage = [&](const T* from, int64_t stride, auto offset, auto swizzle, int tile, uint32_t to)
+      __attribute__((always_inline)) {
+    const char* const p = reinterpret_cast<const char*>(from) + (int64_t)tile * KT * stride;
+    const int left = kv_len - tile * KT;  // keys past the length come as zeros
+    if (left >= KT && !a.wide) {
+      const rsrc_t r = buffer_of(p, 0x7fffffffu);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        if (SEG % NW != 0 && wave + i * NW >= SEG) break;
+        load_lds16(r, offset(i), i * STEP * (uint32_t)stride, to + (wave + i * NW) * 1024);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if (SEG % NW != 0 && wave + i * NW >= SEG) break;
+      const int row = s_row + i * STEP;
+      if (a.wide) {
+        // 32-bit offsets would wrap: a buffer of its own for every key of the load.
+        const int chunk = s_chunk ^ swizzle(row);
+        const bool in = chunk * 8 < a.c.head_dim && row < left;
+        constexpr int keys = RB < 1024 ? 1024 / RB : 1;
+#pragma unroll 1
+        for (int r = 0; r < keys; ++r) {
+          const int first = (wave * 1024 + i * NW * 1024) / RB + r;
+          const rsrc_t one = buffer_of(p + first * stride, 0x7fffffffu);
+          if (row == first) load_lds16(one, in ? chunk * 16u : kOob, 0, to + (wave + i * NW) * 1024);
+        }
+      } else {
+        load_lds16(buffer_of(p, 0x7fffffffu), row < left ? offset(i) : kOob, i * STEP * (uint32_t)stride,
+                   to + (wave + i * NW) * 1024);
+      }
+    }
+  };
+  auto stage_k = [&](int buf, int tile) __attribute__((always_inline)) {
+    stage(kp, ks2, [&](int i) { return k_off[i % KP]; }, L::k_swizzle, tile, lds_base + buf * L::kTile);
+    if (doc_k && wave == 0)
+      load_lds4(buffer_of(doc_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kDoc + buf * 256);
+    if (code_k && wave == NW - 1)
+      load_lds4(buffer_of(code_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kCode + buf * 256);
+  };
+  auto stage_v = [&](int buf, int tile) __attribute__((always_inline)) {
+    stage(vp, vs2, [&](int) { return v_off; }, L::v_swizzle, tile, lds_base + v_at + buf * L::kTile);
+  };
+
+  // -- the products --------------------------------------------------------------------
+  // Operands come from a lane's base plus constants; the permutation, an exclusive or
+  // with the lane's bits, leaves one base for each K step and each block of V values.
+  typedef __attribute__((address_space(3))) unsigned char lds_byte;
+  typedef __attribute__((address_space(3))) const frag lds_frag;
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  lds_byte* const lds0 = (lds_byte*)lds;
+  const uint32_t k_lane = (wk + n) * RB + (half ^ L::k_swizzle(n)) * 16;
+  const int v_row = 4 * half + (lane & 15) / 4;
+  const uint32_t v_lane =
+      (wk + v_row) * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+
+  f16v s[KB];        // scores of the current tile, key block by key block
+  frag p[KW / 16];   // weights of the previous tile
+  auto scores = [&](int buf) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + buf * L::kTile;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      lds_byte* const k = at + (k_lane ^ (ks * 32));
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[kb] = E::mma(*(lds_frag*)(k + kb * 32 * RB), q[ks], ks == 0 ? f16v{} : s[kb]);
+    }
+    ahead<KS * KB, 1>();
+  };
+  auto v_frag = [&](lds_byte* at, int kk) __attribute__((always_inline)) -> frag {  // 32 values of 16 keys (block kk)
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + kk * 16 * RB));
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + kk * 16 * RB + 8 * RB));
+    return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  bool odd = false;  // a tile that a row does not see whole holds an infinity or NaN in V
+  auto values = [&](int buf, bool look) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + v_at + buf * L::kTile;
+    lds_byte* v[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) v[db] = at + (v_lane ^ (db * 64));
+    if (look) {
+      // Rows that do not see all of this tile weigh some of V by 0, which infinities and
+      // NaN survive: 0 times the tile tells whether it has any.
+      f16v z = f16v{};
+#pragma unroll
+      for (int kk = 0; kk < KW / 16; ++kk)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) z = E::mma(v_frag(v[db], kk), frag{}, z);
+      float t = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t += z[r];
+      odd = odd || t != 0.0f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KW / 16; ++kk)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
+    ahead<KW / 16 * DB, 2>();
+  };
+  // The same key by key, each added only to the rows that weigh it.
+  auto values_apart = [&](int buf) __attribute__((always_inline)) {
+    lds_byte* const at = lds0 + v_at + buf * L::kTile;
+#pragma unroll
+    for (int kk = 0; kk < KW / 16; ++kk)
+#pragma unroll 1
+      for (int key = 0; key < 16; ++key) {
+        const int of = (key >> 2) & 1, j = (key & 3) | ((key >> 1) & 4);  // its half and element
+        u4 keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keep[e] = half != of || j >> 1 != e ? 0u : j & 1 ? 0xffff0000u : 0x0000ffffu;
+        const u4 one = __builtin_bit_cast(u4, p[kk]) & keep;
+        const float sees = halves_max(((one[0] | one[1] | one[2] | one[3]) & 0x7fff7fffu) != 0 ? 1.0f : 0.0f);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u4 x = __builtin_bit_cast(u4, v_frag(at + (v_lane ^ (db * 64)), kk)) & keep;
+          const f16v c = E::mma(__builtin_bit_cast(frag, x), __builtin_bit_cast(frag, one), f16v{});
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[db][r] += sees != 0.0f ? c[r] : 0.0f;
+        }
+      }
+  };
+
+  // -- scores to weights -----------------------------------------------------------------
+  auto weights = [&](int buf, int k0, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
+    const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
+    const float unit = a.c.cap > 0 ? 1.0f : a.c.scale * kLog2e;  // what scores are still to be scaled by
+    if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
+      float far = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
+      if (SHAPE == kCap && !__any(!(far <= a.cap_reach))) {
+        // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
+        // less than 8e-8), six plain operations where the exponential and the reciprocal
+        // take a quarter of the rate each.
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float x = s[kb][r], z = x * x;
+            float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
+            t = __builtin_fmaf(t, z, a.cap_fit[2]);
+            t = __builtin_fmaf(t, z, a.cap_fit[1]);
+            t = __builtin_fmaf(t, z, a.cap_fit[0]);
+            s[kb][r] = x * t;
+          }
+      } else {
+        // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2
+        const float in = 2.0f * kLog2e * a.c.scale / a.c.cap, out = kLog2e * a.c.cap;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(s[kb][r] * in);
+            s[kb][r] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
+          }
+      }
+    }
+    if constexpr (SHAPE == kAny) {
+      // The loops below are whole loops a branch: a uniform branch inside would be taken
+      // for every score.
+      const int4* const codes = reinterpret_cast<const int4*>(more + L::kCode + buf * 256 + wk * 4) + half;
+      auto bias = [&](auto coded, auto add) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            int4 c{};
+            if constexpr (decltype(coded)::value) c = codes[8 * kb + 2 * g];
+            const int ck[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[kb][4 * g + e] =
+                  add(s[kb][4 * g + e], decltype(coded)::value ? cq - ck[e] : cq - key0 - (32 * kb + 8 * g + e));
+          }
+      };
+      if (a.c.slopes) {
+        auto add = [&](float x, int diff) __attribute__((always_inline)) {
+          return __builtin_fmaf(x, unit, -slope * fabsf((float)diff));
+        };
+        if (code_k)
+          bias(std::true_type{}, add);
+        else {
+          const float first = (float)(cq - key0);
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[kb][r] = __builtin_fmaf(s[kb][r], unit, -slope * fabsf(first - (float)(32 * kb + 8 * (r / 4) + r % 4)));
+        }
+      }
+      if (table) {
+        const float by = a.c.slopes ? 1.0f : unit;
+        const int last = a.c.table_len - 1, zero = a.c.table_zero;
+        if (a.table_lds) {
+          // Entries in the base of 2.
+          const float* const t = reinterpret_cast<const float*>(more + L::kTable) + g_head * a.c.table_len;
+          auto add = [&](float x, int diff) __attribute__((always_inline)) {
+            return __builtin_fmaf(x, by, t[min(max(diff + zero, 0), last)]);
+          };
+          auto add_hidden = [&](float x, int diff) __attribute__((always_inline)) {
+            const float entry = t[min(max(diff + zero, 0), last)];
+            const float sum = __builtin_fmaf(x, by, entry);
+            return entry == -__builtin_inff() ? entry : sum;
+          };
+          if (hides)
+            code_k ? bias(std::true_type{}, add_hidden) : bias(std::false_type{}, add_hidden);
+          else
+            code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+        } else {
+          const float* const t = table + (int64_t)head * a.c.table_len;
+          auto add = [&](float x, int diff) __attribute__((always_inline)) {
+            const float entry = t[min(max(diff + zero, 0), last)] * kLog2e;
+            const float sum = __builtin_fmaf(x, by, entry);
+            return entry == -__builtin_inff() ? entry : sum;
+          };
+          code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+        }
+      }
+      if (!a.c.slopes && !table && unit != 1.0f) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] *= unit;
+      }
+    }
+    if (partial) {
+      const bool whole = k0 + KW <= pre || (k0 >= w_lo_max && k0 + KW <= w_hi_min);
+      if (!whole) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = key0 + 32 * kb + 8 * (r / 4) + r % 4;
+            s[kb][r] = (key >= lo && key < hi) || key < pre ? s[kb][r] : -__builtin_inff();
+          }
+      }
+      if (doc_k && t_dmin == t_dmax) {
+        const float away = t_dmin == dq ? 0.0f : 1.0f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] = away != 0.0f ? -__builtin_inff() : s[kb][r];
+      } else if (doc_k) {
+        const int4* const docs = reinterpret_cast<const int4*>(more + L::kDoc + buf * 256 + wk * 4) + half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 d = docs[8 * kb + 2 * g];
+            s[kb][4 * g] = d.x == dq ? s[kb][4 * g] : -__builtin_inff();
+            s[kb][4 * g + 1] = d.y == dq ? s[kb][4 * g + 1] : -__builtin_inff();
+            s[kb][4 * g + 2] = d.z == dq ? s[kb][4 * g + 2] : -__builtin_inff();
+            s[kb][4 * g + 3] = d.w == dq ? s[kb][4 * g + 3] : -__builtin_inff();
+          }
+      }
+    }
+
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    top = halves_max(top);
+    // The base of a row's exponents follows its largest score only where that has grown
+    // by more than 2^8: until then weights are at most 256, and nothing is rescaled.
+    if (__any((top - m) * mul > 8.0f)) {
+      const float next = fmaxf(m, top);
+      // A row that has seen nothing yet has no sums to keep (next may be -inf as well).
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= f;
+    }
+    const float base = m == -__builtin_inff() ? 0.0f : m * mul;
+    float sum = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], mul, -base));
+        sum += s[kb][r];
+      }
+    l += sum;  // this half's keys; the halves are added at the end
+#pragma unroll
+    for (int kk = 0; kk < KW / 16; ++kk) {
+      const f16v x = s[kk / 2];
+      p[kk] = kk & 1
+                  ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
+                  : __builtin_convertvector(__builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7), frag);
+    }
+  };
+
+  // -- the walk ------------------------------------------------------------------------
+  // One barrier a tile. While tile t's scores and the previous tile's values are
+  // multiplied, K of the next tile and V of this one are on their way to the buffers
+  // that the last barrier freed; with three buffers, K of the tile after the next and V
+  // of the next, so that two tiles' loads overlap.
+  const bool deep = a.buffers == 3;
+  auto walk = [&](auto apart) __attribute__((always_inline)) {
+    const int chunk = doc_k ? L::kChunk : max(end - begin, 1);
+    for (int c0 = begin; c0 < end; c0 += chunk) {
+      const int c1 = min(end, c0 + chunk);
+      lds_sync();  // the last chunk's tiles and bits have been used
+      if (doc_k) {
+        // Tiles whose documents cannot be a row's are not read: a lane looks at the range
+        // of one tile, a wave at 64.
+        for (int w = wave; w < (c1 - c0 + 63) / 64; w += NW) {
+          const int at = c0 + w * 64 + lane;
+          const int2 r = at < c1 ? doc_ranges[tile_of(at)] : int2{INT32_MAX, INT32_MIN};
+          tile_docs[w * 64 + lane] = r;
+          const uint64_t in = __ballot(r.y >= dmin && r.x <= dmax);
+          if (lane == 0) any[w] = in;
+        }
+        lds_sync();
+      }
+      auto next = [&](int i) __attribute__((always_inline)) {
+        if (doc_k)
+          while (i < c1) {
+            const uint64_t left = any[(i - c0) >> 6] >> ((i - c0) & 63);
+            if (left != 0) {
+              i += __builtin_ctzll(left);
+              break;
+            }
+            i = c0 + (((i - c0) >> 6) + 1) * 64;
+          }
+        return scalar(min(i, c1));
+      };
+      // Tiles i, the next one and (with three buffers) the one after it.
+      int i = next(c0);
+      const bool nothing = i >= c1;
+      int i1 = nothing ? c1 : next(i + 1);
+      if (!nothing) {
+        stage_k(0, tile_of(i));
+        if (deep) {
+          if (i1 < c1) stage_k(1, tile_of(i1));
+          stage_v(0, tile_of(i));
+        }
+      }
+      if (table && !decltype(apart)::value && c0 == begin) load_table();
+      if (nothing) continue;
+      vm_wait<LOADS>(deep ? (i1 < c1 ? 2 : 1) : 0);
+      lds_sync();
+      long long T[6]={0,0,0,0,0,0}; long long t0=clock64(), t1;
+#define TICK(k) { __builtin_amdgcn_sched_barrier(0); t1=clock64(); __builtin_amdgcn_sched_barrier(0); T[k]+=t1-t0; t0=t1; }
+      int buf = 0, before = 0;         // buffers of this tile and of the previous one
+      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
+      while (true) {
+        const bool live = i < c1;
+        const int tile = tile_of(i), k0 = tile * KT + wk, k1 = k0 + KW;
+        bool seen = false, partial = false;
+        int t_dmin = w_dmin, t_dmax = w_dmin, i2 = c1, after = 0, on_way = 0;
+        if (live) {
+          if (doc_k) {
+            const int2 r = tile_docs[i - c0];
+            t_dmin = scalar(r.x);
+            t_dmax = scalar(r.y);
+          }
+          after = buf + 1 == a.buffers ? 0 : buf + 1;
+          if (i1 < c1) i2 = next(i1 + 1);
+          if (deep) {
+            if (i2 < c1) stage_k(after + 1 == a.buffers ? 0 : after + 1, tile_of(i2));
+            if (i1 < c1) stage_v(after, tile_of(i1));
+            on_way = (i2 < c1 ? 1 : 0) + (i1 < c1 ? 1 : 0);
+          } else {
+            if (i1 < c1) stage_k(after, tile_of(i1));
+            stage_v(buf, tile);
+          }
+          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min)) &&
+                 (!doc_k || (t_dmax >= w_dmin && t_dmin <= w_dmax));
+          partial = !(k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min)) ||
+                    (doc_k && !(t_dmin == t_dmax && w_dmin == w_dmax));
+        }
+        TICK(0)
+        if (seen) scores(buf);
+        TICK(1)
+        if (has) {
+          if constexpr (decltype(apart)::value)
+            values_apart(before);
+          else
+            values(before, look);
+        }
+        TICK(2)
+        if (!live) break;
+        if (seen) weights(buf, k0, partial, t_dmin, t_dmax);
+        has = seen;
+        look = partial || hides;
+        TICK(3)
+        vm_wait<LOADS>(on_way);
+        TICK(4)
+        lds_sync();
+        TICK(5)
+        i = i1;
+        i1 = i2;
+        before = buf;
+        buf = after;
+      }
+      if (a.splits==1 && a.part && lane==0) { long long* D=(long long*)a.part + ((long long)blockIdx.x*NW+wave)*8; for(int k=0;k<6;k++) D[k]=T[k]; D[6]=end-begin; }
+    }
+  };
+  walk(std::false_type{});
+  // A workgroup that met such a tile starts over and takes the keys one by one.
+  {
+    int* const flag = reinterpret_cast<int*>(more + L::kRange);
+    lds_sync();
+    if (lane == 0) flag[wave] = 0;
+    if (odd) flag[wave] = 1;
+    lds_sync();
+    int again = 0;
+    for (int i = 0; i < NW; ++i) again |= flag[i];
+    if (__builtin_amdgcn_readfirstlane(again) != 0) {
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i] = f16v{};
+      m = -__builtin_inff();
+      l = 0.0f;
+      walk(std::true_type{});
+    }
+  }
+
+  // -- results -------------------------------------------------------------------------
+  l = halves_sum(l);
+  if constexpr (SHARED) {
+    // The other waves hand their sums to the first, one after the other.
+    float* const box = reinterpret_cast<float*>(lds);
+    for (int w = 1; w < NW; ++w) {
+      lds_sync();  // the tiles, and the last wave's sums, have been used
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f4*>(box + ((i * 4 + g) * 64 + lane) * 4) =
+                f4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+        box[DB * 1024 + lane] = m;
+        box[DB * 1024 + 64 + lane] = l;
+      }
+      lds_sync();
+      if (wave == 0) {
+        const float m2 = box[DB * 1024 + lane], next = fmaxf(m, m2);
+        const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+        const float f2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m2 - next) * mul);
+        m = next;
+        l = l * f1 + box[DB * 1024 + 64 + lane] * f2;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f4 x = *reinterpret_cast<const f4*>(box + ((i * 4 + g) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][4 * g + e] = o[i][4 * g + e] * f1 + x[e] * f2;
+          }
+      }
+    }
+    if (wave != 0) return;
+  }
+  if (a.splits > 1) {
+    if (!real) return;
+    // A range without keys leaves no sums; the join weighs it by 0 and does not use them.
+    const int64_t at = ((int64_t)split * a.c.batch * a.c.k_heads + bh) * a.rows + row;
+    float* const p = a.part + at * a.c.head_dim;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + 8 * g + 4 * half;
+        if (begin < end && d < a.c.head_dim)
+          *reinterpret_cast<f4*>(p + d) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+      }
+    if (half == 0) {
+      a.stat[2 * at] = m * mul;
+      a.stat[2 * at + 1] = l;
+    }
+    return;
+  }
+  const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+  T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
+                head * a.c.out_stride[2];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      // A lane holds four values of every eight; the halves trade so that each stores
+      // eight in a row.
+      uint32_t w[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          typedef float f2 __attribute__((ext_vector_type(2)));
+          typedef T t2 __attribute__((ext_vector_type(2)));
+          const f2 pair = {o[db][4 * (g + e) + 2 * j] * scale, o[db][4 * (g + e) + 2 * j + 1] * scale};
+          w[e][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, t2));
+        }
+      const u2 x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const u2 y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      const int d = db * 32 + 8 * (g + half);
+      if (real && d < a.c.head_dim) *reinterpret_cast<u4*>(op + d) = u4{x[0], y[0], x[1], y[1]};
+    }
+  if (a.c.lse && real && half == 0)
+    a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
+        (m * mul + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Smallest and largest document of each tile of keys: a wave a tile. (Looked over by
+// every workgroup instead, the documents of 16384 keys took each some 30 us.)
+__global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int64_t total) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= total) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t b = at / a.doc_tiles, first = (at - b * a.doc_tiles) * a.doc_tile;
+  int lo = INT32_MAX, hi = INT32_MIN;
+  if (lane < a.doc_tile && first + lane < a.c.k_tokens)
+    lo = hi = a.c.doc_k[b * a.c.doc_k_stride + first + lane];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  if (lane == 0) out[at] = int2{lo, hi};
+}
+
+// Joins the ranges of the keys, a workgroup a row: four values a thread, so that D / 4
+// threads read a range's sums and 1024 / D ranges are read at once. Sums are added in a
+// fixed order.
+template <class T>
+__global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
+  __shared__ float weight[64];
+  __shared__ f4 sums[256];
+  const int64_t total = (int64_t)a.c.batch * a.c.k_heads * a.rows;
+  const int64_t at = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int D = a.c.head_dim, quads = D / 4, steps = 256 / quads;
+  const int step = tid / quads, quad = tid - step * quads;
+  // Every wave looks at the statistics of all ranges (at most 64), a lane each.
+  const bool in = lane < a.splits;
+  const float2 st = in ? *reinterpret_cast<const float2*>(a.stat + 2 * (lane * total + at))
+                       : float2{-__builtin_inff(), 0.0f};
+  f4 o = f4{};
+  const float* const p = a.part + at * D + 4 * quad;
+  float top = st.x;
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  const float w = in ? __builtin_amdgcn_exp2f(st.x - base) : 0.0f;
+  float l = w * st.y;
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
+  if (tid < 64) weight[tid] = w;
+  lds_sync();
+  if (step < steps) {
+#pragma unroll 4
+    for (int s = step; s < a.splits; s += steps) {
+      const float ws = weight[s];
+      const f4 x = *reinterpret_cast<const f4*>(p + s * total * D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = ws != 0.0f ? __builtin_fmaf(ws, x[e], o[e]) : o[e];
+    }
+    sums[tid] = o;
+  }
+  lds_sync();
+  const int64_t bh = at / a.rows;
+  const int row = (int)(at - bh * a.rows);
+  const int b = (int)fdiv((uint32_t)bh, a.by_k_heads), kh = (int)(bh - (int64_t)b * a.c.k_heads);
+  const int token = (int)fdiv((uint32_t)row, a.by_group), head = kh * a.group + row - token * a.group;
+  if (tid < quads) {
+    const int n = min(steps, a.splits);
+    for (int s = 1; s < n; ++s) o += sums[s * quads + tid];
+    const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+    T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
+                  head * a.c.out_stride[2];
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o * scale, t4);
+  }
+  if (a.c.lse && tid == 0)
+    a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
+        (top + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+struct TilePick {
+  void (*fn)(AttnArgs);
+  int bytes[2];  // of LDS with two and three buffers
+  int chunk;     // tiles whose documents' ranges it keeps
+};
+
+template <class T, int DP, int KT, int NW, bool SHARED>
+TilePick pick(Shape shape) {
+  return {shape == kPlain ? attention_tile<T, DP, KT, NW, SHARED, kPlain>
+          : shape == kCap ? attention_tile<T, DP, KT, NW, SHARED, kCap>
+                          : attention_tile<T, DP, KT, NW, SHARED, kAny>,
+          {TileL<DP, KT>::bytes(2), TileL<DP, KT>::bytes(3)},
+          TileL<DP, KT>::kChunk};
+}
+
+template <class T>
+TilePick pick(int d, bool shared, Shape shape) {
+  if (shared) {
+    if (d <= 32) return pick<T, 32, 32, 1, true>(shape);
+    if (d <= 64) return pick<T, 64, 32, 1, true>(shape);
+    if (d <= 96) return pick<T, 96, 32, 1, true>(shape);
+    if (d <= 128) return pick<T, 128, 32, 1, true>(shape);
+    return pick<T, 256, 64, 2, true>(shape);
+  }
+  if (d <= 32) return pick<T, 32, 64, 4, false>(shape);
+  if (d <= 64) return pick<T, 64, 64, 4, false>(shape);
+  if (d <= 96) return pick<T, 96, 64, 4, false>(shape);
+  if (d <= 128) return pick<T, 128, 64, 4, false>(shape);
+  return pick<T, 256, 32, 4, false>(shape);
+}
+
+// Up to 32 rows are shared by two waves, which divide the keys; more take 32 each.
+bool shared_rows(const arthip_attention_args& c) {
+  return (int64_t)c.q_tokens * (c.q_heads / c.k_heads) <= 32;
+}
+int tile_rows(const arthip_attention_args& c) { return shared_rows(c) ? 32 : 128; }
+int tile_keys(const arthip_attention_args& c) { return (c.head_dim > 128) == shared_rows(c) ? 64 : 32; }
+
+}  // namespace
+
+AttnPlan attention_plan(const arthip_attention_args& c) {
+  AttnPlan p{1, 1, 0};
+  if (c.batch == 0 || c.q_tokens == 0 || c.q_heads == 0) return p;
+  const int64_t rows = (int64_t)c.q_tokens * (c.q_heads / c.k_heads);
+  const int per = tile_rows(c), kt = tile_keys(c);
+  const int64_t row_tiles = (rows + per - 1) / per;
+  const int64_t items = (int64_t)c.batch * c.k_heads * row_tiles;
+  // Tiles that a row tile can need at most: a window on both sides bounds them.
+  int64_t tiles = (c.k_tokens + kt - 1) / kt;
+  if (c.left >= 0 && c.right >= 0 && c.prefix == nullptr)
+    tiles = std::min<int64_t>(tiles, ((int64_t)c.left + c.right + std::min<int64_t>(c.q_tokens, per)) / kt + 2);
+{ const char* e1 = getenv("S1"); const char* e2 = getenv("S2"); const char* e3 = getenv("S3"); const int64_t n = e1 ? atoi(e1) : 512, t = e2 ? atoi(e2) : 4, lim = e3 ? atoi(e3) : 256; if (items < lim) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({n / items, tiles / t, 64})); }
+  p.range = (int)std::max<int64_t>(1, (tiles + p.splits - 1) / p.splits);
+  if (p.splits > 1)
+    p.workspace = (size_t)p.splits * c.batch * c.k_heads * rows * (c.head_dim + 2) * sizeof(float);
+  if (c.doc_k != nullptr) {
+    const int64_t n = (c.k_tokens + tile_keys(c) - 1) / tile_keys(c);
+    p.workspace += (size_t)(c.doc_k_stride == 0 ? 1 : c.batch) * n * sizeof(int2);
+  }
+  return p;
+}
+
+hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
+  if (c.batch == 0 || c.q_tokens == 0 || c.q_heads == 0) return hipSuccess;
+  AttnArgs a{};
+  a.c = c;
+  a.group = c.q_heads / c.k_heads;
+  a.rows = c.q_tokens * a.group;
+  const bool shared = shared_rows(c);
+  a.row_tiles = (a.rows + tile_rows(c) - 1) / tile_rows(c);
+  const AttnPlan plan = attention_plan(c);
+  a.splits = plan.splits;
+  a.range = plan.range;
+  a.items = c.batch * c.k_heads * a.row_tiles * a.splits;
+  a.by_group = make_fastdiv((uint32_t)a.group);
+  a.by_k_heads = make_fastdiv((uint32_t)c.k_heads);
+  a.by_row_tiles = make_fastdiv((uint32_t)a.row_tiles);
+  a.by_splits = make_fastdiv((uint32_t)a.splits);
+  const int64_t total = (int64_t)c.batch * c.k_heads * a.rows;
+  a.part = static_cast<float*>(c.workspace);
+  if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
+  const bool f16 = c.dtype == ARTHIP_TYPE_F16;
+  const Shape shape = c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
+  const TilePick k = f16 ? pick<_Float16>(c.head_dim, shared, shape) : pick<__bf16>(c.head_dim, shared, shape);
+  if (shape == kCap) {
+    static constexpr double fit[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825, 0.015486690367999443};
+    const double r = (double)c.scale / c.cap;
+    a.cap_reach = (float)(0.6 / r);
+    for (int i = 0; i < 5; ++i) a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
+  }
+  if (c.doc_k != nullptr && c.k_tokens > 0) {
+    a.doc_tile = tile_keys(c);
+    a.doc_tiles = (c.k_tokens + a.doc_tile - 1) / a.doc_tile;
+    int2* const ranges = reinterpret_cast<int2*>(a.splits > 1 ? a.stat + 2 * a.splits * total : a.part);
+    const int64_t n = (int64_t)(c.doc_k_stride == 0 ? 1 : c.batch) * a.doc_tiles;
+    a.doc_ranges = ranges;
+    hipLaunchKernelGGL(attention_docs, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a, ranges, n);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const int64_t table = c.table == nullptr ? 0 : (int64_t)a.group * c.table_len * 4;
+  a.table_lds = table <= kTableBytes;
+  // Three buffers where workgroups are too few to hide each other's loads, or small.
+  const int64_t room = c.head_dim <= 32 ? INT64_MAX : c.head_dim <= 64 ? 512 : 256;
+  a.buffers = a.items <= room ? 3 : 2;
+  if (getenv("BUF")) a.buffers = atoi(getenv("BUF"));
+  // Offsets of a tile's keys from its first one have 31 bits.
+  const int64_t far = std::max(std::abs(c.k_stride[1]), std::abs(c.v_stride[1]));
+  a.wide = c.k_stride[1] < 0 || c.v_stride[1] < 0 || far * 2 * 64 + 512 > INT32_MAX;
+  a.table_bytes = a.table_lds ? (int)(table + 7) / 8 * 8 : 0;
+  const int bytes = k.bytes[a.buffers - 2] + a.table_bytes + (c.doc_k != nullptr ? k.chunk * 8 : 0);
+  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k.fn, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3(shared ? (c.head_dim > 128 ? 128 : 64) : 256), bytes, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(f16 ? attention_join<_Float16> : attention_join<__bf16>,
+                     dim3((unsigned)total), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace arthip

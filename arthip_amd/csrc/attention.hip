@@ -43,8 +43,10 @@ struct AttnArgs {
   int rows;       // rows of a key head: q_tokens * group
   int row_tiles;  // workgroups along the rows
   int splits;     // workgroups along the keys
+  int range;      // tiles of each but the last
   int items;      // batch * k_heads * row_tiles * splits
   int table_lds;  // the tables of a key head's rows are kept in LDS
+  int table_bytes;  // and take these
   int wide;       // keys further apart than 32-bit offsets reach
   FastDiv by_group, by_k_heads, by_row_tiles, by_splits;
   float cap_reach;  // |q.k| up to which the polynomial holds
@@ -98,20 +100,19 @@ __device__ __forceinline__ float halves_sum(float x) {
 // or with bits of the row, so that the 16 rows of a K operand, and the four rows of a
 // transposed V read, lie on different banks. The permutation is in the addresses that
 // the lanes load from.
-template <int DP>
+template <int DP, int KT>  // values of a head, padded; keys of a tile
 struct TileL {
-  static constexpr int KT = DP > 128 ? 32 : 64;  // keys of a tile
   static constexpr int RB = DP <= 32 ? 64 : DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row
   static constexpr int kTile = KT * RB;
-  static constexpr int kV = 2 * kTile;
-  static constexpr int kChunk = 1024;            // tiles whose documents are looked over at once
-  static constexpr int kDoc = kV + 2 * kTile;    // int32 [2][64]
-  static constexpr int kCode = kDoc + 2 * 64 * 4;
-  static constexpr int kTileDocs = kCode + 2 * 64 * 4;   // int2 a tile: its documents' range
-  static constexpr int kAny = kTileDocs + kChunk * 8;    // bit a tile: some key of a row's document
-  static constexpr int kRange = kAny + kChunk / 8;       // int32 [2][16] documents of the waves
-  static constexpr int kTable = kRange + 2 * 16 * 4;  // fp32 [group][table_len], if it fits
-  static constexpr int kBytes = kTable;
+  static constexpr int kChunk = 1024;  // tiles whose documents are looked over at once
+  // After two K tiles and two V tiles:
+  static constexpr int kRange = 0;                   // int32 [2][16] documents of the waves
+  static constexpr int kDoc = kRange + 2 * 16 * 4;   // int32 [2][64]
+  static constexpr int kCode = kDoc + 2 * 64 * 4;    // int32 [2][64]
+  static constexpr int kAny = kCode + 2 * 64 * 4;    // bit a tile: some key of a row's document
+  static constexpr int kTable = kAny + kChunk / 8;   // fp32 [group][table_len], if it fits
+  // and after that, with documents, int2 a tile: its range of them
+  static constexpr int kBytes = 4 * kTile + kTable;
   static __device__ __forceinline__ int k_swizzle(int row) {
     return RB == 64 ? (row >> 2) & 3 : RB == 128 ? (row >> 1) & 7 : RB == 256 ? row & 15 : row & 7;
   }
@@ -132,17 +133,43 @@ __device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
   return rsrc_t{lo, hi & 0xffffu, bytes, 0x00020000u};
 }
 
-// 16 (4) bytes a lane from the buffer to LDS, lane after lane from `to`. Offsets past
-// the buffer bring zeros. The compiler does not see these loads (its own would make
-// every later LDS read wait for them): vm_wait() stands between them and their use.
-__device__ __forceinline__ void load_lds16(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(to), "v"(at), "s"(from), "s"(base)
-               : "memory");
+// Loads from the buffer to LDS, 16 (4) bytes a lane, lane after lane from `to` on: N
+// loads to consecutive KiB. An instruction's constant goes to both addresses, so that M0
+// is set once (a write of M0 waits for the load before it); the caller's `base` of load i
+// has to take those i KiB out. Offsets past the buffer bring zeros. The compiler does not
+// see these loads (its own would make every later LDS read wait for them): vm_wait()
+// stands between them and their use. Nor does it see that they read scalar registers,
+// which a vector instruction (a lane read back from a spill, a first lane) may have
+// written just before: that takes five wait states, the s_nop.
+template <int N>
+__device__ __forceinline__ void load_lds16(rsrc_t from, const uint32_t (&at)[N], const uint32_t (&base)[N],
+                                           uint32_t to) {
+  static_assert(N == 1 || N == 2 || N == 4, "KiB that the constant reaches");
+  if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, %3 offen lds"
+                 :
+                 : "s"(to), "s"(from), "v"(at[0]), "s"(base[0])
+                 : "memory");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, %4 offen lds\n\t"
+        "buffer_load_dwordx4 %3, %1, %5 offen offset:1024 lds"
+        :
+        : "s"(to), "s"(from), "v"(at[0]), "v"(at[1]), "s"(base[0]), "s"(base[1])
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, %6 offen lds\n\t"
+        "buffer_load_dwordx4 %3, %1, %7 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %4, %1, %8 offen offset:2048 lds\n\t"
+        "buffer_load_dwordx4 %5, %1, %9 offen offset:3072 lds"
+        :
+        : "s"(to), "s"(from), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(base[0]), "s"(base[1]),
+          "s"(base[2]), "s"(base[3])
+        : "memory");
 }
 __device__ __forceinline__ void load_lds4(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :
                : "s"(to), "v"(at), "s"(from), "s"(base)
                : "memory");
@@ -168,20 +195,32 @@ __device__ __forceinline__ void ahead() {
 // of cap, slopes, table and a scale that turns their order.
 enum Shape { kPlain, kCap, kAny };
 
-template <class T, int DP, int NW, Shape SHAPE>
+// SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
+// tile's keys; otherwise each holds 32 rows of its own and takes all keys.
+template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
 __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kAny ? 2 : 3) attention_tile(AttnArgs a) {
-  using L = TileL<DP>;
+  using L = TileL<DP, KT>;
   using E = Elem<T>;
   using frag = typename E::frag;
-  constexpr int KT = L::KT, RB = L::RB, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+  constexpr int RB = L::RB, KW = SHARED ? KT / NW : KT, KB = KW / 32, KS = DP / 16, DB = DP / 32;
+  constexpr int ROWS = SHARED ? 32 : 32 * NW;
   constexpr int SEG = L::kTile / 1024;                // loads of a tile, 1 KiB each
   constexpr int LOADS = (SEG + NW - 1) / NW;          // of a wave
   constexpr uint32_t kOob = 0x80000000u;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  constexpr int v_at = 2 * L::kTile;  // V's buffers
+  unsigned char* const more = lds + 2 * v_at;  // what follows them
+  const uint32_t more_base = lds_base + 2 * v_at;
 
-  const int per = (int)gridDim.x >> 3;
-  int item = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);  // one XCD: neighbours share K, V
+  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
+  // stay on one XCD. A single row tile shares nothing, and sequences of different
+  // lengths are then spread over all.
+  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
+  // stay on one XCD. A single row tile shares nothing: its items go round as they come,
+  // one further each round, so that no XCD gets all the first (long) ranges.
+  const int bid = (int)blockIdx.x, per = (int)gridDim.x >> 3;
+  const int item = a.row_tiles == 1 ? (bid & ~7) + ((bid + (bid >> 3)) & 7) : (bid & 7) * per + (bid >> 3);
   if (item >= a.items) return;
   const int ranges = (int)fdiv((uint32_t)item, a.by_splits);
   const int split = item - ranges * a.splits;
@@ -214,9 +253,11 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
     const int64_t p = (int64_t)q_start + token + a.c.right + 1;
     return p < 0 ? 0 : p > kv_len ? kv_len : (int)p;
   };
-  const int first_row = row_tile * 32 * NW;
-  const int last_row = min(first_row + 32 * NW, a.rows) - 1;
-  const int row = first_row + wave * 32 + n;
+  const int first_row = row_tile * ROWS;
+  const int last_row = min(first_row + ROWS, a.rows) - 1;
+  const int w_row = first_row + (SHARED ? 0 : wave * 32);  // the wave's first
+  const int wk = SHARED ? wave * KW : 0;                   // and its first key of a tile
+  const int row = w_row + n;
   const bool real = row <= last_row;
   const int token = token_of(min(row, last_row));
   const int g_head = min(row, last_row) - token * a.group;
@@ -224,10 +265,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   const int lo = low(token), hi = high(token);
   // The wave's and the workgroup's rows together: all see [lo_max, hi_min), some see
   // [lo_min, hi_max). Positions grow with the row.
-  const int wr0 = min(first_row + wave * 32, last_row), wr1 = min(wr0 + 31, last_row);
+  const int wr0 = min(w_row, last_row), wr1 = min(wr0 + 31, last_row);
   const int w_lo_min = low(token_of(wr0)), w_lo_max = low(token_of(wr1));
   const int w_hi_min = high(token_of(wr0)), w_hi_max = high(token_of(wr1));
-  const bool w_real = first_row + wave * 32 <= last_row;
+  const bool w_real = w_row <= last_row;
   const int g_lo_min = low(token_of(first_row)), g_hi_max = high(token_of(last_row));
 
   frag q[KS];
@@ -251,8 +292,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
   const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
   bool hides = false;  // the table has an entry of -inf
-  if (table) {
-    float* const t = reinterpret_cast<float*>(lds + L::kTable);
+  auto load_table = [&]() __attribute__((always_inline)) {
+    float* const t = reinterpret_cast<float*>(more + L::kTable);
     const int len = a.group * a.c.table_len;
     const float* const from = table + (int64_t)kh * len;
     bool h = false;
@@ -261,31 +302,32 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       if (a.table_lds) t[i] = e * kLog2e;
       h = h || e == -__builtin_inff();
     }
-    int* const flag = reinterpret_cast<int*>(lds + L::kRange);
-    if (__any(h) && lane == 0) flag[wave] = 1;
-    if (!__any(h) && lane == 0) flag[wave] = 0;
+    int* const flag = reinterpret_cast<int*>(more + L::kRange);
+    const int found = __any(h);
+    if (lane == 0) flag[wave] = found;
     lds_sync();
-    for (int i = 0; i < NW; ++i) hides = hides || flag[i] != 0;
-    hides = __builtin_amdgcn_readfirstlane(hides);
-  }
+    int all = 0;
+    for (int i = 0; i < NW; ++i) all |= flag[i];
+    hides = scalar(all) != 0;
+  };
 
   // -- the tiles: those of the prefix, then those of the windows ----------------------
   const int pre_tiles = (pre + KT - 1) / KT;
   const int win_first = max(g_lo_min / KT, pre_tiles);
   const int win_end = g_hi_max > g_lo_min ? (g_hi_max + KT - 1) / KT : 0;
   const int count = pre_tiles + max(win_end - win_first, 0);
-  const int begin = (int)((int64_t)count * split / a.splits);
-  const int end = (int)((int64_t)count * (split + 1) / a.splits);
+  const int begin = min(split * a.range, count);
+  const int end = split == a.splits - 1 ? count : min(begin + a.range, count);
   auto tile_of = [&](int i) __attribute__((always_inline)) { return i < pre_tiles ? i : i - pre_tiles + win_first; };
 
   // Documents: the range of a wave's rows, and of the workgroup's.
-  uint64_t* const any = reinterpret_cast<uint64_t*>(lds + L::kAny);
-  int2* const tile_docs = reinterpret_cast<int2*>(lds + L::kTileDocs);
+  uint64_t* const any = reinterpret_cast<uint64_t*>(more + L::kAny);
+  int2* const tile_docs = reinterpret_cast<int2*>(more + L::kTable + a.table_bytes);
   const int2* const doc_ranges =
       doc_k ? a.doc_ranges + (a.c.doc_k_stride == 0 ? 0 : (int64_t)b * a.doc_tiles) : nullptr;
   int w_dmin = dq, w_dmax = dq, dmin = 0, dmax = 0;
   if (doc_k) {
-    int* const range = reinterpret_cast<int*>(lds + L::kRange);
+    int* const range = reinterpret_cast<int*>(more + L::kRange);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {  // a lane past the last row repeats it
       w_dmin = min(w_dmin, __shfl_xor(w_dmin, o));
@@ -313,47 +355,69 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   float m = -__builtin_inff(), l = 0.0f;
 
   // -- staging -------------------------------------------------------------------------
-  // A wave's loads of a tile are NW KiB apart, whole periods of the permutation, so
-  // that one offset a lane serves them all.
   const T* const kp = static_cast<const T*>(a.c.k) + b * a.c.k_stride[0] + kh * a.c.k_stride[2];
   const T* const vp = static_cast<const T*>(a.c.v) + b * a.c.v_stride[0] + kh * a.c.v_stride[2];
-  const int s_row = (wave * 1024 + lane * 16) / RB;
+  const int s_row = (wave * LOADS * 1024 + lane * 16) / RB;  // of the wave's first load; the others follow
   const int s_chunk = lane * 16 % RB / 16;
-  const int k_chunk = s_chunk ^ L::k_swizzle(s_row), v_chunk = s_chunk ^ L::v_swizzle(s_row);
-  const bool k_in = k_chunk * 8 < a.c.head_dim, v_in = v_chunk * 8 < a.c.head_dim;
   const int64_t ks2 = a.c.k_stride[1] * 2, vs2 = a.c.v_stride[1] * 2;  // bytes
-  auto stage = [&](const T* from, int64_t stride, int chunk, bool in, int tile, uint32_t to) __attribute__((always_inline)) {
+  constexpr int STEP = 1024 / RB;  // rows of a load
+  // K's permutation comes round after 16 rows (8 of 512 bytes), V's after 4.
+  constexpr int KP = (RB == 512 ? 8 : 16) / STEP < LOADS ? (RB == 512 ? 8 : 16) / STEP : LOADS;
+  constexpr int VP = 4 / STEP < 1 ? 1 : 4 / STEP < LOADS ? 4 / STEP : LOADS;
+  uint32_t k_off[KP], v_off[VP];  // a lane's offsets, but for the rows between its loads
+  auto offset_of = [&](int chunk, int64_t stride) __attribute__((always_inline)) {
+    return chunk * 8 < a.c.head_dim ? (uint32_t)(s_row * (int)stride + chunk * 16) : kOob;
+  };
+#pragma unroll
+  for (int i = 0; i < KP; ++i) k_off[i] = offset_of(s_chunk ^ L::k_swizzle(s_row + i * STEP), ks2);
+#pragma unroll
+  for (int i = 0; i < VP; ++i) v_off[i] = offset_of(s_chunk ^ L::v_swizzle(s_row + i * STEP), vs2);
+  constexpr int BACK = 3 * 1024;  // what buffers begin before the tile, for the constants' sake
+  auto stage = [&](const T* from, int64_t stride, auto offset, auto swizzle, int tile, uint32_t to)
+      __attribute__((always_inline)) {
+    if (SEG % NW != 0 && wave * LOADS >= SEG) return;
     const char* const p = reinterpret_cast<const char*>(from) + (int64_t)tile * KT * stride;
     const int left = kv_len - tile * KT;  // keys past the length come as zeros
+    const uint32_t to_wave = to + wave * LOADS * 1024;
+    if (!a.wide) {
+      constexpr int N = LOADS < 4 ? LOADS : 4;
+      static_assert(LOADS % N == 0, "whole blocks of loads");
+      const rsrc_t r = buffer_of(p - BACK, 0x7fffffffu);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      if (SEG % NW != 0 && wave + i * NW >= SEG) break;
-      const int row = s_row + i * NW * 1024 / RB;
-      if (a.wide) {
-        // 32-bit offsets would wrap: a buffer of its own for every key of the load.
-        constexpr int keys = RB < 1024 ? 1024 / RB : 1;
-#pragma unroll 1
-        for (int r = 0; r < keys; ++r) {
-          const int first = (wave * 1024 + i * NW * 1024) / RB + r;
-          const rsrc_t one = buffer_of(p + first * stride, 0x7fffffffu);
-          if (row == first)
-            load_lds16(one, in && row < left ? chunk * 16u : kOob, 0, to + (wave + i * NW) * 1024);
+      for (int i = 0; i < LOADS; i += N) {
+        uint32_t at[N], base[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          base[j] = (i + j) * STEP * (uint32_t)stride + (BACK - j * 1024);
+          at[j] = left >= KT || s_row + (i + j) * STEP < left ? offset(i + j) : kOob;
         }
-      } else {
-        const uint32_t at = (uint32_t)(row * (int)stride + chunk * 16);
-        load_lds16(buffer_of(p, 0x7fffffffu), in && row < left ? at : kOob, 0, to + (wave + i * NW) * 1024);
+        load_lds16<N>(r, at, base, to_wave + i * 1024);
+      }
+    } else {
+      // 32-bit offsets would wrap: a buffer of its own for every key.
+#pragma unroll 1
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = s_row + i * STEP;
+        const int chunk = s_chunk ^ swizzle(row);
+        const uint32_t at[1] = {chunk * 8 < a.c.head_dim && row < left ? chunk * 16u : kOob}, base[1] = {0};
+#pragma unroll 1
+        for (int k = 0; k < STEP; ++k) {
+          const int key = (wave * LOADS + i) * STEP + k;
+          const rsrc_t far = buffer_of(p + key * stride, 0x7fffffffu);
+          if (row == key) load_lds16<1>(far, at, base, to_wave + i * 1024);
+        }
       }
     }
   };
   auto stage_k = [&](int buf, int tile) __attribute__((always_inline)) {
-    stage(kp, ks2, k_chunk, k_in, tile, lds_base + buf * L::kTile);
+    stage(kp, ks2, [&](int i) { return k_off[i % KP]; }, L::k_swizzle, tile, lds_base + buf * L::kTile);
     if (doc_k && wave == 0)
-      load_lds4(buffer_of(doc_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, lds_base + L::kDoc + buf * 256);
+      load_lds4(buffer_of(doc_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kDoc + buf * 256);
     if (code_k && wave == NW - 1)
-      load_lds4(buffer_of(code_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, lds_base + L::kCode + buf * 256);
+      load_lds4(buffer_of(code_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kCode + buf * 256);
   };
   auto stage_v = [&](int buf, int tile) __attribute__((always_inline)) {
-    stage(vp, vs2, v_chunk, v_in, tile, lds_base + L::kV + buf * L::kTile);
+    stage(vp, vs2, [&](int i) { return v_off[i % VP]; }, L::v_swizzle, tile, lds_base + v_at + buf * L::kTile);
   };
 
   // -- the products --------------------------------------------------------------------
@@ -363,13 +427,13 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   typedef __attribute__((address_space(3))) const frag lds_frag;
   typedef __attribute__((address_space(3))) s4 lds_s4;
   lds_byte* const lds0 = (lds_byte*)lds;
-  const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
+  const uint32_t k_lane = (wk + n) * RB + (half ^ L::k_swizzle(n)) * 16;
   const int v_row = 4 * half + (lane & 15) / 4;
   const uint32_t v_lane =
-      v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+      (wk + v_row) * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
 
   f16v s[KB];        // scores of the current tile, key block by key block
-  frag p[KT / 16];   // weights of the previous tile
+  frag p[KW / 16];   // weights of the previous tile
   auto scores = [&](int buf) __attribute__((always_inline)) {
     lds_byte* const at = lds0 + buf * L::kTile;
 #pragma unroll
@@ -387,7 +451,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   };
   bool odd = false;  // a tile that a row does not see whole holds an infinity or NaN in V
   auto values = [&](int buf, bool look) __attribute__((always_inline)) {
-    lds_byte* const at = lds0 + L::kV + buf * L::kTile;
+    lds_byte* const at = lds0 + v_at + buf * L::kTile;
     lds_byte* v[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) v[db] = at + (v_lane ^ (db * 64));
@@ -396,7 +460,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       // NaN survive: 0 times the tile tells whether it has any.
       f16v z = f16v{};
 #pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)
+      for (int kk = 0; kk < KW / 16; ++kk)
 #pragma unroll
         for (int db = 0; db < DB; ++db) z = E::mma(v_frag(v[db], kk), frag{}, z);
       float t = 0.0f;
@@ -405,16 +469,16 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       odd = odd || t != 0.0f;
     }
 #pragma unroll
-    for (int kk = 0; kk < KT / 16; ++kk)
+    for (int kk = 0; kk < KW / 16; ++kk)
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
-    ahead<KT / 16 * DB, 2>();
+    ahead<KW / 16 * DB, 2>();
   };
   // The same key by key, each added only to the rows that weigh it.
   auto values_apart = [&](int buf) __attribute__((always_inline)) {
-    lds_byte* const at = lds0 + L::kV + buf * L::kTile;
+    lds_byte* const at = lds0 + v_at + buf * L::kTile;
 #pragma unroll
-    for (int kk = 0; kk < KT / 16; ++kk)
+    for (int kk = 0; kk < KW / 16; ++kk)
 #pragma unroll 1
       for (int key = 0; key < 16; ++key) {
         const int of = (key >> 2) & 1, j = (key & 3) | ((key >> 1) & 4);  // its half and element
@@ -434,8 +498,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   };
 
   // -- scores to weights -----------------------------------------------------------------
-  auto weights = [&](int buf, int tile, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
-    const int key0 = tile * KT + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
+  auto weights = [&](int buf, int k0, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
+    const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
     const float unit = a.c.cap > 0 ? 1.0f : a.c.scale * kLog2e;  // what scores are still to be scaled by
     if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
       float far = 0.0f;
@@ -473,7 +537,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
     if constexpr (SHAPE == kAny) {
       // The loops below are whole loops a branch: a uniform branch inside would be taken
       // for every score.
-      const int4* const codes = reinterpret_cast<const int4*>(lds + L::kCode + buf * 256) + half;
+      const int4* const codes = reinterpret_cast<const int4*>(more + L::kCode + buf * 256 + wk * 4) + half;
       auto bias = [&](auto coded, auto add) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -508,7 +572,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
         const int last = a.c.table_len - 1, zero = a.c.table_zero;
         if (a.table_lds) {
           // Entries in the base of 2.
-          const float* const t = reinterpret_cast<const float*>(lds + L::kTable) + g_head * a.c.table_len;
+          const float* const t = reinterpret_cast<const float*>(more + L::kTable) + g_head * a.c.table_len;
           auto add = [&](float x, int diff) __attribute__((always_inline)) {
             return __builtin_fmaf(x, by, t[min(max(diff + zero, 0), last)]);
           };
@@ -539,7 +603,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       }
     }
     if (partial) {
-      const bool whole = tile * KT + KT <= pre || (tile * KT >= w_lo_max && tile * KT + KT <= w_hi_min);
+      const bool whole = k0 + KW <= pre || (k0 >= w_lo_max && k0 + KW <= w_hi_min);
       if (!whole) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -556,7 +620,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb][r] = away != 0.0f ? -__builtin_inff() : s[kb][r];
       } else if (doc_k) {
-        const int4* const docs = reinterpret_cast<const int4*>(lds + L::kDoc + buf * 256) + half;
+        const int4* const docs = reinterpret_cast<const int4*>(more + L::kDoc + buf * 256 + wk * 4) + half;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -600,7 +664,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       }
     l += sum;  // this half's keys; the halves are added at the end
 #pragma unroll
-    for (int kk = 0; kk < KT / 16; ++kk) {
+    for (int kk = 0; kk < KW / 16; ++kk) {
       const f16v x = s[kk / 2];
       p[kk] = kk & 1
                   ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
@@ -611,7 +675,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   // -- the walk ------------------------------------------------------------------------
   // One barrier a tile. While tile t's scores and the previous tile's values are
   // multiplied, K of the next tile and V of this one are on their way to the buffers
-  // that the last barrier freed.
+  // that the last barrier freed. (Three buffers, two tiles' loads on their way, were no
+  // faster anywhere, and take the LDS of a second workgroup.)
   auto walk = [&](auto apart) __attribute__((always_inline)) {
     const int chunk = doc_k ? L::kChunk : max(end - begin, 1);
     for (int c0 = begin; c0 < end; c0 += chunk) {
@@ -642,19 +707,20 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
         return scalar(min(i, c1));
       };
       int i = next(c0);
-      int buf = 0;
-      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
-      if (i >= c1) continue;
-      stage_k(0, tile_of(i));
+      const bool nothing = i >= c1;
+      if (!nothing) stage_k(0, tile_of(i));
+      if (table && !decltype(apart)::value && c0 == begin) load_table();
+      if (nothing) continue;
       vm_wait();
       lds_sync();
+      int buf = 0;
+      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
       while (true) {
-        const bool more = i < c1;
-        const int tile = tile_of(i), k0 = tile * KT, k1 = k0 + KT;
+        const bool live = i < c1;
+        const int tile = tile_of(i), k0 = tile * KT + wk, k1 = k0 + KW;
         bool seen = false, partial = false;
-        int t_dmin = w_dmin, t_dmax = w_dmin;
-        int following = i;
-        if (more) {
+        int t_dmin = w_dmin, t_dmax = w_dmin, following = i;
+        if (live) {
           if (doc_k) {
             const int2 r = tile_docs[i - c0];
             t_dmin = scalar(r.x);
@@ -663,7 +729,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
           following = next(i + 1);
           if (following < c1) stage_k(buf ^ 1, tile_of(following));
           stage_v(buf, tile);
-          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min)) && (!doc_k || (t_dmax >= w_dmin && t_dmin <= w_dmax));
+          seen = w_real && (k0 < pre || (k0 < w_hi_max && k1 > w_lo_min)) &&
+                 (!doc_k || (t_dmax >= w_dmin && t_dmin <= w_dmax));
           partial = !(k1 <= pre || (k0 >= w_lo_max && k1 <= w_hi_min)) ||
                     (doc_k && !(t_dmin == t_dmax && w_dmin == w_dmax));
         }
@@ -674,8 +741,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
           else
             values(buf ^ 1, look);
         }
-        if (!more) break;
-        if (seen) weights(buf, tile, partial, t_dmin, t_dmax);
+        if (!live) break;
+        if (seen) weights(buf, k0, partial, t_dmin, t_dmax);
         has = seen;
         look = partial || hides;
         vm_wait();
@@ -688,7 +755,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
   walk(std::false_type{});
   // A workgroup that met such a tile starts over and takes the keys one by one.
   {
-    int* const flag = reinterpret_cast<int*>(lds + L::kRange);
+    int* const flag = reinterpret_cast<int*>(more + L::kRange);
     lds_sync();
     if (lane == 0) flag[wave] = 0;
     if (odd) flag[wave] = 1;
@@ -706,8 +773,43 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
 
   // -- results -------------------------------------------------------------------------
   l = halves_sum(l);
+  if constexpr (SHARED) {
+    // The other waves hand their sums to the first, one after the other.
+    float* const box = reinterpret_cast<float*>(lds);
+    for (int w = 1; w < NW; ++w) {
+      lds_sync();  // the tiles, and the last wave's sums, have been used
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f4*>(box + ((i * 4 + g) * 64 + lane) * 4) =
+                f4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+        box[DB * 1024 + lane] = m;
+        box[DB * 1024 + 64 + lane] = l;
+      }
+      lds_sync();
+      if (wave == 0) {
+        const float m2 = box[DB * 1024 + lane], next = fmaxf(m, m2);
+        const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+        const float f2 = m2 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m2 - next) * mul);
+        m = next;
+        l = l * f1 + box[DB * 1024 + 64 + lane] * f2;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f4 x = *reinterpret_cast<const f4*>(box + ((i * 4 + g) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][4 * g + e] = o[i][4 * g + e] * f1 + x[e] * f2;
+          }
+      }
+    }
+    if (wave != 0) return;
+  }
   if (a.splits > 1) {
     if (!real) return;
+    // A range without keys leaves no sums; the join weighs it by 0 and does not use them.
     const int64_t at = ((int64_t)split * a.c.batch * a.c.k_heads + bh) * a.rows + row;
     float* const p = a.part + at * a.c.head_dim;
 #pragma unroll
@@ -715,7 +817,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = db * 32 + 8 * g + 4 * half;
-        if (d < a.c.head_dim)
+        if (begin < end && d < a.c.head_dim)
           *reinterpret_cast<f4*>(p + d) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
       }
     if (half == 0) {
@@ -771,82 +873,124 @@ __global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int
   if (lane == 0) out[at] = int2{lo, hi};
 }
 
-// Joins the ranges of the keys: a wave a row.
+// Joins the ranges of the keys, a workgroup a row: four values a thread, so that D / 4
+// threads read a range's sums and 1024 / D ranges are read at once. Sums are added in a
+// fixed order.
 template <class T>
 __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
+  __shared__ float weight[64];
+  __shared__ f4 sums[256];
   const int64_t total = (int64_t)a.c.batch * a.c.k_heads * a.rows;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= total) return;
-  const int lane = threadIdx.x & 63;
-  const int D = a.c.head_dim;
-  float top = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.stat[2 * (s * total + at)]);
-  const float base = top == -__builtin_inff() ? 0.0f : top;
-  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(a.stat[2 * (s * total + at)] - base);
-    l = __builtin_fmaf(w, a.stat[2 * (s * total + at) + 1], l);
-    const float* const p = a.part + (s * total + at) * D;
+  const int64_t at = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int D = a.c.head_dim, quads = D / 4, steps = 256 / quads;
+  const int step = tid / quads, quad = tid - step * quads;
+  // Every wave looks at the statistics of all ranges (at most 64), a lane each.
+  const bool in = lane < a.splits;
+  const float2 st = in ? *reinterpret_cast<const float2*>(a.stat + 2 * (lane * total + at))
+                       : float2{-__builtin_inff(), 0.0f};
+  f4 o = f4{};
+  const float* const p = a.part + at * D + 4 * quad;
+  float top = st.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < D) o[i] = __builtin_fmaf(w, p[lane + 64 * i], o[i]);
+  for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  const float w = in ? __builtin_amdgcn_exp2f(st.x - base) : 0.0f;
+  float l = w * st.y;
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
+  if (tid < 64) weight[tid] = w;
+  lds_sync();
+  if (step < steps) {
+#pragma unroll 4
+    for (int s = step; s < a.splits; s += steps) {
+      const float ws = weight[s];
+      const f4 x = *reinterpret_cast<const f4*>(p + s * total * D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = ws != 0.0f ? __builtin_fmaf(ws, x[e], o[e]) : o[e];
+    }
+    sums[tid] = o;
   }
+  lds_sync();
   const int64_t bh = at / a.rows;
   const int row = (int)(at - bh * a.rows);
   const int b = (int)fdiv((uint32_t)bh, a.by_k_heads), kh = (int)(bh - (int64_t)b * a.c.k_heads);
   const int token = (int)fdiv((uint32_t)row, a.by_group), head = kh * a.group + row - token * a.group;
-  const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-  T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
-                head * a.c.out_stride[2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < D) op[lane + 64 * i] = to_elem<T>(o[i] * scale);
-  if (a.c.lse && lane == 0)
+  if (tid < quads) {
+    const int n = min(steps, a.splits);
+    for (int s = 1; s < n; ++s) o += sums[s * quads + tid];
+    const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+    T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
+                  head * a.c.out_stride[2];
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o * scale, t4);
+  }
+  if (a.c.lse && tid == 0)
     a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
         (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 struct TilePick {
   void (*fn)(AttnArgs);
-  int bytes;
+  int threads;
+  int bytes;  // of LDS
+  int chunk;  // tiles whose documents' ranges it keeps
 };
 
-template <class T, int DP, int NW>
+template <class T, int DP, int KT, int NW, bool SHARED>
 TilePick pick(Shape shape) {
-  return {shape == kPlain ? attention_tile<T, DP, NW, kPlain>
-          : shape == kCap ? attention_tile<T, DP, NW, kCap>
-                          : attention_tile<T, DP, NW, kAny>,
-          TileL<DP>::kBytes};
+  return {shape == kPlain ? attention_tile<T, DP, KT, NW, SHARED, kPlain>
+          : shape == kCap ? attention_tile<T, DP, KT, NW, SHARED, kCap>
+                          : attention_tile<T, DP, KT, NW, SHARED, kAny>,
+          NW * 64, TileL<DP, KT>::kBytes, TileL<DP, KT>::kChunk};
 }
 
 template <class T>
-TilePick pick(int d, Shape shape) {
-  if (d <= 32) return pick<T, 32, 4>(shape);
-  if (d <= 64) return pick<T, 64, 4>(shape);
-  if (d <= 96) return pick<T, 96, 4>(shape);
-  if (d <= 128) return pick<T, 128, 4>(shape);
-  return pick<T, 256, 4>(shape);
+TilePick pick(int d, bool shared, Shape shape) {
+  if (shared) {
+    if (d <= 32) return pick<T, 32, 32, 1, true>(shape);
+    if (d <= 64) return pick<T, 64, 32, 1, true>(shape);
+    if (d <= 96) return pick<T, 96, 32, 1, true>(shape);
+    if (d <= 128) return pick<T, 128, 32, 1, true>(shape);
+    return pick<T, 256, 64, 2, true>(shape);
+  }
+  if (d <= 32) return pick<T, 32, 64, 4, false>(shape);
+  if (d <= 64) return pick<T, 64, 64, 4, false>(shape);
+  if (d <= 96) return pick<T, 96, 64, 4, false>(shape);
+  if (d <= 128) return pick<T, 128, 64, 4, false>(shape);
+  return pick<T, 256, 32, 4, false>(shape);
 }
 
-// Keys of a tile (TileL::KT).
-int tile_keys(int d) { return d > 128 ? 32 : 64; }
-
-int waves_of(const arthip_attention_args&) { return 4; }
+// Up to 32 rows are shared by two waves, which divide the keys; more take 32 each.
+bool shared_rows(const arthip_attention_args& c) {
+  return (int64_t)c.q_tokens * (c.q_heads / c.k_heads) <= 32;
+}
+int tile_rows(const arthip_attention_args& c) { return shared_rows(c) ? 32 : 128; }
+int tile_keys(const arthip_attention_args& c) { return (c.head_dim > 128) == shared_rows(c) ? 64 : 32; }
 
 }  // namespace
 
 AttnPlan attention_plan(const arthip_attention_args& c) {
-  AttnPlan p{1, 0};
+  AttnPlan p{1, 1, 0};
   if (c.batch == 0 || c.q_tokens == 0 || c.q_heads == 0) return p;
   const int64_t rows = (int64_t)c.q_tokens * (c.q_heads / c.k_heads);
-  const int per = 32 * waves_of(c);
-  const int64_t items = (int64_t)c.batch * c.k_heads * ((rows + per - 1) / per);
-  const int64_t tiles = (c.k_tokens + 63) / 64;
-  if (items < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, tiles / 4, 64}));
+  const int per = tile_rows(c), kt = tile_keys(c);
+  const int64_t row_tiles = (rows + per - 1) / per;
+  const int64_t items = (int64_t)c.batch * c.k_heads * row_tiles;
+  // Tiles that a row tile can need at most: a window on both sides bounds them.
+  int64_t tiles = (c.k_tokens + kt - 1) / kt;
+  if (c.left >= 0 && c.right >= 0 && c.prefix == nullptr)
+    tiles = std::min<int64_t>(tiles, ((int64_t)c.left + c.right + std::min<int64_t>(c.q_tokens, per)) / kt + 2);
+  // Ranges: enough workgroups for the chip, of at least four tiles. One-wave workgroups
+  // fit a CU four at a time; those of four waves two.
+  const int64_t want = shared_rows(c) ? 1024 : 512;
+  if (items < want / 2)
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + items - 1) / items, tiles / 4, 64}));
+  p.range = (int)std::max<int64_t>(1, (tiles + p.splits - 1) / p.splits);
   if (p.splits > 1)
     p.workspace = (size_t)p.splits * c.batch * c.k_heads * rows * (c.head_dim + 2) * sizeof(float);
   if (c.doc_k != nullptr) {
-    const int64_t n = (c.k_tokens + tile_keys(c.head_dim) - 1) / tile_keys(c.head_dim);
+    const int64_t n = (c.k_tokens + tile_keys(c) - 1) / tile_keys(c);
     p.workspace += (size_t)(c.doc_k_stride == 0 ? 1 : c.batch) * n * sizeof(int2);
   }
   return p;
@@ -858,9 +1002,11 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.c = c;
   a.group = c.q_heads / c.k_heads;
   a.rows = c.q_tokens * a.group;
-  const int nw = waves_of(c);
-  a.row_tiles = (a.rows + 32 * nw - 1) / (32 * nw);
-  a.splits = attention_plan(c).splits;
+  const bool shared = shared_rows(c);
+  a.row_tiles = (a.rows + tile_rows(c) - 1) / tile_rows(c);
+  const AttnPlan plan = attention_plan(c);
+  a.splits = plan.splits;
+  a.range = plan.range;
   a.items = c.batch * c.k_heads * a.row_tiles * a.splits;
   a.by_group = make_fastdiv((uint32_t)a.group);
   a.by_k_heads = make_fastdiv((uint32_t)c.k_heads);
@@ -871,7 +1017,7 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
   const bool f16 = c.dtype == ARTHIP_TYPE_F16;
   const Shape shape = c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
-  TilePick k = f16 ? pick<_Float16>(c.head_dim, shape) : pick<__bf16>(c.head_dim, shape);
+  const TilePick k = f16 ? pick<_Float16>(c.head_dim, shared, shape) : pick<__bf16>(c.head_dim, shared, shape);
   if (shape == kCap) {
     static constexpr double fit[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825, 0.015486690367999443};
     const double r = (double)c.scale / c.cap;
@@ -879,7 +1025,7 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
     for (int i = 0; i < 5; ++i) a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
   }
   if (c.doc_k != nullptr && c.k_tokens > 0) {
-    a.doc_tile = tile_keys(c.head_dim);
+    a.doc_tile = tile_keys(c);
     a.doc_tiles = (c.k_tokens + a.doc_tile - 1) / a.doc_tile;
     int2* const ranges = reinterpret_cast<int2*>(a.splits > 1 ? a.stat + 2 * a.splits * total : a.part);
     const int64_t n = (int64_t)(c.doc_k_stride == 0 ? 1 : c.batch) * a.doc_tiles;
@@ -890,18 +1036,19 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   }
   const int64_t table = c.table == nullptr ? 0 : (int64_t)a.group * c.table_len * 4;
   a.table_lds = table <= kTableBytes;
-  if (a.table_lds) k.bytes += (int)table;
   // Offsets of a tile's keys from its first one have 31 bits.
   const int64_t far = std::max(std::abs(c.k_stride[1]), std::abs(c.v_stride[1]));
   a.wide = c.k_stride[1] < 0 || c.v_stride[1] < 0 || far * 2 * 64 + 512 > INT32_MAX;
+  a.table_bytes = a.table_lds ? (int)(table + 7) / 8 * 8 : 0;
+  const int bytes = k.bytes + a.table_bytes + (c.doc_k != nullptr ? k.chunk * 8 : 0);
   hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, k.bytes);
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k.fn, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3(64 * nw), k.bytes, s, a);
+  hipLaunchKernelGGL(k.fn, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3((unsigned)k.threads), bytes, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   hipLaunchKernelGGL(f16 ? attention_join<_Float16> : attention_join<__bf16>,
-                     dim3((unsigned)((total + 3) / 4)), dim3(256), 0, s, a);
+                     dim3((unsigned)total), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -34,6 +34,7 @@ hipError_t launch_attention(const arthip_attention_args& a, hipStream_t s);
 // How attention divides its work (attention.hip).
 struct AttnPlan {
   int splits;         // ranges of the keys, each its own workgroup; joined by a second kernel
+  int range;          // tiles of each
   size_t workspace;   // bytes
 };
 AttnPlan attention_plan(const arthip_attention_args& a);
