@@ -1041,8 +1041,10 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.wide = c.k_stride[1] < 0 || c.v_stride[1] < 0 || far * 2 * 64 + 512 > INT32_MAX;
   a.table_bytes = a.table_lds ? (int)(table + 7) / 8 * 8 : 0;
   const int bytes = k.bytes + a.table_bytes + (c.doc_k != nullptr ? k.chunk * 8 : 0);
-  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn),
-                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  hipError_t e = hipSuccess;
+  if (bytes > 65536)  // what a kernel may have without asking
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(k.fn, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3((unsigned)k.threads), bytes, s, a);
   e = hipGetLastError();

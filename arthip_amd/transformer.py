@@ -32,38 +32,52 @@ def _need(ok: bool, text: str) -> None:
         raise EngineError(text)
 
 
-def _call(fn, args, stream: int) -> None:
-    if fn(ctypes.byref(args), stream) != 0:
+# What a call's shapes, strides, types and options come to (checked arguments with all
+# pointers empty), so that the next call of the same kind only fills in pointers: a call
+# takes some 8 us instead of 18. Nothing in it depends on a tensor's address or contents.
+_plans: dict = {}
+_PLANS = 512
+
+
+def _keep(key, plan):
+    if len(_plans) >= _PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _tensor(name: str, t) -> None:
+    _need(t is None or isinstance(t, torch.Tensor), f"{name} must be a tensor")
+
+
+def _call(fn, args, device, stream) -> None:
+    """Enqueues on the tensors' device, on its current stream or the one given."""
+    index = device.index
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(ctypes.byref(args), stream)
+    if rc != 0:
         raise EngineError(_lib.last_error() or f"{fn.__name__} failed")
 
 
-class _On:
-    """The device and stream of a call: the tensors' device is made current, and
-    tensors made inside belong to the stream."""
-
-    def __init__(self, device, stream):
-        self.stream = stream
-        self._guards = []
-        if device.index != torch.cuda.current_device():
-            self._guards.append(torch.cuda.device(device))
-        if stream is not None:
-            self._guards.append(torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)))
-        self._device = device
-
-    def __enter__(self):
-        for g in self._guards:
-            g.__enter__()
-        if self.stream is None:
-            self.stream = torch._C._cuda_getCurrentRawStream(self._device.index)
-        return self.stream
-
-    def __exit__(self, *exc):
-        for g in reversed(self._guards):
-            g.__exit__(*exc)
+def _empty(shape, dtype, device, stream):
+    """A result or workspace that belongs to the call's stream."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _check(name: str, t, device, dtype, dim: int | None = None) -> None:
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a tensor on a GPU")
+    _need(t.is_cuda, f"{name} must be a tensor on a GPU")
     _need(t.device == device, f"{name} is on another device")
     _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     _need(dim is None or t.dim() == dim, f"{name} must have {dim} dimensions")
@@ -123,58 +137,69 @@ def rope_axes(q, k, pos, plan: RopePlan, *, q_out=None, k_out=None, inverse: boo
     """Queries [B, L, Hq, D] and keys [B, L, Hk, D] (either may be None) turned by int32
     positions [axes, B, L] (or [axes, L], the same for every batch item). Returns
     (q_out, k_out), new contiguous tensors unless given; q_out=q turns in place."""
+    for name, t in (("q", q), ("k", k), ("pos", pos), ("q_out", q_out), ("k_out", k_out)):
+        _tensor("rope_axes: " + name, t)
+    key = ("rope", _sig(q), _sig(k), _sig(pos), _sig(q_out), _sig(k_out), plan.n, plan.n_axes, plan.pairs,
+           plan.packed.device, inverse)
+    template = _plans.get(key) or _keep(key, _rope_plan(q, k, pos, plan, q_out, k_out, inverse))
+    a = _lib.RopeArgs.from_buffer_copy(template)
+    device = pos.device
+    if q is not None:
+        if q_out is None:
+            q_out = _empty(q.shape, q.dtype, device, stream)
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        if k_out is None:
+            k_out = _empty(k.shape, k.dtype, device, stream)
+        a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
+    a.pos, a.packed = pos.data_ptr(), plan.packed.data_ptr()
+    _call(_lib.lib().arthip_rope_axes, a, device, stream)
+    return q_out, k_out
+
+
+def _contiguous(shape) -> tuple:
+    strides, n = [], 1
+    for size in reversed(shape):
+        strides.append(n)
+        n *= max(size, 1)
+    return tuple(reversed(strides))
+
+
+def _rope_plan(q, k, pos, plan, q_out, k_out, inverse) -> bytes:
     x = q if q is not None else k
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, "rope_axes: q or k must be a tensor on a GPU")
+    _need(x is not None and x.is_cuda, "rope_axes: q or k must be a tensor on a GPU")
     _need(x.dtype in _TYPES, f"rope_axes: unsupported type {x.dtype}")
     _need(x.dim() == 4, "rope_axes: q and k must have 4 dimensions")
+    _need(pos is not None, "rope_axes: pos must be a tensor")
     batch, tokens, _, dim = x.shape
     _check("pos", pos, x.device, torch.int32)
     _need(tuple(pos.shape) in ((plan.n_axes, batch, tokens), (plan.n_axes, tokens)),
           "rope_axes: pos must be [axes, B, L] or [axes, L]")
     _need(plan.packed.device == x.device, "rope_axes: the plan is on another device")
-    lib = _lib.lib()
     a = _lib.RopeArgs()
-    with _On(x.device, stream) as s:
-        outs = []
-        for name, t, out in (("q", q, q_out), ("k", k, k_out)):
-            if t is None:
-                outs.append(None)
-                continue
-            _check(name, t, x.device, x.dtype, 4)
-            _need(t.shape[0] == batch and t.shape[1] == tokens and t.shape[3] == dim,
-                  "rope_axes: q and k must agree in batch, tokens and head_dim")
-            _inner(name, t)
-            if out is None:
-                out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            else:
-                _check(name + "_out", out, x.device, x.dtype, 4)
-                _need(out.shape == t.shape, f"rope_axes: {name}_out must have {name}'s shape")
-                _inner(name + "_out", out)
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_out", out.data_ptr())
-            setattr(a, name + "_heads", t.shape[2])
-            setattr(a, name + "_stride", t.stride()[:3])
-            setattr(a, name + "_out_stride", out.stride()[:3])
-            outs.append(out)
-        a.pos = pos.data_ptr()
-        st = pos.stride()
-        a.pos_stride = st if pos.dim() == 3 else (st[0], 0, st[1])
-        a.packed = plan.packed.data_ptr()
-        a.n_freq, a.dtype, a.pairs, a.inverse = plan.n, _TYPES[x.dtype], plan.pairs, bool(inverse)
-        a.batch, a.tokens, a.head_dim = batch, tokens, dim
-        _call(lib.arthip_rope_axes, a, s)
-    return tuple(outs)
+    for name, t, out in (("q", q, q_out), ("k", k, k_out)):
+        if t is None:
+            _need(out is None, f"rope_axes: {name}_out without {name}")
+            continue
+        _check(name, t, x.device, x.dtype, 4)
+        _need(t.shape[0] == batch and t.shape[1] == tokens and t.shape[3] == dim,
+              "rope_axes: q and k must agree in batch, tokens and head_dim")
+        _inner(name, t)
+        if out is not None:
+            _check(name + "_out", out, x.device, x.dtype, 4)
+            _need(out.shape == t.shape, f"rope_axes: {name}_out must have {name}'s shape")
+            _inner(name + "_out", out)
+        setattr(a, name + "_heads", t.shape[2])
+        setattr(a, name + "_stride", t.stride()[:3])
+        setattr(a, name + "_out_stride", (_contiguous(t.shape) if out is None else out.stride())[:3])
+    st = pos.stride()
+    a.pos_stride = st if pos.dim() == 3 else (st[0], 0, st[1])
+    a.n_freq, a.dtype, a.pairs, a.inverse = plan.n, _TYPES[x.dtype], plan.pairs, bool(inverse)
+    a.batch, a.tokens, a.head_dim = batch, tokens, dim
+    return bytes(a)
 
 
 # -- attention ------------------------------------------------------------------------
-
-def _per_token(name: str, t, device, batch: int, tokens: int):
-    """(pointer, batch stride) of int32 values [B, L] or [L]."""
-    _check(name, t, device, torch.int32)
-    _need(tuple(t.shape) in ((batch, tokens), (tokens,)), f"attention: {name} must be [B, L] or [L]")
-    _inner(name, t)
-    return t.data_ptr(), t.stride(0) if t.dim() == 2 else 0
-
 
 def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: bool = False,
               window=(None, None), q_start=None, kv_len=None, prefix=None, docs=None, codes=None,
@@ -187,7 +212,54 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     (queries', keys'), [B, L] or [L]; slopes is fp32 [Hq], table fp32 [Hq, n]. Returns
     out, or (out, lse) with lse fp32 [B, Hq, Lq]. Without ``workspace`` (uint8) a call
     that needs one makes it."""
-    _need(isinstance(q, torch.Tensor) and q.is_cuda, "attention: q must be a tensor on a GPU")
+    window = tuple(window)
+    doc_q, doc_k = docs or (None, None)
+    code_q, code_k = codes or (None, None)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _need(isinstance(t, torch.Tensor), f"attention: {name} must be a tensor on a GPU")
+    key = ("attention", _sig(q), _sig(k), _sig(v), scale, cap, causal, window, _sig(out), return_lse)
+    plain = (q_start is None and kv_len is None and prefix is None and docs is None and codes is None
+             and slopes is None and table is None)
+    if not plain:
+        more = (q_start, kv_len, prefix, doc_q, doc_k, code_q, code_k, slopes, table)
+        for t in more:
+            _tensor("attention: an option", t)
+        key += tuple(_sig(t) for t in more) + (table_zero,)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix, docs,
+                                          codes, slopes, table, table_zero, out))
+    template, need = plan
+    a = _lib.AttentionArgs.from_buffer_copy(template)
+    device = q.device
+    if out is None:
+        out = _empty(q.shape, q.dtype, device, stream)
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    lse = None
+    if return_lse:
+        lse = _empty((q.shape[0], q.shape[2], q.shape[1]), torch.float32, device, stream)
+        a.lse = lse.data_ptr()
+    if not plain:
+        for name, t in zip(("q_start", "kv_len", "prefix", "doc_q", "doc_k", "code_q", "code_k", "slopes",
+                            "table"), more):
+            if t is not None:
+                setattr(a, name, t.data_ptr())
+    if workspace is None and need > 0:
+        workspace = _empty((need,), torch.uint8, device, stream)
+    elif workspace is not None:
+        _tensor("attention: workspace", workspace)
+        _check("workspace", workspace, device, torch.uint8, 1)
+        _inner("workspace", workspace)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _call(_lib.lib().arthip_attention, a, device, stream)
+    return (out, lse) if return_lse else out
+
+
+def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix, docs, codes, slopes, table,
+                    table_zero, out):
+    """(checked arguments without pointers, bytes of workspace)."""
+    _need(q.is_cuda, "attention: q must be a tensor on a GPU")
     _need(q.dtype in (torch.float16, torch.bfloat16), f"attention: unsupported type {q.dtype}")
     device = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -203,64 +275,54 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
             _check(name, t, device, torch.int32)
             _need(tuple(t.shape) == (batch,) and t.is_contiguous(),
                   f"attention: {name} must be contiguous [B]")
-            setattr(a, name, t.data_ptr())
     for name, pair in (("doc", docs), ("code", codes)):
-        if pair is not None:
-            _need(len(pair) == 2, f"attention: {name}s is a pair of tensors (queries', keys')")
-            for side, t, tokens in (("q", pair[0], q_tokens), ("k", pair[1], k_tokens)):
-                ptr, stride = _per_token(f"{name}_{side}", t, device, batch, tokens)
-                setattr(a, f"{name}_{side}", ptr)
-                setattr(a, f"{name}_{side}_stride", stride)
+        if pair is None:
+            continue
+        _need(len(pair) == 2 and pair[0] is not None and pair[1] is not None,
+              f"attention: {name}s is a pair of tensors (queries', keys')")
+        for side, t, tokens in (("q", pair[0], q_tokens), ("k", pair[1], k_tokens)):
+            _check(f"{name}_{side}", t, device, torch.int32)
+            _need(tuple(t.shape) in ((batch, tokens), (tokens,)),
+                  f"attention: {name}_{side} must be [B, L] or [L]")
+            _inner(f"{name}_{side}", t)
+            setattr(a, f"{name}_{side}", 16)  # any address: which arrays there are decides the workspace
+            setattr(a, f"{name}_{side}_stride", t.stride(0) if t.dim() == 2 else 0)
     if slopes is not None:
         _check("slopes", slopes, device, torch.float32)
         _need(tuple(slopes.shape) == (q_heads,) and slopes.is_contiguous(),
               "attention: slopes must be contiguous [Hq]")
-        a.slopes = slopes.data_ptr()
     if table is not None:
         _check("table", table, device, torch.float32, 2)
         _need(table.shape[0] == q_heads and table.is_contiguous(),
               "attention: table must be contiguous [Hq, n]")
         _need(table.shape[1] > 0, "attention: table without entries")
-        a.table, a.table_len, a.table_zero = table.data_ptr(), table.shape[1], int(table_zero)
+        a.table_len, a.table_zero = table.shape[1], int(table_zero)
     left, right = window
     _need(not causal or right in (None, 0), "attention: causal and a window to the right")
     for side in (left, right):
         _need(side is None or side >= 0, "attention: a window counts keys")
     a.left = -1 if left is None else int(left)
     a.right = 0 if causal else -1 if right is None else int(right)
+    if prefix is not None:
+        a.prefix = 16
     a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     a.cap = float(cap)
     a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.dtype, a.batch, a.q_tokens, a.k_tokens = _TYPES[q.dtype], batch, q_tokens, k_tokens
     a.q_heads, a.k_heads, a.head_dim = q_heads, k_heads, dim
-    lib = _lib.lib()
-    with _On(device, stream) as s:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        else:
-            _check("out", out, device, q.dtype, 4)
-            _need(out.shape == q.shape, "attention: out must have q's shape")
-            _inner("out", out)
-        a.out, a.out_stride = out.data_ptr(), out.stride()[:3]
-        lse = None
-        if return_lse:
-            lse = torch.empty((batch, q_heads, q_tokens), dtype=torch.float32, device=device)
-            a.lse = lse.data_ptr()
-        need = lib.arthip_attention_workspace(ctypes.byref(a))
-        if need > 0 and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        if workspace is not None:
-            _check("workspace", workspace, device, torch.uint8, 1)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        _call(lib.arthip_attention, a, s)
-    return (out, lse) if return_lse else out
+    if out is not None:
+        _tensor("attention: out", out)
+        _check("out", out, device, q.dtype, 4)
+        _need(out.shape == q.shape, "attention: out must have q's shape")
+        _inner("out", out)
+    a.out_stride = (_contiguous(q.shape) if out is None else out.stride())[:3]
+    return bytes(a), _lib.lib().arthip_attention_workspace(ctypes.byref(a))
 
 
 # -- norms around a block ----------------------------------------------------------------
 
 def _spread(name: str, t, shape, device, dtype):
-    """(pointer, batch and token stride) of a tensor that broadcasts to [B, L, C]."""
+    """Batch and token stride of a tensor that broadcasts to [B, L, C]."""
     _check(name, t, device, dtype)
     dims = tuple(t.shape)
     _need(1 <= len(dims) <= 3 and dims[-1] == shape[-1]
@@ -268,7 +330,7 @@ def _spread(name: str, t, shape, device, dtype):
           f"gated_norm: {name} must broadcast to [B, L, C]")
     _inner(name, t)
     strides = (0,) * (3 - len(dims)) + tuple(st if n > 1 else 0 for n, st in zip(dims, t.stride()))
-    return t.data_ptr(), strides[:2]
+    return strides[:2]
 
 
 def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None, gate=None,
@@ -282,8 +344,42 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     fp32. Returns (new residual, h); residual_out=residual updates in place, and without y
     and with a residual_scale of 1 the residual is returned as it is. h has y's type, or
     ``dtype`` where there is no y."""
-    _need(isinstance(residual, torch.Tensor) and residual.is_cuda,
-          "gated_norm: residual must be a tensor on a GPU")
+    _need(isinstance(residual, torch.Tensor), "gated_norm: residual must be a tensor on a GPU")
+    given = (residual, y, gate, mod_scale, mod_shift, post_weight, post_bias, pre_weight, pre_bias,
+             residual_out, h)
+    for t in given:
+        _tensor("gated_norm: an argument", t)
+    key = ("norm", *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in given], post, pre,
+           gate_act, residual_scale, branch_scale, eps, dtype)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _norm_plan(given, post, pre, gate_act, residual_scale, branch_scale, eps, dtype))
+    template, dtype, new_residual, new_h = plan
+    a = _lib.NormArgs.from_buffer_copy(template)
+    device = residual.device
+    a.residual = residual.data_ptr()
+    new = residual
+    if new_residual or residual_out is not None:
+        new = residual_out if residual_out is not None else _empty(residual.shape, residual.dtype, device, stream)
+        a.residual_out = new.data_ptr()
+    if new_h:
+        h = _empty(residual.shape, dtype, device, stream)
+    if h is not None:
+        a.h = h.data_ptr()
+    for name, t in zip(("y", "gate", "mod_scale", "mod_shift", "post_weight", "post_bias", "pre_weight",
+                        "pre_bias"), given[1:9]):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    if a.residual_out or a.h:
+        _call(_lib.lib().arthip_gated_norm, a, device, stream)
+    return new, h
+
+
+def _norm_plan(given, post, pre, gate_act, residual_scale, branch_scale, eps, dtype):
+    """(checked arguments without pointers, type of h, whether a call makes a residual and an h)."""
+    (residual, y, gate, mod_scale, mod_shift, post_weight, post_bias, pre_weight, pre_bias, residual_out,
+     h) = given
+    _need(residual.is_cuda, "gated_norm: residual must be a tensor on a GPU")
     _need(residual.dtype in _TYPES, f"gated_norm: unsupported type {residual.dtype}")
     _need(residual.dim() == 3, "gated_norm: residual must have 3 dimensions")
     _need(post in _NORMS and pre in _NORMS, "gated_norm: a norm is 'rms', 'layer' or None")
@@ -292,7 +388,7 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
           "gated_norm: gate or post norm without y")
     device, shape = residual.device, tuple(residual.shape)
     if y is not None:
-        _need(isinstance(y, torch.Tensor) and y.dtype in _TYPES, "gated_norm: unsupported type of y")
+        _need(y.dtype in _TYPES, "gated_norm: unsupported type of y")
         _need(dtype in (None, y.dtype), "gated_norm: h has y's type")
         dtype = y.dtype
     elif dtype is None:
@@ -300,51 +396,35 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     _need(dtype in _TYPES, f"gated_norm: unsupported type {dtype}")
     a = _lib.NormArgs()
     _inner("residual", residual)
-    a.residual, a.residual_stride = residual.data_ptr(), residual.stride()[:2]
+    a.residual_stride = residual.stride()[:2]
     if y is not None:
         _check("y", y, device, dtype, 3)
         _need(tuple(y.shape) == shape, "gated_norm: y must have the residual's shape")
         _inner("y", y)
-        a.y, a.y_stride = y.data_ptr(), y.stride()[:2]
-    if gate is not None:
-        a.gate, a.gate_stride = _spread("gate", gate, shape, device, dtype)
-    if mod_scale is not None:
-        a.mod_scale, a.mod_scale_stride = _spread("mod_scale", mod_scale, shape, device, dtype)
-    if mod_shift is not None:
-        a.mod_shift, a.mod_shift_stride = _spread("mod_shift", mod_shift, shape, device, dtype)
+        a.y_stride = y.stride()[:2]
+    for name, t in (("gate", gate), ("mod_scale", mod_scale), ("mod_shift", mod_shift)):
+        if t is not None:
+            setattr(a, name + "_stride", _spread(name, t, shape, device, dtype))
     for name, t in (("post_weight", post_weight), ("post_bias", post_bias),
                     ("pre_weight", pre_weight), ("pre_bias", pre_bias)):
         if t is not None:
             _check(name, t, device, torch.float32, 1)
             _need(t.shape[0] == shape[2] and t.is_contiguous(),
                   f"gated_norm: {name} must be contiguous [C]")
-            setattr(a, name, t.data_ptr())
     a.dtype, a.residual_dtype = _TYPES[dtype], _TYPES[residual.dtype]
     a.post, a.pre, a.gate_act = _NORMS[post], _NORMS[pre], _GATES[gate_act]
     a.batch, a.tokens, a.channels = shape
     a.eps, a.residual_scale, a.branch_scale = float(eps), float(residual_scale), float(branch_scale)
-    lib = _lib.lib()
-    with _On(device, stream) as s:
-        if residual_out is None:
-            if y is None and residual_scale == 1.0:
-                new = residual
-            else:
-                new = torch.empty(shape, dtype=residual.dtype, device=device)
-        else:
-            new = residual_out
-            _check("residual_out", new, device, residual.dtype, 3)
-            _need(tuple(new.shape) == shape, "gated_norm: residual_out must have the residual's shape")
-            _inner("residual_out", new)
-        if new is not residual or residual_out is not None:
-            a.residual_out, a.residual_out_stride = new.data_ptr(), new.stride()[:2]
-        if pre not in (None, "none") or mod_scale is not None or mod_shift is not None or h is not None:
-            if h is None:
-                h = torch.empty(shape, dtype=dtype, device=device)
-            else:
-                _check("h", h, device, dtype, 3)
-                _need(tuple(h.shape) == shape, "gated_norm: h must have the residual's shape")
-                _inner("h", h)
-            a.h, a.h_stride = h.data_ptr(), h.stride()[:2]
-        if a.residual_out or a.h:
-            _call(lib.arthip_gated_norm, a, s)
-    return new, h
+    if residual_out is not None:
+        _check("residual_out", residual_out, device, residual.dtype, 3)
+        _need(tuple(residual_out.shape) == shape, "gated_norm: residual_out must have the residual's shape")
+        _inner("residual_out", residual_out)
+    a.residual_out_stride = (_contiguous(shape) if residual_out is None else residual_out.stride())[:2]
+    if h is not None:
+        _check("h", h, device, dtype, 3)
+        _need(tuple(h.shape) == shape, "gated_norm: h must have the residual's shape")
+        _inner("h", h)
+    a.h_stride = (_contiguous(shape) if h is None else h.stride())[:2]
+    normed = pre not in (None, "none") or mod_scale is not None or mod_shift is not None
+    return (bytes(a), dtype, residual_out is None and (y is not None or residual_scale != 1.0),
+            h is None and normed)
