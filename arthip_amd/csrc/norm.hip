@@ -25,12 +25,29 @@ struct NormArgs {
   int row_threads;  // threads of a row: 64, 128, .. 1024
   int rows;         // rows of a workgroup
   float inv_c;
+  FastDiv by_tokens;
 };
 
+// Sum over a wave, the same in every lane: exchanges between lanes inside the vector unit
+// (quads, half rows, rows of 16, then halves), a few clocks each where a shuffle through
+// the LDS path takes its whole latency.
+template <int DPP>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), DPP, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  x = add_dpp<0xb1>(x);   // lanes 1 0 3 2
+  x = add_dpp<0x4e>(x);   // lanes 2 3 0 1
+  x = add_dpp<0x141>(x);  // half rows mirrored
+  x = add_dpp<0x140>(x);  // rows mirrored
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const u2 r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  x = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+  u = __builtin_bit_cast(uint32_t, x);
+  const u2 h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t h0 = h[0], h1 = h[1];
+  return __builtin_bit_cast(float, h0) + __builtin_bit_cast(float, h1);
 }
 
 // Sum over the row's threads. Every thread of the workgroup calls it the same number
@@ -52,87 +69,126 @@ struct RowSum {
   }
 };
 
+// The channels of a thread. Its last chunk, where it would reach past the row, ends with
+// the row instead and repeats `skip` channels of the chunk before it: read and written
+// whole, with the same values, and left out of the sums (all eight where the thread has
+// no chunk).
 template <int N>
-__device__ __forceinline__ void normalize(float (&x)[N][kNormVec], const bool (&live)[N],
-                                          const int (&chan)[N], const NormArgs& a, int kind,
-                                          const float* weight, const float* bias, RowSum& sum) {
-  if (kind == ARTHIP_NORM_NONE) return;
-  const int C = a.c.channels;
-  if (kind == ARTHIP_NORM_LAYER) {
-    float t = 0.0f;
+struct Chans {
+  int at[N], skip[N];
+};
+
+// A thread's channels of a row. Rows of fewer than eight go value by value.
+template <bool FULL, class T, int N>
+__device__ __forceinline__ void load_rows(const T* p, const Chans<N>& c, int C, float (&x)[N][kNormVec]) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+  for (int n = 0; n < N; ++n) {
+    if (!FULL && c.skip[n] >= kNormVec) {
 #pragma unroll
-      for (int i = 0; i < kNormVec; ++i) t += x[n][i];
-    const float mean = sum(t) * a.inv_c;
+      for (int i = 0; i < kNormVec; ++i) x[n][i] = 0.0f;
+    } else if (FULL || C >= kNormVec) {
+      load_chunk<T, kNormVec>(p + c.at[n], x[n]);
+    } else {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int i = 0; i < kNormVec; ++i) x[n][i] = i >= c.skip[n] ? static_cast<float>(p[c.at[n] + i]) : 0.0f;
+    }
+  }
+}
+template <bool FULL, class T, int N>
+__device__ __forceinline__ void store_rows(T* p, const Chans<N>& c, int C, const float (&x)[N][kNormVec]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (!FULL && c.skip[n] >= kNormVec) continue;
+    if (FULL || C >= kNormVec) {
+      store_chunk<T, kNormVec>(p + c.at[n], x[n]);
+    } else {
 #pragma unroll
       for (int i = 0; i < kNormVec; ++i)
-        x[n][i] = live[n] && chan[n] + i < C ? x[n][i] - mean : 0.0f;
+        if (i >= c.skip[n]) p[c.at[n] + i] = to_elem<T>(x[n][i]);
+    }
   }
+}
+
+// Sum of f over a thread's channels.
+template <bool FULL, int N, class F>
+__device__ __forceinline__ float add_up(const float (&x)[N][kNormVec], const Chans<N>& c, F f) {
   float t = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (FULL || !__any(c.skip[n] > 0)) {
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) t = f(x[n][i], t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) t = i >= c.skip[n] ? f(x[n][i], t) : t;
+    }
+  }
+  return t;
+}
+
+template <bool FULL, int N>
+__device__ __forceinline__ void normalize(float (&x)[N][kNormVec], const Chans<N>& c, const NormArgs& a, int kind,
+                                          const float* weight, const float* bias, RowSum& sum) {
+  if (kind == ARTHIP_NORM_NONE) return;
+  if (kind == ARTHIP_NORM_LAYER) {
+    const float mean = sum(add_up<FULL>(x, c, [](float v, float t) { return t + v; })) * a.inv_c;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) x[n][i] -= mean;
+  }
+  const float squares = add_up<FULL>(x, c, [](float v, float t) { return __builtin_fmaf(v, v, t); });
+  const float r = 1.0f / __builtin_sqrtf(sum(squares) * a.inv_c + a.c.eps);
+  float w[N][kNormVec];
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < kNormVec; ++i) t = __builtin_fmaf(x[n][i], x[n][i], t);
-  const float r = 1.0f / __builtin_sqrtf(sum(t) * a.inv_c + a.c.eps);
+    for (int i = 0; i < kNormVec; ++i) x[n][i] *= r;
+  if (weight) {
+    load_rows<FULL>(weight, c, a.c.channels, w);
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (!live[n]) continue;
-    const int left = C - chan[n];
-    float w[kNormVec], b[kNormVec];
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) x[n][i] *= w[n][i];
+  }
+  if (bias) {
+    load_rows<FULL>(bias, c, a.c.channels, w);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) x[n][i] += w[n][i];
+  }
+}
+
+// tanh without branches: near 0, where 1 - 2 / (exp(2 x) + 1) has no digits left, x times
+// a polynomial of x^2 (a Chebyshev fit up to 0.6, off by less than 8e-8).
+__device__ __forceinline__ float tanh_of(float x) {
+  const float z = x * x;
+  float p = 0.01548669f;
+  p = __builtin_fmaf(p, z, -0.05210962f);
+  p = __builtin_fmaf(p, z, 0.13310358f);
+  p = __builtin_fmaf(p, z, -0.33332323f);
+  p = __builtin_fmaf(p, z, 0.99999993f);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__expf(2.0f * x) + 1.0f);
+  return fabsf(x) < 0.6f ? x * p : far;
+}
+
+__device__ __forceinline__ void gates(float (&g)[kNormVec], int act) {
+  if (act == ARTHIP_GATE_TANH) {
+#pragma unroll
+    for (int i = 0; i < kNormVec; ++i) g[i] = tanh_of(g[i]);
+  } else if (act != ARTHIP_GATE_NONE) {
 #pragma unroll
     for (int i = 0; i < kNormVec; ++i) {
-      w[i] = 1.0f;
-      b[i] = 0.0f;
+      const float s = 1.0f / (1.0f + __expf(-g[i]));
+      g[i] = act == ARTHIP_GATE_SILU ? g[i] * s : s;
     }
-    if (left >= kNormVec) {
-      if (weight) load_chunk<float, kNormVec>(weight + chan[n], w);
-      if (bias) load_chunk<float, kNormVec>(bias + chan[n], b);
-    } else {
-      for (int i = 0; i < kNormVec; ++i) {
-        if (weight && i < left) w[i] = weight[chan[n] + i];
-        if (bias && i < left) b[i] = bias[chan[n] + i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kNormVec; ++i) x[n][i] = __builtin_fmaf(x[n][i] * r, w[i], b[i]);
   }
 }
 
-// Eight channels of a row, or the `left` ones that it still has (zeros after them).
-template <class T>
-__device__ __forceinline__ void load_row(const T* p, int left, float (&x)[kNormVec]) {
-  if (left >= kNormVec) {
-    load_chunk<T, kNormVec>(p, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kNormVec; ++i) x[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void store_row(T* p, int left, const float (&x)[kNormVec]) {
-  if (left >= kNormVec) {
-    store_chunk<T, kNormVec>(p, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kNormVec; ++i)
-      if (i < left) p[i] = to_elem<T>(x[i]);
-  }
-}
-
-__device__ __forceinline__ float gate_of(float g, int act) {
-  switch (act) {
-    case ARTHIP_GATE_SIGMOID: return 1.0f / (1.0f + __expf(-g));
-    case ARTHIP_GATE_TANH: return tanhf(g);
-    case ARTHIP_GATE_SILU: return g / (1.0f + __expf(-g));
-    default: return g;
-  }
-}
-
-template <class T, class TR, int N>
+// FULL: every thread's chunks are whole, as where the channels are a power of two from
+// 512 on; the checks of the other kind are a third of the vector work.
+template <class T, class TR, int N, bool FULL>
 __global__ void __launch_bounds__(1024) gated_norm(NormArgs a) {
   __shared__ float part[32];
   const int tid = threadIdx.x;
@@ -144,90 +200,80 @@ __global__ void __launch_bounds__(1024) gated_norm(NormArgs a) {
   // A slot past the last row computes the last one again, so that every thread meets
   // every barrier, and writes nothing.
   const uint32_t row = static_cast<uint32_t>(real ? index : total - 1);
-  const uint32_t b = row / static_cast<uint32_t>(a.c.tokens);
+  const uint32_t b = fdiv(row, a.by_tokens);
   const uint32_t t = row - b * static_cast<uint32_t>(a.c.tokens);
   const int C = a.c.channels;
   RowSum sum{part, tid >> 6, slot * (a.row_threads >> 6), a.row_threads >> 6, 0};
-
   auto at = [&](const int64_t (&stride)[2]) { return b * stride[0] + t * stride[1]; };
 
-  bool live[N];
-  int chan[N];
-  float r[N][kNormVec], y[N][kNormVec];
-  const TR* const res = static_cast<const TR*>(a.c.residual) + at(a.c.residual_stride);
+  Chans<N> c;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    chan[n] = (n * a.row_threads + lane) * kNormVec;
-    live[n] = chan[n] < C;
-#pragma unroll
-    for (int i = 0; i < kNormVec; ++i) r[n][i] = y[n][i] = 0.0f;
-    if (live[n]) load_row(res + chan[n], C - chan[n], r[n]);
+    const int first = (n * a.row_threads + lane) * kNormVec;
+    c.skip[n] = FULL ? 0 : min(max(first + kNormVec - C, 0), kNormVec);
+    // Below 0 where a row has fewer than eight channels: the values skipped are not touched.
+    c.at[n] = first - c.skip[n];
   }
+  float r[N][kNormVec], y[N][kNormVec];
+  load_rows<FULL>(static_cast<const TR*>(a.c.residual) + at(a.c.residual_stride), c, C, r);
+  // In place, no thread may write channels that another one has yet to read.
+  if (!FULL && sum.waves > 1) lds_sync();
   if (a.c.y) {
-    const T* const yp = static_cast<const T*>(a.c.y) + at(a.c.y_stride);
+    load_rows<FULL>(static_cast<const T*>(a.c.y) + at(a.c.y_stride), c, C, y);
+    float g[N][kNormVec];
+    if (a.c.gate) {
+      load_rows<FULL>(static_cast<const T*>(a.c.gate) + at(a.c.gate_stride), c, C, g);
+#pragma unroll
+      for (int n = 0; n < N; ++n) gates(g[n], a.c.gate_act);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < kNormVec; ++i) g[n][i] = 1.0f;
+    }
+    normalize<FULL>(y, c, a, a.c.post, a.c.post_weight, a.c.post_bias, sum);
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      if (live[n]) load_row(yp + chan[n], C - chan[n], y[n]);
-    normalize<N>(y, live, chan, a, a.c.post, a.c.post_weight, a.c.post_bias, sum);
-    const T* const gp = a.c.gate ? static_cast<const T*>(a.c.gate) + at(a.c.gate_stride) : nullptr;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if (!live[n]) continue;
-      float g[kNormVec];
-      if (gp) {
-        load_row(gp + chan[n], C - chan[n], g);
-#pragma unroll
-        for (int i = 0; i < kNormVec; ++i) g[i] = gate_of(g[i], a.c.gate_act);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kNormVec; ++i) g[i] = 1.0f;
-      }
 #pragma unroll
       for (int i = 0; i < kNormVec; ++i)
-        r[n][i] = chan[n] + i < C ? __builtin_fmaf(a.c.branch_scale * g[i], y[n][i],
-                                                   a.c.residual_scale * r[n][i])
-                                  : 0.0f;
-    }
+        r[n][i] = __builtin_fmaf(a.c.branch_scale * g[n][i], y[n][i], a.c.residual_scale * r[n][i]);
   } else {
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < kNormVec; ++i) r[n][i] *= a.c.residual_scale;
   }
-  if (a.c.residual_out && real) {
-    TR* const out = static_cast<TR*>(a.c.residual_out) + at(a.c.residual_out_stride);
+  if (a.c.residual_out && real)
+    store_rows<FULL>(static_cast<TR*>(a.c.residual_out) + at(a.c.residual_out_stride), c, C, r);
+  if (!a.c.h) return;
+  normalize<FULL>(r, c, a, a.c.pre, a.c.pre_weight, a.c.pre_bias, sum);
+  if (a.c.mod_scale) {
+    float m[N][kNormVec];
+    load_rows<FULL>(static_cast<const T*>(a.c.mod_scale) + at(a.c.mod_scale_stride), c, C, m);
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      if (live[n]) store_row(out + chan[n], C - chan[n], r[n]);
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) r[n][i] = __builtin_fmaf(r[n][i], m[n][i], r[n][i]);
   }
-  if (!a.c.h) return;
-  normalize<N>(r, live, chan, a, a.c.pre, a.c.pre_weight, a.c.pre_bias, sum);
-  const T* const sp =
-      a.c.mod_scale ? static_cast<const T*>(a.c.mod_scale) + at(a.c.mod_scale_stride) : nullptr;
-  const T* const fp =
-      a.c.mod_shift ? static_cast<const T*>(a.c.mod_shift) + at(a.c.mod_shift_stride) : nullptr;
-  T* const h = static_cast<T*>(a.c.h) + at(a.c.h_stride);
+  if (a.c.mod_shift) {
+    float m[N][kNormVec];
+    load_rows<FULL>(static_cast<const T*>(a.c.mod_shift) + at(a.c.mod_shift_stride), c, C, m);
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (!live[n]) continue;
-    float m[kNormVec];
-    if (sp) {
-      load_row(sp + chan[n], C - chan[n], m);
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int i = 0; i < kNormVec; ++i) r[n][i] = __builtin_fmaf(r[n][i], m[i], r[n][i]);
-    }
-    if (fp) {
-      load_row(fp + chan[n], C - chan[n], m);
-#pragma unroll
-      for (int i = 0; i < kNormVec; ++i) r[n][i] += m[i];
-    }
-    if (real) store_row(h + chan[n], C - chan[n], r[n]);
+      for (int i = 0; i < kNormVec; ++i) r[n][i] += m[n][i];
   }
+  if (real) store_rows<FULL>(static_cast<T*>(a.c.h) + at(a.c.h_stride), c, C, r);
+}
+
+template <class T, class TR, bool FULL>
+void (*norm_kernel(int n))(NormArgs) {
+  return n == 1 ? gated_norm<T, TR, 1, FULL> : n == 2 ? gated_norm<T, TR, 2, FULL> : gated_norm<T, TR, 4, FULL>;
 }
 
 template <class T, class TR>
-void (*norm_kernel(int n))(NormArgs) {
-  return n == 1 ? gated_norm<T, TR, 1> : n == 2 ? gated_norm<T, TR, 2> : gated_norm<T, TR, 4>;
+void (*norm_kernel(int n, bool full))(NormArgs) {
+  return full ? norm_kernel<T, TR, true>(n) : norm_kernel<T, TR, false>(n);
 }
 
 }  // namespace
@@ -237,19 +283,22 @@ hipError_t launch_norm(const arthip_norm_args& c, hipStream_t s) {
   NormArgs a{};
   a.c = c;
   a.inv_c = 1.0f / static_cast<float>(c.channels);
+  a.by_tokens = make_fastdiv((uint32_t)c.tokens);
   const int chunks = (c.channels + kNormVec - 1) / kNormVec;
   a.row_threads = 64;
   while (a.row_threads < 1024 && a.row_threads * 2 < chunks) a.row_threads *= 2;
   const int n = (chunks + a.row_threads - 1) / a.row_threads;
+  const int held = n == 3 ? 4 : n;  // chunks a thread holds
+  const bool full = c.channels == a.row_threads * held * kNormVec;
   a.rows = a.row_threads < 256 ? 256 / a.row_threads : 1;
   const int64_t total = static_cast<int64_t>(c.batch) * c.tokens;
   if (total < a.rows) a.rows = 1;
   const int64_t blocks = (total + a.rows - 1) / a.rows;
   const bool wide = c.residual_dtype == ARTHIP_TYPE_F32;
   void (*fn)(NormArgs) =
-      c.dtype == ARTHIP_TYPE_F32   ? norm_kernel<float, float>(n)
-      : c.dtype == ARTHIP_TYPE_F16 ? (wide ? norm_kernel<_Float16, float>(n) : norm_kernel<_Float16, _Float16>(n))
-                                   : (wide ? norm_kernel<__bf16, float>(n) : norm_kernel<__bf16, __bf16>(n));
+      c.dtype == ARTHIP_TYPE_F32   ? norm_kernel<float, float>(n, full)
+      : c.dtype == ARTHIP_TYPE_F16 ? (wide ? norm_kernel<_Float16, float>(n, full) : norm_kernel<_Float16, _Float16>(n, full))
+                                   : (wide ? norm_kernel<__bf16, float>(n, full) : norm_kernel<__bf16, __bf16>(n, full));
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3((unsigned)(a.rows * a.row_threads)), 0, s, a);
   return hipGetLastError();
 }

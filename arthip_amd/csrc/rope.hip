@@ -21,6 +21,8 @@ namespace arthip {
 namespace {
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeBatch = 4;            // heads that a thread loads at once
+constexpr int64_t kRopeFill = 512 * 1024;  // threads that fill the chip twice over
 
 struct RopeArgs {
   arthip_rope_args c;
@@ -91,42 +93,38 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes(RopeArgs a) {
   T* const qo = static_cast<T*>(a.c.q_out) + b * a.c.q_out_stride[0] + t * a.c.q_out_stride[1];
   T* const ko = static_cast<T*>(a.c.k_out) + b * a.c.k_out_stride[0] + t * a.c.k_out_stride[1];
   const int heads = a.c.q_heads + a.c.k_heads;
-  for (int head = group; head < heads; head += a.groups) {
-    const bool is_q = head < a.c.q_heads;
-    const int h = is_q ? head : head - a.c.q_heads;
-    const T* const in = is_q ? q + h * a.c.q_stride[2] : k + h * a.c.k_stride[2];
-    T* const out = is_q ? qo + h * a.c.q_out_stride[2] : ko + h * a.c.k_out_stride[2];
-    float x[V], y[V];
-    load_chunk<T, V>(in + first, x);
-    load_chunk<T, V>(in + second, y);
-    if (turn) {
-      if constexpr (PAIRS) {
-        // x and y are the first and second half of the unit's pairs.
+  // Heads in batches: all loads of a batch, then its turns and stores.
+  for (int head = group; head < heads; head += kRopeBatch * a.groups) {
+    float x[kRopeBatch][V], y[kRopeBatch][V];
+    T* out[kRopeBatch];
+#pragma unroll
+    for (int j = 0; j < kRopeBatch; ++j) {
+      const int hj = head + j * a.groups;
+      if (hj >= heads) break;
+      const bool is_q = hj < a.c.q_heads;
+      const int h = is_q ? hj : hj - a.c.q_heads;
+      const T* const in = is_q ? q + h * a.c.q_stride[2] : k + h * a.c.k_stride[2];
+      out[j] = is_q ? qo + h * a.c.q_out_stride[2] : ko + h * a.c.k_out_stride[2];
+      load_chunk<T, V>(in + first, x[j]);
+      load_chunk<T, V>(in + second, y[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kRopeBatch; ++j) {
+      if (head + j * a.groups >= heads) break;
+      if (turn) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float* const half = i < (V + 1) / 2 ? x : y;
-          if constexpr (V == 1) {
-            const float u = x[0], w = y[0];
-            x[0] = u * cs[0] - w * sn[0];
-            y[0] = w * cs[0] + u * sn[0];
-          } else {
-            const int j = 2 * i % V;
-            const float u = half[j], w = half[j + 1];
-            half[j] = u * cs[i] - w * sn[i];
-            half[j + 1] = w * cs[i] + u * sn[i];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float u = x[i], w = y[i];
-          x[i] = u * cs[i] - w * sn[i];
-          y[i] = w * cs[i] + u * sn[i];
+          // Pairs (2f, 2f + 1) are neighbours in the unit's 2 V values, x then y.
+          float& u = PAIRS ? (2 * i < V ? x[j][2 * i % V] : y[j][2 * i % V]) : x[j][i];
+          float& w = PAIRS ? (2 * i + 1 < V ? x[j][(2 * i + 1) % V] : y[j][(2 * i + 1) % V]) : y[j][i];
+          const float u0 = u, w0 = w;
+          u = u0 * cs[i] - w0 * sn[i];
+          w = w0 * cs[i] + u0 * sn[i];
         }
       }
+      store_chunk<T, V>(out[j] + first, x[j]);
+      store_chunk<T, V>(out[j] + second, y[j]);
     }
-    store_chunk<T, V>(out + first, x);
-    store_chunk<T, V>(out + second, y);
   }
 }
 
@@ -160,7 +158,11 @@ hipError_t launch_rope(const arthip_rope_args& c, hipStream_t s) {
   a.turned = c.n_freq / v;
   a.units = a.turned + copied / (2 * v);
   const int64_t tokens = static_cast<int64_t>(c.batch) * c.tokens;
-  a.groups = std::min(heads, kRopeThreads / a.units);
+  // A thread for every head where threads are few; where they fill the chip anyway, one
+  // for up to four heads, which shares the angles among them.
+  a.groups = heads;
+  while (a.groups * kRopeBatch > heads && tokens * a.units * (a.groups / 2) >= kRopeFill) a.groups = (a.groups + 1) / 2;
+  a.groups = std::min(a.groups, kRopeThreads / a.units);
   a.per_token = a.units * a.groups;
   a.per_block = kRopeThreads / a.per_token;
   const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;

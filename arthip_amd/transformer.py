@@ -47,11 +47,11 @@ def _keep(key, plan):
 
 
 def _sig(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
-def _tensor(name: str, t) -> None:
-    _need(t is None or isinstance(t, torch.Tensor), f"{name} must be a tensor")
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise EngineError(f"a {type(t).__name__} where a tensor on a GPU belongs")
+    return t.shape, t.stride(), t.dtype, t.device
 
 
 def _call(fn, args, device, stream) -> None:
@@ -68,8 +68,14 @@ def _call(fn, args, device, stream) -> None:
         raise EngineError(_lib.last_error() or f"{fn.__name__} failed")
 
 
+def _like(t, stream):
+    """A contiguous tensor of t's shape and type that belongs to the call's stream."""
+    if stream is None and t.is_contiguous():
+        return torch.empty_like(t)  # half the time of torch.empty
+    return _empty(t.shape, t.dtype, t.device, stream)
+
+
 def _empty(shape, dtype, device, stream):
-    """A result or workspace that belongs to the call's stream."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
@@ -77,7 +83,7 @@ def _empty(shape, dtype, device, stream):
 
 
 def _check(name: str, t, device, dtype, dim: int | None = None) -> None:
-    _need(t.is_cuda, f"{name} must be a tensor on a GPU")
+    _need(t is not None and t.is_cuda, f"{name} must be a tensor on a GPU")
     _need(t.device == device, f"{name} is on another device")
     _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     _need(dim is None or t.dim() == dim, f"{name} must have {dim} dimensions")
@@ -137,8 +143,6 @@ def rope_axes(q, k, pos, plan: RopePlan, *, q_out=None, k_out=None, inverse: boo
     """Queries [B, L, Hq, D] and keys [B, L, Hk, D] (either may be None) turned by int32
     positions [axes, B, L] (or [axes, L], the same for every batch item). Returns
     (q_out, k_out), new contiguous tensors unless given; q_out=q turns in place."""
-    for name, t in (("q", q), ("k", k), ("pos", pos), ("q_out", q_out), ("k_out", k_out)):
-        _tensor("rope_axes: " + name, t)
     key = ("rope", _sig(q), _sig(k), _sig(pos), _sig(q_out), _sig(k_out), plan.n, plan.n_axes, plan.pairs,
            plan.packed.device, inverse)
     template = _plans.get(key) or _keep(key, _rope_plan(q, k, pos, plan, q_out, k_out, inverse))
@@ -146,11 +150,11 @@ def rope_axes(q, k, pos, plan: RopePlan, *, q_out=None, k_out=None, inverse: boo
     device = pos.device
     if q is not None:
         if q_out is None:
-            q_out = _empty(q.shape, q.dtype, device, stream)
+            q_out = _like(q, stream)
         a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
     if k is not None:
         if k_out is None:
-            k_out = _empty(k.shape, k.dtype, device, stream)
+            k_out = _like(k, stream)
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
     a.pos, a.packed = pos.data_ptr(), plan.packed.data_ptr()
     _call(_lib.lib().arthip_rope_axes, a, device, stream)
@@ -170,7 +174,6 @@ def _rope_plan(q, k, pos, plan, q_out, k_out, inverse) -> bytes:
     _need(x is not None and x.is_cuda, "rope_axes: q or k must be a tensor on a GPU")
     _need(x.dtype in _TYPES, f"rope_axes: unsupported type {x.dtype}")
     _need(x.dim() == 4, "rope_axes: q and k must have 4 dimensions")
-    _need(pos is not None, "rope_axes: pos must be a tensor")
     batch, tokens, _, dim = x.shape
     _check("pos", pos, x.device, torch.int32)
     _need(tuple(pos.shape) in ((plan.n_axes, batch, tokens), (plan.n_axes, tokens)),
@@ -215,15 +218,11 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     window = tuple(window)
     doc_q, doc_k = docs or (None, None)
     code_q, code_k = codes or (None, None)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _need(isinstance(t, torch.Tensor), f"attention: {name} must be a tensor on a GPU")
     key = ("attention", _sig(q), _sig(k), _sig(v), scale, cap, causal, window, _sig(out), return_lse)
     plain = (q_start is None and kv_len is None and prefix is None and docs is None and codes is None
              and slopes is None and table is None)
     if not plain:
         more = (q_start, kv_len, prefix, doc_q, doc_k, code_q, code_k, slopes, table)
-        for t in more:
-            _tensor("attention: an option", t)
         key += tuple(_sig(t) for t in more) + (table_zero,)
     plan = _plans.get(key)
     if plan is None:
@@ -233,7 +232,7 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     a = _lib.AttentionArgs.from_buffer_copy(template)
     device = q.device
     if out is None:
-        out = _empty(q.shape, q.dtype, device, stream)
+        out = _like(q, stream)
     a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     lse = None
     if return_lse:
@@ -247,7 +246,7 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     if workspace is None and need > 0:
         workspace = _empty((need,), torch.uint8, device, stream)
     elif workspace is not None:
-        _tensor("attention: workspace", workspace)
+        _need(isinstance(workspace, torch.Tensor), "workspace must be a tensor on a GPU")
         _check("workspace", workspace, device, torch.uint8, 1)
         _inner("workspace", workspace)
     if workspace is not None:
@@ -259,7 +258,7 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
 def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix, docs, codes, slopes, table,
                     table_zero, out):
     """(checked arguments without pointers, bytes of workspace)."""
-    _need(q.is_cuda, "attention: q must be a tensor on a GPU")
+    _need(q is not None and q.is_cuda, "attention: q must be a tensor on a GPU")
     _need(q.dtype in (torch.float16, torch.bfloat16), f"attention: unsupported type {q.dtype}")
     device = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -311,7 +310,6 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
     a.dtype, a.batch, a.q_tokens, a.k_tokens = _TYPES[q.dtype], batch, q_tokens, k_tokens
     a.q_heads, a.k_heads, a.head_dim = q_heads, k_heads, dim
     if out is not None:
-        _tensor("attention: out", out)
         _check("out", out, device, q.dtype, 4)
         _need(out.shape == q.shape, "attention: out must have q's shape")
         _inner("out", out)
@@ -344,12 +342,10 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     fp32. Returns (new residual, h); residual_out=residual updates in place, and without y
     and with a residual_scale of 1 the residual is returned as it is. h has y's type, or
     ``dtype`` where there is no y."""
-    _need(isinstance(residual, torch.Tensor), "gated_norm: residual must be a tensor on a GPU")
+    _need(residual is not None, "gated_norm: residual must be a tensor on a GPU")
     given = (residual, y, gate, mod_scale, mod_shift, post_weight, post_bias, pre_weight, pre_bias,
              residual_out, h)
-    for t in given:
-        _tensor("gated_norm: an argument", t)
-    key = ("norm", *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in given], post, pre,
+    key = ("norm", *map(_sig, given), post, pre,
            gate_act, residual_scale, branch_scale, eps, dtype)
     plan = _plans.get(key)
     if plan is None:
@@ -360,10 +356,10 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     a.residual = residual.data_ptr()
     new = residual
     if new_residual or residual_out is not None:
-        new = residual_out if residual_out is not None else _empty(residual.shape, residual.dtype, device, stream)
+        new = residual_out if residual_out is not None else _like(residual, stream)
         a.residual_out = new.data_ptr()
     if new_h:
-        h = _empty(residual.shape, dtype, device, stream)
+        h = _like(y, stream) if y is not None else _empty(residual.shape, dtype, device, stream)
     if h is not None:
         a.h = h.data_ptr()
     for name, t in zip(("y", "gate", "mod_scale", "mod_shift", "post_weight", "post_bias", "pre_weight",
