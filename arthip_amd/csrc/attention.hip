@@ -198,7 +198,8 @@ enum Shape { kPlain, kCap, kAny };
 // SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
 // tile's keys; otherwise each holds 32 rows of its own and takes all keys.
 template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
-__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kAny ? 2 : 3) attention_tile(AttnArgs a) {
+__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 && SHAPE == kAny) ? 2 : 3)
+    attention_tile(AttnArgs a) {
   using L = TileL<DP, KT>;
   using E = Elem<T>;
   using frag = typename E::frag;
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
       // The loops below are whole loops a branch: a uniform branch inside would be taken
       // for every score.
       const int4* const codes = reinterpret_cast<const int4*>(more + L::kCode + buf * 256 + wk * 4) + half;
-      auto bias = [&](auto coded, auto add) __attribute__((always_inline)) {
+      auto bias = [&](auto coded, int from, auto add) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -549,7 +550,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               s[kb][4 * g + e] =
-                  add(s[kb][4 * g + e], decltype(coded)::value ? cq - ck[e] : cq - key0 - (32 * kb + 8 * g + e));
+                  add(s[kb][4 * g + e], decltype(coded)::value ? from - ck[e] : from - key0 - (32 * kb + 8 * g + e));
           }
       };
       if (a.c.slopes) {
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
           return __builtin_fmaf(x, unit, -slope * fabsf((float)diff));
         };
         if (code_k)
-          bias(std::true_type{}, add);
+          bias(std::true_type{}, cq, add);
         else {
           const float first = (float)(cq - key0);
 #pragma unroll
@@ -574,25 +575,25 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || SHAPE == kA
           // Entries in the base of 2.
           const float* const t = reinterpret_cast<const float*>(more + L::kTable) + g_head * a.c.table_len;
           auto add = [&](float x, int diff) __attribute__((always_inline)) {
-            return __builtin_fmaf(x, by, t[min(max(diff + zero, 0), last)]);
+            return __builtin_fmaf(x, by, t[min(max(diff, 0), last)]);
           };
           auto add_hidden = [&](float x, int diff) __attribute__((always_inline)) {
-            const float entry = t[min(max(diff + zero, 0), last)];
+            const float entry = t[min(max(diff, 0), last)];
             const float sum = __builtin_fmaf(x, by, entry);
             return entry == -__builtin_inff() ? entry : sum;
           };
           if (hides)
-            code_k ? bias(std::true_type{}, add_hidden) : bias(std::false_type{}, add_hidden);
+            code_k ? bias(std::true_type{}, cq + zero, add_hidden) : bias(std::false_type{}, cq + zero, add_hidden);
           else
-            code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+            code_k ? bias(std::true_type{}, cq + zero, add) : bias(std::false_type{}, cq + zero, add);
         } else {
           const float* const t = table + (int64_t)head * a.c.table_len;
           auto add = [&](float x, int diff) __attribute__((always_inline)) {
-            const float entry = t[min(max(diff + zero, 0), last)] * kLog2e;
+            const float entry = t[min(max(diff, 0), last)] * kLog2e;
             const float sum = __builtin_fmaf(x, by, entry);
             return entry == -__builtin_inff() ? entry : sum;
           };
-          code_k ? bias(std::true_type{}, add) : bias(std::false_type{}, add);
+          code_k ? bias(std::true_type{}, cq + zero, add) : bias(std::false_type{}, cq + zero, add);
         }
       }
       if (!a.c.slopes && !table && unit != 1.0f) {

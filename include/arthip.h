@@ -470,9 +470,9 @@ int arthip_rope_axes(const arthip_rope_args* args, void* stream);
  *                 then - slopes[h] * |cq_i - ck_j| and + table[h][clamp(cq_i - ck_j + table_zero)]
  *   j is visible to i when j < kv_len[b], doc_q[i] == doc_k[j], and either
  *   j < prefix[b] or p_i - left <= j <= p_i + right, with p_i = q_start[b] + i.
- * cq and ck are code_q and code_k, or p_i and j without them. (A two-dimensional
- * table needs one number a token: y * (2 W - 1) + x names every offset inside a
- * window W wide.) A table entry of -inf hides its offset. A query that sees
+ * cq and ck are code_q and code_k, or p_i and j without them; cq + table_zero - ck
+ * has to fit 32 bits. (A two-dimensional table needs one number a token:
+ * y * (2 W - 1) + x names every offset inside a window W wide.) A table entry of -inf hides its offset. A query that sees
  * nothing gives zeros, and -inf as its log-sum. Keys that a query does not see
  * add nothing to it, whatever their K and V hold, NaN and infinities among
  * them. fp16 or bf16. */
