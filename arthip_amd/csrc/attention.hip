@@ -48,7 +48,7 @@ struct AttnArgs {
   int table_lds;  // the tables of a key head's rows are kept in LDS
   int table_bytes;  // and take these
   int wide;       // keys further apart than 32-bit offsets reach
-  FastDiv by_group, by_k_heads, by_row_tiles, by_splits;
+  FastDiv by_group, by_k_heads, by_row_tiles, by_splits, by_rows;
   float cap_reach;  // |q.k| up to which the polynomial holds
   float cap_fit[5];
   const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
@@ -931,6 +931,54 @@ __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
         (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// The same for up to eight ranges of many rows: D / 4 threads a row, which read its ranges
+// one after the other. (A workgroup a row took 41 us for 30740 rows of 80 in four ranges.)
+template <class T>
+__global__ void __launch_bounds__(256) attention_join_few(AttnArgs a) {
+  const int64_t total = (int64_t)a.c.batch * a.c.k_heads * a.rows;
+  const int D = a.c.head_dim, quads = D / 4, rows = 256 / quads;
+  const int slot = threadIdx.x / quads, quad = threadIdx.x - slot * quads;
+  const int64_t at = (int64_t)blockIdx.x * rows + slot;
+  if (slot >= rows || at >= total) return;
+  float2 st[8];
+  f4 x[8];
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= a.splits) break;
+    st[s] = *reinterpret_cast<const float2*>(a.stat + 2 * (s * total + at));
+    x[s] = *reinterpret_cast<const f4*>(a.part + (s * total + at) * D + 4 * quad);
+  }
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= a.splits) break;
+    top = fmaxf(top, st[s].x);
+  }
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  float l = 0.0f;
+  f4 o = f4{};
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= a.splits) break;
+    const float w = __builtin_amdgcn_exp2f(st[s].x - base);
+    l = __builtin_fmaf(w, st[s].y, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = w != 0.0f ? __builtin_fmaf(w, x[s][e], o[e]) : o[e];
+  }
+  const uint32_t bh = fdiv((uint32_t)at, a.by_rows);
+  const int row = (int)at - (int)bh * a.rows;
+  const int b = (int)fdiv(bh, a.by_k_heads), kh = (int)bh - b * a.c.k_heads;
+  const int token = (int)fdiv((uint32_t)row, a.by_group), head = kh * a.group + row - token * a.group;
+  const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+  T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
+                head * a.c.out_stride[2];
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<t4*>(op + 4 * quad) = __builtin_convertvector(o * scale, t4);
+  if (a.c.lse && quad == 0)
+    a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
+        (top + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
 struct TilePick {
   void (*fn)(AttnArgs);
   int threads;
@@ -982,10 +1030,12 @@ AttnPlan attention_plan(const arthip_attention_args& c) {
   int64_t tiles = (c.k_tokens + kt - 1) / kt;
   if (c.left >= 0 && c.right >= 0 && c.prefix == nullptr)
     tiles = std::min<int64_t>(tiles, ((int64_t)c.left + c.right + std::min<int64_t>(c.q_tokens, per)) / kt + 2);
-  // Ranges: enough workgroups for the chip, of at least four tiles. One-wave workgroups
-  // fit a CU four at a time; those of four waves two.
+  // Ranges: enough workgroups for the chip (one-wave workgroups fit a CU four at a time,
+  // those of four waves two), of at least four tiles. From half of that number on only
+  // long walks are divided: 256 items of 64 tiles 91 -> 64 us, of 128 tiles 213 -> 133 us,
+  // but 260 of 25 tiles 54 -> 57 us.
   const int64_t want = shared_rows(c) ? 1024 : 512;
-  if (items < want / 2)
+  if (items < want / 2 || (items < want && tiles >= 32))
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + items - 1) / items, tiles / 4, 64}));
   p.range = (int)std::max<int64_t>(1, (tiles + p.splits - 1) / p.splits);
   if (p.splits > 1)
@@ -1013,6 +1063,7 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.by_k_heads = make_fastdiv((uint32_t)c.k_heads);
   a.by_row_tiles = make_fastdiv((uint32_t)a.row_tiles);
   a.by_splits = make_fastdiv((uint32_t)a.splits);
+  a.by_rows = make_fastdiv((uint32_t)a.rows);
   const int64_t total = (int64_t)c.batch * c.k_heads * a.rows;
   a.part = static_cast<float*>(c.workspace);
   if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
@@ -1050,6 +1101,12 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   hipLaunchKernelGGL(k.fn, dim3((unsigned)((a.items + 7) / 8 * 8)), dim3((unsigned)k.threads), bytes, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
+  if (a.splits <= 8 && total >= 512) {
+    const int rows = 256 / (c.head_dim / 4);
+    hipLaunchKernelGGL(f16 ? attention_join_few<_Float16> : attention_join_few<__bf16>,
+                       dim3((unsigned)((total + rows - 1) / rows)), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(f16 ? attention_join<_Float16> : attention_join<__bf16>,
                      dim3((unsigned)total), dim3(256), 0, s, a);
   return hipGetLastError();
