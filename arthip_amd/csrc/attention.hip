@@ -86,6 +86,31 @@ __device__ __forceinline__ void halves(float x, float& low, float& high) {
   low = __builtin_bit_cast(float, r0);
   high = __builtin_bit_cast(float, r1);
 }
+// f over the values of a wave, the same in every lane: quads, half rows, rows of 16, then
+// halves, inside the vector unit. (A shuffle is an LDS instruction, which the compiler may
+// move between a barrier and the wait before it.)
+template <class X, class F>
+__device__ __forceinline__ X over_wave(X x, F f) {
+  auto dpp = [&](auto control) __attribute__((always_inline)) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(control)::value, 0xf, 0xf, true);
+    x = f(x, __builtin_bit_cast(X, y));
+  };
+  dpp(std::integral_constant<int, 0xb1>{});
+  dpp(std::integral_constant<int, 0x4e>{});
+  dpp(std::integral_constant<int, 0x141>{});
+  dpp(std::integral_constant<int, 0x140>{});
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const u2 r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  x = f(__builtin_bit_cast(X, r0), __builtin_bit_cast(X, r1));
+  u = __builtin_bit_cast(uint32_t, x);
+  const u2 h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t h0 = h[0], h1 = h[1];
+  return f(__builtin_bit_cast(X, h0), __builtin_bit_cast(X, h1));
+}
+__device__ __forceinline__ int wave_min(int x) { return over_wave(x, [](int a, int b) { return min(a, b); }); }
+__device__ __forceinline__ int wave_max(int x) { return over_wave(x, [](int a, int b) { return max(a, b); }); }
+
 __device__ __forceinline__ float halves_max(float x) {
   float a, b;
   halves(x, a, b);
@@ -331,13 +356,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   int w_dmin = dq, w_dmax = dq, dmin = 0, dmax = 0;
   if (doc_k) {
     int* const range = reinterpret_cast<int*>(more + L::kRange);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {  // a lane past the last row repeats it
-      w_dmin = min(w_dmin, __shfl_xor(w_dmin, o));
-      w_dmax = max(w_dmax, __shfl_xor(w_dmax, o));
-    }
-    w_dmin = scalar(w_dmin);
-    w_dmax = scalar(w_dmax);
+    w_dmin = scalar(wave_min(dq));  // a lane past the last row repeats it
+    w_dmax = scalar(wave_max(dq));
     lds_sync();
     if (lane == 0) {
       range[wave] = w_dmin;
@@ -868,11 +888,8 @@ __global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int
   int lo = INT32_MAX, hi = INT32_MIN;
   if (lane < a.doc_tile && first + lane < a.c.k_tokens)
     lo = hi = a.c.doc_k[b * a.c.doc_k_stride + first + lane];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-  }
+  lo = wave_min(lo);
+  hi = wave_max(hi);
   if (lane == 0) out[at] = int2{lo, hi};
 }
 
@@ -894,14 +911,10 @@ __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
                        : float2{-__builtin_inff(), 0.0f};
   f4 o = f4{};
   const float* const p = a.part + at * D + 4 * quad;
-  float top = st.x;
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+  const float top = over_wave(st.x, [](float a, float b) { return fmaxf(a, b); });
   const float base = top == -__builtin_inff() ? 0.0f : top;
   const float w = in ? __builtin_amdgcn_exp2f(st.x - base) : 0.0f;
-  float l = w * st.y;
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
+  const float l = over_wave(w * st.y, [](float a, float b) { return a + b; });
   if (tid < 64) weight[tid] = w;
   lds_sync();
   if (step < steps) {
