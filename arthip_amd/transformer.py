@@ -9,7 +9,8 @@ Tensors are torch tensors on one GPU (torch is used only as device-memory plumbi
 and keep their strides: only the innermost dimension has to be contiguous. Work goes
 to torch's current stream, or to ``stream`` (a raw handle); results that a call makes
 itself belong to that stream. Arguments that do not fit raise :class:`EngineError`
-before anything is launched.
+before anything is launched. Numbers may be tensors or arrays of one value, which are
+read at each call (from a tensor on the GPU with a synchronization).
 """
 
 from __future__ import annotations
@@ -32,9 +33,34 @@ def _need(ok: bool, text: str) -> None:
         raise EngineError(text)
 
 
+def _float(name: str, x) -> float:
+    try:
+        return float(x)
+    except (TypeError, ValueError, RuntimeError):
+        raise EngineError(f"{name} must be a number") from None
+
+
+def _int(name: str, x) -> int:
+    try:
+        n = int(x)
+        if n == x:
+            return n
+    except (TypeError, ValueError, OverflowError, RuntimeError):
+        pass
+    raise EngineError(f"{name} must be a whole number")
+
+
+def _bool(name: str, x) -> bool:
+    try:
+        return bool(x)
+    except (TypeError, ValueError, RuntimeError):
+        raise EngineError(f"{name} must be a truth value") from None
+
+
 # What a call's shapes, strides, types and options come to (checked arguments with all
 # pointers empty), so that the next call of the same kind only fills in pointers: a call
-# takes some 8 us instead of 18. Nothing in it depends on a tensor's address or contents.
+# takes some 8 us instead of 18. Nothing in it depends on a tensor's address or contents:
+# options become plain numbers before they are part of a key.
 _plans: dict = {}
 _PLANS = 512
 
@@ -143,6 +169,7 @@ def rope_axes(q, k, pos, plan: RopePlan, *, q_out=None, k_out=None, inverse: boo
     """Queries [B, L, Hq, D] and keys [B, L, Hk, D] (either may be None) turned by int32
     positions [axes, B, L] (or [axes, L], the same for every batch item). Returns
     (q_out, k_out), new contiguous tensors unless given; q_out=q turns in place."""
+    inverse = _bool("rope_axes: inverse", inverse)
     key = ("rope", _sig(q), _sig(k), _sig(pos), _sig(q_out), _sig(k_out), plan.n, plan.n_axes, plan.pairs,
            plan.packed.device, inverse)
     template = _plans.get(key) or _keep(key, _rope_plan(q, k, pos, plan, q_out, k_out, inverse))
@@ -197,7 +224,7 @@ def _rope_plan(q, k, pos, plan, q_out, k_out, inverse) -> bytes:
         setattr(a, name + "_out_stride", (_contiguous(t.shape) if out is None else out.stride())[:3])
     st = pos.stride()
     a.pos_stride = st if pos.dim() == 3 else (st[0], 0, st[1])
-    a.n_freq, a.dtype, a.pairs, a.inverse = plan.n, _TYPES[x.dtype], plan.pairs, bool(inverse)
+    a.n_freq, a.dtype, a.pairs, a.inverse = plan.n, _TYPES[x.dtype], plan.pairs, inverse
     a.batch, a.tokens, a.head_dim = batch, tokens, dim
     return bytes(a)
 
@@ -215,7 +242,10 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     (queries', keys'), [B, L] or [L]; slopes is fp32 [Hq], table fp32 [Hq, n]. Returns
     out, or (out, lse) with lse fp32 [B, Hq, Lq]. Without ``workspace`` (uint8) a call
     that needs one makes it."""
-    window = tuple(window)
+    scale = None if scale is None else _float("attention: scale", scale)
+    cap, table_zero = _float("attention: cap", cap), _int("attention: table_zero", table_zero)
+    causal = _bool("attention: causal", causal)
+    window = tuple(None if w is None else _int("attention: a window's side", w) for w in window)
     doc_q, doc_k = docs or (None, None)
     code_q, code_k = codes or (None, None)
     key = ("attention", _sig(q), _sig(k), _sig(v), scale, cap, causal, window, _sig(out), return_lse)
@@ -295,17 +325,17 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
         _need(table.shape[0] == q_heads and table.is_contiguous(),
               "attention: table must be contiguous [Hq, n]")
         _need(table.shape[1] > 0, "attention: table without entries")
-        a.table_len, a.table_zero = table.shape[1], int(table_zero)
+        a.table_len, a.table_zero = table.shape[1], table_zero
     left, right = window
     _need(not causal or right in (None, 0), "attention: causal and a window to the right")
     for side in (left, right):
         _need(side is None or side >= 0, "attention: a window counts keys")
-    a.left = -1 if left is None else int(left)
-    a.right = 0 if causal else -1 if right is None else int(right)
+    a.left = -1 if left is None else left
+    a.right = 0 if causal else -1 if right is None else right
     if prefix is not None:
         a.prefix = 16
-    a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    a.cap = float(cap)
+    a.scale = 1.0 / math.sqrt(dim) if scale is None else scale
+    a.cap = cap
     a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]
     a.dtype, a.batch, a.q_tokens, a.k_tokens = _TYPES[q.dtype], batch, q_tokens, k_tokens
     a.q_heads, a.k_heads, a.head_dim = q_heads, k_heads, dim
@@ -343,6 +373,9 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     and with a residual_scale of 1 the residual is returned as it is. h has y's type, or
     ``dtype`` where there is no y."""
     _need(residual is not None, "gated_norm: residual must be a tensor on a GPU")
+    residual_scale = _float("gated_norm: residual_scale", residual_scale)
+    branch_scale = _float("gated_norm: branch_scale", branch_scale)
+    eps = _float("gated_norm: eps", eps)
     given = (residual, y, gate, mod_scale, mod_shift, post_weight, post_bias, pre_weight, pre_bias,
              residual_out, h)
     key = ("norm", *map(_sig, given), post, pre,
@@ -410,7 +443,7 @@ def _norm_plan(given, post, pre, gate_act, residual_scale, branch_scale, eps, dt
     a.dtype, a.residual_dtype = _TYPES[dtype], _TYPES[residual.dtype]
     a.post, a.pre, a.gate_act = _NORMS[post], _NORMS[pre], _GATES[gate_act]
     a.batch, a.tokens, a.channels = shape
-    a.eps, a.residual_scale, a.branch_scale = float(eps), float(residual_scale), float(branch_scale)
+    a.eps, a.residual_scale, a.branch_scale = eps, residual_scale, branch_scale
     if residual_out is not None:
         _check("residual_out", residual_out, device, residual.dtype, 3)
         _need(tuple(residual_out.shape) == shape, "gated_norm: residual_out must have the residual's shape")

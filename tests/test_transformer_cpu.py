@@ -182,3 +182,78 @@ def test_tensors_must_be_on_a_gpu():
         tr.rope_axes(x, x, torch.zeros(1, 1, 2, dtype=torch.int32), tr.RopePlan((16,), device="cpu"))
     with pytest.raises(EngineError, match="on a GPU"):
         tr.gated_norm(torch.zeros(1, 2, 64), pre="rms")
+
+
+# -- the Python layer, with the launch replaced --------------------------------------------
+
+class _Gpu(torch.Tensor):
+    """A host tensor that says it is on a GPU; nothing here launches."""
+    is_cuda = property(lambda self: True)
+
+
+def _gpu(*shape, dtype=torch.float16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Gpu)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The argument structs of the calls made, copied in place of the launch."""
+    seen = []
+    monkeypatch.setattr(tr, "_plans", {})
+    monkeypatch.setattr(tr, "_call", lambda fn, args, device, stream: seen.append(type(args).from_buffer_copy(args)))
+    return seen
+
+
+NUMBERS = [
+    ("norm", "eps", 1e-3), ("norm", "residual_scale", 0.25), ("norm", "branch_scale", 2.0),
+    ("attention", "scale", 0.75), ("attention", "cap", 7.0), ("attention", "table_zero", 3),
+    ("attention", "causal", True), ("rope", "inverse", True),
+]
+
+
+def test_windows_are_read_at_each_call(launches):
+    left, right = torch.tensor(5), torch.tensor(2)
+    _use("attention", window=(left, right))
+    left.fill_(9), right.fill_(0)
+    _use("attention", window=(left, right))
+    assert [(a.left, a.right) for a in launches] == [(5, 2), (9, 0)]
+    for bad in ((1.5, None), ("x", None), (None, torch.ones(2))):
+        with pytest.raises(EngineError, match="window"):
+            _use("attention", window=bad)
+
+
+def _use(op, **kw):
+    if op == "norm":
+        tr.gated_norm(_gpu(1, 2, 64), _gpu(1, 2, 64), pre="rms", **kw)
+    elif op == "attention":
+        tr.attention(_gpu(1, 4, 2, 32), _gpu(1, 4, 2, 32), _gpu(1, 4, 2, 32), table=_gpu(2, 9, dtype=torch.float32),
+                     **kw)
+    else:
+        plan = tr.RopePlan((16,), device="cpu")
+        tr.rope_axes(_gpu(1, 2, 2, 32), None, _gpu(1, 1, 2, dtype=torch.int32), plan, **kw)
+
+
+@pytest.mark.parametrize("op,name,value", NUMBERS)
+def test_numbers_are_read_at_each_call(launches, op, name, value):
+    """A parameter of no dimensions that changes in place between two calls counts with the
+    value that it has at each."""
+    field, first = ("right", -1) if name == "causal" else (name, 0)
+    number = torch.zeros((), dtype=torch.tensor(value).dtype)
+    _use(op, **{name: number})
+    number.copy_(torch.tensor(value))
+    _use(op, **{name: number})
+    assert getattr(launches[0], field) == first
+    assert getattr(launches[1], field) == (0 if name == "causal" else np.float32(value))
+    for other in (value, np.array(value)):
+        _use(op, **{name: other})
+        assert getattr(launches[-1], field) == getattr(launches[1], field)
+
+
+@pytest.mark.parametrize("op,name,value", [n for n in NUMBERS if n[1] not in ("causal", "inverse")])
+@pytest.mark.parametrize("bad", ["much", None, (1.0, 2.0), torch.ones(2)])
+def test_numbers_that_are_none(launches, op, name, value, bad):
+    if name == "scale" and bad is None:
+        return  # 1 / sqrt(D)
+    with pytest.raises(EngineError, match=name):
+        _use(op, **{name: bad})
+    assert not launches
