@@ -785,10 +785,12 @@ int arthip_rope_axes(const arthip_rope_args* args, void* stream) {
 }
 
 size_t arthip_attention_workspace(const arthip_attention_args* args) {
-  if (args == nullptr || args->batch < 0 || args->q_tokens < 0 || args->k_tokens < 0 ||
-      args->k_heads < 1 || args->q_heads < 0 || args->head_dim < 1)
+  try {
+    if (args == nullptr || !arthip::check_attention_shape(*args).empty()) return 0;
+    return arthip::attention_plan(*args).workspace;
+  } catch (const std::exception&) {
     return 0;
-  return arthip::attention_plan(*args).workspace;
+  }
 }
 
 int arthip_attention(const arthip_attention_args* args, void* stream) {

@@ -69,9 +69,8 @@ std::string check_rope(const arthip_rope_args& a) {
   return "";
 }
 
-std::string check_attention(const arthip_attention_args& a) {
+std::string check_attention_shape(const arthip_attention_args& a) {
   const std::string at = "arthip_attention: ";
-  if (a.dtype != ARTHIP_TYPE_F16 && a.dtype != ARTHIP_TYPE_BF16) return at + "type must be fp16 or bf16";
   if (a.batch < 0 || a.q_tokens < 0 || a.k_tokens < 0 || a.q_heads < 0)
     return at + "negative dimension";
   if (a.k_heads < 1 || a.q_heads % a.k_heads != 0)
@@ -86,6 +85,14 @@ std::string check_attention(const arthip_attention_args& a) {
           ((static_cast<int64_t>(a.q_tokens) * (a.q_heads / a.k_heads) + 31) / 32) >
       (int64_t{1} << 24))
     return at + "batch times heads times tokens too large";
+  return "";
+}
+
+std::string check_attention(const arthip_attention_args& a) {
+  const std::string at = "arthip_attention: ";
+  if (a.dtype != ARTHIP_TYPE_F16 && a.dtype != ARTHIP_TYPE_BF16) return at + "type must be fp16 or bf16";
+  const std::string shape = check_attention_shape(a);
+  if (!shape.empty()) return shape;
   if (!std::isfinite(a.scale)) return at + "scale is not finite";
   if (!std::isfinite(a.cap) || a.cap < 0) return at + "cap is negative or not finite";
   if (a.left < -1 || a.right < -1 || a.left > kMaxTokens || a.right > kMaxTokens)

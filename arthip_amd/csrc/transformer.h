@@ -25,13 +25,14 @@ static_assert(sizeof(RopeFreq) == 16, "the packed size is part of the C ABI");
 
 std::string check_rope(const arthip_rope_args& a);
 std::string check_attention(const arthip_attention_args& a);
+std::string check_attention_shape(const arthip_attention_args& a);  // what attention_plan() relies on
 std::string check_norm(const arthip_norm_args& a);
 
 hipError_t launch_rope(const arthip_rope_args& a, hipStream_t s);
 hipError_t launch_norm(const arthip_norm_args& a, hipStream_t s);
 hipError_t launch_attention(const arthip_attention_args& a, hipStream_t s);
 
-// How attention divides its work (attention.hip).
+// How attention divides its work (attention.hip); of arguments whose shape is checked.
 struct AttnPlan {
   int splits;         // ranges of the keys, each its own workgroup; joined by a second kernel
   int range;          // tiles of each

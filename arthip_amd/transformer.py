@@ -298,6 +298,7 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
     k_tokens, k_heads = k.shape[1], k.shape[2]
     _need(tuple(k.shape) == (batch, k_tokens, k_heads, dim) and k.shape == v.shape,
           "attention: k and v must be [B, Lk, Hk, D] of q's batch and head_dim")
+    _need(k_heads > 0 and q_heads % k_heads == 0, "attention: q_heads must be a multiple of k_heads")
     a = _lib.AttentionArgs()
     for name, t in (("q_start", q_start), ("kv_len", kv_len), ("prefix", prefix)):
         if t is not None:

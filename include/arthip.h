@@ -511,7 +511,7 @@ typedef struct arthip_attention_args {
 } arthip_attention_args;
 
 /* Bytes of workspace that arthip_attention needs for these arguments (0 when the
- * keys are not split; pointers are not read). */
+ * keys are not split, or the call refuses the shape; pointers are not read). */
 size_t arthip_attention_workspace(const arthip_attention_args* args);
 int arthip_attention(const arthip_attention_args* args, void* stream);
 

@@ -257,3 +257,26 @@ def test_numbers_that_are_none(launches, op, name, value, bad):
     with pytest.raises(EngineError, match=name):
         _use(op, **{name: bad})
     assert not launches
+
+
+# -- shapes that no operator takes ---------------------------------------------------------
+
+@pytest.mark.parametrize("change", [
+    dict(q_heads=2, k_heads=4), dict(q_heads=3, k_heads=2), dict(head_dim=60), dict(head_dim=512),
+    dict(q_tokens=2 ** 31 - 1), dict(batch=2 ** 24, q_tokens=64),
+])
+def test_attention_shapes_without_a_workspace(change):
+    """No workspace, and a refusal, for shapes that the call does not take."""
+    lib = _lib.lib()
+    a = _attention(k_tokens=100000, **change)
+    assert lib.arthip_attention_workspace(ctypes.byref(a)) == 0
+    assert lib.arthip_attention(ctypes.byref(a), None) == 1
+
+
+def test_attention_fewer_query_heads_than_key_heads(launches):
+    q, k = _gpu(1, 4, 2, 32), _gpu(1, 5000, 4, 32)
+    with pytest.raises(EngineError, match="multiple of k_heads"):
+        tr.attention(q, k, k)
+    with pytest.raises(EngineError, match="multiple of k_heads"):
+        tr.attention(_gpu(1, 4, 3, 32), k[:, :, :2], k[:, :, :2])
+    assert not launches
