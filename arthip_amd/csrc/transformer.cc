@@ -80,10 +80,10 @@ std::string check_attention_shape(const arthip_attention_args& a) {
   if (a.q_tokens > kMaxTokens || a.k_tokens > kMaxTokens ||
       static_cast<int64_t>(a.q_tokens) * (a.q_heads / a.k_heads) > kMaxTokens)
     return at + "too many tokens";
-  // Items of 32 rows and up to 64 ranges of keys number the workgroups in 31 bits.
-  if (static_cast<int64_t>(a.batch) * a.k_heads *
-          ((static_cast<int64_t>(a.q_tokens) * (a.q_heads / a.k_heads) + 31) / 32) >
-      (int64_t{1} << 24))
+  // Items of 32 rows and up to 64 ranges of keys number the workgroups in 31 bits. (A quotient,
+  // as the product can pass 64 bits.)
+  const int64_t items = (static_cast<int64_t>(a.q_tokens) * (a.q_heads / a.k_heads) + 31) / 32;
+  if (items > 0 && static_cast<int64_t>(a.batch) * a.k_heads > (int64_t{1} << 24) / items)
     return at + "batch times heads times tokens too large";
   return "";
 }

@@ -280,3 +280,10 @@ def test_attention_fewer_query_heads_than_key_heads(launches):
     with pytest.raises(EngineError, match="multiple of k_heads"):
         tr.attention(_gpu(1, 4, 3, 32), k[:, :, :2], k[:, :, :2])
     assert not launches
+
+
+@pytest.mark.parametrize("q_tokens", [1, 2 ** 8, 2 ** 9, 2 ** 10, 2 ** 30])
+def test_attention_sizes_whose_product_passes_64_bits(q_tokens):
+    a = _attention(batch=2 ** 30, q_tokens=q_tokens, q_heads=2 ** 30, k_heads=2 ** 30)
+    assert _lib.lib().arthip_attention_workspace(ctypes.byref(a)) == 0
+    _refused(_lib.lib().arthip_attention, a, "too large")
