@@ -1066,6 +1066,8 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   if (c.batch == 0 || c.q_tokens == 0 || c.q_heads == 0) return hipSuccess;
   AttnArgs a{};
   a.c = c;
+  if (c.k_tokens == 0)  // nothing to compare: one side of a pair may be missing
+    a.c.doc_q = a.c.doc_k = a.c.code_q = a.c.code_k = nullptr;
   a.group = c.q_heads / c.k_heads;
   a.rows = c.q_tokens * a.group;
   const bool shared = shared_rows(c);
@@ -1091,7 +1093,7 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
     a.cap_reach = (float)(0.6 / r);
     for (int i = 0; i < 5; ++i) a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
   }
-  if (c.doc_k != nullptr && c.k_tokens > 0) {
+  if (a.c.doc_k != nullptr) {
     a.doc_tile = tile_keys(c);
     a.doc_tiles = (c.k_tokens + a.doc_tile - 1) / a.doc_tile;
     int2* const ranges = reinterpret_cast<int2*>(a.splits > 1 ? a.stat + 2 * a.splits * total : a.part);
@@ -1107,7 +1109,7 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   const int64_t far = std::max(std::abs(c.k_stride[1]), std::abs(c.v_stride[1]));
   a.wide = c.k_stride[1] < 0 || c.v_stride[1] < 0 || far * 2 * 64 + 512 > INT32_MAX;
   a.table_bytes = a.table_lds ? (int)(table + 7) / 8 * 8 : 0;
-  const int bytes = k.bytes + a.table_bytes + (c.doc_k != nullptr ? k.chunk * 8 : 0);
+  const int bytes = k.bytes + a.table_bytes + (a.c.doc_k != nullptr ? k.chunk * 8 : 0);
   hipError_t e = hipSuccess;
   if (bytes > 65536)  // what a kernel may have without asking
     e = hipFuncSetAttribute(reinterpret_cast<const void*>(k.fn), hipFuncAttributeMaxDynamicSharedMemorySize,

@@ -97,12 +97,13 @@ std::string check_attention(const arthip_attention_args& a) {
   if (!std::isfinite(a.cap) || a.cap < 0) return at + "cap is negative or not finite";
   if (a.left < -1 || a.right < -1 || a.left > kMaxTokens || a.right > kMaxTokens)
     return at + "window out of range";
-  if ((a.doc_q == nullptr) != (a.doc_k == nullptr)) return at + "doc_q and doc_k come together";
-  if ((a.code_q == nullptr) != (a.code_k == nullptr)) return at + "code_q and code_k come together";
   if (a.table != nullptr && a.table_len < 1) return at + "table without entries";
   if (a.table != nullptr && (a.table_zero < -kMaxTokens || a.table_zero > kMaxTokens))
     return at + "table_zero out of range";
   if (a.batch == 0 || a.q_tokens == 0 || a.q_heads == 0) return "";
+  // Arrays over no tokens may be NULL: pairs are asked for where both sides have tokens.
+  if (a.k_tokens > 0 && (a.doc_q == nullptr) != (a.doc_k == nullptr)) return at + "doc_q and doc_k come together";
+  if (a.k_tokens > 0 && (a.code_q == nullptr) != (a.code_k == nullptr)) return at + "code_q and code_k come together";
   if (a.q == nullptr || a.out == nullptr) return at + "null query or output buffer";
   if (a.k_tokens > 0 && (a.k == nullptr || a.v == nullptr)) return at + "null key or value buffer";
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16))

@@ -485,7 +485,7 @@ typedef struct arthip_attention_args {
   const int32_t* q_start;   /* [B], or NULL: Lk - Lq */
   const int32_t* kv_len;    /* [B], or NULL: Lk; clamped to [0, Lk] */
   const int32_t* prefix;    /* [B], or NULL: no prefix */
-  const int32_t* doc_q;     /* [B][Lq] with doc_k, or NULL */
+  const int32_t* doc_q;     /* [B][Lq] with doc_k, or NULL (either may be NULL when it has no tokens) */
   const int32_t* doc_k;     /* [B][Lk] */
   const int32_t* code_q;    /* [B][Lq] with code_k, or NULL */
   const int32_t* code_k;    /* [B][Lk] */

@@ -287,3 +287,12 @@ def test_attention_sizes_whose_product_passes_64_bits(q_tokens):
     a = _attention(batch=2 ** 30, q_tokens=q_tokens, q_heads=2 ** 30, k_heads=2 ** 30)
     assert _lib.lib().arthip_attention_workspace(ctypes.byref(a)) == 0
     _refused(_lib.lib().arthip_attention, a, "too large")
+
+
+@pytest.mark.parametrize("empty", [dict(q_tokens=0), dict(batch=0), dict(q_heads=0)])
+def test_calls_without_queries_take_documents_and_codes(empty):
+    """An empty tensor has no address: a pair's one side may be NULL where there is nothing to do."""
+    lib = _lib.lib()
+    for pair in (dict(doc_k=BUF * 8), dict(code_k=BUF * 8), dict(doc_q=BUF * 8, code_q=BUF * 8)):
+        a = _attention(**empty, **pair)
+        assert lib.arthip_attention(ctypes.byref(a), None) == 0, _lib.last_error()

@@ -329,6 +329,23 @@ def test_attention_nothing_to_do():
     assert not out.any() and torch.isneginf(lse).all()
 
 
+@pytest.mark.parametrize("docs", [False, True])
+@pytest.mark.parametrize("codes", [False, True])
+def test_attention_no_tokens_with_documents_and_codes(docs, codes):
+    q, k, v = _qkv(17, BF16, 2, 4, 9, 2, 2, 32)
+
+    def arrays(lq, lk):
+        pair = _ints([1] * lq), _ints([1] * lk)
+        return {**({"docs": pair} if docs else {}),
+                **({"codes": pair, "slopes": torch.ones(2, device="cuda")} if codes else {})}
+
+    assert tr.attention(q[:, :0], k, v, **arrays(0, 9)).shape == (2, 0, 2, 32)
+    assert tr.attention(q[:, :0], k[:, :0], v[:, :0], **arrays(0, 0)).shape == (2, 0, 2, 32)
+    out = torch.full_like(q, math.nan)
+    got, lse = tr.attention(q, k[:, :0], v[:, :0], out=out, return_lse=True, prefix=_ints([0, 3]), **arrays(4, 0))
+    assert got is out and not out.any() and torch.isneginf(lse).all()
+
+
 def test_attention_masks_by_differences():
     """Moving a hidden key or value changes no bit; moving a seen one moves the output
     by its weight (a central difference of the value against the softmax's weight)."""
