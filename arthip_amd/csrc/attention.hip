@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <limits>
 #include <type_traits>
 
 #include "launch.h"
@@ -54,6 +55,7 @@ struct AttnArgs {
   FastDiv by_group, by_k_heads, by_row_tiles, by_splits, by_rows;
   float cap_reach;  // |q.k| up to which the polynomial holds
   float cap_fit[5];
+  float cap_in, cap_out;  // of the exponential's argument and result
   const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
   int doc_tiles, doc_tile;  // tiles of a sequence, keys of a tile
   float* part;    // [splits][batch * k_heads * rows][D] unscaled sums, if splits > 1
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
           }
       } else {
         // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2
-        const float in = 2.0f * kLog2e * a.c.scale / a.c.cap, out = kLog2e * a.c.cap;
+        const float in = a.cap_in, out = a.cap_out;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -1087,11 +1089,21 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   const bool f16 = c.dtype == ARTHIP_TYPE_F16;
   const Shape shape = c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
   const TilePick k = f16 ? pick<_Float16>(c.head_dim, shared, shape) : pick<__bf16>(c.head_dim, shared, shape);
-  if (shape == kCap) {
+  if (c.cap > 0) {
     static constexpr double fit[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825, 0.015486690367999443};
+    // A cap near the ends of its type takes these past theirs: a coefficient that is no number
+    // leaves all scores to the exponential, squares stay below infinity (as 0 times it is NaN),
+    // and factors that a score of 0 or infinity meets stay finite.
+    constexpr double top = std::numeric_limits<float>::max();
     const double r = (double)c.scale / c.cap;
-    a.cap_reach = (float)(0.6 / r);
-    for (int i = 0; i < 5; ++i) a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
+    bool fits = true;
+    for (int i = 0; i < 5; ++i) {
+      a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
+      fits = fits && std::isfinite(a.cap_fit[i]);
+    }
+    a.cap_reach = fits ? (float)std::min(0.6 / std::fabs(r), 1e19) : -1.0f;
+    a.cap_in = (float)std::min(std::max(2.0 * kLog2e * r, -top), top);
+    a.cap_out = (float)std::min((double)kLog2e * c.cap, top / 2);
   }
   if (a.c.doc_k != nullptr) {
     a.doc_tile = tile_keys(c);

@@ -232,6 +232,21 @@ def test_attention_window_table_in_two_dimensions():
     assert not out[:, :, 1].any() and torch.isneginf(lse[:, 1]).all()
 
 
+@pytest.mark.parametrize("cap,bias", [(1e-7, False), (1e-7, True), (1e-30, False), (1e-30, True), (3e38, False)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_attention_caps_at_the_types_ends(cap, bias, zeros):
+    """tanh's argument or its polynomial's coefficients pass the type's range: a cap near 0
+    leaves all keys alike, a huge one changes nothing."""
+    q, k, v = _qkv(52, BF16, 1, 33, 100, 2, 1, 64)
+    if zeros:
+        k.zero_()
+    kw = {"slopes": torch.zeros(2, device="cuda")} if bias else {}
+    out, lse = tr.attention(q, k, v, cap=cap, return_lse=True, **kw)
+    want = ref.attention(q, torch.zeros_like(k) if cap < 1 else k, v)
+    ref.check(lse, want[1], "lse")
+    ref.check(out, want[0], "out")
+
+
 @pytest.mark.parametrize("scale,std", [(0.0, 1.0), (-0.3, 1.0), (3.0, 3.0), (1e-4, 1.0)])
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 def test_attention_scale(scale, std, cap):
