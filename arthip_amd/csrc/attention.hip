@@ -53,7 +53,7 @@ struct AttnArgs {
   int table_bytes;  // and take these
   int wide;       // keys further apart than 32-bit offsets reach
   FastDiv by_group, by_k_heads, by_row_tiles, by_splits, by_rows;
-  float cap_reach;  // |q.k| up to which the polynomial holds
+  float cap_reach;  // |q.k| up to which the polynomial of the capped scores holds
   float cap_fit[5];
   float cap_in, cap_out;  // of the exponential's argument and result
   const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
@@ -532,30 +532,32 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
-      if (SHAPE == kCap && !__any(!(far <= a.cap_reach))) {
-        // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
-        // less than 8e-8), six plain operations where the exponential and the reciprocal
-        // take a quarter of the rate each.
+      // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
+      // less than 8e-8), six plain operations where the exponential and the reciprocal
+      // take a quarter of the rate each.
+      auto near = [&](float x) __attribute__((always_inline)) -> float {
+        const float z = x * x;
+        float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
+        t = __builtin_fmaf(t, z, a.cap_fit[2]);
+        t = __builtin_fmaf(t, z, a.cap_fit[1]);
+        t = __builtin_fmaf(t, z, a.cap_fit[0]);
+        return x * t;
+      };
+      if (!__any(!(far <= a.cap_reach))) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float x = s[kb][r], z = x * x;
-            float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
-            t = __builtin_fmaf(t, z, a.cap_fit[2]);
-            t = __builtin_fmaf(t, z, a.cap_fit[1]);
-            t = __builtin_fmaf(t, z, a.cap_fit[0]);
-            s[kb][r] = x * t;
-          }
+          for (int r = 0; r < 16; ++r) s[kb][r] = near(s[kb][r]);
       } else {
-        // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2
-        const float in = a.cap_in, out = a.cap_out;
+        // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2, whose error
+        // is the cap's, not the score's: small scores keep the polynomial.
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(s[kb][r] * in);
-            s[kb][r] = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
+            const float x = s[kb][r], e = __builtin_amdgcn_exp2f(x * a.cap_in);
+            const float beyond = __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(e + 1.0f), a.cap_out);
+            s[kb][r] = fabsf(x) <= a.cap_reach ? near(x) : beyond;
           }
       }
     }

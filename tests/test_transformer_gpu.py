@@ -215,6 +215,78 @@ def test_attention_bias(lq, lk, cap):
     _attend(q, k, v, table=big, table_zero=4500, cap=cap)
 
 
+def _capped(q, k, v, scale, cap, slopes=None, table=None, table_zero=0):
+    """((out, tolerance), (lse, tolerance)) with capped scores, as transformer_reference but for
+    the cap's error: 2^-20 of the capped score, not of the cap. (cap tanh(s / cap) is no more
+    sensitive to s than s itself; the fit of tanh x / x is off by 8e-8, the form from an
+    exponential above 0.6 by a few 2^-24 of the cap, each with a few roundings.)"""
+    E = ref.E
+    lq, lk, hq, hk, dim = q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3]
+    q64, k64, v64 = (t[0].double().cpu().transpose(0, 1) for t in (q, k, v))
+    k64, v64 = (t.repeat_interleave(hq // hk, 0) for t in (k64, v64))
+    raw = torch.matmul(q64, k64.transpose(1, 2)) * scale
+    s = cap * torch.tanh(raw / cap)
+    d = dim * E * abs(scale) * torch.matmul(q64.abs(), k64.abs().transpose(1, 2)) + 4 * E * raw.abs()
+    d = torch.minimum(d, 2 * s.abs() + 2 * cap) + 2.0 ** -20 * s.abs()
+    diff = torch.arange(lk - lq, lk)[:, None] - torch.arange(lk)
+    if slopes is not None:
+        bias = -slopes.double().cpu()[:, None, None] * diff.abs()
+        s, d = s + bias, d + 4 * E * bias.abs()
+    if table is not None:
+        bias = table.double().cpu()[:, (diff + table_zero).clamp(0, table.shape[1] - 1)]
+        s, d = s + bias, d + 4 * E * bias.abs()
+    top = s.amax(-1, keepdim=True)
+    w = torch.exp(s - top)
+    total = w.sum(-1, keepdim=True)
+    w = w / total
+    dmax = (d + 4 * E * s.abs()).amax(-1, keepdim=True) + 2.0 ** -20 + 4 * E * top.abs() + lk * E
+    u = ref.UNIT[q.dtype]
+    out = torch.matmul(w, v64)
+    tol = u * out.abs() + (u + 2.2 * dmax) * torch.matmul(w, v64.abs()) \
+        + ref.TINY[q.dtype] * (1 + v64.abs().sum(1, keepdim=True))
+    lse = (torch.log(total) + top)[..., 0]
+    return (out.transpose(0, 1)[None], tol.transpose(0, 1)[None]), \
+        (lse[None], dmax[None, ..., 0] + 4 * E * lse.abs()[None])
+
+
+CAPS = [0.5, 20.0, 1e3, 1e4, 1e6, 1e10]
+
+
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("lq,d", [(1, 64), (70, 64), (40, 128)])
+@pytest.mark.parametrize("kind", ["plain", "slopes", "table", "negative"])
+def test_attention_caps_of_any_size(cap, lq, d, kind):
+    """A cap far above the scores leaves them as they are, with a bias and without."""
+    g = _gen(50)
+    q, k, v = _qkv(50, F16, 1, lq, 200, 4, 2, d)
+    kw = {"scale": 0.125, "cap": cap}
+    if kind == "slopes":
+        kw["slopes"] = torch.rand(4, generator=g).cuda() * 0.05
+    elif kind == "table":
+        kw["table"], kw["table_zero"] = _normal(g, 4, 41), 20
+    elif kind == "negative":
+        kw["scale"] = -0.125
+    out, lse = tr.attention(q, k, v, return_lse=True, **kw)
+    want = _capped(q, k, v, **kw)
+    ref.check(lse, want[1], "lse")
+    ref.check(out, want[0], "out")
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+def test_attention_small_scores_beside_capped_ones(slopes):
+    """One row whose scores reach the cap leaves the other rows' small scores exact."""
+    q, k, v = _qkv(51, BF16, 1, 40, 96, 2, 1, 64)
+    q[0, 3], k[0, 50] = 100.0, 1.0  # q . k = 6400
+    kw = {"scale": 1.0, "cap": 8e3}
+    q[0, :3], q[0, 4:] = q[0, :3] * 0.01, q[0, 4:] * 0.01
+    if slopes:
+        kw["slopes"] = torch.tensor([0.01, 0.1], device="cuda")
+    out, lse = tr.attention(q, k, v, return_lse=True, **kw)
+    want = _capped(q, k, v, **kw)
+    ref.check(lse, want[1], "lse")
+    ref.check(out, want[0], "out")
+
+
 def test_attention_window_table_in_two_dimensions():
     g = _gen(10)
     n, d = 7, 32
@@ -232,7 +304,8 @@ def test_attention_window_table_in_two_dimensions():
     assert not out[:, :, 1].any() and torch.isneginf(lse[:, 1]).all()
 
 
-@pytest.mark.parametrize("cap,bias", [(1e-7, False), (1e-7, True), (1e-30, False), (1e-30, True), (3e38, False)])
+@pytest.mark.parametrize("cap,bias", [(1e-7, False), (1e-7, True), (1e-30, False), (1e-30, True), (3e38, False),
+                                      (3e38, True)])
 @pytest.mark.parametrize("zeros", [False, True])
 def test_attention_caps_at_the_types_ends(cap, bias, zeros):
     """tanh's argument or its polynomial's coefficients pass the type's range: a cap near 0
