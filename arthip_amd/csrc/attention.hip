@@ -40,6 +40,13 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kFar = 1 << 30;
+// tanh x / x by powers of x^2, up to x = 0.6.
+constexpr double kTanh[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825,
+                             0.015486690367999443};
+// Up to this cap an error of 2^-22 caps is 2^-16 of a score, far below the rounding of the
+// weights; above it small scores take a form of their own wherever they are. (Both forms for every
+// score: causal 8192 with 32 heads of 128, scores beyond the cap, 740 -> 1069 us.)
+constexpr float kCapSmall = 64.0f;
 
 struct AttnArgs {
   arthip_attention_args c;
@@ -55,7 +62,7 @@ struct AttnArgs {
   FastDiv by_group, by_k_heads, by_row_tiles, by_splits, by_rows;
   float cap_reach;  // |q.k| up to which the polynomial of the capped scores holds
   float cap_fit[5];
-  float cap_in, cap_out;  // of the exponential's argument and result
+  float cap_in, cap_out;  // 2 log2(e) scale / cap and log2(e) cap
   const int2* doc_ranges;  // smallest and largest document of each tile, [batch, or 1][doc_tiles]
   int doc_tiles, doc_tile;  // tiles of a sequence, keys of a tile
   float* part;    // [splits][batch * k_heads * rows][D] unscaled sums, if splits > 1
@@ -220,14 +227,25 @@ __device__ __forceinline__ void ahead() {
   __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
 }
 
-// What the scores go through: nothing (the scale is in the exponent), the cap, or any
-// of cap, slopes, table and a scale that turns their order.
-enum Shape { kPlain, kCap, kAny };
+// What the scores go through: nothing (the scale is in the exponent), a cap up to kCapSmall,
+// any of such a cap, slopes, table and a scale that turns their order, or the same with a
+// larger cap.
+enum Shape { kPlain, kCap, kAny, kLarge };
+
+// cap tanh(x / cap) in the base of 2 of a score x up to 0.6 caps.
+__device__ __forceinline__ float cap_near(const AttnArgs& a, float x) {
+  const float z = x * x;
+  float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
+  t = __builtin_fmaf(t, z, a.cap_fit[2]);
+  t = __builtin_fmaf(t, z, a.cap_fit[1]);
+  t = __builtin_fmaf(t, z, a.cap_fit[0]);
+  return x * t;
+}
 
 // SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
 // tile's keys; otherwise each holds 32 rows of its own and takes all keys.
 template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
-__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 && SHAPE == kAny) ? 2 : 3)
+__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 && SHAPE >= kAny) ? 2 : 3)
     attention_tile(AttnArgs a) {
   using L = TileL<DP, KT>;
   using E = Elem<T>;
@@ -315,10 +333,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   // -- score transforms --------------------------------------------------------------
   // Without cap and bias the scale goes into the exponent's multiply-add.
   const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
-  const float slope = SHAPE == kAny && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
-  const int cq = SHAPE == kAny && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
-  const float* const table = SHAPE == kAny && a.c.table ? a.c.table : nullptr;
-  const int32_t* const code_k = SHAPE == kAny && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
+  const float slope = SHAPE >= kAny && a.c.slopes ? a.c.slopes[head] * kLog2e : 0.0f;
+  const int cq = SHAPE >= kAny && a.c.code_q ? a.c.code_q[b * a.c.code_q_stride + token] : q_start + token;
+  const float* const table = SHAPE >= kAny && a.c.table ? a.c.table : nullptr;
+  const int32_t* const code_k = SHAPE >= kAny && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
   const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
   const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
   bool hides = false;  // the table has an entry of -inf
@@ -526,42 +544,37 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   auto weights = [&](int buf, int k0, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
     const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
     const float unit = a.c.cap > 0 ? 1.0f : a.c.scale * kLog2e;  // what scores are still to be scaled by
-    if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
+    if (SHAPE == kCap || SHAPE == kLarge || (SHAPE == kAny && a.c.cap > 0)) {
       float far = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
-      // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
-      // less than 8e-8), six plain operations where the exponential and the reciprocal
-      // take a quarter of the rate each.
-      auto near = [&](float x) __attribute__((always_inline)) -> float {
-        const float z = x * x;
-        float t = __builtin_fmaf(a.cap_fit[4], z, a.cap_fit[3]);
-        t = __builtin_fmaf(t, z, a.cap_fit[2]);
-        t = __builtin_fmaf(t, z, a.cap_fit[1]);
-        t = __builtin_fmaf(t, z, a.cap_fit[0]);
-        return x * t;
-      };
-      if (!__any(!(far <= a.cap_reach))) {
+      if constexpr (SHAPE != kAny) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = near(s[kb][r]);
+          for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
+      }
+      if (SHAPE != kAny && !__any(!(far <= a.cap_reach))) {
+        // x = score / cap below 0.6: tanh x / x as a polynomial of x^2 (Chebyshev fit, off by
+        // less than 8e-8), six plain operations where the exponential and the reciprocal
+        // take a quarter of the rate each.
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] = cap_near(a, s[kb][r]);
       } else {
-        // cap tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1), in the base of 2, whose error
-        // is the cap's, not the score's: small scores keep the polynomial.
+        // cap tanh x = cap - 2 cap / (exp(2 x) + 1), in the base of 2, off by some 2^-22 of the cap.
+        const float in = a.cap_in, out = a.cap_out;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float x = s[kb][r], e = __builtin_amdgcn_exp2f(x * a.cap_in);
-            const float beyond = __builtin_fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(e + 1.0f), a.cap_out);
-            s[kb][r] = fabsf(x) <= a.cap_reach ? near(x) : beyond;
+            const float x = s[kb][r];
+            const float e = __builtin_amdgcn_exp2f(x * in);
+            const float y = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
+            s[kb][r] = SHAPE == kLarge && fabsf(x) <= a.cap_reach ? cap_near(a, x) : y;
           }
       }
     }
-    if constexpr (SHAPE == kAny) {
+    if constexpr (SHAPE >= kAny) {
       // The loops below are whole loops a branch: a uniform branch inside would be taken
       // for every score.
       const int4* const codes = reinterpret_cast<const int4*>(more + L::kCode + buf * 256 + wk * 4) + half;
@@ -1009,7 +1022,8 @@ template <class T, int DP, int KT, int NW, bool SHARED>
 TilePick pick(Shape shape) {
   return {shape == kPlain ? attention_tile<T, DP, KT, NW, SHARED, kPlain>
           : shape == kCap ? attention_tile<T, DP, KT, NW, SHARED, kCap>
-                          : attention_tile<T, DP, KT, NW, SHARED, kAny>,
+          : shape == kAny ? attention_tile<T, DP, KT, NW, SHARED, kAny>
+                          : attention_tile<T, DP, KT, NW, SHARED, kLarge>,
           NW * 64, TileL<DP, KT>::kBytes, TileL<DP, KT>::kChunk};
 }
 
@@ -1089,23 +1103,25 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
   a.part = static_cast<float*>(c.workspace);
   if (a.splits > 1) a.stat = a.part + a.splits * total * c.head_dim;
   const bool f16 = c.dtype == ARTHIP_TYPE_F16;
-  const Shape shape = c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
+  const Shape shape = c.cap > kCapSmall                                                  ? kLarge
+                      : c.slopes != nullptr || c.table != nullptr || !(c.scale > 0) ? kAny
+                      : c.cap > 0                                                   ? kCap
+                                                                                    : kPlain;
   const TilePick k = f16 ? pick<_Float16>(c.head_dim, shared, shape) : pick<__bf16>(c.head_dim, shared, shape);
   if (c.cap > 0) {
-    static constexpr double fit[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825, 0.015486690367999443};
-    // A cap near the ends of its type takes these past theirs: a coefficient that is no number
-    // leaves all scores to the exponential, squares stay below infinity (as 0 times it is NaN),
-    // and factors that a score of 0 or infinity meets stay finite.
+    // A cap near 0 takes these past their type's end: a coefficient that is no number leaves
+    // all scores to the other form, squares stay below infinity (as 0 times it is NaN), and a
+    // score of 0 meets a finite factor. One above 1e30 changes no score below 4e26.
     constexpr double top = std::numeric_limits<float>::max();
-    const double r = (double)c.scale / c.cap;
+    const double cap = std::min<double>(c.cap, 1e30), r = c.scale / cap;
     bool fits = true;
     for (int i = 0; i < 5; ++i) {
-      a.cap_fit[i] = (float)(fit[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
+      a.cap_fit[i] = (float)(kTanh[i] * std::pow(r, 2 * i) * c.scale * kLog2e);
       fits = fits && std::isfinite(a.cap_fit[i]);
     }
     a.cap_reach = fits ? (float)std::min(0.6 / std::fabs(r), 1e19) : -1.0f;
     a.cap_in = (float)std::min(std::max(2.0 * kLog2e * r, -top), top);
-    a.cap_out = (float)std::min((double)kLog2e * c.cap, top / 2);
+    a.cap_out = (float)(kLog2e * cap);
   }
   if (a.c.doc_k != nullptr) {
     a.doc_tile = tile_keys(c);
