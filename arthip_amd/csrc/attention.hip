@@ -339,15 +339,17 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   const int32_t* const code_k = SHAPE >= kAny && a.c.code_k ? a.c.code_k + b * a.c.code_k_stride : nullptr;
   const int dq = a.c.doc_q ? a.c.doc_q[b * a.c.doc_q_stride + token] : 0;
   const int32_t* const doc_k = a.c.doc_k ? a.c.doc_k + b * a.c.doc_k_stride : nullptr;
-  bool hides = false;  // the table has an entry of -inf
+  // The table has an entry of -inf; one that is not in LDS may (to read it whole costs a
+  // workgroup more than its tiles: one token over 777 keys and 32768 entries 278 us for 17).
+  bool hides = table && !a.table_lds;
   auto load_table = [&]() __attribute__((always_inline)) {
     float* const t = reinterpret_cast<float*>(more + L::kTable);
-    const int len = a.group * a.c.table_len;
+    const int len = a.group * a.c.table_len;  // kTableBytes bound it
     const float* const from = table + (int64_t)kh * len;
     bool h = false;
     for (int i = tid; i < len; i += NW * 64) {
       const float e = from[i];
-      if (a.table_lds) t[i] = e * kLog2e;
+      t[i] = e * kLog2e;
       h = h || e == -__builtin_inff();
     }
     int* const flag = reinterpret_cast<int*>(more + L::kRange);
@@ -749,7 +751,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       int i = next(c0);
       const bool nothing = i >= c1;
       if (!nothing) stage_k(0, tile_of(i));
-      if (table && !decltype(apart)::value && c0 == begin) load_table();
+      if (table && a.table_lds && !decltype(apart)::value && c0 == begin) load_table();
       if (nothing) continue;
       vm_wait();
       lds_sync();

@@ -348,6 +348,26 @@ def test_attention_hidden_values(lq, dtype):
         _attend(q, kb, vb, f"{bad} behind the table", table=table.cuda(), codes=codes)
 
 
+@pytest.mark.parametrize("lq,n", [(1, 41), (1, 9000), (70, 41), (70, 9000), (70, 2 ** 30 + 16)])
+def test_attention_hidden_values_behind_tables_of_any_size(lq, n):
+    """Tables that a workgroup keeps on the chip, that it does not, and of more than 2^31
+    entries a key head; only one of its offsets hides."""
+    q, k, v = _qkv(53, F16, 1, lq, 150, 2, 1, 64)
+    table = torch.zeros(2, n, device="cuda")
+    table[:, 20:30] = _normal(_gen(53), 2, 10)
+    table[:, 40] = -math.inf
+    hidden = torch.arange(150) % 5 == 2
+    codes = _ints([25] * lq), (hidden.int() * -15).cuda()
+    seen = ~hidden
+    want = tr.attention(q, k[:, seen], v[:, seen], table=table, codes=(codes[0], _ints([0] * int(seen.sum()))))
+    for bad in (math.nan, math.inf):
+        kb, vb = k.clone(), v.clone()
+        kb[:, hidden], vb[:, hidden] = bad, bad
+        got = tr.attention(q, kb, vb, table=table, codes=codes)
+        # The same weights in another order of the keys: two roundings of 2^-11 each, of sums of |v| < 5.
+        assert (got.double() - want.double()).abs().max() < 4 * 2 ** -11 * 5
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_hidden_from_some(bad):
     """A key that is not finite reaches the rows that see it and no other."""
