@@ -242,6 +242,13 @@ __device__ __forceinline__ float cap_near(const AttnArgs& a, float x) {
   return x * t;
 }
 
+// A table's entry in the base of 2. Only -inf hides: the least finite numbers, which masks are made
+// of, stay finite.
+__device__ __forceinline__ float entry_of(float e) {
+  const float x = e * kLog2e;
+  return x == -__builtin_inff() && e != -__builtin_inff() ? -__FLT_MAX__ : x;
+}
+
 // SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
 // tile's keys; otherwise each holds 32 rows of its own and takes all keys.
 template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     bool h = false;
     for (int i = tid; i < len; i += NW * 64) {
       const float e = from[i];
-      t[i] = e * kLog2e;
+      t[i] = entry_of(e);
       h = h || e == -__builtin_inff();
     }
     int* const flag = reinterpret_cast<int*>(more + L::kRange);
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         } else {
           const float* const t = table + (int64_t)head * a.c.table_len;
           auto add = [&](float x, int diff) __attribute__((always_inline)) {
-            const float entry = t[min(max(diff, 0), last)] * kLog2e;
+            const float entry = entry_of(t[min(max(diff, 0), last)]);
             const float sum = __builtin_fmaf(x, by, entry);
             return entry == -__builtin_inff() ? entry : sum;
           };

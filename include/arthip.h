@@ -472,10 +472,11 @@ int arthip_rope_axes(const arthip_rope_args* args, void* stream);
  *   j < prefix[b] or p_i - left <= j <= p_i + right, with p_i = q_start[b] + i.
  * cq and ck are code_q and code_k, or p_i and j without them; cq + table_zero - ck
  * has to fit 32 bits. (A two-dimensional table needs one number a token:
- * y * (2 W - 1) + x names every offset inside a window W wide.) A table entry of -inf hides its offset. A query that sees
- * nothing gives zeros, and -inf as its log-sum. Keys that a query does not see
- * add nothing to it, whatever their K and V hold, NaN and infinities among
- * them. fp16 or bf16. */
+ * y * (2 W - 1) + x names every offset inside a window W wide.) A table entry of
+ * -inf hides its offset; the lowest finite numbers do not (entries below -2.3e38
+ * count as that). A query that sees nothing gives zeros, and -inf as its log-sum.
+ * Keys that a query does not see add nothing to it, whatever their K and V hold,
+ * NaN and infinities among them. fp16 or bf16. */
 typedef struct arthip_attention_args {
   const void* q;
   const void* k;            /* may be NULL when k_tokens = 0 */

@@ -368,6 +368,28 @@ def test_attention_hidden_values_behind_tables_of_any_size(lq, n):
         assert (got.double() - want.double()).abs().max() < 4 * 2 ** -11 * 5
 
 
+@pytest.mark.parametrize("n", [41, 9000])
+@pytest.mark.parametrize("lq", [1, 70])
+def test_attention_table_of_the_types_lowest_value(lq, n):
+    """The lowest finite value weighs keys by 0 beside others, and alike where there are no
+    others: it hides nothing."""
+    q, k, v = _qkv(54, F16, 1, lq, 150, 2, 2, 32)
+    low = torch.finfo(F32).min
+    some = torch.zeros(2, n, device="cuda")
+    some[:, 7] = low
+    keys = (torch.arange(150) % 3 == 1)
+    codes = _ints([7] * lq), (keys.int() * 7).cuda()
+    out, lse = tr.attention(q, k, v, table=some, codes=codes, return_lse=True)
+    want = ref.attention(q, k[:, keys], v[:, keys])
+    ref.check(out, want[0], "out beside others")
+    ref.check(lse, want[1], "lse beside others")
+    out, lse = tr.attention(q, k, v, table=torch.full((2, n), low, device="cuda"), return_lse=True)
+    assert torch.isfinite(lse).all() and (lse < -1e38).all()
+    # Every score rounds to the same number, so all keys weigh alike.
+    want = ref.attention(q, torch.zeros_like(k), v)
+    ref.check(out, want[0], "out alone")
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_hidden_from_some(bad):
     """A key that is not finite reaches the rows that see it and no other."""
