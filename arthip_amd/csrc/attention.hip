@@ -463,10 +463,13 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   };
   auto stage_k = [&](int buf, int tile) __attribute__((always_inline)) {
     stage(kp, ks2, [&](int i) { return k_off[i % KP]; }, L::k_swizzle, tile, lds_base + buf * L::kTile);
+    // The tile's documents and codes, those past the length as zeros. (From the tile on: an offset
+    // from the first key would pass 32 bits in the longest caches.)
+    const uint32_t at = lane < kv_len - tile * KT ? lane * 4u : kOob;
     if (doc_k && wave == 0)
-      load_lds4(buffer_of(doc_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kDoc + buf * 256);
+      load_lds4(buffer_of(doc_k + (int64_t)tile * KT, 0x7fffffffu), at, 0, more_base + L::kDoc + buf * 256);
     if (code_k && wave == NW - 1)
-      load_lds4(buffer_of(code_k, (uint32_t)kv_len * 4), lane * 4, tile * KT * 4, more_base + L::kCode + buf * 256);
+      load_lds4(buffer_of(code_k + (int64_t)tile * KT, 0x7fffffffu), at, 0, more_base + L::kCode + buf * 256);
   };
   auto stage_v = [&](int buf, int tile) __attribute__((always_inline)) {
     stage(vp, vs2, [&](int i) { return v_off[i % VP]; }, L::v_swizzle, tile, lds_base + v_at + buf * L::kTile);

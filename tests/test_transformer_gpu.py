@@ -197,6 +197,26 @@ def test_attention_documents_long():
     _attend(q, k, v, docs=(doc_q, doc_k))
 
 
+@pytest.mark.parametrize("lq", [2, 40])
+def test_attention_longest_cache(lq):
+    """2^30 keys, whose documents and codes take 2^32 bytes: the last ones, in turn of the
+    query's document and of another, by their codes' distance. (K and V are one token, repeated.)"""
+    n = 2 ** 30
+    q, k, v = _qkv(55, F16, 1, lq, 1, 1, 1, 32)
+    doc_k = torch.zeros(n, dtype=torch.int32, device="cuda")
+    last = torch.arange(101, device="cuda") % 2 + 1
+    doc_k[-101:] = last
+    code_k = torch.zeros(n, dtype=torch.int32, device="cuda")
+    code_k[-101:] = torch.arange(101, device="cuda") % 7
+    slopes = torch.tensor([0.5], device="cuda")
+    doc_q, code_q = _ints([1] * lq), _ints([3] * lq)
+    far, tail = (t.expand(1, n, 1, 32) for t in (k, v)), (t.expand(1, 101, 1, 32) for t in (k, v))
+    out, lse = tr.attention(q, *far, docs=(doc_q, doc_k), codes=(code_q, code_k), slopes=slopes, return_lse=True)
+    want = ref.attention(q, *tail, docs=(doc_q, doc_k[-101:]), codes=(code_q, code_k[-101:]), slopes=slopes)
+    ref.check(out, want[0], "out")
+    ref.check(lse, want[1], "lse")
+
+
 @pytest.mark.parametrize("cap", [0.0, 5.0])
 @pytest.mark.parametrize("lq,lk", [(1, 100), (81, 81), (200, 70)])
 def test_attention_bias(lq, lk, cap):
