@@ -104,7 +104,10 @@ def _like(t, stream):
 def _empty(shape, dtype, device, stream):
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+    # An external stream of the handle 0 would be one of torch's own streams, not the default one,
+    # and the memory could be given out again there while the call still writes to it.
+    on = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(on):
         return torch.empty(shape, dtype=dtype, device=device)
 
 

@@ -296,3 +296,32 @@ def test_calls_without_queries_take_documents_and_codes(empty):
     for pair in (dict(doc_k=BUF * 8), dict(code_k=BUF * 8), dict(doc_q=BUF * 8, code_q=BUF * 8)):
         a = _attention(**empty, **pair)
         assert lib.arthip_attention(ctypes.byref(a), None) == 0, _lib.last_error()
+
+
+def test_tensors_that_a_call_makes_belong_to_its_stream(monkeypatch):
+    """The handle 0 is the default stream, which no external stream can stand for."""
+    import contextlib
+    used = []
+
+    class External:
+        def __init__(self, handle, device=None):
+            assert handle != 0
+            self.handle = handle
+
+    class Default:
+        handle = 0
+
+    @contextlib.contextmanager
+    def on(stream):
+        used.append(stream.handle)
+        yield
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", External)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: Default())
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    for handle in (0, 4096):
+        tr._empty((2, 3), torch.float32, torch.device("cpu"), handle)
+        tr._like(torch.zeros(2, 3), handle)
+    assert used == [0, 0, 4096, 4096]
+    tr._empty((2, 3), torch.float32, torch.device("cpu"), None)
+    assert len(used) == 4

@@ -668,6 +668,29 @@ def test_streams():
     assert torch.equal(o, want[2])
 
 
+def test_results_belong_to_the_calls_stream():
+    """Also where the handle is the default stream's, 0, as its users pass it."""
+    q, k, v = _qkv(31, F16, 1, 3, 3000, 4, 2, 64)
+    r = _normal(_gen(31), 1, 3, 256, dtype=F16)
+    plan, pos = tr.RopePlan((16, 16)), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    want, y = tr.attention(q, k, v), r.clone()
+
+    def owner(t):
+        at = t.data_ptr()
+        return next(s["stream"] for s in torch.cuda.memory_snapshot()
+                    if s["address"] <= at < s["address"] + s["total_size"])
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.default_stream(), side):
+        out, lse = tr.attention(q, k, v, return_lse=True, stream=stream.cuda_stream)
+        turned, _ = tr.rope_axes(q, None, pos, plan, stream=stream.cuda_stream)
+        new, h = tr.gated_norm(r, y, pre="rms", stream=stream.cuda_stream)
+        stream.synchronize()
+        assert [owner(t) for t in (out, lse, turned, new, h)] == [stream.cuda_stream] * 5
+        assert torch.equal(out, want)
+
+
 def test_graph_replays():
     case = _block_case()
     want = _run(case)
