@@ -43,11 +43,11 @@ def _float(name: str, x) -> float:
 def _int(name: str, x) -> int:
     try:
         n = int(x)
-        if n == x:
+        if n == x and -2 ** 31 <= n < 2 ** 31:
             return n
     except (TypeError, ValueError, OverflowError, RuntimeError):
         pass
-    raise EngineError(f"{name} must be a whole number")
+    raise EngineError(f"{name} must be a whole number of 32 bits")
 
 
 def _bool(name: str, x) -> bool:
@@ -116,6 +116,11 @@ def _check(name: str, t, device, dtype, dim: int | None = None) -> None:
     _need(t.device == device, f"{name} is on another device")
     _need(t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     _need(dim is None or t.dim() == dim, f"{name} must have {dim} dimensions")
+
+
+def _sizes(name: str, t) -> None:
+    """The C structs hold sizes in 32 bits, and ctypes would cut off the rest."""
+    _need(max(t.shape, default=0) < 2 ** 31, f"{name} has too many entries")
 
 
 def _inner(name: str, t) -> None:
@@ -215,6 +220,7 @@ def _rope_plan(q, k, pos, plan, q_out, k_out, inverse) -> bytes:
             _need(out is None, f"rope_axes: {name}_out without {name}")
             continue
         _check(name, t, x.device, x.dtype, 4)
+        _sizes(name, t)
         _need(t.shape[0] == batch and t.shape[1] == tokens and t.shape[3] == dim,
               "rope_axes: q and k must agree in batch, tokens and head_dim")
         _inner(name, t)
@@ -296,6 +302,7 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
     device = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check(name, t, device, q.dtype, 4)
+        _sizes(name, t)
         _inner(name, t)
     batch, q_tokens, q_heads, dim = q.shape
     k_tokens, k_heads = k.shape[1], k.shape[2]
@@ -326,6 +333,7 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
               "attention: slopes must be contiguous [Hq]")
     if table is not None:
         _check("table", table, device, torch.float32, 2)
+        _sizes("table", table)
         _need(table.shape[0] == q_heads and table.is_contiguous(),
               "attention: table must be contiguous [Hq, n]")
         _need(table.shape[1] > 0, "attention: table without entries")
@@ -428,6 +436,7 @@ def _norm_plan(given, post, pre, gate_act, residual_scale, branch_scale, eps, dt
         dtype = residual.dtype if h is None else h.dtype
     _need(dtype in _TYPES, f"gated_norm: unsupported type {dtype}")
     a = _lib.NormArgs()
+    _sizes("residual", residual)
     _inner("residual", residual)
     a.residual_stride = residual.stride()[:2]
     if y is not None:

@@ -325,3 +325,27 @@ def test_tensors_that_a_call_makes_belong_to_its_stream(monkeypatch):
     assert used == [0, 0, 4096, 4096]
     tr._empty((2, 3), torch.float32, torch.device("cpu"), None)
     assert len(used) == 4
+
+
+@pytest.mark.parametrize("kw", [dict(window=(2 ** 32 + 5, None)), dict(window=(None, 2 ** 31)), dict(table_zero=2 ** 32),
+                                dict(table_zero=-2 ** 32 + 1)])
+def test_whole_numbers_past_32_bits(launches, kw):
+    with pytest.raises(EngineError, match="window|table_zero"):
+        _use("attention", **kw)
+    assert not launches
+
+
+def test_sizes_past_32_bits(launches):
+    """Broadcast tensors can name more entries than a size of the C struct holds."""
+    n = 2 ** 32 + 4
+    one, two = _gpu(1, 1, 2, 32), _gpu(1, 4, 2, 32)
+    long = one.expand(1, n, 2, 32)
+    pos = _gpu(1, 1, 1, dtype=torch.int32)
+    row, table = _gpu(1, 1, 64), _gpu(2, 1, dtype=torch.float32)
+    for call in (lambda: tr.attention(two, long, long), lambda: tr.attention(long, two, two),
+                 lambda: tr.rope_axes(long, None, pos.expand(1, 1, n), tr.RopePlan((16,), device="cpu")),
+                 lambda: tr.gated_norm(row.expand(1, n, 64), row.expand(1, n, 64), pre="rms"),
+                 lambda: tr.gated_norm(row.expand(n, 1, 64), row.expand(n, 1, 64), pre="rms")):
+        with pytest.raises(EngineError, match="too"):
+            call()
+    assert not launches
