@@ -57,6 +57,11 @@ def _bool(name: str, x) -> bool:
         raise EngineError(f"{name} must be a truth value") from None
 
 
+def _pair(name: str, x) -> tuple:
+    _need(isinstance(x, (tuple, list)) and len(x) == 2, f"{name} must be a pair")
+    return tuple(x)
+
+
 # What a call's shapes, strides, types and options come to (checked arguments with all
 # pointers empty), so that the next call of the same kind only fills in pointers: a call
 # takes some 8 us instead of 18. Nothing in it depends on a tensor's address or contents:
@@ -254,9 +259,10 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     scale = None if scale is None else _float("attention: scale", scale)
     cap, table_zero = _float("attention: cap", cap), _int("attention: table_zero", table_zero)
     causal = _bool("attention: causal", causal)
-    window = tuple(None if w is None else _int("attention: a window's side", w) for w in window)
-    doc_q, doc_k = docs or (None, None)
-    code_q, code_k = codes or (None, None)
+    window = tuple(None if w is None else _int("attention: a window's side", w)
+                   for w in _pair("attention: window", window))
+    doc_q, doc_k = (None, None) if docs is None else _pair("attention: docs", docs)
+    code_q, code_k = (None, None) if codes is None else _pair("attention: codes", codes)
     key = ("attention", _sig(q), _sig(k), _sig(v), scale, cap, causal, window, _sig(out), return_lse)
     plain = (q_start is None and kv_len is None and prefix is None and docs is None and codes is None
              and slopes is None and table is None)
@@ -318,7 +324,7 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
     for name, pair in (("doc", docs), ("code", codes)):
         if pair is None:
             continue
-        _need(len(pair) == 2 and pair[0] is not None and pair[1] is not None,
+        _need(pair[0] is not None and pair[1] is not None,
               f"attention: {name}s is a pair of tensors (queries', keys')")
         for side, t, tokens in (("q", pair[0], q_tokens), ("k", pair[1], k_tokens)):
             _check(f"{name}_{side}", t, device, torch.int32)
@@ -388,6 +394,8 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     residual_scale = _float("gated_norm: residual_scale", residual_scale)
     branch_scale = _float("gated_norm: branch_scale", branch_scale)
     eps = _float("gated_norm: eps", eps)
+    for name in (post, pre, gate_act):
+        _need(name is None or isinstance(name, str), "gated_norm: norms and gate activations are texts")
     given = (residual, y, gate, mod_scale, mod_shift, post_weight, post_bias, pre_weight, pre_bias,
              residual_out, h)
     key = ("norm", *map(_sig, given), post, pre,

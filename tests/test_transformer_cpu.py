@@ -349,3 +349,29 @@ def test_sizes_past_32_bits(launches):
         with pytest.raises(EngineError, match="too"):
             call()
     assert not launches
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(docs=torch.zeros(2, 4, dtype=torch.int32)), "docs"), (dict(codes=torch.zeros(4, dtype=torch.int32)), "codes"),
+    (dict(docs=(None, None)), "docs"), (dict(docs=(1, 2, 3)), "docs"), (dict(codes=5), "codes"), (dict(docs=()), "docs"),
+    (dict(window=5), "window"), (dict(window=(1, 2, 3)), "window"), (dict(window=None), "window"),
+    (dict(window=torch.tensor(3)), "window"),
+])
+def test_pairs_that_are_none(launches, kw, text):
+    with pytest.raises(EngineError, match=text):
+        _use("attention", **kw)
+    assert not launches
+
+
+def test_lists_are_pairs(launches):
+    docs = [_gpu(4, dtype=torch.int32), _gpu(1, 4, dtype=torch.int32)]
+    _use("attention", docs=docs, codes=docs, window=[3, 1])
+    assert len(launches) == 1 and (launches[0].left, launches[0].right) == (3, 1)
+
+
+@pytest.mark.parametrize("name", ["post", "pre", "gate_act"])
+def test_names_that_are_none(launches, name):
+    for bad in (["rms"], {"rms": 1}, 5):
+        with pytest.raises(EngineError, match="gated_norm"):
+            tr.gated_norm(_gpu(1, 2, 64), _gpu(1, 2, 64), **{name: bad})
+    assert not launches
