@@ -27,6 +27,7 @@ struct NormArgs {
   arthip_norm_args c;
   int row_threads;  // threads of a row: 64, 128, .. 1024
   int rows;         // rows of a workgroup
+  int64_t first;    // row of the launch
   float inv_c;
   FastDiv by_tokens;
 };
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(1024) gated_norm(NormArgs a) {
   const int slot = tid / a.row_threads;
   const int lane = tid - slot * a.row_threads;
   const int64_t total = static_cast<int64_t>(a.c.batch) * a.c.tokens;
-  const int64_t index = static_cast<int64_t>(blockIdx.x) * a.rows + slot;
+  const int64_t index = a.first + static_cast<int64_t>(blockIdx.x) * a.rows + slot;
   const bool real = index < total;
   // A slot past the last row computes the last one again, so that every thread meets
   // every barrier, and writes nothing.
@@ -302,8 +303,12 @@ hipError_t launch_norm(const arthip_norm_args& c, hipStream_t s) {
       c.dtype == ARTHIP_TYPE_F32   ? norm_kernel<float, float>(n, full)
       : c.dtype == ARTHIP_TYPE_F16 ? (wide ? norm_kernel<_Float16, float>(n, full) : norm_kernel<_Float16, _Float16>(n, full))
                                    : (wide ? norm_kernel<__bf16, float>(n, full) : norm_kernel<__bf16, __bf16>(n, full));
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3((unsigned)(a.rows * a.row_threads)), 0, s, a);
-  return hipGetLastError();
+  const int threads = a.rows * a.row_threads;
+  return launch_parts(blocks, threads, [&](int64_t first, unsigned count) {
+    a.first = first * a.rows;
+    hipLaunchKernelGGL(fn, dim3(count), dim3((unsigned)threads), 0, s, a);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace arthip

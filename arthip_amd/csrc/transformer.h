@@ -6,6 +6,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -31,6 +32,18 @@ std::string check_norm(const arthip_norm_args& a);
 hipError_t launch_rope(const arthip_rope_args& a, hipStream_t s);
 hipError_t launch_norm(const arthip_norm_args& a, hipStream_t s);
 hipError_t launch_attention(const arthip_attention_args& a, hipStream_t s);
+
+// Launches a grid of any size: launch(first, count) for runs of workgroups whose threads
+// number fewer than 2^32, which is as many as HIP takes along a dimension.
+template <class F>
+hipError_t launch_parts(int64_t blocks, int threads, F launch) {
+  const int64_t most = ((int64_t{1} << 32) - 1) / threads;
+  for (int64_t first = 0; first < blocks; first += most) {
+    const hipError_t e = launch(first, static_cast<unsigned>(std::min(most, blocks - first)));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 
 // How attention divides its work (attention.hip); of arguments whose shape is checked.
 struct AttnPlan {

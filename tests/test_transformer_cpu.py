@@ -6,6 +6,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -375,3 +378,17 @@ def test_names_that_are_none(launches, name):
         with pytest.raises(EngineError, match="gated_norm"):
             tr.gated_norm(_gpu(1, 2, 64), _gpu(1, 2, 64), **{name: bad})
     assert not launches
+
+
+def test_launches_of_more_threads_than_one_takes(tmp_path):
+    """launch_parts of transformer.h, host code only, built with g++ (tests/launch_parts.cc)."""
+    gxx = shutil.which("g++")
+    if gxx is None or not Path("/opt/rocm/include/hip/hip_runtime.h").exists():
+        pytest.skip("g++ or the HIP headers are not available")
+    here = Path(__file__).resolve().parent
+    exe = tmp_path / "launch_parts"
+    subprocess.run([gxx, "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I",
+                    str(here.parent / "arthip_amd" / "csrc"), str(here / "launch_parts.cc"), "-o", str(exe)],
+                   check=True, capture_output=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr

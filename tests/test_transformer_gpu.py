@@ -617,6 +617,20 @@ def test_gated_norm_large_mean_and_zeros():
     assert torch.isnan(tr.gated_norm(zero, pre="rms", eps=0.0)[1]).all()
 
 
+def test_gated_norm_more_rows_than_a_launch_takes():
+    """2^26 rows of a wave each number 2^32 threads."""
+    n = 2 ** 26 + 5
+    r = _normal(_gen(23), 4099, 8, dtype=F16).repeat(n // 4099 + 1, 1)[:n][None]
+    new, h = tr.gated_norm(r, pre="rms", residual_scale=0.5)
+    want = ref.gated_norm(r[:, :4099], pre="rms", residual_scale=0.5)
+    ref.check(new[:, :4099], want[0], "residual")
+    ref.check(h[:, :4099], want[1], "h")
+    for got in (new, h):  # the rows repeat, so do the results
+        whole = n // 4099 * 4099
+        assert torch.equal(got[0, :whole].view(-1, 4099, 8), got[0, :4099].expand(n // 4099, -1, -1))
+        assert torch.equal(got[0, whole:], got[0, :n - whole])
+
+
 def test_gated_norm_rows_do_not_mix():
     """A row of NaN stays one row, also where rows share a workgroup."""
     for c in (64, 72, 700, 1024):
