@@ -31,6 +31,7 @@ struct RopeArgs {
   int groups;     // threads of a token and unit, heads dealt out in turn
   int per_token;  // units * groups
   int per_block;  // tokens of a workgroup
+  int64_t first;  // token of the launch
 };
 
 // sin and cos of 2 pi x, |x| <= 1/2. The nearest quarter turn comes off exactly, the
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_axes(RopeArgs a) {
   const int rest = tid - slot * a.per_token;
   const int group = rest / a.units;
   const int unit = rest - group * a.units;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * a.per_block + slot;
+  const int64_t token = a.first + static_cast<int64_t>(blockIdx.x) * a.per_block + slot;
   if (slot >= a.per_block || token >= static_cast<int64_t>(a.c.batch) * a.c.tokens) return;
   const uint32_t b = static_cast<uint32_t>(token) / static_cast<uint32_t>(a.c.tokens);
   const uint32_t t = static_cast<uint32_t>(token) - b * static_cast<uint32_t>(a.c.tokens);
@@ -169,8 +170,11 @@ hipError_t launch_rope(const arthip_rope_args& c, hipStream_t s) {
   void (*fn)(RopeArgs) = c.dtype == ARTHIP_TYPE_F16    ? rope_kernel<_Float16>(v, c.pairs != 0)
                          : c.dtype == ARTHIP_TYPE_BF16 ? rope_kernel<__bf16>(v, c.pairs != 0)
                                                        : rope_kernel<float>(v, c.pairs != 0);
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(kRopeThreads), 0, s, a);
-  return hipGetLastError();
+  return launch_parts(blocks, kRopeThreads, [&](int64_t first, unsigned count) {
+    a.first = first * a.per_block;
+    hipLaunchKernelGGL(fn, dim3(count), dim3(kRopeThreads), 0, s, a);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace arthip

@@ -97,6 +97,20 @@ def test_rope_in_place_strides_and_one_side(pairs):
     ref.check(got, ref.rope(q, full, plan.axis, plan.freqs, pairs), "permuted")
 
 
+def test_rope_more_tokens_than_a_launch_takes():
+    """An odd number of pairs goes value by value: 2^24 tokens of 255 pairs take 2^32 threads."""
+    n, step = 2 ** 24 + 3, 1021
+    q, _, pos = _rope_case(F16, 1, step, 1, 1, 510, (255,))
+    plan = tr.RopePlan((255,))
+    want = tr.rope_axes(q, None, pos, plan)[0]
+    ref.check(want, ref.rope(q, pos, plan.axis, plan.freqs), "q")
+    far = q.repeat(1, n // step + 1, 1, 1)[:, :n]
+    tr.rope_axes(far, None, pos.repeat(1, 1, n // step + 1)[:, :, :n], plan, q_out=far)
+    for first in (0, 2 ** 23 // step * step, (n // step - 1) * step, n // step * step):
+        got = far[:, first:first + step]
+        assert torch.equal(got, want[:, :got.shape[1]]), first
+
+
 def test_rope_inverse_is_the_transpose():
     q, k, pos = _rope_case(F32, 1, 40, 2, 2, 64, (16, 16))
     plan = tr.RopePlan((16, 16), theta=500.0)
