@@ -909,8 +909,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 
 // Smallest and largest document of each tile of keys: a wave a tile. (Looked over by
 // every workgroup instead, the documents of 16384 keys took each some 30 us.)
-__global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int64_t total) {
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ void __launch_bounds__(256) attention_docs(AttnArgs a, int2* out, int64_t first_block, int64_t total) {
+  const int64_t at = (first_block + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (at >= total) return;
   const int lane = threadIdx.x & 63;
   const int64_t b = at / a.doc_tiles, first = (at - b * a.doc_tiles) * a.doc_tile;
@@ -1141,8 +1141,10 @@ hipError_t launch_attention(const arthip_attention_args& c, hipStream_t s) {
     int2* const ranges = reinterpret_cast<int2*>(a.splits > 1 ? a.stat + 2 * a.splits * total : a.part);
     const int64_t n = (int64_t)(c.doc_k_stride == 0 ? 1 : c.batch) * a.doc_tiles;
     a.doc_ranges = ranges;
-    hipLaunchKernelGGL(attention_docs, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a, ranges, n);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = launch_parts((n + 3) / 4, 256, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL(attention_docs, dim3(count), dim3(256), 0, s, a, ranges, first, n);
+      return hipGetLastError();
+    });
     if (e != hipSuccess) return e;
   }
   const int64_t table = c.table == nullptr ? 0 : (int64_t)a.group * c.table_len * 4;

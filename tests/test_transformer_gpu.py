@@ -231,6 +231,21 @@ def test_attention_longest_cache(lq):
     ref.check(lse, want[1], "lse")
 
 
+def test_attention_documents_of_several_longest_caches():
+    """Two sequences of 2^30 keys have 2^26 tiles, whose documents take 2^32 threads to look over.
+    (The second one's documents are the first's, four keys on.)"""
+    n = 2 ** 30
+    q, k, v = _qkv(56, BF16, 2, 1, 1, 1, 1, 32)
+    store = torch.zeros(n + 4, dtype=torch.int32, device="cuda")
+    store[-50:] = torch.arange(50, device="cuda") % 2 + 1
+    docs = (_ints([[1], [2]]), store.as_strided((2, n), (4, 1)))
+    out, lse = tr.attention(q, k.expand(2, n, 1, 32), v.expand(2, n, 1, 32), docs=docs, return_lse=True)
+    tail = [t.expand(2, 50, 1, 32) for t in (k, v)]
+    want = ref.attention(q, *tail, docs=(docs[0], docs[1][:, -50:]))
+    ref.check(out, want[0], "out")
+    ref.check(lse, want[1], "lse")
+
+
 @pytest.mark.parametrize("cap", [0.0, 5.0])
 @pytest.mark.parametrize("lq,lk", [(1, 100), (81, 81), (200, 70)])
 def test_attention_bias(lq, lk, cap):
