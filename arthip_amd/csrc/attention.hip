@@ -249,6 +249,15 @@ __device__ __forceinline__ float entry_of(float e) {
   return x == -__builtin_inff() && e != -__builtin_inff() ? -__FLT_MAX__ : x;
 }
 
+// A mean of finite values stays in their type's range: the weights' rounding (2^-11) can take one of
+// fp16's largest numbers out of it.
+template <class T>
+__device__ __forceinline__ float in_range(float x) {
+  if constexpr (std::is_same_v<T, _Float16>)
+    return fabsf(x) < __builtin_inff() ? __builtin_amdgcn_fmed3f(x, -65504.0f, 65504.0f) : x;
+  return x;
+}
+
 // SHARED: the waves of a workgroup hold the same (up to) 32 rows and divide each
 // tile's keys; otherwise each holds 32 rows of its own and takes all keys.
 template <class T, int DP, int KT, int NW, bool SHARED, Shape SHAPE>
@@ -894,7 +903,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         for (int j = 0; j < 2; ++j) {
           typedef float f2 __attribute__((ext_vector_type(2)));
           typedef T t2 __attribute__((ext_vector_type(2)));
-          const f2 pair = {o[db][4 * (g + e) + 2 * j] * scale, o[db][4 * (g + e) + 2 * j + 1] * scale};
+          const f2 pair = {in_range<T>(o[db][4 * (g + e) + 2 * j] * scale),
+                           in_range<T>(o[db][4 * (g + e) + 2 * j + 1] * scale)};
           w[e][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, t2));
         }
       const u2 x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
@@ -968,7 +978,9 @@ __global__ void __launch_bounds__(256) attention_join(AttnArgs a) {
     T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
                   head * a.c.out_stride[2];
     typedef T t4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o * scale, t4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = in_range<T>(o[e] * scale);
+    *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o, t4);
   }
   if (a.c.lse && tid == 0)
     a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
@@ -1017,7 +1029,9 @@ __global__ void __launch_bounds__(256) attention_join_few(AttnArgs a) {
   T* const op = static_cast<T*>(a.c.out) + b * a.c.out_stride[0] + token * a.c.out_stride[1] +
                 head * a.c.out_stride[2];
   typedef T t4 __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<t4*>(op + 4 * quad) = __builtin_convertvector(o * scale, t4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = in_range<T>(o[e] * scale);
+  *reinterpret_cast<t4*>(op + 4 * quad) = __builtin_convertvector(o, t4);
   if (a.c.lse && quad == 0)
     a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
         (top + __builtin_amdgcn_logf(l)) * kLn2;

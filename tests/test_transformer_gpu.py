@@ -454,6 +454,23 @@ def test_attention_hidden_from_some(bad):
     assert torch.isfinite(out[:, :70]).all() and torch.isnan(out[:, 70:]).all()
 
 
+@pytest.mark.parametrize("lq,lk", [(1, 64), (40, 200), (1, 4000)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_values_at_the_types_end(lq, lk, sign):
+    """A mean of fp16's largest number is that number, also where the weights' own rounding
+    (here up, by 2^-11) makes more of it."""
+    q = torch.zeros(1, lq, 1, 8, dtype=F16, device="cuda")
+    k = torch.zeros(1, lk, 1, 8, dtype=F16, device="cuda")
+    q[..., 0], k[:, 0, :, 0] = 1, 1
+    v = torch.full_like(k, sign * torch.finfo(F16).max)
+    # All keys but the first weigh 0.500245, next to the middle of two fp16 numbers.
+    out = tr.attention(q, k, v, scale=-math.log(0.500245))
+    assert torch.equal(out, v[:, :1].expand(1, lq, 1, 8))
+    v[:, :, :, 3] = math.inf
+    out = tr.attention(q, k, v, scale=-math.log(0.500245))
+    assert torch.isposinf(out[..., 3]).all() and torch.equal(out[..., 4:], v[:, :1, :, 4:].expand(1, lq, 1, 4))
+
+
 def test_attention_layouts():
     """Heads before tokens, one projection's views, a broadcast key, gaps between tokens."""
     g = _gen(14)
