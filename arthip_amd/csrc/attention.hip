@@ -74,6 +74,7 @@ struct Elem;
 template <>
 struct Elem<_Float16> {
   typedef h8 frag;
+  static constexpr float kZero = 0x1p-25f;  // numbers of 0 and more up to here round to 0
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -81,6 +82,7 @@ struct Elem<_Float16> {
 template <>
 struct Elem<__bf16> {
   typedef b8 frag;
+  static constexpr float kZero = 0.0f;  // as the exponential's are 2^-126 or more, or 0
   static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -538,7 +540,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
     ahead<KW / 16 * DB, 2>();
   };
-  // The same key by key, each added only to the rows that weigh it.
+  // The same key by key, each added only to the rows that see it. (Weights that round to 0 are -0
+  // there, as an infinity or NaN counts with any weight; those of hidden keys are +0.)
   auto values_apart = [&](int buf) __attribute__((always_inline)) {
     lds_byte* const at = lds0 + v_at + buf * L::kTile;
 #pragma unroll
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
         for (int e = 0; e < 4; ++e) keep[e] = half != of || j >> 1 != e ? 0u : j & 1 ? 0xffff0000u : 0x0000ffffu;
         const u4 one = __builtin_bit_cast(u4, p[kk]) & keep;
-        const float sees = halves_max(((one[0] | one[1] | one[2] | one[3]) & 0x7fff7fffu) != 0 ? 1.0f : 0.0f);
+        const float sees = halves_max((one[0] | one[1] | one[2] | one[3]) != 0 ? 1.0f : 0.0f);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const u4 x = __builtin_bit_cast(u4, v_frag(at + (v_lane ^ (db * 64)), kk)) & keep;
@@ -562,7 +565,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   };
 
   // -- scores to weights -----------------------------------------------------------------
-  auto weights = [&](int buf, int k0, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
+  auto weights = [&](auto apart, int buf, int k0, bool partial, int t_dmin, int t_dmax) __attribute__((always_inline)) {
     const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
     const float unit = a.c.cap > 0 ? 1.0f : a.c.scale * kLog2e;  // what scores are still to be scaled by
     if (SHAPE == kCap || SHAPE == kLarge || (SHAPE == kAny && a.c.cap > 0)) {
@@ -720,8 +723,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], mul, -base));
-        sum += s[kb][r];
+        const float x = s[kb][r], w = __builtin_amdgcn_exp2f(__builtin_fmaf(x, mul, -base));
+        sum += w;
+        s[kb][r] = decltype(apart)::value && w <= E::kZero && x != -__builtin_inff() ? -0.0f : w;
       }
     l += sum;  // this half's keys; the halves are added at the end
 #pragma unroll
@@ -803,7 +807,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
             values(buf ^ 1, look);
         }
         if (!live) break;
-        if (seen) weights(buf, k0, partial, t_dmin, t_dmax);
+        if (seen) weights(apart, buf, k0, partial, t_dmin, t_dmax);
         has = seen;
         look = partial || hides;
         vm_wait();

@@ -471,6 +471,23 @@ def test_attention_values_at_the_types_end(lq, lk, sign):
     assert torch.isposinf(out[..., 3]).all() and torch.equal(out[..., 4:], v[:, :1, :, 4:].expand(1, lq, 1, 4))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("depth", [20.0, 200.0])
+def test_attention_seen_values_of_small_weight(dtype, bad, depth):
+    """A value that is not finite reaches the rows that see it also where its weight rounds
+    to 0, in tiles that other rows do not see whole."""
+    q, k, v = _qkv(57, dtype, 1, 100, 100, 2, 1, 64)
+    q[..., 0], k[..., 0] = 1, 0
+    k[0, 70, 0] = 0
+    k[0, 70, 0, 0] = -depth  # e^-depth beside the others
+    v[0, 70, 0, 5] = bad
+    out = tr.attention(q, k, v, causal=True, scale=1.0)
+    assert torch.isfinite(out[:, :70]).all()
+    assert not torch.isfinite(out[0, 71:, :, 5]).any()
+    assert torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 6:]).all()
+
+
 def test_attention_layouts():
     """Heads before tokens, one projection's views, a broadcast key, gaps between tokens."""
     g = _gen(14)
