@@ -4,11 +4,13 @@ layouts, lengths, masks, strides, streams, graphs and values that are not finite
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
+from arthip_amd import _lib
 from arthip_amd import transformer as tr
 from arthip_amd.engine import EngineError
 from tests import transformer_reference as ref
@@ -850,3 +852,68 @@ def test_refusals():
         with pytest.raises(EngineError, match=text):
             tr.gated_norm(r, args.pop("y"), **args)
     assert torch.isfinite(tr.attention(q, k, v)).all()  # nothing was left behind
+
+
+# -- strides that torch cannot make -----------------------------------------------------------------
+
+def _flipped(t, dims):
+    """t's values in memory that goes backwards along some dimensions: (memory, address, strides)."""
+    mem = t.flip(dims).contiguous()
+    strides = list(mem.stride())
+    at = mem.data_ptr()
+    for d in dims:
+        at += (t.shape[d] - 1) * strides[d] * t.element_size()
+        strides[d] = -strides[d]
+    return mem, at, strides
+
+
+@pytest.mark.parametrize("dims", [(0,), (1,), (2,), (0, 1, 2)])
+def test_negative_strides(dims):
+    """Through the C entry points: every tensor backwards along the dimensions, outputs too."""
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for lq, lk in ((1, 70), (70, 70), (150, 1000)):
+        q, k, v = _qkv(60, F16, 2, lq, lk, 4, 2, 64)
+        want = tr.attention(q, k, v, causal=True)
+        a = _lib.AttentionArgs()
+        kept = []
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", torch.zeros_like(q))):
+            mem, at, strides = _flipped(t, dims)
+            kept.append(mem)
+            setattr(a, name, at)
+            setattr(a, name + "_stride", tuple(strides[:3]))
+        a.scale, a.left, a.right = 0.125, -1, 0
+        a.batch, a.q_tokens, a.k_tokens, a.q_heads, a.k_heads, a.head_dim = 2, lq, lk, 4, 2, 64
+        work = torch.empty(lib.arthip_attention_workspace(ctypes.byref(a)), dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+        assert lib.arthip_attention(ctypes.byref(a), stream) == 0, _lib.last_error()
+        assert torch.equal(kept[3].flip(dims), want), (lq, lk)
+
+    q, k, pos = _rope_case(BF16, 2, 9, 3, 3, 64, (8, 24))
+    plan = tr.RopePlan((8, 24))
+    want = tr.rope_axes(q, k, pos, plan)
+    a = _lib.RopeArgs()
+    kept = {}
+    for name, t in (("q", q), ("k", k), ("q_out", torch.zeros_like(q)), ("k_out", torch.zeros_like(k))):
+        kept[name], at, strides = _flipped(t, dims)
+        setattr(a, name, at)
+        setattr(a, name + "_stride", tuple(strides[:3]))
+    kept["pos"], a.pos, strides = _flipped(pos, dims)
+    a.pos_stride, a.packed = tuple(strides), plan.packed.data_ptr()
+    a.n_freq, a.dtype, a.batch, a.tokens, a.q_heads, a.k_heads, a.head_dim = 32, 1, 2, 9, 3, 3, 64
+    assert lib.arthip_rope_axes(ctypes.byref(a), stream) == 0, _lib.last_error()
+    assert torch.equal(kept["q_out"].flip(dims), want[0]) and torch.equal(kept["k_out"].flip(dims), want[1])
+
+    rows = [d for d in dims if d < 2] or [0, 1]
+    g = _gen(61)
+    r, y, gate = (_normal(g, 2, 9, 200, dtype=F16) for _ in range(3))
+    want = tr.gated_norm(r, y, post="rms", gate=gate, gate_act="tanh", pre="layer")
+    a = _lib.NormArgs()
+    for name, t in (("residual", r), ("y", y), ("gate", gate), ("residual_out", torch.zeros_like(r)),
+                    ("h", torch.zeros_like(r))):
+        kept[name], at, strides = _flipped(t, rows)
+        setattr(a, name, at)
+        setattr(a, name + "_stride", tuple(strides[:2]))
+    a.post, a.pre, a.gate_act, a.batch, a.tokens, a.channels = 1, 2, 2, 2, 9, 200
+    a.eps, a.residual_scale, a.branch_scale = 1e-6, 1.0, 1.0
+    assert lib.arthip_gated_norm(ctypes.byref(a), stream) == 0, _lib.last_error()
+    assert torch.equal(kept["residual_out"].flip(rows), want[0]) and torch.equal(kept["h"].flip(rows), want[1])
