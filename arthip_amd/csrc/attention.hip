@@ -39,7 +39,6 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kFar = 1 << 30;
 // tanh x / x by powers of x^2, up to x = 0.6.
 constexpr double kTanh[5] = {0.9999999283998549, -0.33332323371192635, 0.13310358022610624, -0.05210962448570825,
                              0.015486690367999443};
@@ -305,8 +304,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   auto token_of = [&](int row) __attribute__((always_inline)) { return (int)fdiv((uint32_t)row, a.by_group); };
   auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int kv_len = scalar(a.c.kv_len ? min(max(a.c.kv_len[b], 0), a.c.k_tokens) : a.c.k_tokens);
-  const int q_start =
-      scalar(a.c.q_start ? min(max(a.c.q_start[b], -kFar), kFar) : a.c.k_tokens - a.c.q_tokens);
+  const int q_start = scalar(a.c.q_start ? a.c.q_start[b] : a.c.k_tokens - a.c.q_tokens);
   const int pre = scalar(a.c.prefix ? min(max(a.c.prefix[b], 0), kv_len) : 0);
   // Keys [lo, hi) that a window leaves to a token (and those below pre).
   auto low = [&](int token) __attribute__((always_inline)) -> int {

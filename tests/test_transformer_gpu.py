@@ -172,6 +172,20 @@ def test_attention_window(window):
     _attend(q, k, v, window=window, q_start=_ints([500]))
 
 
+@pytest.mark.parametrize("lq", [1, 90])
+def test_attention_positions_far_from_the_keys(lq):
+    """Positions of 31 bits keep their place: a window ends before the keys or reaches them."""
+    q, k, v = _qkv(58, F16, 2, lq, 100, 2, 1, 32)
+    top = 2 ** 31 - 200
+    reach = 2 ** 30
+    for start, window in ((top, (reach, None)), (top, (reach, 0)), (-top, (None, reach)), (-top, (0, reach))):
+        out, lse = tr.attention(q, k, v, window=window, q_start=_ints([start, start]), return_lse=True)
+        assert not out.any() and torch.isneginf(lse).all(), (start, window)
+    _attend(q, k, v, window=(reach, None), q_start=_ints([reach, reach + 50]))
+    _attend(q, k, v, window=(None, reach), q_start=_ints([-reach, -reach + 50]))
+    _attend(q, k, v, window=(None, 0), q_start=_ints([top, -top]))
+
+
 @pytest.mark.parametrize("lq", [1, 5, 140])
 def test_attention_prefix_and_lengths(lq):
     q, k, v = _qkv(6, BF16, 4, lq, 190, 4, 2, 64)
