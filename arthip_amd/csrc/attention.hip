@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const char* const p = reinterpret_cast<const char*>(from) + (int64_t)tile * KT * stride;
     const int left = kv_len - tile * KT;  // keys past the length come as zeros
     const uint32_t to_wave = to + wave * LOADS * 1024;
-    if (!a.wide) {
+    if (__builtin_expect(!a.wide, 1)) {
       constexpr int N = LOADS < 4 ? LOADS : 4;
       static_assert(LOADS % N == 0, "whole blocks of loads");
       const rsrc_t r = buffer_of(p - BACK, 0x7fffffffu);
@@ -474,11 +474,12 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     stage(kp, ks2, [&](int i) { return k_off[i % KP]; }, L::k_swizzle, tile, lds_base + buf * L::kTile);
     // The tile's documents and codes, those past the length as zeros. (From the tile on: an offset
     // from the first key would pass 32 bits in the longest caches.)
-    const uint32_t at = lane < kv_len - tile * KT ? lane * 4u : kOob;
     if (doc_k && wave == 0)
-      load_lds4(buffer_of(doc_k + (int64_t)tile * KT, 0x7fffffffu), at, 0, more_base + L::kDoc + buf * 256);
+      load_lds4(buffer_of(doc_k + (int64_t)tile * KT, (uint32_t)min(kv_len - tile * KT, KT) * 4), lane * 4, 0,
+                more_base + L::kDoc + buf * 256);
     if (code_k && wave == NW - 1)
-      load_lds4(buffer_of(code_k + (int64_t)tile * KT, 0x7fffffffu), at, 0, more_base + L::kCode + buf * 256);
+      load_lds4(buffer_of(code_k + (int64_t)tile * KT, (uint32_t)min(kv_len - tile * KT, KT) * 4), lane * 4, 0,
+                more_base + L::kCode + buf * 256);
   };
   auto stage_v = [&](int buf, int tile) __attribute__((always_inline)) {
     stage(vp, vs2, [&](int i) { return v_off[i % VP]; }, L::v_swizzle, tile, lds_base + v_at + buf * L::kTile);
@@ -816,7 +817,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     }
   };
   walk(std::false_type{});
-  // A workgroup that met such a tile starts over and takes the keys one by one.
+  // A workgroup that met such a tile starts over and takes the keys one by one. (Rarely, and so it
+  // is called: this and `wide` hold scalar registers against the loop otherwise, 465 us for 450
+  // in windows.)
   {
     int* const flag = reinterpret_cast<int*>(more + L::kRange);
     lds_sync();
@@ -825,7 +828,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     lds_sync();
     int again = 0;
     for (int i = 0; i < NW; ++i) again |= flag[i];
-    if (__builtin_amdgcn_readfirstlane(again) != 0) {
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(again) != 0, 0)) {
 #pragma unroll
       for (int i = 0; i < DB; ++i) o[i] = f16v{};
       m = -__builtin_inff();
