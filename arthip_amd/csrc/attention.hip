@@ -1095,11 +1095,23 @@ AttnPlan attention_plan(const arthip_attention_args& c) {
   if (c.left >= 0 && c.right >= 0 && c.prefix == nullptr)
     tiles = std::min<int64_t>(tiles, ((int64_t)c.left + c.right + std::min<int64_t>(c.q_tokens, per)) / kt + 2);
   // Ranges: enough workgroups for the chip (one-wave workgroups fit a CU four at a time,
-  // those of four waves two), of at least four tiles. From half of that number on only
-  // long walks are divided: 256 items of 64 tiles 91 -> 64 us, of 128 tiles 213 -> 133 us,
-  // but 260 of 25 tiles 54 -> 57 us.
-  const int64_t want = shared_rows(c) ? 1024 : 512;
-  if (items < want / 2 || (items < want && tiles >= 32))
+  // those of four waves two), of at least four tiles. From half of that number on walks of 32
+  // tiles or more are divided where the halves take fewer turns of the chip than half of the
+  // whole ones', by the workgroups that it holds at once: with four waves two a CU, three for
+  // heads of up to 64 (with a bias 32), one above 128. Whole and halved, us:
+  //   four waves, heads of 128: 256 items 32 tiles 65, 56; 260 items 70, 87, 64 tiles 131, 150
+  //   heads of 64: 300 items 64 tiles 95, 79; 400 items 95, 114. Of 256: 260 items 287, 248; 400 288, 331
+  //   one wave, heads of 128: 512 items 32 tiles 51, 49; 520 items 52, 68. Of 64: 640 items 64 tiles
+  //   73, 70; 704 items 79, 83. Of 32: 640 items 64 tiles 55, 59, 128 tiles 125, 112
+  const bool shared = shared_rows(c);
+  const int64_t want = shared ? 1024 : 512;
+  const bool biased = c.slopes != nullptr || c.table != nullptr || c.cap > kCapSmall;
+  const bool five = c.head_dim == 64 || (c.head_dim <= 32 && tiles >= 128);
+  const int64_t slots = c.head_dim > 128 ? 256
+                        : shared         ? (five ? 1280 : 1024)
+                                         : (c.head_dim <= (biased ? 32 : 64) ? 768 : 512);
+  const bool halve = tiles >= 32 && (2 * items + slots - 1) / slots < 2 * ((items + slots - 1) / slots);
+  if (items < want / 2 || (items < want && halve))
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(want + items - 1) / items, tiles / 4, 64}));
   p.range = (int)std::max<int64_t>(1, (tiles + p.splits - 1) / p.splits);
   if (p.splits > 1)

@@ -350,8 +350,9 @@ def _attention_plan(q, k, v, scale, cap, causal, window, q_start, kv_len, prefix
         _need(side is None or side >= 0, "attention: a window counts keys")
     a.left = -1 if left is None else left
     a.right = 0 if causal else -1 if right is None else right
-    if prefix is not None:
-        a.prefix = 16
+    for name, t in (("prefix", prefix), ("slopes", slopes), ("table", table)):
+        if t is not None:
+            setattr(a, name, 16)
     a.scale = 1.0 / math.sqrt(dim) if scale is None else scale
     a.cap = cap
     a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]

@@ -511,8 +511,9 @@ typedef struct arthip_attention_args {
   int32_t head_dim;         /* a multiple of 8 up to 256 */
 } arthip_attention_args;
 
-/* Bytes of workspace that arthip_attention needs for these arguments (0 when the
- * keys are not split, or the call refuses the shape; pointers are not read). */
+/* Bytes of workspace that arthip_attention needs for these arguments: for the parts of
+ * keys that are split, and for documents. 0 where there is neither, or the call refuses
+ * the shape. Of pointers it counts which are given; they are not read. */
 size_t arthip_attention_workspace(const arthip_attention_args* args);
 int arthip_attention(const arthip_attention_args* args, void* stream);
 

@@ -392,3 +392,26 @@ def test_launches_of_more_threads_than_one_takes(tmp_path):
                    check=True, capture_output=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("rows,heads,dim,more,split", [
+    (13 * 128, 20, 128, {}, False),  # 260 workgroups of a CU's two: their halves would take three turns
+    (16 * 128, 16, 128, {}, True), (20 * 128, 15, 64, {}, True), (20 * 128, 20, 64, {}, False),
+    (20 * 128, 15, 64, dict(slopes=BUF * 8), False), (20 * 128, 15, 64, dict(cap=100.0), False),
+    (20 * 128, 15, 32, dict(slopes=BUF * 8), True), (1, 512, 128, {}, True), (1, 640, 128, {}, False),
+    (13 * 128, 20, 256, {}, True), (16 * 128, 16, 256, {}, False), (25 * 128, 20, 256, {}, False),
+    (1, 640, 64, {}, True), (1, 672, 64, {}, False), (1, 576, 48, {}, False), (1, 512, 256, {}, False),
+])
+def test_attention_divides_long_walks_into_what_the_chip_holds_at_once(rows, heads, dim, more, split):
+    a = _attention(batch=1, q_tokens=rows, k_tokens=4096, q_heads=heads, k_heads=heads, head_dim=dim, **more)
+    assert (_lib.lib().arthip_attention_workspace(ctypes.byref(a)) > 0) == split
+
+
+def test_attention_workspace_counts_the_bias(launches):
+    """The Python layer sizes the workspace for the call's own arguments."""
+    q, k = _gpu(1, 20 * 128, 15, 64), _gpu(1, 4096, 15, 64)
+    for kw in (dict(slopes=_gpu(15, dtype=torch.float32)), dict(table=_gpu(15, 5, dtype=torch.float32)), dict(cap=100.0)):
+        tr.attention(q, k, k, **kw)
+        assert not launches[-1].workspace
+    tr.attention(q, k, k)
+    assert launches[-1].workspace_bytes > 0
