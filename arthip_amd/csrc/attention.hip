@@ -13,8 +13,8 @@
 // V's rows are fetched in the accumulator's order, by transposing LDS reads.)
 //
 // Statistics are fp32 in the base of 2. P is rounded to the element type for the
-// second product (it lies in [0, 256], see weights()); its sum is taken before the
-// rounding. fp16 and bf16 run alike: 8192 x 8192 keys, 32 heads of 128: 1135 us, 969
+// second product (it lies in [0, 2^8], fp16's in [0, 2^15], see weights()); its sum is taken
+// before the rounding. fp16 and bf16 run alike: 8192 x 8192 keys, 32 heads of 128: 1135 us, 969
 // TFLOP/s, 79% of a large library product; heads of 64: 664 us, bound by the vector work
 // of the exponentials; one token over 16384 keys: 4.8 TB/s.
 
@@ -74,6 +74,7 @@ template <>
 struct Elem<_Float16> {
   typedef h8 frag;
   static constexpr float kZero = 0x1p-25f;  // numbers of 0 and more up to here round to 0
+  static constexpr float kRaise = 7.0f;     // weights are up to 2^(8 + 7), see weights()
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -82,6 +83,7 @@ template <>
 struct Elem<__bf16> {
   typedef b8 frag;
   static constexpr float kZero = 0.0f;  // as the exponential's are 2^-126 or more, or 0
+  static constexpr float kRaise = 0.0f;
   static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -716,7 +718,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] *= f;
     }
-    const float base = m == -__builtin_inff() ? 0.0f : m * mul;
+    // fp16's weights are raised to the top of its range, so that small ones, of which a long
+    // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
+    const float base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -887,7 +891,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
           *reinterpret_cast<f4*>(p + d) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
       }
     if (half == 0) {
-      a.stat[2 * at] = m * mul;
+      a.stat[2 * at] = m * mul - E::kRaise;
       a.stat[2 * at + 1] = l;
     }
     return;
@@ -919,7 +923,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     }
   if (a.c.lse && real && half == 0)
     a.c.lse[((int64_t)b * a.c.q_heads + head) * a.c.q_tokens + token] =
-        (m * mul + __builtin_amdgcn_logf(l)) * kLn2;
+        (m * mul - E::kRaise + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Smallest and largest document of each tile of keys: a wave a tile. (Looked over by

@@ -488,6 +488,29 @@ def test_attention_values_at_the_types_end(lq, lk, sign):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lq,hq", [(1, 8), (8192, 8)])
+@pytest.mark.parametrize("depth", [14.0, 17.5, 19.0])
+def test_attention_many_keys_of_small_weight(dtype, lq, hq, depth):
+    """One key far above 2^17 others, whose weights lie among fp16's subnormal numbers or below
+    but add up. The first key's V is 0, the others' 1: the result is their share."""
+    n = 2 ** 17
+    q = torch.zeros(1, lq, hq, 32, dtype=dtype, device="cuda")
+    k = torch.zeros(1, n, hq, 32, dtype=dtype, device="cuda")
+    v = torch.ones(1, n, hq, 32, dtype=dtype, device="cuda")
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = depth, 1, 0
+    out, lse = tr.attention(q, k, v, scale=1.0, return_lse=True)
+    tail = (n - 1) * math.exp(-depth)
+    want = tail / (1 + tail)
+    # Each weight's rounding to the type (fp16: 2^-11, subnormal from 2^-14 / 128 on, where a
+    # weight is off by 2^-25 / 128 at most), the exponential's argument (2^-20), the result's own rounding.
+    u = ref.UNIT[dtype]
+    small = n * 2.0 ** -32 if dtype == F16 else 0.0
+    assert (out.double() - want).abs().max() < (2 * u + 2 ** -18) * want + small + ref.TINY[dtype]
+    # The running sum's additions, as in transformer_reference.attention.
+    assert (lse.double() - (depth + math.log1p(tail))).abs().max() < n * ref.E + 1e-5
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("depth", [20.0, 200.0])
 def test_attention_seen_values_of_small_weight(dtype, bad, depth):
