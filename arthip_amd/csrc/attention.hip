@@ -14,9 +14,11 @@
 //
 // Statistics are fp32 in the base of 2. P is rounded to the element type for the
 // second product (it lies in [0, 2^8], fp16's in [0, 2^15], see weights()); its sum is taken
-// before the rounding. fp16 and bf16 run alike: 8192 x 8192 keys, 32 heads of 128: 1135 us, 969
-// TFLOP/s, 79% of a large library product; heads of 64: 664 us, bound by the vector work
-// of the exponentials; one token over 16384 keys: 4.8 TB/s.
+// before the rounding. fp16 and bf16 run alike: 8192 x 8192 keys, 32 heads of 128: 1125 us, 977
+// TFLOP/s, 79% of a large library product; heads of 64: 664 us. No unit is full there (vector
+// 41%, matrix 42% busy; 59% and 35% with heads of 64): a wave's products and its exponentials
+// follow one another, and two or three waves a SIMD cover only part of that. One token over
+// 16384 keys: 4.8 TB/s.
 
 #include <hip/hip_runtime.h>
 
@@ -280,12 +282,11 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   unsigned char* const more = lds + 2 * v_at;  // what follows them
   const uint32_t more_base = lds_base + 2 * v_at;
 
-  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
-  // stay on one XCD. A single row tile shares nothing, and sequences of different
-  // lengths are then spread over all.
-  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: they
-  // stay on one XCD. A single row tile shares nothing: its items go round as they come,
-  // one further each round, so that no XCD gets all the first (long) ranges.
+  // Workgroups go round the eight XCDs. Row tiles of one key head share K and V: each XCD
+  // takes an eighth of them in order (even for causal rows where batch times key heads is a
+  // multiple of 8; one key head alone gives the busiest XCD 1.87 times the mean). A single row
+  // tile shares nothing: its items go round as they come, one further each round, so that no
+  // XCD gets all the first (long) ranges.
   const int bid = (int)blockIdx.x, per = (int)gridDim.x >> 3;
   const int item = a.row_tiles == 1 ? (bid & ~7) + ((bid + (bid >> 3)) & 7) : (bid & 7) * per + (bid >> 3);
   if (item >= a.items) return;
@@ -1078,7 +1079,8 @@ TilePick pick(int d, bool shared, Shape shape) {
   return pick<T, 256, 32, 4, false>(shape);
 }
 
-// Up to 32 rows are shared by two waves, which divide the keys; more take 32 each.
+// Up to 32 rows are one wave's, or above heads of 128 two waves', which divide the keys; of more rows
+// each of four waves takes 32.
 bool shared_rows(const arthip_attention_args& c) {
   return (int64_t)c.q_tokens * (c.q_heads / c.k_heads) <= 32;
 }
