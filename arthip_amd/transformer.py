@@ -58,8 +58,12 @@ def _bool(name: str, x) -> bool:
 
 
 def _pair(name: str, x) -> tuple:
-    _need(isinstance(x, (tuple, list)) and len(x) == 2, f"{name} must be a pair")
-    return tuple(x)
+    try:
+        pair = tuple(x)
+    except TypeError:
+        pair = ()
+    _need(len(pair) == 2, f"{name} must be a pair")
+    return pair
 
 
 # What a call's shapes, strides, types and options come to (checked arguments with all
@@ -261,8 +265,12 @@ def attention(q, k, v, *, scale: float | None = None, cap: float = 0.0, causal: 
     causal = _bool("attention: causal", causal)
     window = tuple(None if w is None else _int("attention: a window's side", w)
                    for w in _pair("attention: window", window))
-    doc_q, doc_k = (None, None) if docs is None else _pair("attention: docs", docs)
-    code_q, code_k = (None, None) if codes is None else _pair("attention: codes", codes)
+    for name, x in (("docs", docs), ("codes", codes)):
+        _need(not isinstance(x, torch.Tensor), f"attention: {name} must be a pair of tensors")
+    docs = None if docs is None else _pair("attention: docs", docs)
+    codes = None if codes is None else _pair("attention: codes", codes)
+    doc_q, doc_k = docs or (None, None)
+    code_q, code_k = codes or (None, None)
     key = ("attention", _sig(q), _sig(k), _sig(v), scale, cap, causal, window, _sig(out), return_lse)
     plain = (q_start is None and kv_len is None and prefix is None and docs is None and codes is None
              and slopes is None and table is None)

@@ -372,6 +372,12 @@ def test_lists_are_pairs(launches):
     assert len(launches) == 1 and (launches[0].left, launches[0].right) == (3, 1)
 
 
+def test_windows_of_any_two_numbers(launches):
+    for window in (np.array([3, 1]), torch.tensor([3, 1]), iter((3, 1)), torch.Size((3, 1))):
+        _use("attention", window=window)
+        assert (launches[-1].left, launches[-1].right) == (3, 1)
+
+
 @pytest.mark.parametrize("name", ["post", "pre", "gate_act"])
 def test_names_that_are_none(launches, name):
     for bad in (["rms"], {"rms": 1}, 5):
