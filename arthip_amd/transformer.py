@@ -395,7 +395,7 @@ def gated_norm(residual, y=None, *, post=None, post_weight=None, post_bias=None,
     """The norms before and after a block with its gate and residual scale, on tokens
     [B, L, C]; see arthip_gated_norm. ``post`` and ``pre`` are "rms", "layer" or None,
     ``gate_act`` is "none", "sigmoid", "tanh" or "silu"; gate, mod_scale and mod_shift
-    broadcast to [B, L, C], weights and biases are fp32 [C]. The residual has y's type or
+    broadcast to [B, L, C] (no gate is one of 1), weights and biases are fp32 [C]. The residual has y's type or
     fp32. Returns (new residual, h); residual_out=residual updates in place, and without y
     and with a residual_scale of 1 the residual is returned as it is. h has y's type, or
     ``dtype`` where there is no y."""

@@ -538,7 +538,7 @@ typedef struct arthip_norm_args {
   const void* y;               /* or NULL */
   void* residual_out;          /* may be residual with its strides (in place); or NULL */
   void* h;                     /* or NULL */
-  const void* gate;            /* or NULL: 1 */
+  const void* gate;            /* or NULL: 1, through gate_act */
   const void* mod_scale;       /* or NULL: 0 */
   const void* mod_shift;       /* or NULL: 0 */
   const float* post_weight;    /* [C], or NULL: 1 */

@@ -667,6 +667,21 @@ def test_gated_norm(dtype, res, b, l, c, post, pre, gate, act, mod, bias):
     assert out is place and torch.equal(place, new)
 
 
+@pytest.mark.parametrize("act", ["none", "sigmoid", "tanh", "silu"])
+@pytest.mark.parametrize("c", [5, 512, 975])
+def test_gated_norm_activation_without_a_gate(act, c):
+    """No gate stands for a gate of 1, which goes through the activation."""
+    g = _gen(24)
+    r, y = _normal(g, 2, 9, c, dtype=BF16), _normal(g, 2, 9, c, dtype=BF16)
+    kw = {"post": "rms", "pre": "layer", "gate_act": act, "branch_scale": 0.7}
+    want = ref.gated_norm(r, y, **kw)
+    new, h = tr.gated_norm(r, y, **kw)
+    ref.check(new, want[0], "residual")
+    ref.check(h, want[1], "h")
+    for got, of_one in zip((new, h), tr.gated_norm(r, y, gate=torch.ones(c, dtype=BF16, device="cuda"), **kw)):
+        assert torch.equal(got, of_one)
+
+
 def test_gated_norm_parts_alone():
     """The first norm of a network (no branch), the last residual (no norm after it)."""
     g = _gen(20)
