@@ -228,14 +228,18 @@ __global__ void __launch_bounds__(1024) gated_norm(NormArgs a) {
     float g[N][kNormVec];
     if (a.c.gate) {
       load_rows<FULL>(static_cast<const T*>(a.c.gate) + at(a.c.gate_stride), c, C, g);
+#pragma unroll
+      for (int n = 0; n < N; ++n) gates(g[n], a.c.gate_act);
     } else {
+      float one[kNormVec];
+#pragma unroll
+      for (int i = 0; i < kNormVec; ++i) one[i] = 1.0f;
+      gates(one, a.c.gate_act);
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < kNormVec; ++i) g[n][i] = 1.0f;
+        for (int i = 0; i < kNormVec; ++i) g[n][i] = one[0];
     }
-#pragma unroll
-    for (int n = 0; n < N; ++n) gates(g[n], a.c.gate_act);
     normalize<FULL>(y, c, a, a.c.post, a.c.post_weight, a.c.post_bias, sum);
 #pragma unroll
     for (int n = 0; n < N; ++n)
