@@ -90,6 +90,56 @@ class NormArgs(ctypes.Structure):
                 + [(n, ctypes.c_float) for n in ("eps", "residual_scale", "branch_scale")])
 
 
+class Pages(ctypes.Structure):
+    """arthip_pages."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("pages", "kv_len", "q_offsets")]
+                + [("pages_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("batch", "tokens", "max_pages", "pool_pages", "page_size",
+                                                 "k_heads", "head_dim", "dtype")])
+
+
+class CacheWriteArgs(ctypes.Structure):
+    """arthip_cache_write_args."""
+    _fields_ = ([("p", Pages)]
+                + [(n, ctypes.c_void_p) for n in ("k", "v", "k_cache", "v_cache", "positions",
+                                                  "token_positions")]
+                + [("k_stride", _I64x2), ("v_stride", _I64x2), ("k_cache_stride", _I64x3),
+                   ("v_cache_stride", _I64x3), ("positions_stride", _I64x2)]
+                + [(n, ctypes.c_int32) for n in ("slots", "pad")])
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """arthip_paged_attention_args."""
+    _fields_ = ([("p", Pages)]
+                + [(n, ctypes.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "lse", "workspace")]
+                + [("workspace_bytes", ctypes.c_uint64)]
+                + [("q_stride", _I64x2), ("out_stride", _I64x2), ("k_cache_stride", _I64x3),
+                   ("v_cache_stride", _I64x3)]
+                + [("scale", ctypes.c_float), ("cap", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("q_heads", "causal", "left", "pad")])
+
+
+class KeyWeightsArgs(ctypes.Structure):
+    """arthip_key_weights_args."""
+    _fields_ = ([("p", Pages)]
+                + [(n, ctypes.c_void_p) for n in ("q", "k_cache", "lse", "weights", "out", "workspace")]
+                + [("workspace_bytes", ctypes.c_uint64)]
+                + [("q_stride", _I64x2), ("k_cache_stride", _I64x3), ("weights_stride", _I64x2),
+                   ("out_stride", _I64x2)]
+                + [(n, ctypes.c_float) for n in ("scale", "cap", "decay")]
+                + [(n, ctypes.c_int32) for n in ("q_heads", "causal", "left", "slots", "pad")])
+
+
+class CacheEvictArgs(ctypes.Structure):
+    """arthip_cache_evict_args."""
+    _fields_ = ([("p", Pages)]
+                + [(n, ctypes.c_void_p) for n in ("k_cache", "v_cache", "weights", "positions", "new_len",
+                                                  "weights_out", "positions_out", "kept")]
+                + [("k_cache_stride", _I64x3), ("v_cache_stride", _I64x3), ("weights_stride", _I64x2),
+                   ("positions_stride", _I64x2)]
+                + [(n, ctypes.c_int32) for n in ("slots", "keep", "recent", "first")])
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     c_int, c_size, c_void, c_char = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
     i32p = ctypes.POINTER(ctypes.c_int)
@@ -168,6 +218,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     sig("arthip_attention_workspace", c_size, ctypes.POINTER(AttentionArgs))
     sig("arthip_attention", c_int, ctypes.POINTER(AttentionArgs), c_void)
     sig("arthip_gated_norm", c_int, ctypes.POINTER(NormArgs), c_void)
+    sig("arthip_cache_write", c_int, ctypes.POINTER(CacheWriteArgs), c_void)
+    sig("arthip_paged_attention_workspace", c_size, ctypes.POINTER(PagedAttentionArgs))
+    sig("arthip_paged_attention", c_int, ctypes.POINTER(PagedAttentionArgs), c_void)
+    sig("arthip_key_weights_workspace", c_size, ctypes.POINTER(KeyWeightsArgs))
+    sig("arthip_key_weights", c_int, ctypes.POINTER(KeyWeightsArgs), c_void)
+    sig("arthip_cache_evict", c_int, ctypes.POINTER(CacheEvictArgs), c_void)
     sig("arthip_f32_to_f16", ctypes.c_uint16, ctypes.c_float)
     sig("arthip_f16_to_f32", ctypes.c_float, ctypes.c_uint16)
     sig("arthip_f32_to_f16_no_subnormals", ctypes.c_uint16, ctypes.c_float)
@@ -191,7 +247,9 @@ EXPORTED_SYMBOLS = (
     "arthip_conv3x3_packed_halfs", "arthip_conv3x3_bias_len", "arthip_conv3x3_pack",
     "arthip_conv3x3_f16_nhwc", "arthip_conv3x3_block_f16_nhwc", "arthip_conv3x3_limits", "arthip_padded_dims",
     "arthip_rope_packed_bytes", "arthip_rope_pack", "arthip_rope_axes", "arthip_attention_workspace",
-    "arthip_attention", "arthip_gated_norm", "arthip_f32_to_f16",
+    "arthip_attention", "arthip_gated_norm", "arthip_cache_write", "arthip_paged_attention_workspace",
+    "arthip_paged_attention", "arthip_key_weights_workspace", "arthip_key_weights", "arthip_cache_evict",
+    "arthip_f32_to_f16",
     "arthip_f16_to_f32", "arthip_f32_to_f16_no_subnormals", "arthip_last_error", "arthip_version",
 )
 

@@ -16,6 +16,7 @@
 #include "half.h"
 #include "launch.h"
 #include "pack.h"
+#include "paged.h"
 #include "transformer.h"
 
 static_assert(ARTHIP_DEBUG_POISON == arthip::kDebugPoison &&
@@ -809,6 +810,68 @@ int arthip_gated_norm(const arthip_norm_args* args, void* stream) {
     const std::string wrong = arthip::check_norm(*args);
     if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
     return launched("arthip_gated_norm", arthip::launch_norm(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Paged cache
+// ---------------------------------------------------------------------------
+
+int arthip_cache_write(const arthip_cache_write_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_cache_write: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_cache_write(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_cache_write",
+                    arthip::launch_cache_write(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+size_t arthip_paged_attention_workspace(const arthip_paged_attention_args* args) {
+  try {
+    if (args == nullptr || !arthip::check_paged_attention_shape(*args).empty()) return 0;
+    return arthip::paged_plan(*args).workspace();
+  } catch (const std::exception&) {
+    return 0;
+  }
+}
+
+int arthip_paged_attention(const arthip_paged_attention_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_paged_attention: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_paged_attention(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_paged_attention",
+                    arthip::launch_paged_attention(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+size_t arthip_key_weights_workspace(const arthip_key_weights_args* args) {
+  try {
+    if (args == nullptr || !arthip::check_key_weights_shape(*args).empty()) return 0;
+    return arthip::key_weights_plan(*args).workspace;
+  } catch (const std::exception&) {
+    return 0;
+  }
+}
+
+int arthip_key_weights(const arthip_key_weights_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_key_weights: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_key_weights(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_key_weights",
+                    arthip::launch_key_weights(*args, static_cast<hipStream_t>(stream)));
+  });
+}
+
+int arthip_cache_evict(const arthip_cache_evict_args* args, void* stream) {
+  return guard(ARTHIP_ERR_BUILD, nullptr, 0, "", [&]() -> int {
+    if (args == nullptr) return fail("arthip_cache_evict: null arguments", ARTHIP_ERR_BUILD);
+    const std::string wrong = arthip::check_cache_evict(*args);
+    if (!wrong.empty()) return fail(wrong, ARTHIP_ERR_BUILD);
+    return launched("arthip_cache_evict",
+                    arthip::launch_cache_evict(*args, static_cast<hipStream_t>(stream)));
   });
 }
 

@@ -1,0 +1,849 @@
+// Attention of new tokens over a paged cache (arthip_paged_attention).
+//
+// The query heads that share a key head are rows of one matrix. A row tile is as many whole
+// tokens of a sequence as fit 32 rows a wave; a workgroup walks a row tile's keys in tiles
+// that it stages in LDS. Both products are v_mfma_f32_32x32x16 with the keys of the first as
+// rows, S^T = K Q^T: a lane holds 16 keys of ONE query, and the accumulator, packed to the
+// element type, is the right operand of O^T += V^T P^T. Statistics are fp32 in the base of 2;
+// P is rounded to the element type (it lies in [0, 2^8], fp16's in [0, 2^15]), its sum is taken
+// before.
+//
+// Lengths are known on the device alone, and differ: one call holds prompts beside single
+// tokens. So the work is divided there. The key tiles that the row tiles need, all sequences'
+// in a row, are cut into equal ranges, one a workgroup; a range may end inside a row tile, whose
+// parts a second kernel joins in a fixed order. Every wave finds its range's beginning from the
+// lengths, a lane (or some) a sequence.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "attention_dev.h"
+#include "launch.h"
+#include "paged.h"
+#include "paged_dev.h"
+
+namespace arthip {
+
+namespace {
+
+// What the scores go through: nothing (the scale is in the exponent), a cap up to kCapSmall, or
+// any cap and scale.
+enum Shape { kPlain, kCap, kAny };
+
+struct PagedArgs {
+  arthip_paged_attention_args c;
+  int group;        // query heads of a key head
+  int tile_tokens;  // tokens of a row tile
+  int ranges;       // workgroups
+  int row_slots;    // rows kept of a part of a row tile
+  int lanes;        // that count one sequence's tiles together, if `before` is not there
+  int wave_rows;    // 32 rows a workgroup rather than 128
+  FastDiv by_group, by_page, by_lanes;
+  CapFit cap;
+  const int64_t* before;  // key tiles of the sequences before each [batch + 1], of all key heads
+  float* sums;   // [2 ranges][row_slots][D] unscaled: parts that begin inside a row tile, parts that end inside
+  float* stats;  // [2 ranges][row_slots][2] maximum (base 2) and sum
+  int4* pieces;  // [ranges + 1] of a row tile that begins in a range and ends in another: sequence, key
+                 // head, tile, number of parts. The last: ranges that there are.
+};
+
+constexpr int kLeast = 4;  // key tiles of a range, where there are that many
+
+// Key tiles of a row tile: from `first` on, `count` of them. KT: log2 of the keys of one.
+struct Span {
+  int first, count;
+};
+template <int KT>
+__device__ __forceinline__ Span span_of(const PagedArgs& a, const Sequence& s, int tile) {
+  const int from = tile * a.tile_tokens, to = min(from + a.tile_tokens, s.tokens);
+  const int lo = a.c.left < 0 ? 0 : min(max(s.start() + from - a.c.left, 0), s.len);
+  const int hi = a.c.causal ? min(max(s.start() + to, 0), s.len) : s.len;
+  const int first = lo >> KT;
+  return {first, hi > lo ? ((hi + (1 << KT) - 1) >> KT) - first : 0};
+}
+// Row tiles count as one key tile at least: their rows are written.
+template <int KT>
+__device__ __forceinline__ int units_of(const PagedArgs& a, const Sequence& s, int tile) {
+  return max(span_of<KT>(a, s, tile).count, 1);
+}
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, const Sequence& s) {
+  return (s.tokens + a.tile_tokens - 1) / a.tile_tokens;
+}
+
+__device__ __forceinline__ int64_t shuffle(int64_t x, int lane) { return __shfl((long long)x, lane); }
+
+// Where a unit lies.
+struct Place {
+  int b, head, tile, unit;  // unit: of the row tile's
+};
+
+// The units before each sequence, by one workgroup: a wave a sequence, then a running sum.
+template <int KT>
+__global__ void __launch_bounds__(1024) paged_count(PagedArgs a, int64_t* before) {
+  __shared__ int64_t box[16];
+  __shared__ int64_t carry;
+  const arthip_pages& p = a.c.p;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) {
+    carry = 0;
+    before[0] = 0;
+  }
+  for (int b0 = 0; b0 < p.batch; b0 += 1024) {
+    // 16 waves, 64 sequences each; lane i keeps the i-th one's units.
+    int64_t mine = 0;
+    for (int i = 0; i < 64; ++i) {
+      const int b = b0 + wave * 64 + i;
+      if (b >= p.batch) break;
+      const Sequence s = sequence_of(p, b);
+      const int tiles = tiles_of(a, s);
+      int64_t n = 0;
+      for (int t = lane; t < tiles; t += 64) n += units_of<KT>(a, s, t);
+#pragma unroll
+      for (int step = 32; step > 0; step /= 2) n += shuffle(n, lane ^ step);
+      if (lane == i) mine = n * p.k_heads;
+    }
+    int64_t sum = mine;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int64_t y = shuffle(sum, max(lane - step, 0));
+      sum += lane >= step ? y : 0;
+    }
+    lds_sync();
+    if (lane == 63) box[wave] = sum;
+    lds_sync();
+    int64_t base = carry;
+    for (int w = 0; w < wave; ++w) base += box[w];
+    const int b = b0 + wave * 64 + lane;
+    if (b < p.batch) before[b + 1] = base + sum;
+    lds_sync();
+    if (threadIdx.x == 1023) carry = base + sum;
+    lds_sync();
+  }
+}
+
+// A wave's view of the batch: units of each sequence (64 at most, `lanes` lanes each) or the
+// counted ones.
+template <int KT>
+struct Finder {
+  int64_t end, units;  // lane's sequence: units up to its end, and its own, of one key head
+  int64_t total;
+
+  __device__ __forceinline__ void count(const PagedArgs& a, int lane) {
+    const arthip_pages& p = a.c.p;
+    if (a.before != nullptr) {
+      total = a.before[p.batch];
+      return;
+    }
+    const int b = (int)fdiv((uint32_t)lane, a.by_lanes), sub = lane - b * a.lanes;
+    int64_t n = 0;
+    if (b < p.batch) {
+      const Sequence s = sequence_of(p, b);
+      const int tiles = tiles_of(a, s);
+      for (int t = sub; t < tiles; t += a.lanes) n += units_of<KT>(a, s, t);
+    }
+    for (int step = 1; step < a.lanes; step *= 2) n += shuffle(n, lane ^ step);
+    units = n;
+    int64_t sum = sub == 0 ? n * p.k_heads : 0;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int64_t y = shuffle(sum, max(lane - step, 0));
+      sum += lane >= step ? y : 0;
+    }
+    end = sum;  // the same for a sequence's lanes
+    total = shuffle(sum, 63);
+  }
+
+  // The place of unit x, below `total` (uniform).
+  __device__ __forceinline__ Place find(const PagedArgs& a, int64_t x, int lane) const {
+    const arthip_pages& p = a.c.p;
+    Place at;
+    int64_t one;  // units of a key head
+    if (a.before != nullptr) {
+      int lo = 0, n = p.batch;  // the last sequence whose units begin at or before x
+      while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool in = lane * step < n && a.before[lo + min(lane * step, n - 1)] <= x;
+        const int skip = (__popcll(__ballot(in)) - 1) * step;
+        lo += skip;
+        n = min(step, n - skip);
+      }
+      at.b = __builtin_amdgcn_readfirstlane(lo);
+      const int64_t first = a.before[at.b];
+      one = (a.before[at.b + 1] - first) / p.k_heads;
+      x -= first;
+    } else {
+      const int of = __popcll(__ballot(end <= x));  // lanes of earlier sequences
+      at.b = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)of, a.by_lanes));
+      one = shuffle(units, of);
+      x -= shuffle(end, of) - one * p.k_heads;
+    }
+    at.head = __builtin_amdgcn_readfirstlane((int)(x / one));
+    x -= at.head * one;
+    const Sequence s = sequence_of(p, at.b);
+    for (int t0 = 0;; t0 += 64) {
+      const int t = t0 + lane;
+      const uint32_t n = t < tiles_of(a, s) ? (uint32_t)units_of<KT>(a, s, t) : 0;
+      uint32_t sum = n;
+#pragma unroll
+      for (int step = 1; step < 64; step *= 2) {
+        const uint32_t y = __shfl(sum, max(lane - step, 0));
+        sum += lane >= step ? y : 0;
+      }
+      const uint32_t all = __shfl(sum, 63);
+      if (x >= all && all > 0) {
+        x -= all;
+        continue;
+      }
+      const int of = min(__popcll(__ballot((int64_t)sum <= x)), 63);
+      at.tile = __builtin_amdgcn_readfirstlane(t0 + of);
+      at.unit = __builtin_amdgcn_readfirstlane((int)(x - (__shfl(sum, of) - __shfl(n, of))));
+      return at;
+    }
+  }
+};
+
+template <class T, int DP, int KT, int NW, Shape SHAPE>
+__global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 && SHAPE == kAny) ? 2 : 3)
+    paged_tile(PagedArgs a) {
+  using L = TileL<DP, KT>;
+  using E = Elem<T>;
+  using frag = typename E::frag;
+  constexpr int LOG = KT == 64 ? 6 : 5;
+  static_assert(1 << LOG == KT, "keys of a tile");
+  constexpr int RB = L::RB, KB = KT / 32, KS = DP / 16, DB = DP / 32;
+  constexpr int SEG = L::kTile / 1024;                 // loads of a tile, 1 KiB each
+  constexpr int LOADS = (SEG + NW - 1) / NW;           // of a wave
+  constexpr int STEP = 1024 / RB;                      // keys of a load
+  constexpr int WK = LOADS * STEP;                     // keys that a wave loads: in one page each 16
+  constexpr int NG = WK > 16 ? WK / 16 : 1;            // pages at most
+  constexpr int GL = LOADS / NG;                       // loads of a page
+  static_assert(SEG % NW == 0 && LOADS % NG == 0 && (WK <= 16 || WK % 16 == 0), "whole pages a wave");
+  constexpr uint32_t kOob = 0x80000000u;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  constexpr int v_at = 2 * L::kTile;  // V's buffers
+
+  const arthip_pages& pg = a.c.p;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int n = lane & 31;     // the lane's row of the wave's 32
+  const int half = lane >> 5;  // which keys and values of it
+  auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto scalar64 = [&](int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)scalar((int)x) | (uint64_t)(uint32_t)scalar((int)(x >> 32)) << 32);
+  };
+
+  // -- the workgroup's range ---------------------------------------------------------
+  // Workgroups go round the eight XCDs: each takes an eighth of the ranges in a row, as row tiles
+  // of one key head share K and V.
+  Finder<LOG> finder;
+  finder.count(a, lane);
+  const int64_t total = scalar64(finder.total);
+  const int live = total >= (int64_t)a.ranges * kLeast ? a.ranges : max((int)total / kLeast, total > 0 ? 1 : 0);
+  const int per = (live + 7) >> 3;
+  const int range = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  if (blockIdx.x == 0 && tid == 0) a.pieces[a.ranges] = int4{live, 0, 0, 0};
+  if (((int)blockIdx.x >> 3) >= per || range >= live) return;
+  const int64_t share = scalar64(total / live);
+  const int more = scalar((int)(total - share * live));  // ranges of one unit more
+  int64_t at = range * share + min(range, more);
+  const int64_t range_end = at + share + (range < more ? 1 : 0);
+  Place place = finder.find(a, at, lane);
+  place = {scalar(place.b), scalar(place.head), scalar(place.tile), scalar(place.unit)};
+
+  // -- what does not change from row tile to row tile ----------------------------------
+  const int my_token = (int)fdiv((uint32_t)(wave * 32 + n), a.by_group);  // of the row tile
+  const int g_head = wave * 32 + n - my_token * a.group;
+  const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
+  const int s_row = (wave * LOADS * 1024 + lane * 16) / RB;  // tile's key of the wave's first load
+  const int s_chunk = lane * 16 % RB / 16;
+  const int l_row = lane * 16 / RB;  // the same of the load's keys
+  const int ks2 = (int)a.c.k_cache_stride[1] * 2, vs2 = (int)a.c.v_cache_stride[1] * 2;  // bytes
+  constexpr int KP = (RB == 512 ? 8 : 16) / STEP < LOADS ? (RB == 512 ? 8 : 16) / STEP : LOADS;
+  constexpr int VP = 4 / STEP < 1 ? 1 : 4 / STEP < LOADS ? 4 / STEP : LOADS;
+  uint32_t k_off[KP], v_off[VP];  // a lane's offsets, but for the keys between its loads
+  auto offset_of = [&](int chunk, int stride) __attribute__((always_inline)) {
+    return chunk * 8 < pg.head_dim ? (uint32_t)(l_row * stride + chunk * 16) : kOob;
+  };
+#pragma unroll
+  for (int i = 0; i < KP; ++i) k_off[i] = offset_of(s_chunk ^ L::k_swizzle(s_row + i * STEP), ks2);
+#pragma unroll
+  for (int i = 0; i < VP; ++i) v_off[i] = offset_of(s_chunk ^ L::v_swizzle(s_row + i * STEP), vs2);
+  typedef __attribute__((address_space(3))) unsigned char lds_byte;
+  typedef __attribute__((address_space(3))) const frag lds_frag;
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  lds_byte* const lds0 = (lds_byte*)lds;
+  const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
+  const int v_row = 4 * half + (lane & 15) / 4;
+  const uint32_t v_lane =
+      v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+
+  while (true) {
+    // -- a row tile, or a part of it ----------------------------------------------------
+    Sequence seq = sequence_of(pg, place.b);
+    seq.first = scalar(seq.first);
+    seq.tokens = scalar(seq.tokens);
+    seq.len = scalar(seq.len);
+    const int token0 = place.tile * a.tile_tokens;
+    const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;  // of the row tile
+    const Span span = span_of<LOG>(a, seq, place.tile);
+    const int units = max(span.count, 1);
+    const int take = (int)min((int64_t)(units - place.unit), range_end - at);
+    const int begin = span.first + min(place.unit, span.count), end = span.first + min(place.unit + take, span.count);
+    const int32_t* const pages = pg.pages + place.b * pg.pages_stride;
+    const int kv_len = seq.len, start = seq.start();
+    // Keys [lo, hi) that a token sees.
+    auto low = [&](int token) __attribute__((always_inline)) -> int {
+      return a.c.left < 0 ? 0 : min(max(start + token - a.c.left, 0), kv_len);
+    };
+    auto high = [&](int token) __attribute__((always_inline)) -> int {
+      return a.c.causal ? min(max(start + token + 1, 0), kv_len) : kv_len;
+    };
+    const bool real = wave * 32 + n < rows, w_real = wave * 32 < rows;
+    const int token = token0 + (real ? my_token : 0);
+    const int head = place.head * a.group + (real ? g_head : 0);
+    const int lo = low(token), hi = high(token);
+    // The wave's rows together: all see [w_lo_max, w_hi_min), some see [w_lo_min, w_hi_max).
+    const int t_first = token0 + (int)fdiv((uint32_t)min(wave * 32, rows - 1), a.by_group);
+    const int t_last = token0 + (int)fdiv((uint32_t)min(wave * 32 + 31, rows - 1), a.by_group);
+    const int w_lo_min = low(t_first), w_lo_max = low(t_last);
+    const int w_hi_min = high(t_first), w_hi_max = high(t_last);
+
+    frag q[KS];
+    {
+      const T* const qp = static_cast<const T*>(a.c.q) + (seq.first + token) * a.c.q_stride[0] + head * a.c.q_stride[1];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        q[s] = real && d < pg.head_dim ? *reinterpret_cast<const frag*>(qp + d) : frag{};
+      }
+    }
+    f16v o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f16v{};
+    float m = -__builtin_inff(), l = 0.0f;
+
+    // -- staging -------------------------------------------------------------------------
+    // The page of each 16 keys that the wave loads of a tile. (Slots past the length are not read,
+    // whatever their page.)
+    struct Pages {
+      int of[NG];
+    };
+    auto ask = [&](int tile) __attribute__((always_inline)) {
+      Pages r;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int slot = tile * KT + wave * WK + g * 16;
+        r.of[g] = pages[min((int)fdiv((uint32_t)slot, a.by_page), pg.max_pages - 1)];
+      }
+      return r;
+    };
+    constexpr int BACK = 3 * 1024;  // what buffers begin before the rows, for the constants' sake
+    auto stage = [&](const void* pool, const int64_t* stride, int slot_bytes, auto offset, int tile, const Pages& in,
+                     uint32_t to) __attribute__((always_inline)) {
+      const int left = kv_len - tile * KT;  // keys past the length come as zeros
+      const uint32_t to_wave = to + wave * LOADS * 1024;
+      constexpr int N = GL < 4 ? GL : 4;
+      static_assert(GL % N == 0, "whole blocks of loads");
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int slot = tile * KT + wave * WK + g * 16;
+        const int page = in.of[g], of = (int)fdiv((uint32_t)slot, a.by_page);
+        const char* const p = static_cast<const char*>(pool) +
+                              (page * stride[0] + (slot - of * pg.page_size) * stride[1] + place.head * stride[2]) * 2;
+        // A page outside the pool comes as zeros as well.
+        const rsrc_t r = buffer_of(p - BACK, (uint32_t)page < (uint32_t)pg.pool_pages ? 0x7fffffffu : 0u);
+#pragma unroll
+        for (int i = 0; i < GL; i += N) {
+          uint32_t at_lane[N], base[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int load = g * GL + i + j;
+            base[j] = (i + j) * STEP * (uint32_t)slot_bytes + (BACK - j * 1024);
+            at_lane[j] = left >= KT || s_row + load * STEP < left ? offset(load) : kOob;
+          }
+          load_lds16<N>(r, at_lane, base, to_wave + (g * GL + i) * 1024);
+        }
+      }
+    };
+    auto stage_k = [&](int buf, int tile, const Pages& in) __attribute__((always_inline)) {
+      stage(a.c.k_cache, a.c.k_cache_stride, ks2, [&](int i) { return k_off[i % KP]; }, tile, in,
+            lds_base + buf * L::kTile);
+    };
+    auto stage_v = [&](int buf, int tile, const Pages& in) __attribute__((always_inline)) {
+      stage(a.c.v_cache, a.c.v_cache_stride, vs2, [&](int i) { return v_off[i % VP]; }, tile, in,
+            lds_base + v_at + buf * L::kTile);
+    };
+
+    // -- the products --------------------------------------------------------------------
+    f16v s[KB];        // scores of the current tile, key block by key block
+    frag p[KT / 16];   // weights of the previous tile
+    auto scores = [&](int buf) __attribute__((always_inline)) {
+      lds_byte* const from = lds0 + buf * L::kTile;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        lds_byte* const k = from + (k_lane ^ (ks * 32));
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = E::mma(*(lds_frag*)(k + kb * 32 * RB), q[ks], ks == 0 ? f16v{} : s[kb]);
+      }
+      ahead<KS * KB, 1>();
+    };
+    auto v_frag = [&](lds_byte* from, int kk) __attribute__((always_inline)) -> frag {  // 32 values of 16 keys
+      const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + kk * 16 * RB));
+      const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + kk * 16 * RB + 8 * RB));
+      return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    bool odd = false;  // a tile that a row does not see whole holds an infinity or NaN in V
+    auto values = [&](int buf, bool look) __attribute__((always_inline)) {
+      lds_byte* const from = lds0 + v_at + buf * L::kTile;
+      lds_byte* v[DB];
+#pragma unroll
+      for (int db = 0; db < DB; ++db) v[db] = from + (v_lane ^ (db * 64));
+      if (look) {
+        // Rows that do not see all of this tile weigh some of V by 0, which infinities and
+        // NaN survive: 0 times the tile tells whether it has any.
+        f16v z = f16v{};
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) z = E::mma(v_frag(v[db], kk), frag{}, z);
+        float t = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t += z[r];
+        odd = odd || t != 0.0f;
+      }
+#pragma unroll
+      for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
+      ahead<KT / 16 * DB, 2>();
+    };
+    // The same key by key, each added only to the rows that see it. (Weights that round to 0 are -0
+    // there, as an infinity or NaN counts with any weight; those of hidden keys are +0.)
+    auto values_apart = [&](int buf) __attribute__((always_inline)) {
+      lds_byte* const from = lds0 + v_at + buf * L::kTile;
+#pragma unroll
+      for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll 1
+        for (int key = 0; key < 16; ++key) {
+          const int of = (key >> 2) & 1, j = (key & 3) | ((key >> 1) & 4);  // its half and element
+          u4 keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) keep[e] = half != of || j >> 1 != e ? 0u : j & 1 ? 0xffff0000u : 0x0000ffffu;
+          const u4 one = __builtin_bit_cast(u4, p[kk]) & keep;
+          const float sees = halves_max((one[0] | one[1] | one[2] | one[3]) != 0 ? 1.0f : 0.0f);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u4 x = __builtin_bit_cast(u4, v_frag(from + (v_lane ^ (db * 64)), kk)) & keep;
+            const f16v c = E::mma(__builtin_bit_cast(frag, x), __builtin_bit_cast(frag, one), f16v{});
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[db][r] += sees != 0.0f ? c[r] : 0.0f;
+          }
+        }
+    };
+
+    // -- scores to weights -----------------------------------------------------------------
+    auto weights = [&](auto apart, int k0, bool partial) __attribute__((always_inline)) {
+      const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
+      if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
+        float far = 0.0f;
+        if constexpr (SHAPE == kCap) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
+        }
+        if (SHAPE == kCap && !__any(!(far <= a.cap.reach))) {
+          // Small scores: six plain operations where the exponential and the reciprocal take a
+          // quarter of the rate each.
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] = cap_near(a.cap, s[kb][r]);
+        } else {
+          // Off by some 2^-22 of the cap; large caps choose score by score.
+          const float in = a.cap.in, out = a.cap.out;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float x = s[kb][r];
+              const float e = __builtin_amdgcn_exp2f(x * in);
+              const float y = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
+              s[kb][r] = SHAPE == kAny && fabsf(x) <= a.cap.reach ? cap_near(a.cap, x) : y;
+            }
+        }
+      } else if constexpr (SHAPE == kAny) {
+        const float unit = a.c.scale * kLog2e;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb][r] *= unit;
+      }
+      if (partial) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = key0 + 32 * kb + 8 * (r / 4) + r % 4;
+            s[kb][r] = key >= lo && key < hi ? s[kb][r] : -__builtin_inff();
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+      top = halves_max(top);
+      // The base of a row's exponents follows its largest score only where that has grown
+      // by more than 2^8: until then weights are at most 256, and nothing is rescaled.
+      if (__any((top - m) * mul > 8.0f)) {
+        const float next = fmaxf(m, top);
+        // A row that has seen nothing yet has no sums to keep (next may be -inf as well).
+        const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= f;
+      }
+      // fp16's weights are raised to the top of its range, so that small ones, of which a long
+      // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
+      const float base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+      float sum = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = s[kb][r], w = __builtin_amdgcn_exp2f(__builtin_fmaf(x, mul, -base));
+          sum += w;
+          s[kb][r] = decltype(apart)::value && w <= E::kZero && x != -__builtin_inff() ? -0.0f : w;
+        }
+      l += sum;  // this half's keys; the halves are added at the end
+#pragma unroll
+      for (int kk = 0; kk < KT / 16; ++kk) {
+        const f16v x = s[kk / 2];
+        p[kk] = kk & 1
+                    ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
+                    : __builtin_convertvector(__builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7), frag);
+      }
+    };
+
+    // -- the walk ------------------------------------------------------------------------
+    // One barrier a tile. While tile t's scores and the previous tile's values are multiplied, K of
+    // the next tile and V of this one are on their way to the buffers that the last barrier freed,
+    // and the pages of the tile after the next are asked for.
+    auto settle = [&](Pages& x) __attribute__((always_inline)) {  // after the wait for the loads
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        asm volatile("" : "+v"(x.of[g]));
+        x.of[g] = scalar(x.of[g]);
+      }
+    };
+    auto walk = [&](auto apart) __attribute__((always_inline)) {
+      lds_sync();  // the last walk's tiles have been used
+      if (begin >= end) return;
+      Pages here = ask(begin), next = here;
+      settle(here);
+      stage_k(0, begin, here);
+      if (begin + 1 < end) next = ask(begin + 1);
+      vm_wait();
+      settle(next);
+      lds_sync();
+      int buf = 0;
+      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
+      for (int t = begin;; ++t) {
+        const bool on = t < end;
+        const int k0 = t * KT, k1 = k0 + KT;
+        bool seen = false, partial = false;
+        Pages then = next;
+        if (on) {
+          if (t + 1 < end) stage_k(buf ^ 1, t + 1, next);
+          stage_v(buf, t, here);
+          if (t + 2 < end) then = ask(t + 2);
+          seen = w_real && k0 < w_hi_max && k1 > w_lo_min;
+          partial = !(k0 >= w_lo_max && k1 <= w_hi_min);
+        }
+        if (seen) scores(buf);
+        if (has) {
+          if constexpr (decltype(apart)::value)
+            values_apart(buf ^ 1);
+          else
+            values(buf ^ 1, look);
+        }
+        if (!on) break;
+        if (seen) weights(apart, k0, partial);
+        has = seen;
+        look = partial;
+        vm_wait();
+        settle(then);
+        lds_sync();
+        here = next;
+        next = then;
+        buf ^= 1;
+      }
+    };
+    walk(std::false_type{});
+    // A workgroup that met such a tile starts over and takes the keys one by one.
+    {
+      int* const flag = reinterpret_cast<int*>(lds);
+      lds_sync();
+      if (lane == 0) flag[wave] = 0;
+      if (odd) flag[wave] = 1;
+      lds_sync();
+      int again = 0;
+      for (int i = 0; i < NW; ++i) again |= flag[i];
+      if (__builtin_expect(scalar(again) != 0, 0)) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] = f16v{};
+        m = -__builtin_inff();
+        l = 0.0f;
+        walk(std::true_type{});
+      }
+    }
+
+    // -- results -------------------------------------------------------------------------
+    l = halves_sum(l);
+    if (take < units) {
+      if (real) {
+        const int64_t row = (int64_t)(2 * range + (place.unit == 0 ? 1 : 0)) * a.row_slots + wave * 32 + n;
+        float* const part = a.sums + row * pg.head_dim;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int d = db * 32 + 8 * g + 4 * half;
+            if (d < pg.head_dim)
+              *reinterpret_cast<f4*>(part + d) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+          }
+        if (half == 0) {
+          a.stats[2 * row] = m * mul - E::kRaise;
+          a.stats[2 * row + 1] = l;
+        }
+      }
+    } else {
+      const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+      T* const op = static_cast<T*>(a.c.out) + (seq.first + token) * a.c.out_stride[0] + head * a.c.out_stride[1];
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+          // A lane holds four values of every eight; the halves trade so that each stores
+          // eight in a row.
+          uint32_t w[2][2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              typedef float f2 __attribute__((ext_vector_type(2)));
+              typedef T t2 __attribute__((ext_vector_type(2)));
+              const f2 pair = {in_range<T>(o[db][4 * (g + e) + 2 * j] * scale),
+                               in_range<T>(o[db][4 * (g + e) + 2 * j + 1] * scale)};
+              w[e][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, t2));
+            }
+          const u2 x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+          const u2 y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+          const int d = db * 32 + 8 * (g + half);
+          if (real && d < pg.head_dim) *reinterpret_cast<u4*>(op + d) = u4{x[0], y[0], x[1], y[1]};
+        }
+      if (a.c.lse && real && half == 0)
+        a.c.lse[(int64_t)(seq.first + token) * a.c.q_heads + head] =
+            (m * mul - E::kRaise + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+    const int64_t tile_end = at + units - place.unit;
+    at += take;
+    if (at >= range_end) {
+      if (tid == 0) {
+        // Whether a row tile begins here and ends in a later range.
+        int parts = 0;
+        if (tile_end > at && place.unit == 0) {
+          const int64_t last = tile_end - 1, longer = more * (share + 1);
+          parts = (int)(last < longer ? last / (share + 1) : more + (last - longer) / share) - range + 1;
+        }
+        a.pieces[range] = int4{place.b, place.head, place.tile, parts};
+      }
+      return;
+    }
+    place.unit = 0;
+    if (++place.tile == tiles_of(a, seq)) {
+      place.tile = 0;
+      if (++place.head == pg.k_heads) {
+        place.head = 0;
+        // Units are left, so there is a next one (if no one changes the lengths meanwhile).
+        do ++place.b;
+        while (place.b < pg.batch && scalar(sequence_of(pg, place.b).tokens) == 0);
+        place.b = scalar(min(place.b, pg.batch - 1));
+      }
+    }
+  }
+}
+
+// Joins the parts of row tiles that several ranges share, in their order: a workgroup some rows of
+// the tile that begins in range blockIdx.x. Four values a thread: D / 4 threads read a part's row,
+// 1024 / D parts are read at once.
+template <class T>
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
+  __shared__ float weight[2048];
+  __shared__ f4 sums[256];
+  __shared__ float box[8];
+  const arthip_pages& pg = a.c.p;
+  const int range = blockIdx.x;
+  if (range >= a.pieces[a.ranges].x) return;
+  const int4 piece = a.pieces[range];
+  const int parts = piece.w;
+  if (parts == 0) return;
+  const Sequence seq = sequence_of(pg, piece.x);
+  const int token0 = piece.z * a.tile_tokens;
+  const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int D = pg.head_dim, quads = D / 4, steps = 256 / quads;
+  const int step = tid / quads, quad = tid - step * quads;
+  // Part s of a row: the first is one that ends inside its tile, the others begin inside.
+  auto slot = [&](int s, int row) __attribute__((always_inline)) {
+    return (int64_t)(2 * (range + s) + (s == 0 ? 1 : 0)) * a.row_slots + row;
+  };
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    lds_sync();  // the last row's weights and sums have been read
+    float top = -__builtin_inff();
+    for (int s = tid; s < parts; s += 256) top = fmaxf(top, a.stats[2 * slot(s, row)]);
+    top = over_wave(top, [](float x, float y) { return fmaxf(x, y); });
+    if (lane == 0) box[wave] = top;
+    lds_sync();
+    top = fmaxf(fmaxf(box[0], box[1]), fmaxf(box[2], box[3]));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float l = 0.0f;
+    for (int s = tid; s < parts; s += 256) {
+      const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * slot(s, row));
+      const float w = __builtin_amdgcn_exp2f(st.x - base);
+      weight[s] = w;
+      l = __builtin_fmaf(w, st.y, l);
+    }
+    l = over_wave(l, [](float x, float y) { return x + y; });
+    if (lane == 0) box[4 + wave] = l;
+    lds_sync();
+    l = (box[4] + box[5]) + (box[6] + box[7]);
+    f4 o = f4{};
+    if (step < steps) {
+#pragma unroll 4
+      for (int s = step; s < parts; s += steps) {
+        const float ws = weight[s];
+        const f4 x = *reinterpret_cast<const f4*>(a.sums + slot(s, row) * D + 4 * quad);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = ws != 0.0f ? __builtin_fmaf(ws, x[e], o[e]) : o[e];
+      }
+      sums[tid] = o;
+    }
+    lds_sync();
+    const int of = (int)fdiv((uint32_t)row, a.by_group);
+    const int64_t token = seq.first + token0 + of;
+    const int head = piece.y * a.group + row - of * a.group;
+    if (tid < quads) {
+      const int n = min(steps, parts);
+      for (int s = 1; s < n; ++s) o += sums[s * quads + tid];
+      const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+      T* const op = static_cast<T*>(a.c.out) + token * a.c.out_stride[0] + head * a.c.out_stride[1];
+      typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = in_range<T>(o[e] * scale);
+      *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o, t4);
+    }
+    if (a.c.lse && tid == 0) a.c.lse[token * a.c.q_heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+}
+
+struct TilePick {
+  void (*fn)(PagedArgs);
+  int threads;
+  int bytes;  // of LDS
+};
+
+template <class T, int DP, int KT, int NW>
+TilePick pick(Shape shape) {
+  return {shape == kPlain ? paged_tile<T, DP, KT, NW, kPlain>
+          : shape == kCap ? paged_tile<T, DP, KT, NW, kCap>
+                          : paged_tile<T, DP, KT, NW, kAny>,
+          NW * 64, 4 * TileL<DP, KT>::kTile};
+}
+
+template <class T>
+TilePick pick(int d, bool one_wave, Shape shape) {
+  if (one_wave) {
+    if (d <= 32) return pick<T, 32, 32, 1>(shape);
+    if (d <= 64) return pick<T, 64, 32, 1>(shape);
+    if (d <= 96) return pick<T, 96, 32, 1>(shape);
+    if (d <= 128) return pick<T, 128, 32, 1>(shape);
+    return pick<T, 256, 32, 1>(shape);
+  }
+  if (d <= 32) return pick<T, 32, 64, 4>(shape);
+  if (d <= 64) return pick<T, 64, 64, 4>(shape);
+  if (d <= 96) return pick<T, 96, 64, 4>(shape);
+  if (d <= 128) return pick<T, 128, 64, 4>(shape);
+  return pick<T, 256, 32, 4>(shape);
+}
+
+}  // namespace
+
+PagedPlan paged_plan(const arthip_paged_attention_args& c) {
+  PagedPlan p{};
+  if (c.p.batch == 0 || c.p.tokens == 0 || c.q_heads == 0) return p;
+  const int group = c.q_heads / c.p.k_heads;
+  const int64_t rows = (int64_t)c.p.tokens * group;
+  p.one_wave = group <= 32 && rows <= (int64_t)32 * c.p.batch;
+  const int tile = p.one_wave ? 32 : 128;
+  p.tile_tokens = tile / group;
+  p.row_slots = (int)std::min<int64_t>(tile, rows);
+  p.ranges = c.p.head_dim > 128 ? (p.one_wave ? 512 : 256) : p.one_wave ? 1024 : c.p.head_dim <= 64 ? 768 : 512;
+  p.counted = c.p.batch > 64;
+  const size_t parts = (size_t)2 * p.ranges * p.row_slots;
+  p.sums = parts * c.p.head_dim * sizeof(float);
+  p.stats = parts * 2 * sizeof(float);
+  p.pieces = (size_t)(p.ranges + 1) * sizeof(int4);
+  p.before = p.counted ? ((size_t)c.p.batch + 1) * sizeof(int64_t) : 0;
+  return p;
+}
+
+hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStream_t s) {
+  if (c.p.batch == 0 || c.p.tokens == 0 || c.q_heads == 0) return hipSuccess;
+  const PagedPlan plan = paged_plan(c);
+  PagedArgs a{};
+  a.c = c;
+  a.group = c.q_heads / c.p.k_heads;
+  a.tile_tokens = plan.tile_tokens;
+  a.ranges = plan.ranges;
+  a.row_slots = plan.row_slots;
+  a.lanes = 64;
+  while (a.lanes * c.p.batch > 64 && a.lanes > 1) a.lanes /= 2;
+  a.by_group = make_fastdiv((uint32_t)a.group);
+  a.by_page = make_fastdiv((uint32_t)c.p.page_size);
+  a.by_lanes = make_fastdiv((uint32_t)a.lanes);
+  if (c.cap > 0) a.cap = make_cap(c.cap, c.scale);
+  char* at = static_cast<char*>(c.workspace);
+  a.sums = reinterpret_cast<float*>(at);
+  a.stats = reinterpret_cast<float*>(at += plan.sums);
+  a.pieces = reinterpret_cast<int4*>(at += plan.stats);
+  int64_t* const before = reinterpret_cast<int64_t*>(at += plan.pieces);
+  const bool f16 = c.p.dtype == ARTHIP_TYPE_F16;
+  const Shape shape = c.cap > kCapSmall || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
+  const TilePick k =
+      f16 ? pick<_Float16>(c.p.head_dim, plan.one_wave, shape) : pick<__bf16>(c.p.head_dim, plan.one_wave, shape);
+  if (plan.counted) {
+    a.before = before;
+    const bool small = plan.one_wave || c.p.head_dim > 128;  // tiles of 32 keys
+    hipLaunchKernelGGL(small ? paged_count<5> : paged_count<6>, dim3(1), dim3(1024), 0, s, a, before);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(k.fn, dim3((unsigned)a.ranges), dim3((unsigned)k.threads), k.bytes, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(f16 ? paged_join<_Float16> : paged_join<__bf16>,
+                     dim3((unsigned)a.ranges, plan.one_wave ? 4 : 16), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace arthip

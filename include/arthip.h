@@ -564,6 +564,149 @@ typedef struct arthip_norm_args {
 int arthip_gated_norm(const arthip_norm_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* A paged cache of keys and values (device buffers)                          */
+/*                                                                           */
+/* For networks that read a clip or a text piece by piece: new tokens are    */
+/* written into the cache, look at it, leave a weight on the keys that they   */
+/* looked at, and the keys with little weight are evicted. The rules of the   */
+/* transformer operators hold: validated on the host, enqueued, nothing       */
+/* allocated, capturable, the same bits for the same inputs; fp16 or bf16.    */
+/*                                                                           */
+/* The pool holds `pool_pages` pages of `page_size` slots (a multiple of 16), */
+/* [pool_pages][page_size][k_heads][D] by strides. Slot s of sequence b lies  */
+/* in page pages[b][s / page_size]. kv_len[b] counts its slots in use, the     */
+/* new tokens among them, and is clamped to [0, max_pages * page_size]. New    */
+/* tokens are packed: those of sequence b are rows q_offsets[b] to             */
+/* q_offsets[b + 1] - 1 (clamped to [0, tokens]) of `tokens` rows, and take    */
+/* its last slots; without q_offsets each sequence has one (tokens = batch).   */
+/* Rows behind the last sequence are left as they are. All of this is read on  */
+/* the device when the call runs, so a captured call may be replayed as        */
+/* lengths and pages change. Pages outside the pool are neither read nor       */
+/* written: keys there count as zeros. A page belongs to one sequence; where   */
+/* a written page is named twice, either's rows may end up in it.              */
+/* ------------------------------------------------------------------------ */
+
+typedef struct arthip_pages {
+  const int32_t* pages;      /* [batch][max_pages]; the pages of a sequence are contiguous */
+  const int32_t* kv_len;     /* [batch] */
+  const int32_t* q_offsets;  /* [batch + 1], or NULL: one new token a sequence */
+  int64_t pages_stride;      /* of a sequence, in entries */
+  int32_t batch, tokens;     /* tokens: rows of all new tokens */
+  int32_t max_pages, pool_pages, page_size;
+  int32_t k_heads;
+  int32_t head_dim;          /* a multiple of 8 up to 256 */
+  int32_t dtype;             /* ARTHIP_TYPE_F16 or ARTHIP_TYPE_BF16 */
+} arthip_pages;
+
+/* The new tokens' keys and values into the cache. With `positions`, the slots' positions
+ * [batch][k_heads][slots] get those of their tokens (slots from `slots` on are left out). */
+typedef struct arthip_cache_write_args {
+  arthip_pages p;
+  const void* k;                   /* [tokens][k_heads][D] */
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  int32_t* positions;              /* or NULL */
+  const int32_t* token_positions;  /* [tokens], with positions */
+  int64_t k_stride[2];             /* token, head: multiples of 8, as all data is 16-byte aligned */
+  int64_t v_stride[2];
+  int64_t k_cache_stride[3];       /* page, slot, head: multiples of 8; a slot's from 0 to 2^24 */
+  int64_t v_cache_stride[3];
+  int64_t positions_stride[2];     /* sequence, head; slots are contiguous */
+  int32_t slots;
+  int32_t pad;
+} arthip_cache_write_args;
+
+int arthip_cache_write(const arthip_cache_write_args* args, void* stream);
+
+/* out = softmax(score) V of the new tokens' queries [tokens][q_heads][D] over their sequence's
+ * slots; each run of q_heads / k_heads (up to 128) query heads shares a key head. score(i, j) =
+ * scale * q_i . k_j, then cap * tanh(score / cap) if cap > 0. Token i of n new ones has the
+ * position p = kv_len - n + i and sees slots j < kv_len with p - left <= j and, if causal,
+ * j <= p. A token that sees nothing gives zeros, and -inf as its log-sum. Slots that a token does
+ * not see add nothing to it, whatever they hold. */
+typedef struct arthip_paged_attention_args {
+  arthip_pages p;
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  float* lse;               /* [tokens][q_heads] contiguous, natural log; or NULL */
+  void* workspace;          /* arthip_paged_attention_workspace bytes, for this call's time on its stream */
+  uint64_t workspace_bytes;
+  int64_t q_stride[2];      /* token, head */
+  int64_t out_stride[2];
+  int64_t k_cache_stride[3];
+  int64_t v_cache_stride[3];
+  float scale, cap;         /* cap 0: none */
+  int32_t q_heads;
+  int32_t causal;
+  int32_t left;             /* -1: no limit */
+  int32_t pad;
+} arthip_paged_attention_args;
+
+/* Bytes of workspace for these sizes, whatever the lengths; 0 where the call refuses them. */
+size_t arthip_paged_attention_workspace(const arthip_paged_attention_args* args);
+int arthip_paged_attention(const arthip_paged_attention_args* args, void* stream);
+
+/* What the new tokens looked at: for each slot and key head
+ *   out[b][h][j] = decay * weights[b][h][j] + sum of exp(score(i, j) - lse[i])
+ * over the new tokens i that see slot j and the query heads that share key head h, with the
+ * scores of arthip_paged_attention and its lse. The new tokens' own slots start from 0 instead of
+ * the old weight, as do all with a decay of 0 (then weights may be NULL); slots from kv_len on
+ * get 0. A token whose lse is -inf adds nothing. */
+typedef struct arthip_key_weights_args {
+  arthip_pages p;
+  const void* q;            /* [tokens][q_heads][D] */
+  const void* k_cache;
+  const float* lse;         /* [tokens][q_heads] contiguous */
+  const float* weights;     /* [batch][k_heads][slots] */
+  float* out;               /* may be weights with its strides (in place) */
+  void* workspace;          /* arthip_key_weights_workspace bytes */
+  uint64_t workspace_bytes;
+  int64_t q_stride[2];      /* token, head: from 0 to 2^24 */
+  int64_t k_cache_stride[3];
+  int64_t weights_stride[2];  /* sequence, head; slots are contiguous */
+  int64_t out_stride[2];
+  float scale, cap, decay;
+  int32_t q_heads;
+  int32_t causal;
+  int32_t left;
+  int32_t slots;            /* of weights and out; weight on later slots is left out */
+  int32_t pad;
+} arthip_key_weights_args;
+
+size_t arthip_key_weights_workspace(const arthip_key_weights_args* args);
+int arthip_key_weights(const arthip_key_weights_args* args, void* stream);
+
+/* Cuts each sequence to `keep` slots, a key head at a time. Of n = min(kv_len, slots) slots more
+ * than `keep` the protected ones stay first, then those with the largest weight (a NaN counts less
+ * than any number); equals go to the lowest slot. Protected are slots whose position is among the
+ * last `recent` up to the largest of them, or below `first`; a slot's position is itself, or
+ * positions[b][h][slot]. Staying slots from `keep` on move, in order, into the others below `keep`,
+ * in order; the rest stay where they are, as does what lies behind. Sequences of up to `keep`
+ * slots stay whole. A move from or to a page outside the pool is left out. Results of slots past
+ * the new length: weight 0, kept -1, position -1. */
+typedef struct arthip_cache_evict_args {
+  arthip_pages p;           /* tokens and q_offsets are not used */
+  void* k_cache;
+  void* v_cache;
+  const float* weights;     /* [batch][k_heads][slots] */
+  const int32_t* positions; /* the same, or NULL */
+  int32_t* new_len;         /* [batch] min(n, keep); or NULL */
+  float* weights_out;       /* [batch][k_heads][slots] contiguous, no input; or NULL */
+  int32_t* positions_out;   /* the same, with positions; or NULL */
+  int32_t* kept;            /* [batch][k_heads][keep] contiguous: the slot that is now in each */
+  int64_t k_cache_stride[3];
+  int64_t v_cache_stride[3];
+  int64_t weights_stride[2];    /* sequence, head; slots are contiguous */
+  int64_t positions_stride[2];
+  int32_t slots, keep, recent, first;  /* recent + first up to keep */
+} arthip_cache_evict_args;
+
+int arthip_cache_evict(const arthip_cache_evict_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Helpers                                                                   */
 /* ------------------------------------------------------------------------ */
 
