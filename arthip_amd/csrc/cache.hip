@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "launch.h"
 #include "paged.h"
@@ -90,15 +91,24 @@ __device__ __forceinline__ uint32_t ordered(float w) {
   return w != w ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of x over the threads before this one, and over all (16 waves).
+// Sum of x over the lanes up to this one, inside the vector unit: rows of 16, then across them.
+__device__ __forceinline__ uint32_t up_to(uint32_t x) {
+  auto add = [&](auto control, auto rows) __attribute__((always_inline)) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xf, false);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return x;
+}
+
+// Sum of x over the threads before this one, and over all (16 waves). Its halves are two sums.
 __device__ __forceinline__ uint64_t scan(uint64_t x, uint64_t* box, uint64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t sum = x;
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    const uint64_t y = __shfl_up((unsigned long long)sum, step);
-    sum += lane >= step ? y : 0;
-  }
+  const uint64_t sum = up_to((uint32_t)x) | (uint64_t)up_to((uint32_t)(x >> 32)) << 32;
   lds_sync();  // the box has been read
   if (lane == 63) box[wave] = sum;
   lds_sync();
