@@ -7,10 +7,10 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "attention_dev.h"
 #include "launch.h"
 #include "paged.h"
 #include "paged_dev.h"
-#include "token_dev.h"
 #include "transformer.h"
 
 namespace arthip {
@@ -81,8 +81,10 @@ struct EvictArgs {
   FastDiv by_page, by_heads, by_head_chunks;
 };
 
-constexpr int kThreads = 1024;
-constexpr int kMoves = 4096;    // slots listed in LDS at once
+constexpr int kWaves = 16;       // of the selecting workgroup
+constexpr int kThreads = 64 * kWaves;
+constexpr int kBins = 2048;      // 11 bits of a key at a time: 11, 11, 10
+constexpr int kMoves = 8192;     // slots listed in LDS at once
 constexpr int kMovesHere = 256;  // up to this many the selecting workgroup moves the rows itself
 
 // A weight as a number whose order is the weights': NaN is 0, less than -inf.
@@ -105,23 +107,6 @@ __device__ __forceinline__ uint32_t up_to(uint32_t x) {
   return x;
 }
 
-// Sum of x over the threads before this one, and over all (16 waves). Its halves are two sums.
-__device__ __forceinline__ uint64_t scan(uint64_t x, uint64_t* box, uint64_t& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t sum = up_to((uint32_t)x) | (uint64_t)up_to((uint32_t)(x >> 32)) << 32;
-  lds_sync();  // the box has been read
-  if (lane == 63) box[wave] = sum;
-  lds_sync();
-  uint64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    before += w < wave ? box[w] : 0;
-    total += box[w];
-  }
-  return before + sum - x;
-}
-
 // 16 bytes of a slot's key and of its value to another slot.
 __device__ __forceinline__ void move_chunk(const EvictArgs& a, const int32_t* pages, int head, int part, int from,
                                            int to) {
@@ -138,21 +123,23 @@ __device__ __forceinline__ void move_chunk(const EvictArgs& a, const int32_t* pa
   *reinterpret_cast<u4*>(v + v_to) = y;
 }
 
-// The slots of one key head of one sequence: a thread holds E of them in a row (E = 0: as many as
-// there are, read again each time). The `keep`-th largest key is found bit by bit from the top: a
-// candidate stands if at least `keep` keys reach it. Waves count with ballots, so that equal
-// weights cost no more than others, as they would in a histogram's counters.
-template <int E, bool HERE>
+// The slots of one key head of one sequence, by one workgroup. The `keep`-th largest key is found
+// 11 bits at a time from a histogram of the keys that share the bits before; then each wave ranks
+// the holes and the movers of a run of slots. Keys are read anew in every pass, 64 in a row a wave:
+// they come from the L2 (32768 slots: some 1 us a pass).
+template <bool HERE>
 __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
-  __shared__ uint64_t box[kThreads / 64];
-  __shared__ int counts[32];
-  __shared__ int newest_box;
-  __shared__ int list[kMoves];
+  __shared__ int bins[kBins];
+  __shared__ int box[3][kWaves];
+  __shared__ int found[3];
+  __shared__ int list[HERE ? kMovesHere : kMoves];
   __shared__ int holes_at[HERE ? kMovesHere : 1];
+  constexpr int kList = HERE ? kMovesHere : kMoves;
   const arthip_pages& p = a.c.p;
   const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = (int)fdiv(blockIdx.x, a.by_heads), head = (int)blockIdx.x - b * p.k_heads;
-  const int n = min(slots_of(p, b), a.c.slots), keep = a.c.keep;
+  const int n = __builtin_amdgcn_readfirstlane(min(slots_of(p, b), a.c.slots)), keep = a.c.keep;
   const float* const w = a.c.weights + b * a.c.weights_stride[0] + head * a.c.weights_stride[1];
   const int32_t* const place =
       a.c.positions == nullptr ? nullptr : a.c.positions + b * a.c.positions_stride[0] + head * a.c.positions_stride[1];
@@ -181,105 +168,147 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
     return;
   }
 
-  const int each = E > 0 ? E : (n + kThreads - 1) / kThreads;
-  const int first = tid * each;
   int newest = n - 1;
   if (place != nullptr) {
-    if (tid == 0) newest_box = INT32_MIN;
-    lds_sync();
     int top = INT32_MIN;
     for (int s = tid; s < n; s += kThreads) top = max(top, place[s]);
-    atomicMax(&newest_box, top);
+    top = over_wave(top, [](int x, int y) { return max(x, y); });
+    if (lane == 0) box[0][wave] = top;
     lds_sync();
-    newest = newest_box;
+    newest = box[0][0];
+    for (int i = 1; i < kWaves; ++i) newest = max(newest, box[0][i]);
   }
   auto key_of = [&](int s) __attribute__((always_inline)) -> uint32_t {
-    if (s >= n) return 0u;
     const int64_t t = place != nullptr ? place[s] : s;
-    return t > (int64_t)newest - a.c.recent || t < a.c.first ? UINT32_MAX : ordered(w[s]);
-  };
-  uint32_t keys[E > 0 ? E : 1];
-  if constexpr (E > 0) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) keys[i] = key_of(first + i);
-  }
-  auto each_key = [&](auto f) __attribute__((always_inline)) {
-    if constexpr (E > 0) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) f(first + i, keys[i]);
-    } else {
-      for (int i = 0; i < each; ++i) f(first + i, key_of(first + i));
-    }
+    const uint32_t u = ordered(w[s]);
+    return t > (int64_t)newest - a.c.recent || t < a.c.first ? UINT32_MAX : u;
   };
 
   // -- the keep-th largest key ---------------------------------------------------------
-  if (tid < 32) counts[tid] = 0;
-  lds_sync();
-  uint32_t least = 0;
-  int reach = n;  // keys of `least` or more
-  for (int bit = 31; bit >= 0 && reach != keep; --bit) {
-    const uint32_t candidate = least | 1u << bit;
-    int count = 0;
-    each_key([&](int, uint32_t key) { count += __popcll(__ballot(key >= candidate)); });
-    if (lane == 0) atomicAdd(&counts[bit], count);
+  uint32_t least = 0;  // its bits so far
+  int want = keep;     // it is the want-th largest of the keys that share them
+  bool ties = false;   // of which not all stay
+  for (int level = 0; level < 3; ++level) {
+    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
     lds_sync();
-    const int all = counts[bit];
-    if (all >= keep) {
-      least = candidate;
-      reach = all;
+    for (int s = tid; s < n; s += kThreads) {
+      const uint32_t key = key_of(s);
+      bool in = level == 0 || key >> (shift + width) == least >> (shift + width);
+      const int bin = (int)(key >> shift) & ((1 << width) - 1);
+      // Equal keys are common (weights of 0, protected slots) and would meet in one counter: two
+      // of a wave's bins are counted by ballots.
+#pragma unroll
+      for (int round = 0; round < 2; ++round) {
+        const uint64_t left = __ballot(in);
+        if (left == 0) break;
+        const int first = __builtin_amdgcn_readlane(bin, __builtin_ctzll(left));
+        const bool same = in && bin == first;
+        const int count = __popcll(__ballot(same));
+        if (lane == (int)__builtin_ctzll(left)) atomicAdd(&bins[first], count);
+        in = in && !same;
+      }
+      if (in) atomicAdd(&bins[bin], 1);
     }
+    lds_sync();
+    // Two bins a thread, the largest keys first: the bin in which the want-th key lies.
+    const int top = kBins - 1 - 2 * tid;
+    const int c0 = bins[top], c1 = bins[top - 1];
+    const int sum = (int)up_to((uint32_t)(c0 + c1));
+    if (lane == 63) box[level][wave] = sum;
+    lds_sync();
+    int before = sum - c0 - c1;
+    for (int i = 0; i < wave; ++i) before += box[level][i];
+    const bool here = before < want && want <= before + c0 + c1;
+    if (here) {
+      const bool second = want > before + c0;
+      found[0] = top - (second ? 1 : 0);
+      found[1] = want - before - (second ? c0 : 0);
+      found[2] = second ? c1 : c0;
+    }
+    lds_sync();
+    least |= (uint32_t)found[0] << shift;
+    want = found[1];
+    ties = found[2] != want;
+    lds_sync();
+    if (!ties) break;  // all keys from here on stay
   }
-  // Of the equals of the least, the lowest slots make up for what the larger leave.
-  int equals_before = 0, equals = 0;
-  uint64_t total;
-  const bool ties = reach != keep;
-  if (ties) {
-    uint64_t here = 0;
-    each_key([&](int s, uint32_t key) { here += s < n && key == least; });
-    equals_before = (int)scan(here, box, total);
-    equals = keep - (reach - (int)total);
-  }
-  auto each_slot = [&](auto f) __attribute__((always_inline)) {
-    int seen = equals_before;
-    each_key([&](int s, uint32_t key) {
-      bool stay = key >= least && s < n;
-      if (ties && key == least && s < n) stay = seen++ < equals;
-      f(s, stay);
-    });
-  };
 
   // -- holes below the budget and slots past it that stay, by their ranks -----------------
-  uint64_t mine = 0;  // holes, and movers above them
-  each_slot([&](int s, bool stay) {
-    mine += s < keep && !stay ? 1 : 0;
-    mine += s >= keep && stay ? uint64_t{1} << 32 : 0;
-  });
-  const uint64_t before = scan(mine, box, total);
-  const int moves = (int)(uint32_t)total;
-  each_slot([&](int s, bool stay) {
-    if (s < keep && stay) stays(s, s);
-  });
-  for (int from = 0; from < moves; from += kMoves) {
-    lds_sync();  // the list has been read
-    int rank = (int)(before >> 32) - from;
-    each_slot([&](int s, bool stay) {
-      if (s < keep || !stay) return;
-      if ((uint32_t)rank < (uint32_t)kMoves) list[rank] = s;
-      ++rank;
-    });
+  const int run = ((n + kWaves - 1) / kWaves + 63) & ~63;  // slots of a wave
+  const int begin = min(wave * run, n), end = min(begin + run, n);
+  auto all_waves = [&](int mine, int (&of)[kWaves], int& total) __attribute__((always_inline)) {
+    if (lane == 0) of[wave] = mine;
     lds_sync();
-    rank = (int)(uint32_t)before - from;
-    each_slot([&](int s, bool stay) {
-      if (s >= keep || stay) return;
-      if ((uint32_t)rank < (uint32_t)kMoves) {
-        stays(s, list[rank]);
-        if constexpr (HERE) holes_at[rank] = s;
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < kWaves; ++i) {
+      before += i < wave ? of[i] : 0;
+      total += of[i];
+    }
+    return before;
+  };
+  // Of the equals of the least, the lowest `want` slots stay.
+  int equals_before = 0, total;
+  if (ties) {
+    int equals = 0;
+    for (int s0 = begin; s0 < end; s0 += 64) {
+      const int s = s0 + lane;
+      equals += __popcll(__ballot(s < end && key_of(min(s, n - 1)) == least));
+    }
+    equals_before = all_waves(equals, box[0], total);
+  }
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  auto each_slot = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, it stays)
+    int seen = equals_before;
+    for (int s0 = begin; s0 < end; s0 += 64) {
+      const int s = s0 + lane;
+      const uint32_t key = key_of(min(s, n - 1));
+      bool stay = s < end && key >= least;
+      if (ties) {
+        const bool equal = s < end && key == least;
+        const uint64_t mask = __ballot(equal);
+        if (equal) stay = seen + __popcll(mask & below) < want;
+        seen += __popcll(mask);
       }
-      ++rank;
+      f(s, s < end, stay);
+    }
+  };
+  int holes = 0, movers = 0;
+  each_slot([&](int s, bool is, bool stay) {
+    holes += __popcll(__ballot(is && s < keep && !stay));
+    movers += __popcll(__ballot(is && s >= keep && stay));
+  });
+  const int holes_before = all_waves(holes, box[1], total);
+  const int moves = total;
+  const int movers_before = all_waves(movers, box[2], total);
+  for (int from = 0; from == 0 || from < moves; from += kList) {
+    if (movers > 0) {
+      int rank = movers_before - from;
+      each_slot([&](int s, bool is, bool stay) {
+        const bool mover = is && s >= keep && stay;
+        const uint64_t mask = __ballot(mover);
+        const int mine = rank + __popcll(mask & below);
+        if (mover && (uint32_t)mine < (uint32_t)kList) list[mine] = s;
+        rank += __popcll(mask);
+      });
+    }
+    lds_sync();
+    int rank = holes_before - from;
+    each_slot([&](int s, bool is, bool stay) {
+      const bool hole = is && s < keep && !stay;
+      const uint64_t mask = __ballot(hole);
+      const int mine = rank + __popcll(mask & below);
+      if (hole && (uint32_t)mine < (uint32_t)kList) {
+        stays(s, list[mine]);
+        if constexpr (HERE) holes_at[mine] = s;
+      }
+      if (from == 0 && is && s < keep && stay) stays(s, s);
+      rank += __popcll(mask);
     });
+    lds_sync();  // the list has been read
   }
   if constexpr (HERE) {
-    lds_sync();
     const int32_t* const pages = p.pages + b * p.pages_stride;
     for (int i = tid; i < moves * a.head_chunks; i += kThreads) {
       const int m = (int)fdiv((uint32_t)i, a.by_head_chunks), part = i - m * a.head_chunks;
@@ -302,11 +331,6 @@ __global__ void __launch_bounds__(256) evict_move(EvictArgs a, int64_t first_blo
   const int b = (int)fdiv((uint32_t)at, a.by_heads), head = (int)at - b * p.k_heads;
   const int32_t* const pages = p.pages + b * p.pages_stride;
   move_chunk(a, pages, head, part, from, s);
-}
-
-template <int E>
-void (*select_of(bool here))(EvictArgs) {
-  return here ? evict_select<E, true> : evict_select<E, false>;
 }
 
 }  // namespace
@@ -338,13 +362,7 @@ hipError_t launch_cache_evict(const arthip_cache_evict_args& c, hipStream_t s) {
   const int64_t heads = (int64_t)c.p.batch * c.p.k_heads;
   const int most = std::min(c.keep, std::max(0, c.slots - c.keep));  // moves of a key head
   const bool here = most <= kMovesHere;
-  const int each = (c.slots + kThreads - 1) / kThreads;
-  const auto fn = each <= 4    ? select_of<4>(here)
-                  : each <= 8  ? select_of<8>(here)
-                  : each <= 16 ? select_of<16>(here)
-                  : each <= 32 ? select_of<32>(here)
-                               : select_of<0>(here);
-  hipLaunchKernelGGL(fn, dim3((unsigned)heads), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(here ? evict_select<true> : evict_select<false>, dim3((unsigned)heads), dim3(kThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || here) return e;
   const int per = 256 / a.head_chunks;

@@ -46,9 +46,14 @@ struct PagedArgs {
   const int64_t* before;  // key tiles of the sequences before each [batch + 1], of all key heads
   float* sums;   // [2 ranges][row_slots][D] unscaled: parts that begin inside a row tile, parts that end inside
   float* stats;  // [2 ranges][row_slots][2] maximum (base 2) and sum
+  int* odd;      // [ranges][4 waves] kHead, kTail, kWhole
   int4* pieces;  // [ranges + 1] of a row tile that begins in a range and ends in another: sequence, key
                  // head, tile, number of parts. The last: ranges that there are.
 };
+
+// Parts of row tiles in which a row met an infinity or NaN that it may not see: the one that begins
+// inside its tile, the one that ends inside, whole row tiles.
+constexpr int kHead = 1, kTail = 2, kWhole = 4;
 
 constexpr int kLeast = 4;  // key tiles of a range, where there are that many
 
@@ -79,6 +84,21 @@ __device__ __forceinline__ int64_t shuffle(int64_t x, int lane) { return __shfl(
 struct Place {
   int b, head, tile, unit;  // unit: of the row tile's
 };
+
+// The row tile after a place's; false where there is none (which the units rule out, if no one changes
+// the lengths meanwhile).
+__device__ __forceinline__ bool next_tile(const PagedArgs& a, const Sequence& s, Place& at) {
+  at.unit = 0;
+  if (++at.tile < tiles_of(a, s)) return true;
+  at.tile = 0;
+  if (++at.head < a.c.p.k_heads) return true;
+  at.head = 0;
+  do ++at.b;
+  while (at.b < a.c.p.batch && sequence_of(a.c.p, at.b).tokens == 0);
+  const bool is = at.b < a.c.p.batch;
+  at.b = min(at.b, a.c.p.batch - 1);
+  return is;
+}
 
 // The units before each sequence, by one workgroup: a wave a sequence, then a running sum.
 template <int KT>
@@ -229,9 +249,6 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   const arthip_pages& pg = a.c.p;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = tid & 63;
-  const int n = lane & 31;     // the lane's row of the wave's 32
-  const int half = lane >> 5;  // which keys and values of it
   auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   auto scalar64 = [&](int64_t x) {
     return (int64_t)((uint64_t)(uint32_t)scalar((int)x) | (uint64_t)(uint32_t)scalar((int)(x >> 32)) << 32);
@@ -241,7 +258,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   // Workgroups go round the eight XCDs: each takes an eighth of the ranges in a row, as row tiles
   // of one key head share K and V.
   Finder<LOG> finder;
-  finder.count(a, lane);
+  finder.count(a, tid & 63);
   const int64_t total = scalar64(finder.total);
   const int live = total >= (int64_t)a.ranges * kLeast ? a.ranges : max((int)total / kLeast, total > 0 ? 1 : 0);
   const int per = (live + 7) >> 3;
@@ -252,37 +269,45 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   const int more = scalar((int)(total - share * live));  // ranges of one unit more
   int64_t at = range * share + min(range, more);
   const int64_t range_end = at + share + (range < more ? 1 : 0);
-  Place place = finder.find(a, at, lane);
+  Place place = finder.find(a, at, tid & 63);
   place = {scalar(place.b), scalar(place.head), scalar(place.tile), scalar(place.unit)};
 
-  // -- what does not change from row tile to row tile ----------------------------------
-  const int my_token = (int)fdiv((uint32_t)(wave * 32 + n), a.by_group);  // of the row tile
-  const int g_head = wave * 32 + n - my_token * a.group;
-  const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
-  const int s_row = (wave * LOADS * 1024 + lane * 16) / RB;  // tile's key of the wave's first load
-  const int s_chunk = lane * 16 % RB / 16;
-  const int l_row = lane * 16 / RB;  // the same of the load's keys
-  const int ks2 = (int)a.c.k_cache_stride[1] * 2, vs2 = (int)a.c.v_cache_stride[1] * 2;  // bytes
-  constexpr int KP = (RB == 512 ? 8 : 16) / STEP < LOADS ? (RB == 512 ? 8 : 16) / STEP : LOADS;
-  constexpr int VP = 4 / STEP < 1 ? 1 : 4 / STEP < LOADS ? 4 / STEP : LOADS;
-  uint32_t k_off[KP], v_off[VP];  // a lane's offsets, but for the keys between its loads
-  auto offset_of = [&](int chunk, int stride) __attribute__((always_inline)) {
-    return chunk * 8 < pg.head_dim ? (uint32_t)(l_row * stride + chunk * 16) : kOob;
-  };
-#pragma unroll
-  for (int i = 0; i < KP; ++i) k_off[i] = offset_of(s_chunk ^ L::k_swizzle(s_row + i * STEP), ks2);
-#pragma unroll
-  for (int i = 0; i < VP; ++i) v_off[i] = offset_of(s_chunk ^ L::v_swizzle(s_row + i * STEP), vs2);
-  typedef __attribute__((address_space(3))) unsigned char lds_byte;
-  typedef __attribute__((address_space(3))) const frag lds_frag;
-  typedef __attribute__((address_space(3))) s4 lds_s4;
-  lds_byte* const lds0 = (lds_byte*)lds;
-  const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
-  const int v_row = 4 * half + (lane & 15) / 4;
-  const uint32_t v_lane =
-      v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+  int odd = 0;  // what the wave met
 
   while (true) {
+    // -- the lane's part -----------------------------------------------------------------
+    // (Found again for every row tile: what would be kept across them is registers that the walk
+    // needs. Spilled ones come back by loads that wait for the tiles' own.)
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int n = lane & 31;     // its row of the wave's 32
+    const int half = lane >> 5;  // which keys and values of it
+    const int my_token = (int)fdiv((uint32_t)(wave * 32 + n), a.by_group);  // of the row tile
+    const int g_head = wave * 32 + n - my_token * a.group;
+    const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
+    const int s_row = (wave * LOADS * 1024 + lane * 16) / RB;  // tile's key of the wave's first load
+    const int s_chunk = lane * 16 % RB / 16;
+    const int l_row = lane * 16 / RB;  // the same of the load's keys
+    const int ks2 = (int)a.c.k_cache_stride[1] * 2, vs2 = (int)a.c.v_cache_stride[1] * 2;  // bytes
+    constexpr int KP = (RB == 512 ? 8 : 16) / STEP < LOADS ? (RB == 512 ? 8 : 16) / STEP : LOADS;
+    constexpr int VP = 4 / STEP < 1 ? 1 : 4 / STEP < LOADS ? 4 / STEP : LOADS;
+    uint32_t k_off[KP], v_off[VP];  // a lane's offsets, but for the keys between its loads
+    auto offset_of = [&](int chunk, int stride) __attribute__((always_inline)) {
+      return chunk * 8 < pg.head_dim ? (uint32_t)(l_row * stride + chunk * 16) : kOob;
+    };
+#pragma unroll
+    for (int i = 0; i < KP; ++i) k_off[i] = offset_of(s_chunk ^ L::k_swizzle(s_row + i * STEP), ks2);
+#pragma unroll
+    for (int i = 0; i < VP; ++i) v_off[i] = offset_of(s_chunk ^ L::v_swizzle(s_row + i * STEP), vs2);
+    typedef __attribute__((address_space(3))) unsigned char lds_byte;
+    typedef __attribute__((address_space(3))) const frag lds_frag;
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    lds_byte* const lds0 = (lds_byte*)lds;
+    const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
+    const int v_row = 4 * half + (lane & 15) / 4;
+    const uint32_t v_lane =
+        v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
+
     // -- a row tile, or a part of it ----------------------------------------------------
     Sequence seq = sequence_of(pg, place.b);
     seq.first = scalar(seq.first);
@@ -397,57 +422,19 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + kk * 16 * RB + 8 * RB));
       return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    bool odd = false;  // a tile that a row does not see whole holds an infinity or NaN in V
-    auto values = [&](int buf, bool look) __attribute__((always_inline)) {
+    auto values = [&](int buf) __attribute__((always_inline)) {
       lds_byte* const from = lds0 + v_at + buf * L::kTile;
       lds_byte* v[DB];
 #pragma unroll
       for (int db = 0; db < DB; ++db) v[db] = from + (v_lane ^ (db * 64));
-      if (look) {
-        // Rows that do not see all of this tile weigh some of V by 0, which infinities and
-        // NaN survive: 0 times the tile tells whether it has any.
-        f16v z = f16v{};
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) z = E::mma(v_frag(v[db], kk), frag{}, z);
-        float t = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) t += z[r];
-        odd = odd || t != 0.0f;
-      }
 #pragma unroll
       for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
       ahead<KT / 16 * DB, 2>();
     };
-    // The same key by key, each added only to the rows that see it. (Weights that round to 0 are -0
-    // there, as an infinity or NaN counts with any weight; those of hidden keys are +0.)
-    auto values_apart = [&](int buf) __attribute__((always_inline)) {
-      lds_byte* const from = lds0 + v_at + buf * L::kTile;
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)
-#pragma unroll 1
-        for (int key = 0; key < 16; ++key) {
-          const int of = (key >> 2) & 1, j = (key & 3) | ((key >> 1) & 4);  // its half and element
-          u4 keep;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) keep[e] = half != of || j >> 1 != e ? 0u : j & 1 ? 0xffff0000u : 0x0000ffffu;
-          const u4 one = __builtin_bit_cast(u4, p[kk]) & keep;
-          const float sees = halves_max((one[0] | one[1] | one[2] | one[3]) != 0 ? 1.0f : 0.0f);
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const u4 x = __builtin_bit_cast(u4, v_frag(from + (v_lane ^ (db * 64)), kk)) & keep;
-            const f16v c = E::mma(__builtin_bit_cast(frag, x), __builtin_bit_cast(frag, one), f16v{});
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[db][r] += sees != 0.0f ? c[r] : 0.0f;
-          }
-        }
-    };
-
     // -- scores to weights -----------------------------------------------------------------
-    auto weights = [&](auto apart, int k0, bool partial) __attribute__((always_inline)) {
+    auto weights = [&](int k0, bool partial) __attribute__((always_inline)) {
       const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
       if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
         float far = 0.0f;
@@ -520,9 +507,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float x = s[kb][r], w = __builtin_amdgcn_exp2f(__builtin_fmaf(x, mul, -base));
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], mul, -base));
           sum += w;
-          s[kb][r] = decltype(apart)::value && w <= E::kZero && x != -__builtin_inff() ? -0.0f : w;
+          s[kb][r] = w;
         }
       l += sum;  // this half's keys; the halves are added at the end
 #pragma unroll
@@ -545,9 +532,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         x.of[g] = scalar(x.of[g]);
       }
     };
-    auto walk = [&](auto apart) __attribute__((always_inline)) {
-      lds_sync();  // the last walk's tiles have been used
-      if (begin >= end) return;
+    lds_sync();  // the last row tile has been used
+    if (begin < end) {
       Pages here = ask(begin), next = here;
       settle(here);
       stage_k(0, begin, here);
@@ -556,7 +542,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       settle(next);
       lds_sync();
       int buf = 0;
-      bool has = false, look = false;  // weights of the previous tile; some row sees not all of it
+      bool has = false;  // weights of the previous tile
       for (int t = begin;; ++t) {
         const bool on = t < end;
         const int k0 = t * KT, k1 = k0 + KT;
@@ -570,16 +556,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
           partial = !(k0 >= w_lo_max && k1 <= w_hi_min);
         }
         if (seen) scores(buf);
-        if (has) {
-          if constexpr (decltype(apart)::value)
-            values_apart(buf ^ 1);
-          else
-            values(buf ^ 1, look);
-        }
+        if (has) values(buf ^ 1);
         if (!on) break;
-        if (seen) weights(apart, k0, partial);
+        if (seen) weights(k0, partial);
         has = seen;
-        look = partial;
         vm_wait();
         settle(then);
         lds_sync();
@@ -587,24 +567,33 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         next = then;
         buf ^= 1;
       }
-    };
-    walk(std::false_type{});
-    // A workgroup that met such a tile starts over and takes the keys one by one.
-    {
-      int* const flag = reinterpret_cast<int*>(lds);
-      lds_sync();
-      if (lane == 0) flag[wave] = 0;
-      if (odd) flag[wave] = 1;
-      lds_sync();
-      int again = 0;
-      for (int i = 0; i < NW; ++i) again |= flag[i];
-      if (__builtin_expect(scalar(again) != 0, 0)) {
+    }
+
+    // Rows that do not see all of a tile weigh some of V by 0, which infinities and NaN survive. Where
+    // the sums are not finite, such tiles are looked over, and those row tiles that met one are found
+    // anew by the joining kernel.
+    float rest = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DB; ++i) o[i] = f16v{};
-        m = -__builtin_inff();
-        l = 0.0f;
-        walk(std::true_type{});
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rest = __builtin_fmaf(o[i][r], 0.0f, rest);
+    if (__builtin_expect(__any(rest != 0.0f), 0)) {
+      bool found = false;
+      for (int t = begin; t < end; ++t) {
+        if (!w_real || t * KT >= w_hi_max || t * KT + KT <= w_lo_min) continue;
+        if (t * KT >= w_lo_max && t * KT + KT <= w_hi_min) continue;
+        for (int i = lane; i < KT * (DP / 8); i += 64) {
+          const int slot = t * KT + i / (DP / 8), d = i % (DP / 8) * 8;
+          if (slot >= kv_len || d >= pg.head_dim) continue;
+          const int64_t row = row_of(pg, a.by_page, pages, slot, a.c.v_cache_stride);
+          if (row == -1) continue;
+          const frag x = *reinterpret_cast<const frag*>(static_cast<const T*>(a.c.v_cache) + row +
+                                                        place.head * a.c.v_cache_stride[2] + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) found = found || !(fabsf((float)x[e]) < __builtin_inff());
+        }
       }
+      if (__any(found)) odd |= take == units ? kWhole : place.unit == 0 ? kTail : kHead;
     }
 
     // -- results -------------------------------------------------------------------------
@@ -658,6 +647,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const int64_t tile_end = at + units - place.unit;
     at += take;
     if (at >= range_end) {
+      if ((tid & 63) == 0) a.odd[range * 4 + wave] = odd;
       if (tid == 0) {
         // Whether a row tile begins here and ends in a later range.
         int parts = 0;
@@ -669,90 +659,182 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       }
       return;
     }
-    place.unit = 0;
-    if (++place.tile == tiles_of(a, seq)) {
-      place.tile = 0;
-      if (++place.head == pg.k_heads) {
-        place.head = 0;
-        // Units are left, so there is a next one (if no one changes the lengths meanwhile).
-        do ++place.b;
-        while (place.b < pg.batch && scalar(sequence_of(pg, place.b).tokens) == 0);
-        place.b = scalar(min(place.b, pg.batch - 1));
+    next_tile(a, seq, place);
+    place = {scalar(place.b), scalar(place.head), scalar(place.tile), 0};
+  }
+}
+
+// One row by itself, from the definition: the rows of a workgroup's share of a row tile one after the
+// other, each key added only to the rows that see it (an infinity whatever its weight).
+template <class T>
+__device__ __forceinline__ void rows_apart(const PagedArgs& a, int b, int kh, int tile, float* weight, float* box) {
+  const arthip_pages& pg = a.c.p;
+  const Sequence seq = sequence_of(pg, b);
+  const int32_t* const pages = pg.pages + b * pg.pages_stride;
+  const int token0 = tile * a.tile_tokens, rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    const int of = (int)fdiv((uint32_t)row, a.by_group), token = token0 + of;
+    const int head = kh * a.group + row - of * a.group, place = seq.start() + token;
+    const int lo = a.c.left < 0 ? 0 : min(max(place - a.c.left, 0), seq.len);
+    const int hi = a.c.causal ? min(max(place + 1, 0), seq.len) : seq.len;
+    const T* const q = static_cast<const T*>(a.c.q) + (seq.first + token) * a.c.q_stride[0] + head * a.c.q_stride[1];
+    auto score = [&](int slot) {  // in the base of 2
+      const int64_t at = row_of(pg, a.by_page, pages, slot, a.c.k_cache_stride);
+      float x = 0.0f;
+      if (at != -1) {
+        const T* const k = static_cast<const T*>(a.c.k_cache) + at + kh * a.c.k_cache_stride[2];
+        for (int d = 0; d < pg.head_dim; ++d) x = __builtin_fmaf((float)q[d], (float)k[d], x);
       }
+      if (!(a.c.cap > 0)) return x * (a.c.scale * kLog2e);
+      if (fabsf(x) <= a.cap.reach) return cap_near(a.cap, x);
+      const float e = __builtin_amdgcn_exp2f(x * a.cap.in);
+      return __builtin_fmaf(-2.0f * a.cap.out, __builtin_amdgcn_rcpf(e + 1.0f), a.cap.out);
+    };
+    auto over_all = [&](float x, auto f) {
+      x = over_wave(x, f);
+      lds_sync();
+      if (lane == 0) box[wave] = x;
+      lds_sync();
+      return f(f(box[0], box[1]), f(box[2], box[3]));
+    };
+    float top = -__builtin_inff();
+    for (int slot = lo + tid; slot < hi; slot += 256) top = fmaxf(top, score(slot));
+    top = over_all(top, [](float x, float y) { return fmaxf(x, y); });
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float l = 0.0f, o = 0.0f;  // o: value tid of the head
+    for (int slot0 = lo; slot0 < hi; slot0 += 256) {
+      const int n = min(256, hi - slot0);
+      lds_sync();
+      if (tid < n) {
+        const float w = __builtin_amdgcn_exp2f(score(slot0 + tid) - base);
+        weight[tid] = w;
+        l += w;
+      }
+      lds_sync();
+      if (tid < pg.head_dim)
+        for (int i = 0; i < n; ++i) {
+          const int64_t at = row_of(pg, a.by_page, pages, slot0 + i, a.c.v_cache_stride);
+          if (at == -1) continue;
+          const float x = (float)static_cast<const T*>(a.c.v_cache)[at + kh * a.c.v_cache_stride[2] + tid];
+          const float w = weight[i];
+          o += w == 0.0f && !(fabsf(x) < __builtin_inff()) ? x : w * x;
+        }
     }
+    l = over_all(l, [](float x, float y) { return x + y; });
+    T* const op = static_cast<T*>(a.c.out) + (seq.first + token) * a.c.out_stride[0] + head * a.c.out_stride[1];
+    if (tid < pg.head_dim) op[tid] = to_elem<T>(in_range<T>(l == 0.0f ? 0.0f : o * (1.0f / l)));
+    if (a.c.lse && tid == 0)
+      a.c.lse[(int64_t)(seq.first + token) * a.c.q_heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
 // Joins the parts of row tiles that several ranges share, in their order: a workgroup some rows of
-// the tile that begins in range blockIdx.x. Four values a thread: D / 4 threads read a part's row,
-// 1024 / D parts are read at once.
-template <class T>
+// the tile that begins in range blockIdx.x. Four values a thread, D / 4 threads a row; where the rows
+// do not fill the workgroup, several such groups take a row's parts in turn.
+template <class T, int KT>
 __global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
-  __shared__ float weight[2048];
   __shared__ f4 sums[256];
-  __shared__ float box[8];
+  __shared__ float2 stats[256];
+  __shared__ int met;
   const arthip_pages& pg = a.c.p;
-  const int range = blockIdx.x;
-  if (range >= a.pieces[a.ranges].x) return;
+  const int range = blockIdx.x, live = a.pieces[a.ranges].x;
+  if (range >= live) return;
   const int4 piece = a.pieces[range];
-  const int parts = piece.w;
+  const int parts = piece.w, waves = a.wave_rows ? 1 : 4;
+  int odd = 0;
+  for (int w = 0; w < waves; ++w) odd |= a.odd[range * 4 + w];
+  if (__builtin_expect((odd & kWhole) != 0, 0)) {
+    // All whole row tiles of the range, once more.
+    const int lane = threadIdx.x & 63;
+    Finder<KT> finder;
+    finder.count(a, lane);
+    const int64_t share = finder.total / live;
+    const int more = (int)(finder.total - share * live);
+    int64_t at = range * share + min(range, more);
+    const int64_t range_end = at + share + (range < more ? 1 : 0);
+    Place place = finder.find(a, at, lane);
+    while (true) {
+      const Sequence seq = sequence_of(pg, place.b);
+      const int units = units_of<KT>(a, seq, place.tile);
+      if (place.unit == 0 && at + units <= range_end)
+        rows_apart<T>(a, place.b, place.head, place.tile, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
+      at += units - place.unit;
+      if (at >= range_end) break;
+      if (!next_tile(a, seq, place)) break;
+    }
+  }
   if (parts == 0) return;
+  if (threadIdx.x == 0) met = odd & kTail;
+  lds_sync();
+  for (int s = 1 + (int)threadIdx.x; s < parts; s += 256) {
+    int part_odd = 0;
+    for (int w = 0; w < waves; ++w) part_odd |= a.odd[(range + s) * 4 + w];
+    if (part_odd & kHead) met = kHead;
+  }
+  lds_sync();
+  if (__builtin_expect(met != 0, 0)) {
+    rows_apart<T>(a, piece.x, piece.y, piece.z, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
+    return;
+  }
   const Sequence seq = sequence_of(pg, piece.x);
   const int token0 = piece.z * a.tile_tokens;
   const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int D = pg.head_dim, quads = D / 4, steps = 256 / quads;
-  const int step = tid / quads, quad = tid - step * quads;
-  // Part s of a row: the first is one that ends inside its tile, the others begin inside.
-  auto slot = [&](int s, int row) __attribute__((always_inline)) {
-    return (int64_t)(2 * (range + s) + (s == 0 ? 1 : 0)) * a.row_slots + row;
-  };
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-    lds_sync();  // the last row's weights and sums have been read
-    float top = -__builtin_inff();
-    for (int s = tid; s < parts; s += 256) top = fmaxf(top, a.stats[2 * slot(s, row)]);
-    top = over_wave(top, [](float x, float y) { return fmaxf(x, y); });
-    if (lane == 0) box[wave] = top;
-    lds_sync();
-    top = fmaxf(fmaxf(box[0], box[1]), fmaxf(box[2], box[3]));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float l = 0.0f;
-    for (int s = tid; s < parts; s += 256) {
-      const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * slot(s, row));
-      const float w = __builtin_amdgcn_exp2f(st.x - base);
-      weight[s] = w;
-      l = __builtin_fmaf(w, st.y, l);
-    }
-    l = over_wave(l, [](float x, float y) { return x + y; });
-    if (lane == 0) box[4 + wave] = l;
-    lds_sync();
-    l = (box[4] + box[5]) + (box[6] + box[7]);
+  const int quads = pg.head_dim / 4, groups = 256 / quads;
+  const int group = (int)threadIdx.x / quads, quad = (int)threadIdx.x - group * quads;
+  const int share = (rows + (int)gridDim.y - 1) / (int)gridDim.y;
+  const int first = (int)blockIdx.y * share, last = min(first + share, rows);
+  const int steps = min(max(groups / max(share, 1), 1), parts);  // groups of a row
+  const int at_once = groups / steps;
+  const int step = group % steps;
+  for (int row0 = first; row0 < last; row0 += at_once) {
+    const int row = row0 + group / steps;
+    const bool in = row < last && group / steps < at_once;
+    float top = -__builtin_inff(), l = 0.0f;
     f4 o = f4{};
-    if (step < steps) {
+    if (in) {
+      // Part s: the first is one that ends inside its tile, the others begin inside.
+      int64_t at = (int64_t)(2 * (range + step) + (step == 0 ? 1 : 0)) * a.row_slots + row;
 #pragma unroll 4
       for (int s = step; s < parts; s += steps) {
-        const float ws = weight[s];
-        const f4 x = *reinterpret_cast<const f4*>(a.sums + slot(s, row) * D + 4 * quad);
+        const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * at);
+        const f4 x = *reinterpret_cast<const f4*>(a.sums + at * pg.head_dim + 4 * quad);
+        at += ((int64_t)2 * steps - (s == 0 ? 1 : 0)) * a.row_slots;
+        const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
+        top = next;
+        l = l * f + st.y * w;
+        // (A part that weighs nothing beside another is left out, whatever it holds.)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = ws != 0.0f ? __builtin_fmaf(ws, x[e], o[e]) : o[e];
+        for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
       }
-      sums[tid] = o;
+      stats[threadIdx.x] = float2{top, l};
+      sums[threadIdx.x] = o;
     }
-    lds_sync();
-    const int of = (int)fdiv((uint32_t)row, a.by_group);
-    const int64_t token = seq.first + token0 + of;
-    const int head = piece.y * a.group + row - of * a.group;
-    if (tid < quads) {
-      const int n = min(steps, parts);
-      for (int s = 1; s < n; ++s) o += sums[s * quads + tid];
+    if (steps > 1) lds_sync();
+    if (in && step == 0) {
+      for (int s = 1; s < steps; ++s) {
+        const float2 st = stats[threadIdx.x + s * quads];
+        const f4 x = sums[threadIdx.x + s * quads];
+        const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
+        top = next;
+        l = l * f + st.y * w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
+      }
+      const int of = (int)fdiv((uint32_t)row, a.by_group);
+      const int64_t token = seq.first + token0 + of;
+      const int head = piece.y * a.group + row - of * a.group;
       const float scale = l == 0.0f ? 0.0f : 1.0f / l;
       T* const op = static_cast<T*>(a.c.out) + token * a.c.out_stride[0] + head * a.c.out_stride[1];
       typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = in_range<T>(o[e] * scale);
-      *reinterpret_cast<t4*>(op + 4 * tid) = __builtin_convertvector(o, t4);
+      *reinterpret_cast<t4*>(op + 4 * quad) = __builtin_convertvector(o, t4);
+      if (a.c.lse && quad == 0) a.c.lse[token * a.c.q_heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
     }
-    if (a.c.lse && tid == 0) a.c.lse[token * a.c.q_heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+    if (steps > 1) lds_sync();  // the sums have been read
   }
 }
 
@@ -802,7 +884,7 @@ PagedPlan paged_plan(const arthip_paged_attention_args& c) {
   const size_t parts = (size_t)2 * p.ranges * p.row_slots;
   p.sums = parts * c.p.head_dim * sizeof(float);
   p.stats = parts * 2 * sizeof(float);
-  p.pieces = (size_t)(p.ranges + 1) * sizeof(int4);
+  p.pieces = (size_t)(2 * p.ranges + 1) * sizeof(int4);  // and what the waves met
   p.before = p.counted ? ((size_t)c.p.batch + 1) * sizeof(int64_t) : 0;
   return p;
 }
@@ -816,6 +898,7 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   a.tile_tokens = plan.tile_tokens;
   a.ranges = plan.ranges;
   a.row_slots = plan.row_slots;
+  a.wave_rows = plan.one_wave;
   a.lanes = 64;
   while (a.lanes * c.p.batch > 64 && a.lanes > 1) a.lanes /= 2;
   a.by_group = make_fastdiv((uint32_t)a.group);
@@ -826,14 +909,15 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   a.sums = reinterpret_cast<float*>(at);
   a.stats = reinterpret_cast<float*>(at += plan.sums);
   a.pieces = reinterpret_cast<int4*>(at += plan.stats);
+  a.odd = reinterpret_cast<int*>(a.pieces + a.ranges + 1);
   int64_t* const before = reinterpret_cast<int64_t*>(at += plan.pieces);
   const bool f16 = c.p.dtype == ARTHIP_TYPE_F16;
   const Shape shape = c.cap > kCapSmall || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
   const TilePick k =
       f16 ? pick<_Float16>(c.p.head_dim, plan.one_wave, shape) : pick<__bf16>(c.p.head_dim, plan.one_wave, shape);
+  const bool small = plan.one_wave || c.p.head_dim > 128;  // tiles of 32 keys
   if (plan.counted) {
     a.before = before;
-    const bool small = plan.one_wave || c.p.head_dim > 128;  // tiles of 32 keys
     hipLaunchKernelGGL(small ? paged_count<5> : paged_count<6>, dim3(1), dim3(1024), 0, s, a, before);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -841,8 +925,9 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   hipLaunchKernelGGL(k.fn, dim3((unsigned)a.ranges), dim3((unsigned)k.threads), k.bytes, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(f16 ? paged_join<_Float16> : paged_join<__bf16>,
-                     dim3((unsigned)a.ranges, plan.one_wave ? 4 : 16), dim3(256), 0, s, a);
+  const auto join = f16 ? (small ? paged_join<_Float16, 5> : paged_join<_Float16, 6>)
+                        : (small ? paged_join<__bf16, 5> : paged_join<__bf16, 6>);
+  hipLaunchKernelGGL(join, dim3((unsigned)a.ranges, plan.one_wave ? 4 : 16), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
