@@ -202,6 +202,32 @@ __device__ __forceinline__ void load_lds16(rsrc_t from, const uint32_t (&at)[N],
           "s"(base[2]), "s"(base[3])
         : "memory");
 }
+// The same with everything but the buffer's address in the lanes' offsets.
+template <int N>
+__device__ __forceinline__ void load_lds16(rsrc_t from, const uint32_t (&at)[N], uint32_t to) {
+  static_assert(N == 1 || N == 2 || N == 4, "KiB that the constant reaches");
+  if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds"
+                 :
+                 : "s"(to), "s"(from), "v"(at[0])
+                 : "memory");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %3, %1, 0 offen offset:1024 lds"
+        :
+        : "s"(to), "s"(from), "v"(at[0]), "v"(at[1])
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %3, %1, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %4, %1, 0 offen offset:2048 lds\n\t"
+        "buffer_load_dwordx4 %5, %1, 0 offen offset:3072 lds"
+        :
+        : "s"(to), "s"(from), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+        : "memory");
+}
 __device__ __forceinline__ void load_lds4(rsrc_t from, uint32_t at, uint32_t base, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :

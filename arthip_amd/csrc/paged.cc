@@ -46,7 +46,10 @@ std::string check_pool(const std::string& at, const arthip_pages& p, const void*
   if (pool == nullptr && p.pool_pages > 0 && p.max_pages > 0) return at + "null " + name;
   if (!aligned(pool, 16)) return at + name + " must be aligned to 16 bytes";
   if (!multiples(stride, 3)) return at + name + ": strides must be multiples of 8 elements";
-  if (stride[1] < 0 || stride[1] > kMaxSlotStride) return at + name + ": a slot's stride must be from 0 to 2^24";
+  // Kernels address a page, and a slot in it, by 32 bits each.
+  if (stride[0] < 0 || stride[0] > kMaxTokens) return at + name + ": a page's stride must be from 0 to 2^30";
+  if (stride[1] < 0 || stride[1] > kMaxSlotStride || stride[1] * p.page_size > kMaxTokens)
+    return at + name + ": a slot's stride must be from 0 to 2^24, and a page's slots within 2^30";
   return "";
 }
 

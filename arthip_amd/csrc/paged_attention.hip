@@ -55,7 +55,11 @@ struct PagedArgs {
 // inside its tile, the one that ends inside, whole row tiles.
 constexpr int kHead = 1, kTail = 2, kWhole = 4;
 
-constexpr int kLeast = 4;  // key tiles of a range, where there are that many
+#ifndef KSTART
+#define KSTART 2
+#endif
+constexpr int kStart = KSTART;
+constexpr int kLeast = 4 + kStart;  // units of a range, where there are that many
 
 // Key tiles of a row tile: from `first` on, `count` of them. KT: log2 of the keys of one.
 struct Span {
@@ -69,10 +73,10 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, const Sequence& s, i
   const int first = lo >> KT;
   return {first, hi > lo ? ((hi + (1 << KT) - 1) >> KT) - first : 0};
 }
-// Row tiles count as one key tile at least: their rows are written.
+// The units of a row tile: its key tiles, and before them kStart for what it takes to begin and end one.
 template <int KT>
 __device__ __forceinline__ int units_of(const PagedArgs& a, const Sequence& s, int tile) {
-  return max(span_of<KT>(a, s, tile).count, 1);
+  return span_of<KT>(a, s, tile).count + kStart;
 }
 __device__ __forceinline__ int tiles_of(const PagedArgs& a, const Sequence& s) {
   return (s.tokens + a.tile_tokens - 1) / a.tile_tokens;
@@ -288,17 +292,20 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const int s_row = (wave * LOADS * 1024 + lane * 16) / RB;  // tile's key of the wave's first load
     const int s_chunk = lane * 16 % RB / 16;
     const int l_row = lane * 16 / RB;  // the same of the load's keys
-    const int ks2 = (int)a.c.k_cache_stride[1] * 2, vs2 = (int)a.c.v_cache_stride[1] * 2;  // bytes
-    constexpr int KP = (RB == 512 ? 8 : 16) / STEP < LOADS ? (RB == 512 ? 8 : 16) / STEP : LOADS;
-    constexpr int VP = 4 / STEP < 1 ? 1 : 4 / STEP < LOADS ? 4 / STEP : LOADS;
-    uint32_t k_off[KP], v_off[VP];  // a lane's offsets, but for the keys between its loads
-    auto offset_of = [&](int chunk, int stride) __attribute__((always_inline)) {
-      return chunk * 8 < pg.head_dim ? (uint32_t)(l_row * stride + chunk * 16) : kOob;
-    };
+    // A lane's offsets of a page's loads. (Less what an instruction's constant adds to both addresses:
+    // buffers begin BACK before the rows.)
+    constexpr int BACK = 3 * 1024;
+    uint32_t k_off[GL], v_off[GL];
 #pragma unroll
-    for (int i = 0; i < KP; ++i) k_off[i] = offset_of(s_chunk ^ L::k_swizzle(s_row + i * STEP), ks2);
-#pragma unroll
-    for (int i = 0; i < VP; ++i) v_off[i] = offset_of(s_chunk ^ L::v_swizzle(s_row + i * STEP), vs2);
+    for (int i = 0; i < GL; ++i) {
+      auto offset = [&](int chunk, int64_t stride) __attribute__((always_inline)) {
+        return chunk * 8 < pg.head_dim
+                   ? (uint32_t)((l_row + i * STEP) * (int)stride * 2 + chunk * 16 + BACK - i % 4 * 1024)
+                   : kOob;
+      };
+      k_off[i] = offset(s_chunk ^ L::k_swizzle(s_row + i * STEP), a.c.k_cache_stride[1]);
+      v_off[i] = offset(s_chunk ^ L::v_swizzle(s_row + i * STEP), a.c.v_cache_stride[1]);
+    }
     typedef __attribute__((address_space(3))) unsigned char lds_byte;
     typedef __attribute__((address_space(3))) const frag lds_frag;
     typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -316,9 +323,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const int token0 = place.tile * a.tile_tokens;
     const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;  // of the row tile
     const Span span = span_of<LOG>(a, seq, place.tile);
-    const int units = max(span.count, 1);
+    const int units = span.count + kStart;
     const int take = (int)min((int64_t)(units - place.unit), range_end - at);
-    const int begin = span.first + min(place.unit, span.count), end = span.first + min(place.unit + take, span.count);
+    const int begin = span.first + max(place.unit - kStart, 0), end = span.first + max(place.unit + take - kStart, 0);
     const int32_t* const pages = pg.pages + place.b * pg.pages_stride;
     const int kv_len = seq.len, start = seq.start();
     // Keys [lo, hi) that a token sees.
@@ -332,11 +339,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const int token = token0 + (real ? my_token : 0);
     const int head = place.head * a.group + (real ? g_head : 0);
     const int lo = low(token), hi = high(token);
-    // The wave's rows together: all see [w_lo_max, w_hi_min), some see [w_lo_min, w_hi_max).
+    // The wave's rows all see [w_lo_max, w_hi_min).
     const int t_first = token0 + (int)fdiv((uint32_t)min(wave * 32, rows - 1), a.by_group);
     const int t_last = token0 + (int)fdiv((uint32_t)min(wave * 32 + 31, rows - 1), a.by_group);
-    const int w_lo_min = low(t_first), w_lo_max = low(t_last);
-    const int w_hi_min = high(t_first), w_hi_max = high(t_last);
+    const int w_lo_max = low(t_last), w_hi_min = high(t_first);
 
     frag q[KS];
     {
@@ -353,76 +359,84 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     float m = -__builtin_inff(), l = 0.0f;
 
     // -- staging -------------------------------------------------------------------------
-    // The page of each 16 keys that the wave loads of a tile. (Slots past the length are not read,
-    // whatever their page.)
-    struct Pages {
-      int of[NG];
+    // Where each 16 keys that the wave loads of a tile lie: their page, then their bytes in the pools
+    // from the head on, less BACK, and the buffers' size (0 outside the pool: zeros). (Slots past the
+    // length are not read, whatever their page.)
+    struct Spot {
+      int page[NG];
+      uint64_t k[NG], v[NG];
+      uint32_t size[NG];
     };
-    auto ask = [&](int tile) __attribute__((always_inline)) {
-      Pages r;
+    const uint64_t k_head = reinterpret_cast<uint64_t>(a.c.k_cache) + place.head * a.c.k_cache_stride[2] * 2 - BACK;
+    const uint64_t v_head = reinterpret_cast<uint64_t>(a.c.v_cache) + place.head * a.c.v_cache_stride[2] * 2 - BACK;
+    auto ask = [&](Spot& x, int tile) __attribute__((always_inline)) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int slot = tile * KT + wave * WK + g * 16;
-        r.of[g] = pages[min((int)fdiv((uint32_t)slot, a.by_page), pg.max_pages - 1)];
+        x.page[g] = pages[min((int)fdiv((uint32_t)slot, a.by_page), pg.max_pages - 1)];
       }
-      return r;
     };
-    constexpr int BACK = 3 * 1024;  // what buffers begin before the rows, for the constants' sake
-    auto stage = [&](const void* pool, const int64_t* stride, int slot_bytes, auto offset, int tile, const Pages& in,
+    auto settle = [&](Spot& x, int tile) __attribute__((always_inline)) {  // after the wait for the loads
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        asm volatile("" : "+v"(x.page[g]));
+        const uint32_t page = (uint32_t)scalar(x.page[g]);
+        const int slot = tile * KT + wave * WK + g * 16;
+        const uint32_t in = (uint32_t)(slot - (int)fdiv((uint32_t)slot, a.by_page) * pg.page_size);
+        x.k[g] = k_head + (uint64_t)page * (uint32_t)(a.c.k_cache_stride[0] * 2) + in * (uint32_t)(a.c.k_cache_stride[1] * 2);
+        x.v[g] = v_head + (uint64_t)page * (uint32_t)(a.c.v_cache_stride[0] * 2) + in * (uint32_t)(a.c.v_cache_stride[1] * 2);
+        x.size[g] = page < (uint32_t)pg.pool_pages ? 0x7fffffffu : 0u;
+      }
+    };
+    auto stage = [&](const uint64_t (&from)[NG], const uint32_t (&size)[NG], const uint32_t (&offset)[GL], int tile,
                      uint32_t to) __attribute__((always_inline)) {
       const int left = kv_len - tile * KT;  // keys past the length come as zeros
       const uint32_t to_wave = to + wave * LOADS * 1024;
       constexpr int N = GL < 4 ? GL : 4;
       static_assert(GL % N == 0, "whole blocks of loads");
+      auto loads = [&](auto all) __attribute__((always_inline)) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int slot = tile * KT + wave * WK + g * 16;
-        const int page = in.of[g], of = (int)fdiv((uint32_t)slot, a.by_page);
-        const char* const p = static_cast<const char*>(pool) +
-                              (page * stride[0] + (slot - of * pg.page_size) * stride[1] + place.head * stride[2]) * 2;
-        // A page outside the pool comes as zeros as well.
-        const rsrc_t r = buffer_of(p - BACK, (uint32_t)page < (uint32_t)pg.pool_pages ? 0x7fffffffu : 0u);
+        for (int g = 0; g < NG; ++g) {
+          const rsrc_t r = {(uint32_t)from[g], (uint32_t)(from[g] >> 32) & 0xffffu, size[g], 0x00020000u};
 #pragma unroll
-        for (int i = 0; i < GL; i += N) {
-          uint32_t at_lane[N], base[N];
+          for (int i = 0; i < GL; i += N) {
+            uint32_t at_lane[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const int load = g * GL + i + j;
-            base[j] = (i + j) * STEP * (uint32_t)slot_bytes + (BACK - j * 1024);
-            at_lane[j] = left >= KT || s_row + load * STEP < left ? offset(load) : kOob;
+            for (int j = 0; j < N; ++j)
+              at_lane[j] = decltype(all)::value || s_row + (g * GL + i + j) * STEP < left ? offset[i + j] : kOob;
+            load_lds16<N>(r, at_lane, to_wave + (g * GL + i) * 1024);
           }
-          load_lds16<N>(r, at_lane, base, to_wave + (g * GL + i) * 1024);
         }
-      }
+      };
+      if (left >= KT)
+        loads(std::true_type{});
+      else
+        loads(std::false_type{});
     };
-    auto stage_k = [&](int buf, int tile, const Pages& in) __attribute__((always_inline)) {
-      stage(a.c.k_cache, a.c.k_cache_stride, ks2, [&](int i) { return k_off[i % KP]; }, tile, in,
-            lds_base + buf * L::kTile);
+    auto stage_k = [&](int buf, int tile, const Spot& in) __attribute__((always_inline)) {
+      stage(in.k, in.size, k_off, tile, lds_base + buf * L::kTile);
     };
-    auto stage_v = [&](int buf, int tile, const Pages& in) __attribute__((always_inline)) {
-      stage(a.c.v_cache, a.c.v_cache_stride, vs2, [&](int i) { return v_off[i % VP]; }, tile, in,
-            lds_base + v_at + buf * L::kTile);
+    auto stage_v = [&](int buf, int tile, const Spot& in) __attribute__((always_inline)) {
+      stage(in.v, in.size, v_off, tile, lds_base + v_at + buf * L::kTile);
     };
 
     // -- the products --------------------------------------------------------------------
-    f16v s[KB];        // scores of the current tile, key block by key block
-    frag p[KT / 16];   // weights of the previous tile
-    auto scores = [&](int buf) __attribute__((always_inline)) {
+    f16v s[KB];  // scores of a tile, key block by key block
+    auto scores = [&](int buf, f16v (&x)[KB]) __attribute__((always_inline)) {
       lds_byte* const from = lds0 + buf * L::kTile;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         lds_byte* const k = from + (k_lane ^ (ks * 32));
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) s[kb] = E::mma(*(lds_frag*)(k + kb * 32 * RB), q[ks], ks == 0 ? f16v{} : s[kb]);
+        for (int kb = 0; kb < KB; ++kb) x[kb] = E::mma(*(lds_frag*)(k + kb * 32 * RB), q[ks], ks == 0 ? f16v{} : x[kb]);
       }
-      ahead<KS * KB, 1>();
     };
     auto v_frag = [&](lds_byte* from, int kk) __attribute__((always_inline)) -> frag {  // 32 values of 16 keys
       const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + kk * 16 * RB));
       const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(from + kk * 16 * RB + 8 * RB));
       return __builtin_bit_cast(frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto values = [&](int buf) __attribute__((always_inline)) {
+    auto values = [&](int buf, const frag (&p)[KT / 16]) __attribute__((always_inline)) {
       lds_byte* const from = lds0 + v_at + buf * L::kTile;
       lds_byte* v[DB];
 #pragma unroll
@@ -431,10 +445,12 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] = E::mma(v_frag(v[db], kk), p[kk], o[db]);
-      ahead<KT / 16 * DB, 2>();
     };
+
     // -- scores to weights -----------------------------------------------------------------
-    auto weights = [&](int k0, bool partial) __attribute__((always_inline)) {
+    // The scores in the base of 2 or, plain ones, still to be scaled by `mul`; hidden ones -inf. Then
+    // the row's base, from the largest of them.
+    auto ready = [&](int k0, bool partial) __attribute__((always_inline)) {
       const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
       if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
         float far = 0.0f;
@@ -499,73 +515,81 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= f;
       }
-      // fp16's weights are raised to the top of its range, so that small ones, of which a long
-      // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
-      const float base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
-      float sum = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], mul, -base));
-          sum += w;
-          s[kb][r] = w;
-        }
-      l += sum;  // this half's keys; the halves are added at the end
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk) {
-        const f16v x = s[kk / 2];
-        p[kk] = kk & 1
-                    ? __builtin_convertvector(__builtin_shufflevector(x, x, 8, 9, 10, 11, 12, 13, 14, 15), frag)
-                    : __builtin_convertvector(__builtin_shufflevector(x, x, 0, 1, 2, 3, 4, 5, 6, 7), frag);
-      }
     };
 
     // -- the walk ------------------------------------------------------------------------
-    // One barrier a tile. While tile t's scores and the previous tile's values are multiplied, K of
-    // the next tile and V of this one are on their way to the buffers that the last barrier freed,
-    // and the pages of the tile after the next are asked for.
-    auto settle = [&](Pages& x) __attribute__((always_inline)) {  // after the wait for the loads
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        asm volatile("" : "+v"(x.of[g]));
-        x.of[g] = scalar(x.of[g]);
-      }
-    };
+    // One barrier a tile. While the weights of tile t are found, the scores of tile t + 1 are
+    // multiplied, in one run of instructions: a product takes the matrix unit 32 clocks, in which the
+    // wave's exponentials go on. Then t's values are multiplied. K of tile t + 2 and V of tile t + 1
+    // are on their way meanwhile to the buffers that the last barrier freed, and the page of the tile
+    // after them is asked for.
     lds_sync();  // the last row tile has been used
     if (begin < end) {
-      Pages here = ask(begin), next = here;
-      settle(here);
+      Spot here, next, then;
+      ask(here, begin);
+      ask(next, min(begin + 1, end - 1));
+      ask(then, min(begin + 2, end - 1));
+      settle(here, begin);
       stage_k(0, begin, here);
-      if (begin + 1 < end) next = ask(begin + 1);
+      settle(next, begin + 1);
+      if (begin + 1 < end) stage_k(1, begin + 1, next);
+      stage_v(0, begin, here);
       vm_wait();
-      settle(next);
+      settle(then, begin + 2);
       lds_sync();
-      int buf = 0;
-      bool has = false;  // weights of the previous tile
-      for (int t = begin;; ++t) {
-        const bool on = t < end;
-        const int k0 = t * KT, k1 = k0 + KT;
-        bool seen = false, partial = false;
-        Pages then = next;
-        if (on) {
-          if (t + 1 < end) stage_k(buf ^ 1, t + 1, next);
-          stage_v(buf, t, here);
-          if (t + 2 < end) then = ask(t + 2);
-          seen = w_real && k0 < w_hi_max && k1 > w_lo_min;
-          partial = !(k0 >= w_lo_max && k1 <= w_hi_min);
-        }
-        if (seen) scores(buf);
-        if (has) values(buf ^ 1);
-        if (!on) break;
-        if (seen) weights(k0, partial);
-        has = seen;
-        vm_wait();
-        settle(then);
-        lds_sync();
-        here = next;
+      if (w_real) scores(0, s);
+      lds_sync();  // K's first buffer has been used
+      for (int t = begin; t < end; ++t) {
+        const int buf = (t - begin) & 1, k0 = t * KT;
+        if (t + 2 < end) stage_k(buf, t + 2, then);
+        if (t + 1 < end) stage_v(buf ^ 1, t + 1, next);
         next = then;
-        buf ^= 1;
+        ask(then, min(t + 3, end - 1));
+        if (w_real) {
+          ready(k0, !(k0 >= w_lo_max && k0 + KT <= w_hi_min));
+          // fp16's weights are raised to the top of its range, so that small ones, of which a long
+          // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
+          const float base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+          f16v following[KB];
+          frag p[KT / 16];
+          float sum = 0.0f;
+          {
+            // A product, the operand of the fourth after it, and its share of the exponentials.
+            constexpr int N = KS * KB, A = N < 4 ? N : 4;
+            lds_byte* const from = lds0 + (buf ^ 1) * L::kTile;
+            frag k[N];
+            auto read = [&](int i) __attribute__((always_inline)) {
+              k[i] = *(lds_frag*)(from + (k_lane ^ (i / KB * 32)) + i % KB * 32 * RB);
+            };
+#pragma unroll
+            for (int i = 0; i < A; ++i) read(i);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              following[i % KB] = E::mma(k[i], q[i / KB], i < KB ? f16v{} : following[i % KB]);
+              if (i + A < N) read(i + A);
+#pragma unroll
+              for (int e = i * 16 * KB / N; e < (i + 1) * 16 * KB / N; ++e) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], mul, -base));
+                sum += w;
+                s[e / 16][e % 16] = w;
+                if (e % 16 == 7)
+                  p[e / 8] = __builtin_convertvector(__builtin_shufflevector(s[e / 16], s[e / 16], 0, 1, 2, 3, 4, 5, 6, 7), frag);
+                if (e % 16 == 15)
+                  p[e / 8] = __builtin_convertvector(
+                      __builtin_shufflevector(s[e / 16], s[e / 16], 8, 9, 10, 11, 12, 13, 14, 15), frag);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          l += sum;  // this half's keys; the halves are added at the end
+          values(buf, p);
+          ahead<KT / 16 * DB, 2>();
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) s[kb] = following[kb];
+        }
+        vm_wait();
+        settle(then, t + 3);
+        lds_sync();
       }
     }
 
@@ -580,8 +604,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     if (__builtin_expect(__any(rest != 0.0f), 0)) {
       bool found = false;
       for (int t = begin; t < end; ++t) {
-        if (!w_real || t * KT >= w_hi_max || t * KT + KT <= w_lo_min) continue;
-        if (t * KT >= w_lo_max && t * KT + KT <= w_hi_min) continue;
+        if (!w_real || (t * KT >= w_lo_max && t * KT + KT <= w_hi_min)) continue;
         for (int i = lane; i < KT * (DP / 8); i += 64) {
           const int slot = t * KT + i / (DP / 8), d = i % (DP / 8) * 8;
           if (slot >= kv_len || d >= pg.head_dim) continue;

@@ -610,7 +610,7 @@ typedef struct arthip_cache_write_args {
   const int32_t* token_positions;  /* [tokens], with positions */
   int64_t k_stride[2];             /* token, head: multiples of 8, as all data is 16-byte aligned */
   int64_t v_stride[2];
-  int64_t k_cache_stride[3];       /* page, slot, head: multiples of 8; a slot's from 0 to 2^24 */
+  int64_t k_cache_stride[3];       /* page (0 to 2^30), slot (0 to 2^24, page_size times it 2^30), head: multiples of 8 */
   int64_t v_cache_stride[3];
   int64_t positions_stride[2];     /* sequence, head; slots are contiguous */
   int32_t slots;

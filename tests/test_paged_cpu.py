@@ -82,7 +82,9 @@ def test_page_refusals(name, make, change, text):
 @pytest.mark.parametrize("change,text", [
     (dict(k_cache=None), "null k_cache"), (dict(k_cache=BUF + 8), "aligned"),
     (dict(k_cache_stride=(2048, 132, 64)), "multiples of 8"), (dict(k_cache_stride=(2048, 2 ** 24 + 8, 64)), "slot's stride"),
-    (dict(k_cache_stride=(2048, -128, 64)), "slot's stride"),
+    (dict(k_cache_stride=(2048, -128, 64)), "slot's stride"), (dict(k_cache_stride=(-2048, 128, 64)), "page's stride"),
+    (dict(k_cache_stride=(2 ** 30 + 8, 128, 64)), "page's stride"),
+    (dict(page_size=128, k_cache_stride=(2048, 2 ** 24, 64)), "slots within"),
 ])
 @pytest.mark.parametrize("name,make", CALLS)
 def test_pool_refusals(name, make, change, text):
