@@ -120,6 +120,20 @@ __device__ __forceinline__ X over_wave(X x, F f) {
 __device__ __forceinline__ int wave_min(int x) { return over_wave(x, [](int a, int b) { return min(a, b); }); }
 __device__ __forceinline__ int wave_max(int x) { return over_wave(x, [](int a, int b) { return max(a, b); }); }
 
+// Sum of x over the lanes up to this one, inside the vector unit: rows of 16, then across them.
+__device__ __forceinline__ uint32_t up_to(uint32_t x) {
+  auto add = [&](auto control, auto rows) __attribute__((always_inline)) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xf, false);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return x;
+}
+
 __device__ __forceinline__ float halves_max(float x) {
   float a, b;
   halves(x, a, b);

@@ -93,20 +93,6 @@ __device__ __forceinline__ uint32_t ordered(float w) {
   return w != w ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of x over the lanes up to this one, inside the vector unit: rows of 16, then across them.
-__device__ __forceinline__ uint32_t up_to(uint32_t x) {
-  auto add = [&](auto control, auto rows) __attribute__((always_inline)) {
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xf, false);
-  };
-  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
-  return x;
-}
-
 // 16 bytes of a slot's key and of its value to another slot.
 __device__ __forceinline__ void move_chunk(const EvictArgs& a, const int32_t* pages, int head, int part, int from,
                                            int to) {
@@ -123,15 +109,15 @@ __device__ __forceinline__ void move_chunk(const EvictArgs& a, const int32_t* pa
   *reinterpret_cast<u4*>(v + v_to) = y;
 }
 
-// The slots of one key head of one sequence, by one workgroup. The `keep`-th largest key is found
-// 11 bits at a time from a histogram of the keys that share the bits before; then each wave ranks
-// the holes and the movers of a run of slots. Keys are read anew in every pass, 64 in a row a wave:
-// they come from the L2 (32768 slots: some 1 us a pass).
-template <bool HERE>
+// The slots of one key head of one sequence, by one workgroup. A wave holds the keys of a run of
+// slots in registers, 64 slots in a row an instruction, E times (E = 0: more than fit, read anew in
+// every pass). The `keep`-th largest key is found 11 bits at a time from a histogram of the keys that
+// share the bits before; then each wave ranks the holes and the movers of its run.
+template <int E, bool HERE>
 __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
-  __shared__ int bins[kBins];
-  __shared__ int box[3][kWaves];
-  __shared__ int found[3];
+  __shared__ int bins[3][kBins];
+  __shared__ int box[5][kWaves];
+  __shared__ int found[3][3];
   __shared__ int list[HERE ? kMovesHere : kMoves];
   __shared__ int holes_at[HERE ? kMovesHere : 1];
   constexpr int kList = HERE ? kMovesHere : kMoves;
@@ -149,39 +135,84 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   int32_t* const kept = a.c.kept + at * keep;
   const int used = min(n, keep);
   if (head == 0 && tid == 0 && a.c.new_len != nullptr) a.c.new_len[b] = used;
-  for (int s = used + tid; s < a.c.slots; s += kThreads) {
-    if (w_out != nullptr) w_out[s] = 0.0f;
-    if (place_out != nullptr) place_out[s] = -1;
-  }
   auto stays = [&](int s, int from) __attribute__((always_inline)) {
     kept[s] = from;
     if (w_out != nullptr) w_out[s] = w[from];
     if (place_out != nullptr) place_out[s] = place[from];
   };
-  if (n <= keep) {
-    for (int s = tid; s < keep; s += kThreads) {
-      if (s < n)
-        stays(s, s);
-      else
-        kept[s] = -1;
+  auto rest = [&]() __attribute__((always_inline)) {  // what lies behind
+    for (int s = used + tid; s < a.c.slots; s += kThreads) {
+      if (w_out != nullptr) w_out[s] = 0.0f;
+      if (place_out != nullptr) place_out[s] = -1;
     }
+    for (int s = used + tid; s < keep; s += kThreads) kept[s] = -1;
+  };
+  if (n <= keep) {
+    for (int s = tid; s < n; s += kThreads) stays(s, s);
+    rest();
     return;
   }
 
+  // -- the keys --------------------------------------------------------------------------
+  const int each = (n + kThreads - 1) / kThreads;
+  const int begin = min(wave * each * 64, n), end = min(begin + each * 64, n);  // the wave's slots
+  uint32_t keys[E > 0 ? E : 1];
+  int places[E > 0 ? E : 1];
   int newest = n - 1;
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < each) {
+        const int s = min(begin + i * 64 + lane, n - 1);
+        keys[i] = __builtin_bit_cast(uint32_t, w[s]);
+        if (place != nullptr) places[i] = place[s];
+      }
+  }
+  for (int i = tid; i < 3 * kBins; i += kThreads) bins[0][i] = 0;
   if (place != nullptr) {
     int top = INT32_MIN;
-    for (int s = tid; s < n; s += kThreads) top = max(top, place[s]);
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i < each) top = max(top, places[i]);  // (past the run: the last slot's)
+    } else {
+      for (int s = tid; s < n; s += kThreads) top = max(top, place[s]);
+    }
     top = over_wave(top, [](int x, int y) { return max(x, y); });
-    if (lane == 0) box[0][wave] = top;
-    lds_sync();
-    newest = box[0][0];
-    for (int i = 1; i < kWaves; ++i) newest = max(newest, box[0][i]);
+    if (lane == 0) box[3][wave] = top;
   }
-  auto key_of = [&](int s) __attribute__((always_inline)) -> uint32_t {
-    const int64_t t = place != nullptr ? place[s] : s;
-    const uint32_t u = ordered(w[s]);
-    return t > (int64_t)newest - a.c.recent || t < a.c.first ? UINT32_MAX : u;
+  lds_sync();
+  if (place != nullptr) {
+    newest = box[3][0];
+    for (int i = 1; i < kWaves; ++i) newest = max(newest, box[3][i]);
+  }
+  auto key = [&](float weight, int64_t t) __attribute__((always_inline)) -> uint32_t {
+    return t > (int64_t)newest - a.c.recent || t < a.c.first ? UINT32_MAX : ordered(weight);
+  };
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < each)
+        keys[i] = key(__builtin_bit_cast(float, keys[i]), place != nullptr ? places[i] : begin + i * 64 + lane);
+  }
+  auto each_slot = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, its key)
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i < each) f(begin + i * 64 + lane, begin + i * 64 + lane < end, keys[i]);
+    } else {
+      constexpr int kOnce = 8;  // loads in flight
+      for (int s0 = begin; s0 < end; s0 += 64 * kOnce) {
+        uint32_t x[kOnce];
+#pragma unroll
+        for (int i = 0; i < kOnce; ++i) {
+          const int s = min(s0 + i * 64 + lane, n - 1);
+          x[i] = key(w[s], place != nullptr ? place[s] : s);
+        }
+#pragma unroll
+        for (int i = 0; i < kOnce; ++i) f(s0 + i * 64 + lane, s0 + i * 64 + lane < end, x[i]);
+      }
+    }
   };
 
   // -- the keep-th largest key ---------------------------------------------------------
@@ -190,53 +221,43 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   bool ties = false;   // of which not all stay
   for (int level = 0; level < 3; ++level) {
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
-    lds_sync();
-    for (int s = tid; s < n; s += kThreads) {
-      const uint32_t key = key_of(s);
-      bool in = level == 0 || key >> (shift + width) == least >> (shift + width);
-      const int bin = (int)(key >> shift) & ((1 << width) - 1);
-      // Equal keys are common (weights of 0, protected slots) and would meet in one counter: two
-      // of a wave's bins are counted by ballots.
-#pragma unroll
-      for (int round = 0; round < 2; ++round) {
-        const uint64_t left = __ballot(in);
-        if (left == 0) break;
-        const int first = __builtin_amdgcn_readlane(bin, __builtin_ctzll(left));
-        const bool same = in && bin == first;
-        const int count = __popcll(__ballot(same));
-        if (lane == (int)__builtin_ctzll(left)) atomicAdd(&bins[first], count);
-        in = in && !same;
+    int* const mine = bins[level];
+    each_slot([&](int, bool is, uint32_t x) __attribute__((always_inline)) {
+      const bool in = is && (level == 0 || x >> (shift + width) == least >> (shift + width));
+      const int bin = (int)(x >> shift) & ((1 << width) - 1);
+      const uint64_t mask = __ballot(in);
+      if (mask == 0) return;
+      // Equal keys (weights of 0, protected slots) would meet in one counter.
+      const int first = __builtin_amdgcn_readlane(bin, __builtin_ctzll(mask));
+      if (__ballot(in && bin != first) == 0) {
+        if (lane == 0) atomicAdd(&mine[first], __popcll(mask));
+      } else if (in) {
+        atomicAdd(&mine[bin], 1);
       }
-      if (in) atomicAdd(&bins[bin], 1);
-    }
+    });
     lds_sync();
     // Two bins a thread, the largest keys first: the bin in which the want-th key lies.
     const int top = kBins - 1 - 2 * tid;
-    const int c0 = bins[top], c1 = bins[top - 1];
+    const int c0 = mine[top], c1 = mine[top - 1];
     const int sum = (int)up_to((uint32_t)(c0 + c1));
     if (lane == 63) box[level][wave] = sum;
     lds_sync();
     int before = sum - c0 - c1;
     for (int i = 0; i < wave; ++i) before += box[level][i];
-    const bool here = before < want && want <= before + c0 + c1;
-    if (here) {
+    if (before < want && want <= before + c0 + c1) {
       const bool second = want > before + c0;
-      found[0] = top - (second ? 1 : 0);
-      found[1] = want - before - (second ? c0 : 0);
-      found[2] = second ? c1 : c0;
+      found[level][0] = top - (second ? 1 : 0);
+      found[level][1] = want - before - (second ? c0 : 0);
+      found[level][2] = second ? c1 : c0;
     }
     lds_sync();
-    least |= (uint32_t)found[0] << shift;
-    want = found[1];
-    ties = found[2] != want;
-    lds_sync();
+    least |= (uint32_t)found[level][0] << shift;
+    want = found[level][1];
+    ties = found[level][2] != want;
     if (!ties) break;  // all keys from here on stay
   }
 
   // -- holes below the budget and slots past it that stay, by their ranks -----------------
-  const int run = ((n + kWaves - 1) / kWaves + 63) & ~63;  // slots of a wave
-  const int begin = min(wave * run, n), end = min(begin + run, n);
   auto all_waves = [&](int mine, int (&of)[kWaves], int& total) __attribute__((always_inline)) {
     if (lane == 0) of[wave] = mine;
     lds_sync();
@@ -252,40 +273,43 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   int equals_before = 0, total;
   if (ties) {
     int equals = 0;
-    for (int s0 = begin; s0 < end; s0 += 64) {
-      const int s = s0 + lane;
-      equals += __popcll(__ballot(s < end && key_of(min(s, n - 1)) == least));
-    }
-    equals_before = all_waves(equals, box[0], total);
+    each_slot([&](int, bool is, uint32_t x) { equals += __popcll(__ballot(is && x == least)); });
+    equals_before = all_waves(equals, box[4], total);
   }
   const uint64_t below = (uint64_t{1} << lane) - 1;
-  auto each_slot = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, it stays)
+  auto each_stay = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, it stays)
     int seen = equals_before;
-    for (int s0 = begin; s0 < end; s0 += 64) {
-      const int s = s0 + lane;
-      const uint32_t key = key_of(min(s, n - 1));
-      bool stay = s < end && key >= least;
+    each_slot([&](int s, bool is, uint32_t x) __attribute__((always_inline)) {
+      bool stay = is && x >= least;
       if (ties) {
-        const bool equal = s < end && key == least;
+        const bool equal = is && x == least;
         const uint64_t mask = __ballot(equal);
         if (equal) stay = seen + __popcll(mask & below) < want;
         seen += __popcll(mask);
       }
-      f(s, s < end, stay);
-    }
+      f(s, is, stay);
+    });
   };
   int holes = 0, movers = 0;
-  each_slot([&](int s, bool is, bool stay) {
+  each_stay([&](int s, bool is, bool stay) {
     holes += __popcll(__ballot(is && s < keep && !stay));
     movers += __popcll(__ballot(is && s >= keep && stay));
   });
-  const int holes_before = all_waves(holes, box[1], total);
-  const int moves = total;
-  const int movers_before = all_waves(movers, box[2], total);
+  if (lane == 0) {
+    box[0][wave] = holes;
+    box[1][wave] = movers;
+  }
+  lds_sync();
+  int holes_before = 0, movers_before = 0, moves = 0;
+  for (int i = 0; i < kWaves; ++i) {
+    holes_before += i < wave ? box[0][i] : 0;
+    movers_before += i < wave ? box[1][i] : 0;
+    moves += box[0][i];
+  }
   for (int from = 0; from == 0 || from < moves; from += kList) {
     if (movers > 0) {
       int rank = movers_before - from;
-      each_slot([&](int s, bool is, bool stay) {
+      each_stay([&](int s, bool is, bool stay) __attribute__((always_inline)) {
         const bool mover = is && s >= keep && stay;
         const uint64_t mask = __ballot(mover);
         const int mine = rank + __popcll(mask & below);
@@ -295,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
     }
     lds_sync();
     int rank = holes_before - from;
-    each_slot([&](int s, bool is, bool stay) {
+    each_stay([&](int s, bool is, bool stay) __attribute__((always_inline)) {
       const bool hole = is && s < keep && !stay;
       const uint64_t mask = __ballot(hole);
       const int mine = rank + __popcll(mask & below);
@@ -315,6 +339,7 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
       move_chunk(a, pages, head, part, list[m], holes_at[m]);
     }
   }
+  rest();
 }
 
 // The rows that evict_select found to move: a thread 16 bytes of a slot's key and value. Rows come
@@ -331,6 +356,11 @@ __global__ void __launch_bounds__(256) evict_move(EvictArgs a, int64_t first_blo
   const int b = (int)fdiv((uint32_t)at, a.by_heads), head = (int)at - b * p.k_heads;
   const int32_t* const pages = p.pages + b * p.pages_stride;
   move_chunk(a, pages, head, part, from, s);
+}
+
+template <int E>
+void (*select_of(bool here))(EvictArgs) {
+  return here ? evict_select<E, true> : evict_select<E, false>;
 }
 
 }  // namespace
@@ -362,7 +392,9 @@ hipError_t launch_cache_evict(const arthip_cache_evict_args& c, hipStream_t s) {
   const int64_t heads = (int64_t)c.p.batch * c.p.k_heads;
   const int most = std::min(c.keep, std::max(0, c.slots - c.keep));  // moves of a key head
   const bool here = most <= kMovesHere;
-  hipLaunchKernelGGL(here ? evict_select<true> : evict_select<false>, dim3((unsigned)heads), dim3(kThreads), 0, s, a);
+  const int each = (c.slots + kThreads - 1) / kThreads;
+  const auto fn = each <= 4 ? select_of<4>(here) : select_of<0>(here);
+  hipLaunchKernelGGL(fn, dim3((unsigned)heads), dim3(kThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || here) return e;
   const int per = 256 / a.head_chunks;

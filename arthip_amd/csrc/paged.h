@@ -30,7 +30,6 @@ struct PagedPlan {
   bool one_wave;     // 32 rows a workgroup instead of 128
   int tile_tokens;   // new tokens of a row tile, with all heads of a key head
   int ranges;        // workgroups, each a range of the key tiles of all row tiles
-  int row_slots;     // rows that a range keeps of a row tile which it shares with others
   bool counted;      // a kernel of its own counts the tiles before each sequence
   size_t sums, stats, pieces, before;  // bytes of the workspace's parts, in this order
   size_t workspace() const { return sums + stats + pieces + before; }

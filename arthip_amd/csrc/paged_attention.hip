@@ -38,28 +38,27 @@ struct PagedArgs {
   int group;        // query heads of a key head
   int tile_tokens;  // tokens of a row tile
   int ranges;       // workgroups
-  int row_slots;    // rows kept of a part of a row tile
   int lanes;        // that count one sequence's tiles together, if `before` is not there
-  int wave_rows;    // 32 rows a workgroup rather than 128
   FastDiv by_group, by_page, by_lanes;
   CapFit cap;
   const int64_t* before;  // key tiles of the sequences before each [batch + 1], of all key heads
-  float* sums;   // [2 ranges][row_slots][D] unscaled: parts that begin inside a row tile, parts that end inside
-  float* stats;  // [2 ranges][row_slots][2] maximum (base 2) and sum
-  int* odd;      // [ranges][4 waves] kHead, kTail, kWhole
-  int4* pieces;  // [ranges + 1] of a row tile that begins in a range and ends in another: sequence, key
-                 // head, tile, number of parts. The last: ranges that there are.
+  // Parts of row tiles, two a range: the one that begins inside its tile, the one that ends inside.
+  float* sums;    // [2 ranges][waves][padded D / 8][64 lanes][4] unscaled, as the lanes hold them
+  float2* stats;  // [2 ranges][32 waves] of a row: maximum (base 2) and sum
+  int4* pieces;   // [ranges] the row tile that begins in a range and ends in another: sequence, key head,
+                  // tile, number of parts (0: none) and 2^16 times what the waves met
 };
 
 // Parts of row tiles in which a row met an infinity or NaN that it may not see: the one that begins
 // inside its tile, the one that ends inside, whole row tiles.
 constexpr int kHead = 1, kTail = 2, kWhole = 4;
+constexpr int kMaxRanges = 1024, kAgain = 1 << 16;
+// Workgroups that join. (16 single tokens with 512, 1024 and 2048: 113, 118, 124 us; prompts beside
+// tokens 466, 471, 468.)
+constexpr int kJoiners = 512;
 
-#ifndef KSTART
-#define KSTART 2
-#endif
-constexpr int kStart = KSTART;
-constexpr int kLeast = 4 + kStart;  // units of a range, where there are that many
+constexpr int kStart = 2;
+constexpr int kLeast = 4;  // units of a range, where there are that many
 
 // Key tiles of a row tile: from `first` on, `count` of them. KT: log2 of the keys of one.
 struct Span {
@@ -229,6 +228,57 @@ struct Finder {
   }
 };
 
+__device__ __forceinline__ int ranges_of(const PagedArgs& a, int64_t total) {
+  return total >= (int64_t)a.ranges * kLeast ? a.ranges : max((int)total / kLeast, total > 0 ? 1 : 0);
+}
+
+// One workgroup's range of the units: about as many as any other's. A cut that would leave only a
+// little (a 32nd of a range, or four tiles) of a row tile on one side goes to that tile's end: two parts more cost
+// more than they balance (256 tokens over 32765 keys: 147 us, 136 so).
+struct Range {
+  int64_t at, cut, slack;  // where it is, where it is cut off
+  int64_t total;           // units of all ranges,
+  int live;                // and their number
+  Place place;
+
+  // False where there is no range of this number.
+  template <int KT>
+  __device__ __forceinline__ bool begin(const PagedArgs& a, const Finder<KT>& finder, int ranges, int range, int lane) {
+    auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    total = finder.total;
+    live = ranges;
+    at = range * total / live;
+    cut = (range + 1) * total / live;
+    const int64_t share = total / live;
+    slack = min(share >> 3, max(share >> 5, (int64_t)4));
+    const Place p = finder.find(a, at, lane);
+    place = {scalar(p.b), scalar(p.head), scalar(p.tile), scalar(p.unit)};
+    if (place.unit == 0) return true;
+    const Sequence s = sequence_of(a.c.p, place.b);
+    const int left = units_of<KT>(a, s, place.tile) - place.unit;
+    if (place.unit <= slack) {
+      at -= place.unit;
+      place.unit = 0;
+    } else if (left <= slack) {
+      at += left;
+      return next_tile(a, s, place);
+    }
+    return true;
+  }
+  // Units to take of the row tile at hand, which has `units`.
+  __device__ __forceinline__ int take(int units) const {
+    const int64_t start = at - place.unit, end = start + units;
+    if (cut >= end || (cut - start > slack && end - cut <= slack)) return units - place.unit;
+    return cut - start <= slack ? 0 : (int)(cut - at);
+  }
+  // Whether the range ends with them.
+  __device__ __forceinline__ bool last(int units) const { return cut <= at - place.unit + units; }
+  // The range in which a row tile ends that has `units` and begins here.
+  __device__ __forceinline__ int end_of(int units) const {
+    return (int)(((at + units - slack) * live - 1) / total);
+  }
+};
+
 template <class T, int DP, int KT, int NW, Shape SHAPE>
 __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 && SHAPE == kAny) ? 2 : 3)
     paged_tile(PagedArgs a) {
@@ -263,20 +313,35 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   // of one key head share K and V.
   Finder<LOG> finder;
   finder.count(a, tid & 63);
-  const int64_t total = scalar64(finder.total);
-  const int live = total >= (int64_t)a.ranges * kLeast ? a.ranges : max((int)total / kLeast, total > 0 ? 1 : 0);
+  const int live = scalar(ranges_of(a, finder.total));
   const int per = (live + 7) >> 3;
   const int range = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-  if (blockIdx.x == 0 && tid == 0) a.pieces[a.ranges] = int4{live, 0, 0, 0};
+  if ((int)blockIdx.x >= live && tid == 0) a.pieces[blockIdx.x] = int4{};  // no such range
   if (((int)blockIdx.x >> 3) >= per || range >= live) return;
-  const int64_t share = scalar64(total / live);
-  const int more = scalar((int)(total - share * live));  // ranges of one unit more
-  int64_t at = range * share + min(range, more);
-  const int64_t range_end = at + share + (range < more ? 1 : 0);
-  Place place = finder.find(a, at, tid & 63);
-  place = {scalar(place.b), scalar(place.head), scalar(place.tile), scalar(place.unit)};
-
+  Range r;
+  if (!r.begin(a, finder, live, range, tid & 63)) {
+    if (tid == 0) a.pieces[range] = int4{};
+    return;
+  }
+  r.total = scalar64(r.total);
+  r.slack = scalar64(r.slack);
+  r.at = scalar64(r.at);
+  r.cut = scalar64(r.cut);
+  Place place = {scalar(r.place.b), scalar(r.place.head), scalar(r.place.tile), scalar(r.place.unit)};
   int odd = 0;  // what the wave met
+  // The last of a range: the row tile that it shares with later ones, if any.
+  auto finish = [&](int4 piece) __attribute__((always_inline)) {
+    if constexpr (NW > 1) {
+      int* const flag = reinterpret_cast<int*>(lds);
+      lds_sync();
+      if ((tid & 63) == 0) flag[wave] = odd;
+      lds_sync();
+      odd = 0;
+      for (int i = 0; i < NW; ++i) odd |= flag[i];
+    }
+    piece.w |= odd << 16;
+    if (tid == 0) a.pieces[range] = piece;
+  };
 
   while (true) {
     // -- the lane's part -----------------------------------------------------------------
@@ -324,7 +389,13 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;  // of the row tile
     const Span span = span_of<LOG>(a, seq, place.tile);
     const int units = span.count + kStart;
-    const int take = (int)min((int64_t)(units - place.unit), range_end - at);
+    r.place.unit = place.unit;
+    const int take = r.take(units);
+    const bool last = r.last(units);
+    if (take == 0) {
+      finish(int4{});
+      return;
+    }
     const int begin = span.first + max(place.unit - kStart, 0), end = span.first + max(place.unit + take - kStart, 0);
     const int32_t* const pages = pg.pages + place.b * pg.pages_stride;
     const int kv_len = seq.len, start = seq.start();
@@ -623,20 +694,15 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     l = halves_sum(l);
     if (take < units) {
       if (real) {
-        const int64_t row = (int64_t)(2 * range + (place.unit == 0 ? 1 : 0)) * a.row_slots + wave * 32 + n;
-        float* const part = a.sums + row * pg.head_dim;
+        const int64_t part = 2 * range + (place.unit == 0 ? 1 : 0);
+        f4* const sums = reinterpret_cast<f4*>(a.sums) + (part * NW + wave) * (DP / 8) * 64 + lane;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int d = db * 32 + 8 * g + 4 * half;
-            if (d < pg.head_dim)
-              *reinterpret_cast<f4*>(part + d) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-          }
-        if (half == 0) {
-          a.stats[2 * row] = m * mul - E::kRaise;
-          a.stats[2 * row + 1] = l;
-        }
+          for (int g = 0; g < 4; ++g)
+            if (db * 32 + 8 * g < pg.head_dim)
+              sums[(db * 4 + g) * 64] = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+        if (half == 0) a.stats[(part * NW + wave) * 32 + n] = float2{m * mul - E::kRaise, l};
       }
     } else {
       const float scale = l == 0.0f ? 0.0f : 1.0f / l;
@@ -667,21 +733,12 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         a.c.lse[(int64_t)(seq.first + token) * a.c.q_heads + head] =
             (m * mul - E::kRaise + __builtin_amdgcn_logf(l)) * kLn2;
     }
-    const int64_t tile_end = at + units - place.unit;
-    at += take;
-    if (at >= range_end) {
-      if ((tid & 63) == 0) a.odd[range * 4 + wave] = odd;
-      if (tid == 0) {
-        // Whether a row tile begins here and ends in a later range.
-        int parts = 0;
-        if (tile_end > at && place.unit == 0) {
-          const int64_t last = tile_end - 1, longer = more * (share + 1);
-          parts = (int)(last < longer ? last / (share + 1) : more + (last - longer) / share) - range + 1;
-        }
-        a.pieces[range] = int4{place.b, place.head, place.tile, parts};
-      }
+    if (last) {
+      finish({place.b, place.head, place.tile,
+              place.unit == 0 && take < units ? r.end_of(units) - range + 1 : 0});
       return;
     }
+    r.at += take;
     next_tile(a, seq, place);
     place = {scalar(place.b), scalar(place.head), scalar(place.tile), 0};
   }
@@ -690,13 +747,14 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 // One row by itself, from the definition: the rows of a workgroup's share of a row tile one after the
 // other, each key added only to the rows that see it (an infinity whatever its weight).
 template <class T>
-__device__ __forceinline__ void rows_apart(const PagedArgs& a, int b, int kh, int tile, float* weight, float* box) {
+__device__ __forceinline__ void rows_apart(const PagedArgs& a, int b, int kh, int tile, int index, int wide,
+                                           float* weight, float* box) {
   const arthip_pages& pg = a.c.p;
   const Sequence seq = sequence_of(pg, b);
   const int32_t* const pages = pg.pages + b * pg.pages_stride;
   const int token0 = tile * a.tile_tokens, rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+  for (int row = index; row < rows; row += wide) {
     const int of = (int)fdiv((uint32_t)row, a.by_group), token = token0 + of;
     const int head = kh * a.group + row - of * a.group, place = seq.start() + token;
     const int lo = a.c.left < 0 ? 0 : min(max(place - a.c.left, 0), seq.len);
@@ -752,100 +810,105 @@ __device__ __forceinline__ void rows_apart(const PagedArgs& a, int b, int kh, in
   }
 }
 
-// Joins the parts of row tiles that several ranges share, in their order: a workgroup some rows of
-// the tile that begins in range blockIdx.x. Four values a thread, D / 4 threads a row; where the rows
-// do not fill the workgroup, several such groups take a row's parts in turn.
-template <class T, int KT>
-__global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
-  __shared__ f4 sums[256];
-  __shared__ float2 stats[256];
-  __shared__ int met;
+// A workgroup's share of a job of the joining kernel: the parts of the row tile that begins in a range,
+// in their order, four values of a row a thread; where there are fewer of these than threads, several
+// threads take an item's parts in turn.
+template <class T, int DP, int KT, int NW>
+__device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* sums, float2* stats, int* met) {
   const arthip_pages& pg = a.c.p;
-  const int range = blockIdx.x, live = a.pieces[a.ranges].x;
-  if (range >= live) return;
-  const int4 piece = a.pieces[range];
-  const int parts = piece.w, waves = a.wave_rows ? 1 : 4;
-  int odd = 0;
-  for (int w = 0; w < waves; ++w) odd |= a.odd[range * 4 + w];
-  if (__builtin_expect((odd & kWhole) != 0, 0)) {
+  const int range = job & ~kAgain, tid = threadIdx.x;
+  if (__builtin_expect((job & kAgain) != 0, 0)) {
     // All whole row tiles of the range, once more.
-    const int lane = threadIdx.x & 63;
+    const int lane = tid & 63;
     Finder<KT> finder;
     finder.count(a, lane);
-    const int64_t share = finder.total / live;
-    const int more = (int)(finder.total - share * live);
-    int64_t at = range * share + min(range, more);
-    const int64_t range_end = at + share + (range < more ? 1 : 0);
-    Place place = finder.find(a, at, lane);
-    while (true) {
-      const Sequence seq = sequence_of(pg, place.b);
-      const int units = units_of<KT>(a, seq, place.tile);
-      if (place.unit == 0 && at + units <= range_end)
-        rows_apart<T>(a, place.b, place.head, place.tile, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
-      at += units - place.unit;
-      if (at >= range_end) break;
-      if (!next_tile(a, seq, place)) break;
+    Range r;
+    bool on = r.begin(a, finder, ranges_of(a, finder.total), range, lane);
+    while (on) {
+      const Sequence seq = sequence_of(pg, r.place.b);
+      const int units = units_of<KT>(a, seq, r.place.tile);
+      if (r.take(units) == units)
+        rows_apart<T>(a, r.place.b, r.place.head, r.place.tile, index, wide, reinterpret_cast<float*>(sums),
+                      reinterpret_cast<float*>(stats));
+      if (r.last(units)) break;
+      r.at += units - r.place.unit;
+      on = next_tile(a, seq, r.place);
     }
-  }
-  if (parts == 0) return;
-  if (threadIdx.x == 0) met = odd & kTail;
-  lds_sync();
-  for (int s = 1 + (int)threadIdx.x; s < parts; s += 256) {
-    int part_odd = 0;
-    for (int w = 0; w < waves; ++w) part_odd |= a.odd[(range + s) * 4 + w];
-    if (part_odd & kHead) met = kHead;
-  }
-  lds_sync();
-  if (__builtin_expect(met != 0, 0)) {
-    rows_apart<T>(a, piece.x, piece.y, piece.z, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
     return;
   }
+  const int4 piece = a.pieces[range];
+  const int parts = piece.w & 0xffff;
+  lds_sync();  // the last job is done
+  if (tid == 0) *met = piece.w >> 16 & kTail;
+  lds_sync();
+  for (int s = 1 + tid; s < parts; s += 256)
+    if (a.pieces[range + s].w >> 16 & kHead) *met = kHead;
   const Sequence seq = sequence_of(pg, piece.x);
   const int token0 = piece.z * a.tile_tokens;
   const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
-  const int quads = pg.head_dim / 4, groups = 256 / quads;
-  const int group = (int)threadIdx.x / quads, quad = (int)threadIdx.x - group * quads;
-  const int share = (rows + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int first = (int)blockIdx.y * share, last = min(first + share, rows);
-  const int steps = min(max(groups / max(share, 1), 1), parts);  // groups of a row
-  const int at_once = groups / steps;
-  const int step = group % steps;
-  for (int row0 = first; row0 < last; row0 += at_once) {
-    const int row = row0 + group / steps;
-    const bool in = row < last && group / steps < at_once;
+  // Items: four values of a row, the rows of a quad one after the other, as they lie in the parts.
+  const int items = rows * (pg.head_dim / 4);
+  const int share = (items + wide - 1) / wide;
+  const int first = index * share, last = min(first + share, items);
+  const int steps = max(min(256 / max(share, 1), parts), 1);  // threads of an item
+  const int at_once = 256 / steps, step = tid / at_once;
+  lds_sync();
+  if (__builtin_expect(*met != 0, 0)) {
+    lds_sync();
+    rows_apart<T>(a, piece.x, piece.y, piece.z, index, wide, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
+    return;
+  }
+  for (int item0 = first; item0 < last; item0 += at_once) {
+    const int item = item0 + tid - step * at_once;
+    const bool in = item < last && step < steps;
+    const int quad = item / rows, row = item - quad * rows;
+    const int wave = NW == 1 ? 0 : row >> 5, n = row & 31;
     float top = -__builtin_inff(), l = 0.0f;
     f4 o = f4{};
+    auto merge = [&](float2 st, f4 x) __attribute__((always_inline)) {
+      const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
+      const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
+      top = next;
+      l = l * f + st.y * w;
+      // (A part that weighs nothing beside another is left out, whatever it holds.)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
+    };
     if (in) {
-      // Part s: the first is one that ends inside its tile, the others begin inside.
-      int64_t at = (int64_t)(2 * (range + step) + (step == 0 ? 1 : 0)) * a.row_slots + row;
-#pragma unroll 4
-      for (int s = step; s < parts; s += steps) {
-        const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * at);
-        const f4 x = *reinterpret_cast<const f4*>(a.sums + at * pg.head_dim + 4 * quad);
-        at += ((int64_t)2 * steps - (s == 0 ? 1 : 0)) * a.row_slots;
-        const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
-        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
-        top = next;
-        l = l * f + st.y * w;
-        // (A part that weighs nothing beside another is left out, whatever it holds.)
+      const f4* const sums_at = reinterpret_cast<const f4*>(a.sums) + wave * (DP / 8) * 64 + (quad >> 1) * 64 +
+                                (quad & 1) * 32 + n;
+      const float2* const stats_at = a.stats + wave * 32 + n;
+      auto take = [&](auto once) __attribute__((always_inline)) {  // so many loads in flight
+        constexpr int kOnce = decltype(once)::value;
+        for (int s0 = step; s0 < parts; s0 += kOnce * steps) {
+          f4 x[kOnce];
+          float2 st[kOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
-      }
-      stats[threadIdx.x] = float2{top, l};
-      sums[threadIdx.x] = o;
+          for (int i = 0; i < kOnce; ++i) {
+            const int s = min(s0 + i * steps, parts - 1);
+            // The first part is one that ends inside its tile, the others begin inside.
+            const int64_t part = 2 * (range + s) + (s == 0 ? 1 : 0);
+            x[i] = sums_at[part * NW * (DP / 8) * 64];
+            st[i] = stats_at[part * NW * 32];
+          }
+#pragma unroll
+          for (int i = 0; i < kOnce; ++i)
+            if (s0 + i * steps < parts) merge(st[i], x[i]);
+        }
+      };
+      if (parts <= 2 * steps)
+        take(std::integral_constant<int, 2>{});
+      else
+        take(std::integral_constant<int, 8>{});
     }
-    if (steps > 1) lds_sync();
+    if (steps > 1) {
+      stats[tid] = float2{top, l};
+      sums[tid] = o;
+      lds_sync();
+      if (in && step == 0)
+        for (int s = 1; s < steps; ++s) merge(stats[tid + s * at_once], sums[tid + s * at_once]);
+    }
     if (in && step == 0) {
-      for (int s = 1; s < steps; ++s) {
-        const float2 st = stats[threadIdx.x + s * quads];
-        const f4 x = sums[threadIdx.x + s * quads];
-        const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
-        const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
-        top = next;
-        l = l * f + st.y * w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
-      }
       const int of = (int)fdiv((uint32_t)row, a.by_group);
       const int64_t token = seq.first + token0 + of;
       const int head = piece.y * a.group + row - of * a.group;
@@ -861,34 +924,73 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
   }
 }
 
+// Joins the parts of row tiles that several ranges share.
+template <class T, int DP, int KT, int NW>
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
+  __shared__ f4 sums[256];
+  __shared__ float2 stats[256];
+  __shared__ int met;
+  __shared__ int box[4];
+  __shared__ int list[2 * kMaxRanges];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // The ranges in which such a row tile begins, and those with whole row tiles to find anew.
+  constexpr int kEach = kMaxRanges / 256;
+  int mine[2 * kEach], count = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int range = tid * kEach + i, w = range < a.ranges ? a.pieces[range].w : 0;
+    mine[2 * i] = (w & 0xffff) != 0 ? range : -1;
+    mine[2 * i + 1] = (w >> 16 & kWhole) != 0 ? range | kAgain : -1;
+    count += (mine[2 * i] >= 0) + (mine[2 * i + 1] >= 0);
+  }
+  const int sum = (int)up_to((uint32_t)count);
+  if (lane == 63) box[wave] = sum;
+  lds_sync();
+  int jobs = 0, at = sum - count;
+  for (int i = 0; i < 4; ++i) {
+    at += i < wave ? box[i] : 0;
+    jobs += box[i];
+  }
+  if (jobs == 0) return;
+#pragma unroll
+  for (int i = 0; i < 2 * kEach; ++i)
+    if (mine[i] >= 0) list[at++] = mine[i];
+  lds_sync();
+  // Workgroups of a job; and the job and share of this one.
+  const int wide = min(max((int)gridDim.x / jobs, 1), 16);
+  for (int job = blockIdx.x; job < jobs * wide; job += gridDim.x)
+    join_one<T, DP, KT, NW>(a, list[job / wide], job % wide, wide, sums, stats, &met);
+}
+
 struct TilePick {
   void (*fn)(PagedArgs);
+  void (*join)(PagedArgs);
+  void (*count)(PagedArgs, int64_t*);
   int threads;
   int bytes;  // of LDS
 };
 
 template <class T, int DP, int KT, int NW>
 TilePick pick(Shape shape) {
+  constexpr int LOG = KT == 64 ? 6 : 5;
   return {shape == kPlain ? paged_tile<T, DP, KT, NW, kPlain>
           : shape == kCap ? paged_tile<T, DP, KT, NW, kCap>
                           : paged_tile<T, DP, KT, NW, kAny>,
-          NW * 64, 4 * TileL<DP, KT>::kTile};
+          paged_join<T, DP, LOG, NW>, paged_count<LOG>, NW * 64, 4 * TileL<DP, KT>::kTile};
 }
+
+// Values of a head, padded.
+int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
 template <class T>
 TilePick pick(int d, bool one_wave, Shape shape) {
-  if (one_wave) {
-    if (d <= 32) return pick<T, 32, 32, 1>(shape);
-    if (d <= 64) return pick<T, 64, 32, 1>(shape);
-    if (d <= 96) return pick<T, 96, 32, 1>(shape);
-    if (d <= 128) return pick<T, 128, 32, 1>(shape);
-    return pick<T, 256, 32, 1>(shape);
+  switch (padded(d)) {
+    case 32: return one_wave ? pick<T, 32, 32, 1>(shape) : pick<T, 32, 64, 4>(shape);
+    case 64: return one_wave ? pick<T, 64, 32, 1>(shape) : pick<T, 64, 64, 4>(shape);
+    case 96: return one_wave ? pick<T, 96, 32, 1>(shape) : pick<T, 96, 64, 4>(shape);
+    case 128: return one_wave ? pick<T, 128, 32, 1>(shape) : pick<T, 128, 64, 4>(shape);
+    default: return one_wave ? pick<T, 256, 32, 1>(shape) : pick<T, 256, 32, 4>(shape);
   }
-  if (d <= 32) return pick<T, 32, 64, 4>(shape);
-  if (d <= 64) return pick<T, 64, 64, 4>(shape);
-  if (d <= 96) return pick<T, 96, 64, 4>(shape);
-  if (d <= 128) return pick<T, 128, 64, 4>(shape);
-  return pick<T, 256, 32, 4>(shape);
 }
 
 }  // namespace
@@ -901,13 +1003,12 @@ PagedPlan paged_plan(const arthip_paged_attention_args& c) {
   p.one_wave = group <= 32 && rows <= (int64_t)32 * c.p.batch;
   const int tile = p.one_wave ? 32 : 128;
   p.tile_tokens = tile / group;
-  p.row_slots = (int)std::min<int64_t>(tile, rows);
   p.ranges = c.p.head_dim > 128 ? (p.one_wave ? 512 : 256) : p.one_wave ? 1024 : c.p.head_dim <= 64 ? 768 : 512;
   p.counted = c.p.batch > 64;
-  const size_t parts = (size_t)2 * p.ranges * p.row_slots;
-  p.sums = parts * c.p.head_dim * sizeof(float);
-  p.stats = parts * 2 * sizeof(float);
-  p.pieces = (size_t)(2 * p.ranges + 1) * sizeof(int4);  // and what the waves met
+  const size_t rows_kept = (size_t)2 * p.ranges * tile;
+  p.sums = rows_kept * padded(c.p.head_dim) * sizeof(float);
+  p.stats = rows_kept * sizeof(float2);
+  p.pieces = (size_t)p.ranges * sizeof(int4);
   p.before = p.counted ? ((size_t)c.p.batch + 1) * sizeof(int64_t) : 0;
   return p;
 }
@@ -920,8 +1021,6 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   a.group = c.q_heads / c.p.k_heads;
   a.tile_tokens = plan.tile_tokens;
   a.ranges = plan.ranges;
-  a.row_slots = plan.row_slots;
-  a.wave_rows = plan.one_wave;
   a.lanes = 64;
   while (a.lanes * c.p.batch > 64 && a.lanes > 1) a.lanes /= 2;
   a.by_group = make_fastdiv((uint32_t)a.group);
@@ -930,27 +1029,23 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   if (c.cap > 0) a.cap = make_cap(c.cap, c.scale);
   char* at = static_cast<char*>(c.workspace);
   a.sums = reinterpret_cast<float*>(at);
-  a.stats = reinterpret_cast<float*>(at += plan.sums);
+  a.stats = reinterpret_cast<float2*>(at += plan.sums);
   a.pieces = reinterpret_cast<int4*>(at += plan.stats);
-  a.odd = reinterpret_cast<int*>(a.pieces + a.ranges + 1);
   int64_t* const before = reinterpret_cast<int64_t*>(at += plan.pieces);
   const bool f16 = c.p.dtype == ARTHIP_TYPE_F16;
   const Shape shape = c.cap > kCapSmall || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
   const TilePick k =
       f16 ? pick<_Float16>(c.p.head_dim, plan.one_wave, shape) : pick<__bf16>(c.p.head_dim, plan.one_wave, shape);
-  const bool small = plan.one_wave || c.p.head_dim > 128;  // tiles of 32 keys
   if (plan.counted) {
     a.before = before;
-    hipLaunchKernelGGL(small ? paged_count<5> : paged_count<6>, dim3(1), dim3(1024), 0, s, a, before);
+    hipLaunchKernelGGL(k.count, dim3(1), dim3(1024), 0, s, a, before);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL(k.fn, dim3((unsigned)a.ranges), dim3((unsigned)k.threads), k.bytes, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const auto join = f16 ? (small ? paged_join<_Float16, 5> : paged_join<_Float16, 6>)
-                        : (small ? paged_join<__bf16, 5> : paged_join<__bf16, 6>);
-  hipLaunchKernelGGL(join, dim3((unsigned)a.ranges, plan.one_wave ? 4 : 16), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(k.join, dim3(kJoiners), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
