@@ -143,10 +143,9 @@ std::string check_key_weights_shape(const arthip_key_weights_args& a) {
   if (!wrong.empty()) return wrong;
   if (a.q_heads == 0) return at + "no query heads";
   if (a.slots < 0 || a.slots > kMaxTokens) return at + "slots out of range";
-  // Items of 128 keys and up to 64 ranges of rows number the workgroups in 31 bits, and the
-  // workspace's sums in 64.
+  // A launch takes fewer than 2^32 threads, of 256 for every 128 slots of a head.
   const int64_t items = (static_cast<int64_t>(a.slots) + 127) / 128;
-  if (items > 0 && static_cast<int64_t>(a.p.batch) * a.p.k_heads > (int64_t{1} << 24) / items)
+  if (items > 0 && static_cast<int64_t>(a.p.batch) * a.p.k_heads > (int64_t{1} << 23) / items)
     return at + "batch times heads times slots too large";
   return "";
 }
@@ -201,7 +200,7 @@ std::string check_cache_evict(const arthip_cache_evict_args& a) {
   if (a.recent < 0 || a.first < 0 || static_cast<int64_t>(a.recent) + a.first > a.keep)
     return at + "recent and first must be positive and add up to keep at most";
   if (p.batch == 0 || a.slots == 0) return "";
-  if (static_cast<int64_t>(p.batch) * p.k_heads > INT32_MAX / 64) return at + "batch times heads too large";
+  if (static_cast<int64_t>(p.batch) * p.k_heads > int64_t{1} << 21) return at + "batch times heads too large";
   if (a.weights == nullptr) return at + "null weights";
   if (a.kept == nullptr) return at + "null kept";
   if (a.positions_out != nullptr && a.positions == nullptr) return at + "positions_out without positions";

@@ -38,8 +38,9 @@ PagedPlan paged_plan(const arthip_paged_attention_args& a);
 
 // How the key weights are divided (key_weights.hip); of arguments whose shape is checked.
 struct KeyWeightsPlan {
-  int blocks;   // of 32 keys a wave
-  int splits;   // ranges of the rows, each its own workgroup; joined by a second kernel
+  int tiles;    // workgroups along the slots
+  int splits;   // and along the rows, whose sums a second kernel joins
+  int stream;   // few rows: slots of a workgroup (of one wave); 0: many
   size_t workspace;
 };
 KeyWeightsPlan key_weights_plan(const arthip_key_weights_args& a);
