@@ -135,16 +135,18 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   int32_t* const kept = a.c.kept + at * keep;
   const int used = min(n, keep);
   if (head == 0 && tid == 0 && a.c.new_len != nullptr) a.c.new_len[b] = used;
+  // (Where rows are moved by a kernel of their own, that one writes the weights and positions too.)
   auto stays = [&](int s, int from) __attribute__((always_inline)) {
     kept[s] = from;
-    if (w_out != nullptr) w_out[s] = w[from];
-    if (place_out != nullptr) place_out[s] = place[from];
+    if (HERE && w_out != nullptr) w_out[s] = w[from];
+    if (HERE && place_out != nullptr) place_out[s] = place[from];
   };
   auto rest = [&]() __attribute__((always_inline)) {  // what lies behind
-    for (int s = used + tid; s < a.c.slots; s += kThreads) {
-      if (w_out != nullptr) w_out[s] = 0.0f;
-      if (place_out != nullptr) place_out[s] = -1;
-    }
+    if constexpr (HERE)
+      for (int s = used + tid; s < a.c.slots; s += kThreads) {
+        if (w_out != nullptr) w_out[s] = 0.0f;
+        if (place_out != nullptr) place_out[s] = -1;
+      }
     for (int s = used + tid; s < keep; s += kThreads) kept[s] = -1;
   };
   if (n <= keep) {
@@ -157,25 +159,37 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   const int each = (n + kThreads - 1) / kThreads;
   const int begin = min(wave * each * 64, n), end = min(begin + each * 64, n);  // the wave's slots
   uint32_t keys[E > 0 ? E : 1];
-  int places[E > 0 ? E : 1];
   int newest = n - 1;
-  if constexpr (E > 0) {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < each) {
-        const int s = min(begin + i * 64 + lane, n - 1);
-        keys[i] = __builtin_bit_cast(uint32_t, w[s]);
-        if (place != nullptr) places[i] = place[s];
-      }
-  }
-  for (int i = tid; i < 3 * kBins; i += kThreads) bins[0][i] = 0;
-  if (place != nullptr) {
-    int top = INT32_MIN;
+  constexpr int kOnce = E > 0 && E < 8 ? E : 8;  // loads in flight
+  // f(i, the lane's slot), i counting the wave's 64 slots in a row. (What is known of some of them is
+  // kept from the others, or their addresses fill the registers.)
+  auto each_run = [&](auto f) __attribute__((always_inline)) {
     if constexpr (E > 0) {
+      int slot = begin + lane;
 #pragma unroll
       for (int i = 0; i < E; ++i)
-        if (i < each) top = max(top, places[i]);  // (past the run: the last slot's)
+        if (i < each) {
+          if (i % kOnce == 0) {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+v"(slot));
+          }
+          f(i, slot + i % kOnce * 64);
+          if (i % kOnce == kOnce - 1) slot += kOnce * 64;
+        }
+    }
+  };
+  for (int i = tid; i < 3 * kBins; i += kThreads) bins[0][i] = 0;
+  int places[E > 0 && E <= kOnce ? E : 1];  // short runs' are loaded once
+  if (place != nullptr) {
+    int top = INT32_MIN;
+    if constexpr (E > 0 && E <= kOnce) {
+      each_run([&](int i, int slot) __attribute__((always_inline)) {
+        places[i] = place[min(slot, n - 1)];  // (past the run: the last slot's)
+        keys[i] = __builtin_bit_cast(uint32_t, w[min(slot, n - 1)]);
+      });
+      each_run([&](int i, int) __attribute__((always_inline)) { top = max(top, places[i]); });
     } else {
+#pragma unroll 8
       for (int s = tid; s < n; s += kThreads) top = max(top, place[s]);
     }
     top = over_wave(top, [](int x, int y) { return max(x, y); });
@@ -189,19 +203,17 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   auto key = [&](float weight, int64_t t) __attribute__((always_inline)) -> uint32_t {
     return t > (int64_t)newest - a.c.recent || t < a.c.first ? UINT32_MAX : ordered(weight);
   };
-  if constexpr (E > 0) {
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < each)
-        keys[i] = key(__builtin_bit_cast(float, keys[i]), place != nullptr ? places[i] : begin + i * 64 + lane);
-  }
+  each_run([&](int i, int slot) __attribute__((always_inline)) {
+    const int s = min(slot, n - 1);
+    if (E <= kOnce && place != nullptr)
+      keys[i] = key(__builtin_bit_cast(float, keys[i]), places[E <= kOnce ? i : 0]);
+    else
+      keys[i] = key(w[s], place != nullptr ? place[s] : s);
+  });
   auto each_slot = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, its key)
     if constexpr (E > 0) {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (i < each) f(begin + i * 64 + lane, begin + i * 64 + lane < end, keys[i]);
+      each_run([&](int i, int slot) __attribute__((always_inline)) { f(slot, slot < end, keys[i]); });
     } else {
-      constexpr int kOnce = 8;  // loads in flight
       for (int s0 = begin; s0 < end; s0 += 64 * kOnce) {
         uint32_t x[kOnce];
 #pragma unroll
@@ -258,23 +270,14 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   }
 
   // -- holes below the budget and slots past it that stay, by their ranks -----------------
-  auto all_waves = [&](int mine, int (&of)[kWaves], int& total) __attribute__((always_inline)) {
-    if (lane == 0) of[wave] = mine;
-    lds_sync();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < kWaves; ++i) {
-      before += i < wave ? of[i] : 0;
-      total += of[i];
-    }
-    return before;
-  };
   // Of the equals of the least, the lowest `want` slots stay.
-  int equals_before = 0, total;
+  int equals_before = 0;
   if (ties) {
     int equals = 0;
     each_slot([&](int, bool is, uint32_t x) { equals += __popcll(__ballot(is && x == least)); });
-    equals_before = all_waves(equals, box[4], total);
+    if (lane == 0) box[4][wave] = equals;
+    lds_sync();
+    for (int i = 0; i < wave; ++i) equals_before += box[4][i];
   }
   const uint64_t below = (uint64_t{1} << lane) - 1;
   auto each_stay = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, it stays)
@@ -343,19 +346,38 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
 }
 
 // The rows that evict_select found to move: a thread 16 bytes of a slot's key and value. Rows come
-// from slots past the budget and go to slots below it, so that no order is needed.
-__global__ void __launch_bounds__(256) evict_move(EvictArgs a, int64_t first_block, int blocks) {
+// from slots past the budget and go to slots below it, so that no order is needed. The workgroups
+// from `movers` on write the weights and positions.
+constexpr int kSlots = 2048;  // of such a workgroup
+
+__global__ void __launch_bounds__(256) evict_move(EvictArgs a, int64_t first_block, int blocks, int movers) {
   const arthip_pages& p = a.c.p;
   const int64_t block = first_block + blockIdx.x, at = block / blocks;
+  const int index = (int)(block - at * blocks);
+  const int b = (int)fdiv((uint32_t)at, a.by_heads), head = (int)at - b * p.k_heads;
+  const int32_t* const kept = a.c.kept + at * a.c.keep;
+  if (index >= movers) {
+    const float* const w = a.c.weights + b * a.c.weights_stride[0] + head * a.c.weights_stride[1];
+    const int s0 = (index - movers) * kSlots;
+#pragma unroll
+    for (int i = 0; i < kSlots; i += 256) {
+      const int s = s0 + i + (int)threadIdx.x;
+      if (s >= a.c.slots) return;
+      const int from = s < a.c.keep ? kept[s] : -1;
+      if (a.c.weights_out != nullptr) a.c.weights_out[at * a.c.slots + s] = from < 0 ? 0.0f : w[from];
+      if (a.c.positions_out != nullptr)
+        a.c.positions_out[at * a.c.slots + s] =
+            from < 0 ? -1 : a.c.positions[b * a.c.positions_stride[0] + head * a.c.positions_stride[1] + from];
+    }
+    return;
+  }
   const int per = 256 / a.head_chunks;  // slots of a workgroup
   const int of = (int)fdiv(threadIdx.x, a.by_head_chunks), part = (int)threadIdx.x - of * a.head_chunks;
-  const int s = (int)(block - at * blocks) * per + of;
+  const int s = index * per + of;
   if (of >= per || s >= a.c.keep) return;
-  const int from = a.c.kept[at * a.c.keep + s];
+  const int from = kept[s];
   if (from < 0 || from == s) return;
-  const int b = (int)fdiv((uint32_t)at, a.by_heads), head = (int)at - b * p.k_heads;
-  const int32_t* const pages = p.pages + b * p.pages_stride;
-  move_chunk(a, pages, head, part, from, s);
+  move_chunk(a, p.pages + b * p.pages_stride, head, part, from, s);
 }
 
 template <int E>
@@ -393,14 +415,19 @@ hipError_t launch_cache_evict(const arthip_cache_evict_args& c, hipStream_t s) {
   const int most = std::min(c.keep, std::max(0, c.slots - c.keep));  // moves of a key head
   const bool here = most <= kMovesHere;
   const int each = (c.slots + kThreads - 1) / kThreads;
-  const auto fn = each <= 4 ? select_of<4>(here) : select_of<0>(here);
+  // (32768 slots of 32 key heads, keys in registers and read anew: 57 and 68 us.)
+  const auto fn = each <= 4    ? select_of<4>(here)
+                  : each <= 16 ? select_of<16>(here)
+                  : each <= 40 ? select_of<40>(here)
+                               : select_of<0>(here);
   hipLaunchKernelGGL(fn, dim3((unsigned)heads), dim3(kThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || here) return e;
   const int per = 256 / a.head_chunks;
-  const int64_t blocks = ((int64_t)c.keep + per - 1) / per;
+  const int movers = (c.keep + per - 1) / per;
+  const int blocks = movers + (c.slots + kSlots - 1) / kSlots;
   return launch_parts(heads * blocks, 256, [&](int64_t first, unsigned count) {
-    hipLaunchKernelGGL(evict_move, dim3(count), dim3(256), 0, s, a, first, (int)blocks);
+    hipLaunchKernelGGL(evict_move, dim3(count), dim3(256), 0, s, a, first, blocks, movers);
     return hipGetLastError();
   });
 }

@@ -90,17 +90,20 @@ struct Place {
 
 // The row tile after a place's; false where there is none (which the units rule out, if no one changes
 // the lengths meanwhile).
-__device__ __forceinline__ bool next_tile(const PagedArgs& a, const Sequence& s, Place& at) {
+__device__ __forceinline__ bool next_tile(const PagedArgs& a, Sequence& s, Place& at) {
   at.unit = 0;
   if (++at.tile < tiles_of(a, s)) return true;
   at.tile = 0;
   if (++at.head < a.c.p.k_heads) return true;
   at.head = 0;
-  do ++at.b;
-  while (at.b < a.c.p.batch && sequence_of(a.c.p, at.b).tokens == 0);
-  const bool is = at.b < a.c.p.batch;
-  at.b = min(at.b, a.c.p.batch - 1);
-  return is;
+  do {
+    if (++at.b >= a.c.p.batch) {
+      at.b = a.c.p.batch - 1;
+      return false;
+    }
+    s = sequence_of(a.c.p, at.b);
+  } while (s.tokens == 0);
+  return true;
 }
 
 // The units before each sequence, by one workgroup: a wave a sequence, then a running sum.
@@ -153,6 +156,7 @@ template <int KT>
 struct Finder {
   int64_t end, units;  // lane's sequence: units up to its end, and its own, of one key head
   int64_t total;
+  Sequence mine;       // and itself
 
   __device__ __forceinline__ void count(const PagedArgs& a, int lane) {
     const arthip_pages& p = a.c.p;
@@ -162,10 +166,10 @@ struct Finder {
     }
     const int b = (int)fdiv((uint32_t)lane, a.by_lanes), sub = lane - b * a.lanes;
     int64_t n = 0;
+    mine = sequence_of(p, min(b, p.batch - 1));
     if (b < p.batch) {
-      const Sequence s = sequence_of(p, b);
-      const int tiles = tiles_of(a, s);
-      for (int t = sub; t < tiles; t += a.lanes) n += units_of<KT>(a, s, t);
+      const int tiles = tiles_of(a, mine);
+      for (int t = sub; t < tiles; t += a.lanes) n += units_of<KT>(a, mine, t);
     }
     for (int step = 1; step < a.lanes; step *= 2) n += shuffle(n, lane ^ step);
     units = n;
@@ -179,8 +183,8 @@ struct Finder {
     total = shuffle(sum, 63);
   }
 
-  // The place of unit x, below `total` (uniform).
-  __device__ __forceinline__ Place find(const PagedArgs& a, int64_t x, int lane) const {
+  // The place of unit x, below `total` (uniform), and its sequence.
+  __device__ __forceinline__ Place find(const PagedArgs& a, int64_t x, int lane, Sequence& s) const {
     const arthip_pages& p = a.c.p;
     Place at;
     int64_t one;  // units of a key head
@@ -197,15 +201,16 @@ struct Finder {
       const int64_t first = a.before[at.b];
       one = (a.before[at.b + 1] - first) / p.k_heads;
       x -= first;
+      s = sequence_of(p, at.b);
     } else {
       const int of = __popcll(__ballot(end <= x));  // lanes of earlier sequences
       at.b = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)of, a.by_lanes));
       one = shuffle(units, of);
+      s = {__shfl(mine.first, of), __shfl(mine.tokens, of), __shfl(mine.len, of)};
       x -= shuffle(end, of) - one * p.k_heads;
     }
     at.head = __builtin_amdgcn_readfirstlane((int)(x / one));
     x -= at.head * one;
-    const Sequence s = sequence_of(p, at.b);
     for (int t0 = 0;; t0 += 64) {
       const int t = t0 + lane;
       const uint32_t n = t < tiles_of(a, s) ? (uint32_t)units_of<KT>(a, s, t) : 0;
@@ -240,6 +245,7 @@ struct Range {
   int64_t total;           // units of all ranges,
   int live;                // and their number
   Place place;
+  Sequence seq;            // the place's
 
   // False where there is no range of this number.
   template <int KT>
@@ -251,17 +257,18 @@ struct Range {
     cut = (range + 1) * total / live;
     const int64_t share = total / live;
     slack = min(share >> 3, max(share >> 5, (int64_t)4));
-    const Place p = finder.find(a, at, lane);
+    Sequence s;
+    const Place p = finder.find(a, at, lane, s);
     place = {scalar(p.b), scalar(p.head), scalar(p.tile), scalar(p.unit)};
+    seq = {scalar(s.first), scalar(s.tokens), scalar(s.len)};
     if (place.unit == 0) return true;
-    const Sequence s = sequence_of(a.c.p, place.b);
-    const int left = units_of<KT>(a, s, place.tile) - place.unit;
+    const int left = units_of<KT>(a, seq, place.tile) - place.unit;
     if (place.unit <= slack) {
       at -= place.unit;
       place.unit = 0;
     } else if (left <= slack) {
       at += left;
-      return next_tile(a, s, place);
+      return next_tile(a, seq, place);
     }
     return true;
   }
@@ -328,6 +335,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   r.at = scalar64(r.at);
   r.cut = scalar64(r.cut);
   Place place = {scalar(r.place.b), scalar(r.place.head), scalar(r.place.tile), scalar(r.place.unit)};
+  Sequence seq = {scalar(r.seq.first), scalar(r.seq.tokens), scalar(r.seq.len)};
   int odd = 0;  // what the wave met
   // The last of a range: the row tile that it shares with later ones, if any.
   auto finish = [&](int4 piece) __attribute__((always_inline)) {
@@ -381,10 +389,6 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         v_row * RB + ((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::v_swizzle(v_row)) * 16 + (lane & 1) * 8;
 
     // -- a row tile, or a part of it ----------------------------------------------------
-    Sequence seq = sequence_of(pg, place.b);
-    seq.first = scalar(seq.first);
-    seq.tokens = scalar(seq.tokens);
-    seq.len = scalar(seq.len);
     const int token0 = place.tile * a.tile_tokens;
     const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;  // of the row tile
     const Span span = span_of<LOG>(a, seq, place.tile);
@@ -741,6 +745,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     r.at += take;
     next_tile(a, seq, place);
     place = {scalar(place.b), scalar(place.head), scalar(place.tile), 0};
+    seq = {scalar(seq.first), scalar(seq.tokens), scalar(seq.len)};
   }
 }
 
@@ -825,14 +830,13 @@ __device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* s
     Range r;
     bool on = r.begin(a, finder, ranges_of(a, finder.total), range, lane);
     while (on) {
-      const Sequence seq = sequence_of(pg, r.place.b);
-      const int units = units_of<KT>(a, seq, r.place.tile);
+      const int units = units_of<KT>(a, r.seq, r.place.tile);
       if (r.take(units) == units)
         rows_apart<T>(a, r.place.b, r.place.head, r.place.tile, index, wide, reinterpret_cast<float*>(sums),
                       reinterpret_cast<float*>(stats));
       if (r.last(units)) break;
       r.at += units - r.place.unit;
-      on = next_tile(a, seq, r.place);
+      on = next_tile(a, r.seq, r.place);
     }
     return;
   }
