@@ -72,6 +72,7 @@ struct Elem<_Float16> {
   typedef h8 frag;
   static constexpr float kZero = 0x1p-25f;  // numbers of 0 and more up to here round to 0
   static constexpr float kRaise = 7.0f;     // weights are up to 2^(8 + 7), see weights()
+  static constexpr float kMost = 0x1p+15f;  // sum of weights that each are numbers of the type
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -81,6 +82,7 @@ struct Elem<__bf16> {
   typedef b8 frag;
   static constexpr float kZero = 0.0f;  // as the exponential's are 2^-126 or more, or 0
   static constexpr float kRaise = 0.0f;
+  static constexpr float kMost = 0x1p+10f;  // values up to 2^-10 of the type's largest stay finite
   static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }

@@ -44,6 +44,7 @@ struct KeyArgs {
 };
 
 constexpr int kRows = 64;  // of a tile
+constexpr int kStarts = 4 * kRows * 4;  // bytes of their exponents' starts in LDS
 constexpr int kItems = 2048;    // workgroups that many rows are divided into (1024: 284 us for 268 below)
 constexpr int kStreams = 5120;  // and waves that few rows are (2560, 10240: 78 and 76 us for 73.5)
 
@@ -542,8 +543,13 @@ hipError_t launch_key_weights(const arthip_key_weights_args& c, hipStream_t s) {
     hipLaunchKernelGGL(fn, dim3((unsigned)a.items), dim3(64), 0, s, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(fn, dim3((unsigned)a.items), dim3(256), 2 * tile_bytes(c.p.head_dim), s, a);
-  const hipError_t e = hipGetLastError();
+  const int bytes = 2 * tile_bytes(c.p.head_dim);
+  hipError_t e = hipSuccess;
+  if (bytes + kStarts > 65536)  // what a kernel may have without asking
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(fn, dim3((unsigned)a.items), dim3(256), bytes, s, a);
+  e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t total = heads * c.slots;
   return launch_parts((total + 255) / 256, 256, [&](int64_t first, unsigned count) {

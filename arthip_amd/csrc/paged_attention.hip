@@ -5,7 +5,7 @@
 // that it stages in LDS. Both products are v_mfma_f32_32x32x16 with the keys of the first as
 // rows, S^T = K Q^T: a lane holds 16 keys of ONE query, and the accumulator, packed to the
 // element type, is the right operand of O^T += V^T P^T. Statistics are fp32 in the base of 2;
-// P is rounded to the element type (it lies in [0, 2^8], fp16's in [0, 2^15]), its sum is taken
+// P is rounded to the element type (it lies in [0, 2^10], fp16's in [0, 2^15]), its sum is taken
 // before.
 //
 // Lengths are known on the device alone, and differ: one call holds prompts beside single
@@ -204,7 +204,7 @@ struct Finder {
       s = sequence_of(p, at.b);
     } else {
       const int of = __popcll(__ballot(end <= x));  // lanes of earlier sequences
-      at.b = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)of, a.by_lanes));
+      at.b = __builtin_amdgcn_readfirstlane(min((int)fdiv((uint32_t)of, a.by_lanes), p.batch - 1));
       one = shuffle(units, of);
       s = {__shfl(mine.first, of), __shfl(mine.tokens, of), __shfl(mine.len, of)};
       x -= shuffle(end, of) - one * p.k_heads;
@@ -303,6 +303,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   constexpr int GL = LOADS / NG;                       // loads of a page
   static_assert(SEG % NW == 0 && LOADS % NG == 0 && (WK <= 16 || WK % 16 == 0), "whole pages a wave");
   constexpr uint32_t kOob = 0x80000000u;
+  constexpr bool kLazy = DP > 64;  // see follow()
+  // A wave at its exponentials goes before one at its products where the vector unit has more to do
+  // (heads of 64, 8160 over 40800: 1265 -> 1203 us; capped heads of 128 110 -> 106; plain ones 454 -> 472).
+  constexpr bool kFirst = DP <= 64 || SHAPE != kPlain;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   constexpr int v_at = 2 * L::kTile;  // V's buffers
@@ -523,8 +527,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     };
 
     // -- scores to weights -----------------------------------------------------------------
-    // The scores in the base of 2 or, plain ones, still to be scaled by `mul`; hidden ones -inf. Then
-    // the row's base, from the largest of them.
+    // The scores in the base of 2 or, plain ones, still to be scaled by `mul`; hidden ones -inf.
     auto ready = [&](int k0, bool partial) __attribute__((always_inline)) {
       const int key0 = k0 + 4 * half;  // key of element r of block kb: key0 + 32 kb + 8 (r / 4) + r % 4
       if (SHAPE == kCap || (SHAPE == kAny && a.c.cap > 0)) {
@@ -571,24 +574,39 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
             s[kb][r] = key >= lo && key < hi ? s[kb][r] : -__builtin_inff();
           }
       }
+    };
+    auto largest = [&]() __attribute__((always_inline)) {
       float top = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-      top = halves_max(top);
-      // The base of a row's exponents follows its largest score only where that has grown
-      // by more than 2^8: until then weights are at most 256, and nothing is rescaled.
-      if (__any((top - m) * mul > 8.0f)) {
-        const float next = fmaxf(m, top);
-        // A row that has seen nothing yet has no sums to keep (next may be -inf as well).
-        const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
-        m = next;
-        l *= f;
+      return halves_max(top);
+    };
+    // A row's base is a score near its largest so far; this makes it the largest. Where that has not
+    // grown by more than 2^8 or so nothing is rescaled. Heads above 64 take no maximum to see whether
+    // it has: the weights' sum tells (also of a row that has seen nothing yet, whose base of -inf makes
+    // it infinite or NaN), and they are found again. (Prompts beside single tokens 462 -> 448 us;
+    // narrower heads have no registers for it.)
+    auto follow = [&]() __attribute__((always_inline)) {
+      const float next = fmaxf(m, largest());
+      // A row that has seen nothing yet has no sums to keep (next may be -inf as well).
+      const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - next) * mul);
+      m = next;
+      l *= f;
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
+      for (int i = 0; i < DB; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][r] *= f;
+        for (int r = 0; r < 16; ++r) o[i][r] *= f;
+    };
+    // The weights of the scores against a row's base, packed; their sum.
+    auto weight = [&](int e, float base, float& sum, float (&w)[8], frag (&p)[KT / 16]) __attribute__((always_inline)) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], mul, -base));
+      sum += x;
+      w[e % 8] = x;
+      if (e % 8 == 7) {
+        typedef float f8 __attribute__((ext_vector_type(8)));
+        p[e / 8] = __builtin_convertvector(f8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, frag);
       }
     };
 
@@ -622,12 +640,16 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
         ask(then, min(t + 3, end - 1));
         if (w_real) {
           ready(k0, !(k0 >= w_lo_max && k0 + KT <= w_hi_min));
+          if constexpr (!kLazy) {
+            if (__any((largest() - m) * mul > 8.0f)) follow();
+          }
           // fp16's weights are raised to the top of its range, so that small ones, of which a long
           // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
-          const float base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+          float base = (!kLazy && m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
           f16v following[KB];
           frag p[KT / 16];
-          float sum = 0.0f;
+          float w[8], sum = 0.0f;
+          if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
           {
             // A product, the operand of the fourth after it, and its share of the exponentials.
             constexpr int N = KS * KB, A = N < 4 ? N : 4;
@@ -643,17 +665,19 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
               following[i % KB] = E::mma(k[i], q[i / KB], i < KB ? f16v{} : following[i % KB]);
               if (i + A < N) read(i + A);
 #pragma unroll
-              for (int e = i * 16 * KB / N; e < (i + 1) * 16 * KB / N; ++e) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], mul, -base));
-                sum += w;
-                s[e / 16][e % 16] = w;
-                if (e % 16 == 7)
-                  p[e / 8] = __builtin_convertvector(__builtin_shufflevector(s[e / 16], s[e / 16], 0, 1, 2, 3, 4, 5, 6, 7), frag);
-                if (e % 16 == 15)
-                  p[e / 8] = __builtin_convertvector(
-                      __builtin_shufflevector(s[e / 16], s[e / 16], 8, 9, 10, 11, 12, 13, 14, 15), frag);
-              }
+              for (int e = i * 16 * KB / N; e < (i + 1) * 16 * KB / N; ++e) weight(e, base, sum, w, p);
               __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
+          if (kLazy && __any(!(sum <= E::kMost))) {
+            follow();
+            base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+            sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16 * KB; ++e) {
+              weight(e, base, sum, w, p);
+              if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // or registers run out
             }
           }
           l += sum;  // this half's keys; the halves are added at the end

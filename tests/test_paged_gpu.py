@@ -162,6 +162,9 @@ ATTENTION = [
     (BF16, 4, 2, 96, 16, [(1, 80), (1, 1)], {"cap": 50.0, "left": 20}),
     (F16, 4, 2, 64, 16, [(1, 3 + 5 * (i % 13)) for i in range(100)], {}),       # more sequences than lanes
     (BF16, 2, 2, 64, 16, [((i * 7) % 50 if i % 3 else 0, 50 + i) for i in range(70)], {}),
+    (F16, 4, 1, 64, 16, [(40, 300)] + [(1, 20 + i) for i in range(20)], {}),    # few rows a sequence but in one
+    (BF16, 8, 2, 128, 32, [(1, 2000 - 31 * i) for i in range(64)], {}),         # as many sequences as lanes
+    (F16, 16, 1, 256, 16, [(100, 600), (1, 900)], {}),
 ]
 
 
@@ -230,6 +233,37 @@ def test_attention_hidden_infinities(dtype, d):
             c.v[page, at, 0, 3] = value
         c.k[int(c.table[0, (lk - 1) // 16]), (lk - 1) % 16, 1] = math.nan
         _attend(c, q, f"{n} over {lk}")
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F16, 128), (BF16, 128), (BF16, 32)])
+def test_attention_scores_that_grow(dtype, d):
+    """Scores that rise by hundreds from tile to tile, and fall again; hidden keys are the largest."""
+    for n, lk in ((70, 500), (1, 700)):
+        c = Cache([(n, lk)], 1, d, dtype)
+        for slot in range(lk):
+            page, at = int(c.table[0, slot // 16]), slot % 16
+            c.k[page, at] *= 0.25 + 4 * min(slot, lk - slot) / lk
+        c.k[int(c.table[0, (lk - 1) // 16]), (lk - 1) % 16] *= 8
+        _attend(c, c.normal(n, 4, d, std=6.0))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_means_of_the_largest_numbers(dtype):
+    """A mean of the type's largest numbers, less the weights' room, is finite."""
+    top = 65504.0 if dtype == F16 else 2.0 ** 117
+    c = Cache([(40, 300), (1, 3000)], 1, 128, dtype)
+    c.v[~torch.isnan(c.v)] = top
+    q = c.normal(41, 4, 128)
+    k, v, pages, kv_len, offsets = c.cuda()
+    out = paged.paged_attention(q.cuda(), k, v, pages, kv_len, offsets)
+    assert (out.float() / top - 1).abs().max() <= 2 * ref.UNIT[dtype]
+
+
+def test_attention_sequences_that_share_pages():
+    """A common beginning lies in the cache once."""
+    c = Cache([(3, 70), (1, 66)], 2, 64, F16)
+    c.table[1, :4] = c.table[0, :4]
+    _attend(c, c.normal(4, 4, 64))
 
 
 def test_attention_same_bits_whatever_the_stream():
