@@ -39,7 +39,8 @@ struct PagedArgs {
   int tile_tokens;  // tokens of a row tile
   int ranges;       // workgroups
   int lanes;        // that count one sequence's tiles together, if `before` is not there
-  FastDiv by_group, by_page, by_lanes;
+  int few;          // 31 bits hold the units, times `ranges`
+  FastDiv by_group, by_page, by_lanes, by_heads;
   CapFit cap;
   const int64_t* before;  // key tiles of the sequences before each [batch + 1], of all key heads
   // Parts of row tiles, two a range: the one that begins inside its tile, the one that ends inside.
@@ -151,12 +152,14 @@ __global__ void __launch_bounds__(1024) paged_count(PagedArgs a, int64_t* before
 }
 
 // A wave's view of the batch: units of each sequence (64 at most, `lanes` lanes each) or the
-// counted ones.
+// counted ones. Where 31 bits hold all units times the ranges, sums and quotients are of 32 bits and
+// stay in the vector unit.
 template <int KT>
 struct Finder {
-  int64_t end, units;  // lane's sequence: units up to its end, and its own, of one key head
-  int64_t total;
-  Sequence mine;       // and itself
+  int64_t end;     // units of one key head up to the lane's share of its sequence
+  uint32_t end32;  // the same, if they are few
+  int64_t total;   // of all key heads
+  Sequence mine;   // the lane's
 
   __device__ __forceinline__ void count(const PagedArgs& a, int lane) {
     const arthip_pages& p = a.c.p;
@@ -171,23 +174,26 @@ struct Finder {
       const int tiles = tiles_of(a, mine);
       for (int t = sub; t < tiles; t += a.lanes) n += units_of<KT>(a, mine, t);
     }
-    for (int step = 1; step < a.lanes; step *= 2) n += shuffle(n, lane ^ step);
-    units = n;
-    int64_t sum = sub == 0 ? n * p.k_heads : 0;
+    if (a.few) {
+      end32 = up_to((uint32_t)n);
+      total = (int64_t)__builtin_amdgcn_readlane((int)end32, 63) * p.k_heads;
+      return;
+    }
+    end = n;
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
-      const int64_t y = shuffle(sum, max(lane - step, 0));
-      sum += lane >= step ? y : 0;
+      const int64_t y = shuffle(end, max(lane - step, 0));
+      end += lane >= step ? y : 0;
     }
-    end = sum;  // the same for a sequence's lanes
-    total = shuffle(sum, 63);
+    total = shuffle(end, 63) * p.k_heads;
   }
 
   // The place of unit x, below `total` (uniform), and its sequence.
   __device__ __forceinline__ Place find(const PagedArgs& a, int64_t x, int lane, Sequence& s) const {
+    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    auto from = [&](int v, int of) { return __builtin_amdgcn_readlane(v, scalar(of)); };
     const arthip_pages& p = a.c.p;
     Place at;
-    int64_t one;  // units of a key head
     if (a.before != nullptr) {
       int lo = 0, n = p.batch;  // the last sequence whose units begin at or before x
       while (n > 1) {
@@ -197,37 +203,42 @@ struct Finder {
         lo += skip;
         n = min(step, n - skip);
       }
-      at.b = __builtin_amdgcn_readfirstlane(lo);
-      const int64_t first = a.before[at.b];
-      one = (a.before[at.b + 1] - first) / p.k_heads;
-      x -= first;
+      at.b = scalar(lo);
+      const int64_t first = a.before[at.b], one = (a.before[at.b + 1] - first) / p.k_heads;
       s = sequence_of(p, at.b);
+      at.head = scalar((int)((x - first) / one));
+      x -= first + at.head * one;
     } else {
-      const int of = __popcll(__ballot(end <= x));  // lanes of earlier sequences
-      at.b = __builtin_amdgcn_readfirstlane(min((int)fdiv((uint32_t)of, a.by_lanes), p.batch - 1));
-      one = shuffle(units, of);
-      s = {__shfl(mine.first, of), __shfl(mine.tokens, of), __shfl(mine.len, of)};
-      x -= shuffle(end, of) - one * p.k_heads;
+      // A sequence's key heads follow one another: its first unit is as many times the units of one
+      // key head before it.
+      const int of = a.few ? __popcll(__ballot(end32 <= fdiv((uint32_t)x, a.by_heads)))
+                           : __popcll(__ballot(end <= x / p.k_heads));  // lanes before unit x's
+      at.b = scalar(min((int)fdiv((uint32_t)of, a.by_lanes), p.batch - 1));
+      const int first = at.b * a.lanes, last = first + a.lanes - 1;
+      s = {from(mine.first, first), from(mine.tokens, first), from(mine.len, first)};
+      if (a.few) {
+        const uint32_t before = at.b > 0 ? (uint32_t)from((int)end32, first - 1) : 0u;
+        const uint32_t one = (uint32_t)from((int)end32, last) - before, left = (uint32_t)x - before * (uint32_t)p.k_heads;
+        at.head = scalar((int)(left / one));
+        x = left - (uint32_t)at.head * one;
+      } else {
+        const int64_t before = at.b > 0 ? shuffle(end, first - 1) : 0, one = shuffle(end, last) - before;
+        x -= before * p.k_heads;
+        at.head = scalar((int)(x / one));
+        x -= at.head * one;
+      }
     }
-    at.head = __builtin_amdgcn_readfirstlane((int)(x / one));
-    x -= at.head * one;
     for (int t0 = 0;; t0 += 64) {
       const int t = t0 + lane;
       const uint32_t n = t < tiles_of(a, s) ? (uint32_t)units_of<KT>(a, s, t) : 0;
-      uint32_t sum = n;
-#pragma unroll
-      for (int step = 1; step < 64; step *= 2) {
-        const uint32_t y = __shfl(sum, max(lane - step, 0));
-        sum += lane >= step ? y : 0;
-      }
-      const uint32_t all = __shfl(sum, 63);
+      const uint32_t sum = up_to(n), all = (uint32_t)from((int)sum, 63);
       if (x >= all && all > 0) {
         x -= all;
         continue;
       }
       const int of = min(__popcll(__ballot((int64_t)sum <= x)), 63);
-      at.tile = __builtin_amdgcn_readfirstlane(t0 + of);
-      at.unit = __builtin_amdgcn_readfirstlane((int)(x - (__shfl(sum, of) - __shfl(n, of))));
+      at.tile = scalar(t0 + of);
+      at.unit = scalar((int)(x - ((uint32_t)from((int)sum, of) - (uint32_t)from((int)n, of))));
       return at;
     }
   }
@@ -238,8 +249,8 @@ __device__ __forceinline__ int ranges_of(const PagedArgs& a, int64_t total) {
 }
 
 // One workgroup's range of the units: about as many as any other's. A cut that would leave only a
-// little (a 32nd of a range, or four tiles) of a row tile on one side goes to that tile's end: two parts more cost
-// more than they balance (256 tokens over 32765 keys: 147 us, 136 so).
+// little (a 32nd of a range, or four tiles) of a row tile on one side goes to that tile's end: two
+// parts more cost more than they balance (256 tokens over 32765 keys: 147 us, 136 so).
 struct Range {
   int64_t at, cut, slack;  // where it is, where it is cut off
   int64_t total;           // units of all ranges,
@@ -253,9 +264,17 @@ struct Range {
     auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     total = finder.total;
     live = ranges;
-    at = range * total / live;
-    cut = (range + 1) * total / live;
-    const int64_t share = total / live;
+    int64_t share;
+    if (a.few) {
+      const uint32_t all = (uint32_t)total, n = (uint32_t)live;
+      at = (uint32_t)range * all / n;
+      cut = (uint32_t)(range + 1) * all / n;
+      share = all / n;
+    } else {
+      at = range * total / live;
+      cut = (range + 1) * total / live;
+      share = total / live;
+    }
     slack = min(share >> 3, max(share >> 5, (int64_t)4));
     Sequence s;
     const Place p = finder.find(a, at, lane, s);
@@ -1054,6 +1073,10 @@ hipError_t launch_paged_attention(const arthip_paged_attention_args& c, hipStrea
   a.by_group = make_fastdiv((uint32_t)a.group);
   a.by_page = make_fastdiv((uint32_t)c.p.page_size);
   a.by_lanes = make_fastdiv((uint32_t)a.lanes);
+  a.by_heads = make_fastdiv((uint32_t)c.p.k_heads);
+  const int64_t tiles = ((int64_t)c.p.tokens / a.tile_tokens + 1) * c.p.batch;  // whatever q_offsets hold
+  const int64_t units = ((int64_t)c.p.max_pages * c.p.page_size + 31) / 32 + 1 + kStart;
+  a.few = tiles < INT32_MAX / units / c.p.k_heads / a.ranges;
   if (c.cap > 0) a.cap = make_cap(c.cap, c.scale);
   char* at = static_cast<char*>(c.workspace);
   a.sums = reinterpret_cast<float*>(at);
