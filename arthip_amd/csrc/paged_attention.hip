@@ -860,7 +860,8 @@ __device__ __forceinline__ void rows_apart(const PagedArgs& a, int b, int kh, in
 
 // A workgroup's share of a job of the joining kernel: the parts of the row tile that begins in a range,
 // in their order, four values of a row a thread; where there are fewer of these than threads, several
-// threads take an item's parts in turn.
+// threads take an item's parts in turn. What costs time is that loads wait: four items a thread, two
+// parts of each at a time, are in flight (prompts 456 -> 449 us against one item a thread).
 template <class T, int DP, int KT, int NW>
 __device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* sums, float2* stats, int* met) {
   const arthip_pages& pg = a.c.p;
@@ -893,7 +894,9 @@ __device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* s
   const Sequence seq = sequence_of(pg, piece.x);
   const int token0 = piece.z * a.tile_tokens;
   const int rows = min(a.tile_tokens, seq.tokens - token0) * a.group;
-  // Items: four values of a row, the rows of a quad one after the other, as they lie in the parts.
+  // Items: four values of a row, the rows of a quad one after the other, as they lie in the parts, or
+  // 8 rows of 8 quads, so that out is written 64 bytes at a time.
+  const bool blocks = rows % 8 == 0 && pg.head_dim % 32 == 0;
   const int items = rows * (pg.head_dim / 4);
   const int share = (items + wide - 1) / wide;
   const int first = index * share, last = min(first + share, items);
@@ -905,70 +908,98 @@ __device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* s
     rows_apart<T>(a, piece.x, piece.y, piece.z, index, wide, reinterpret_cast<float*>(sums), reinterpret_cast<float*>(stats));
     return;
   }
-  for (int item0 = first; item0 < last; item0 += at_once) {
-    const int item = item0 + tid - step * at_once;
-    const bool in = item < last && step < steps;
-    const int quad = item / rows, row = item - quad * rows;
-    const int wave = NW == 1 ? 0 : row >> 5, n = row & 31;
-    float top = -__builtin_inff(), l = 0.0f;
-    f4 o = f4{};
-    auto merge = [&](float2 st, f4 x) __attribute__((always_inline)) {
-      const float next = fmaxf(top, st.x), base = next == -__builtin_inff() ? 0.0f : next;
-      const float f = __builtin_amdgcn_exp2f(top - base), w = __builtin_amdgcn_exp2f(st.x - base);
-      top = next;
-      l = l * f + st.y * w;
-      // (A part that weighs nothing beside another is left out, whatever it holds.)
+  // COUNT items a thread and ONCE parts of each at a time, all in flight.
+  auto join = [&](auto count, auto once) __attribute__((always_inline)) {
+    constexpr int COUNT = decltype(count)::value, ONCE = decltype(once)::value;
+    for (int item0 = first; item0 < last; item0 += COUNT * at_once) {
+      int row[COUNT], quad[COUNT];
+      float top[COUNT], l[COUNT];
+      f4 o[COUNT];
+      bool in[COUNT];
+      const f4* sums_at[COUNT];
+      const float2* stats_at[COUNT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (f != 0.0f ? o[e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
-    };
-    if (in) {
-      const f4* const sums_at = reinterpret_cast<const f4*>(a.sums) + wave * (DP / 8) * 64 + (quad >> 1) * 64 +
-                                (quad & 1) * 32 + n;
-      const float2* const stats_at = a.stats + wave * 32 + n;
-      auto take = [&](auto once) __attribute__((always_inline)) {  // so many loads in flight
-        constexpr int kOnce = decltype(once)::value;
-        for (int s0 = step; s0 < parts; s0 += kOnce * steps) {
-          f4 x[kOnce];
-          float2 st[kOnce];
+      for (int c = 0; c < COUNT; ++c) {
+        const int item = min(item0 + c * at_once + tid - step * at_once, last - 1);
+        in[c] = item0 + c * at_once + tid - step * at_once < last && step < steps;
+        if (blocks) {
+          const int block = item >> 6, quads = block / (rows / 8);
+          row[c] = (block - quads * (rows / 8)) * 8 + (item & 7);
+          quad[c] = quads * 8 + (item >> 3 & 7);
+        } else {
+          quad[c] = item / rows;
+          row[c] = item - quad[c] * rows;
+        }
+        const int wave = NW == 1 ? 0 : row[c] >> 5, n = row[c] & 31;
+        sums_at[c] = reinterpret_cast<const f4*>(a.sums) + wave * (DP / 8) * 64 + (quad[c] >> 1) * 64 +
+                     (quad[c] & 1) * 32 + n;
+        stats_at[c] = a.stats + wave * 32 + n;
+        top[c] = -__builtin_inff();
+        l[c] = 0.0f;
+        o[c] = f4{};
+      }
+      auto merge = [&](int c, float2 st, f4 x) __attribute__((always_inline)) {
+        const float next = fmaxf(top[c], st.x), base = next == -__builtin_inff() ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f(top[c] - base), w = __builtin_amdgcn_exp2f(st.x - base);
+        top[c] = next;
+        l[c] = l[c] * f + st.y * w;
+        // (A part that weighs nothing beside another is left out, whatever it holds.)
 #pragma unroll
-          for (int i = 0; i < kOnce; ++i) {
+        for (int e = 0; e < 4; ++e) o[c][e] = (f != 0.0f ? o[c][e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
+      };
+      if (step < steps) {
+        for (int s0 = step; s0 < parts; s0 += ONCE * steps) {
+          f4 x[COUNT][ONCE];
+          float2 st[COUNT][ONCE];
+#pragma unroll
+          for (int i = 0; i < ONCE; ++i) {
             const int s = min(s0 + i * steps, parts - 1);
             // The first part is one that ends inside its tile, the others begin inside.
             const int64_t part = 2 * (range + s) + (s == 0 ? 1 : 0);
-            x[i] = sums_at[part * NW * (DP / 8) * 64];
-            st[i] = stats_at[part * NW * 32];
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) {
+              x[c][i] = sums_at[c][part * NW * (DP / 8) * 64];
+              st[c][i] = stats_at[c][part * NW * 32];
+            }
           }
 #pragma unroll
-          for (int i = 0; i < kOnce; ++i)
-            if (s0 + i * steps < parts) merge(st[i], x[i]);
-        }
-      };
-      if (parts <= 2 * steps)
-        take(std::integral_constant<int, 2>{});
-      else
-        take(std::integral_constant<int, 8>{});
-    }
-    if (steps > 1) {
-      stats[tid] = float2{top, l};
-      sums[tid] = o;
-      lds_sync();
-      if (in && step == 0)
-        for (int s = 1; s < steps; ++s) merge(stats[tid + s * at_once], sums[tid + s * at_once]);
-    }
-    if (in && step == 0) {
-      const int of = (int)fdiv((uint32_t)row, a.by_group);
-      const int64_t token = seq.first + token0 + of;
-      const int head = piece.y * a.group + row - of * a.group;
-      const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-      T* const op = static_cast<T*>(a.c.out) + token * a.c.out_stride[0] + head * a.c.out_stride[1];
-      typedef T t4 __attribute__((ext_vector_type(4)));
+          for (int i = 0; i < ONCE; ++i)
+            if (s0 + i * steps < parts)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = in_range<T>(o[e] * scale);
-      *reinterpret_cast<t4*>(op + 4 * quad) = __builtin_convertvector(o, t4);
-      if (a.c.lse && quad == 0) a.c.lse[token * a.c.q_heads + head] = (top + __builtin_amdgcn_logf(l)) * kLn2;
+              for (int c = 0; c < COUNT; ++c) merge(c, st[c][i], x[c][i]);
+        }
+      }
+      if (COUNT == 1 && steps > 1) {
+        stats[tid] = float2{top[0], l[0]};
+        sums[tid] = o[0];
+        lds_sync();
+        if (in[0] && step == 0)
+          for (int s = 1; s < steps; ++s) merge(0, stats[tid + s * at_once], sums[tid + s * at_once]);
+      }
+#pragma unroll
+      for (int c = 0; c < COUNT; ++c) {
+        if (!in[c] || step != 0) continue;
+        const int of = (int)fdiv((uint32_t)row[c], a.by_group);
+        const int64_t token = seq.first + token0 + of;
+        const int head = piece.y * a.group + row[c] - of * a.group;
+        const float scale = l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+        T* const op = static_cast<T*>(a.c.out) + token * a.c.out_stride[0] + head * a.c.out_stride[1];
+        typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][e] = in_range<T>(o[c][e] * scale);
+        *reinterpret_cast<t4*>(op + 4 * quad[c]) = __builtin_convertvector(o[c], t4);
+        if (a.c.lse && quad[c] == 0) a.c.lse[token * a.c.q_heads + head] = (top[c] + __builtin_amdgcn_logf(l[c])) * kLn2;
+      }
+      if (COUNT == 1 && steps > 1) lds_sync();  // the sums have been read
     }
-    if (steps > 1) lds_sync();  // the sums have been read
-  }
+  };
+  using std::integral_constant;
+  if (share > 256)  // (steps is 1)
+    join(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  else if (parts <= 2 * steps)
+    join(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  else
+    join(integral_constant<int, 1>{}, integral_constant<int, 8>{});
 }
 
 // Joins the parts of row tiles that several ranges share.
