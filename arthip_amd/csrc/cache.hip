@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   const int begin = min(wave * each * 64, n), end = min(begin + each * 64, n);  // the wave's slots
   uint32_t keys[E > 0 ? E : 1];
   int newest = n - 1;
-  constexpr int kOnce = E > 0 && E < 8 ? E : 8;  // loads in flight
+  constexpr int kOnce = E == 4 ? 4 : E == 40 ? 20 : 8;  // 64 slots each whose addresses are known together
   // f(i, the lane's slot), i counting the wave's 64 slots in a row. (What is known of some of them is
   // kept from the others, or their addresses fill the registers.)
   auto each_run = [&](auto f) __attribute__((always_inline)) {
@@ -179,14 +179,18 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
     }
   };
   for (int i = tid; i < 3 * kBins; i += kThreads) bins[0][i] = 0;
-  int places[E > 0 && E <= kOnce ? E : 1];  // short runs' are loaded once
+  // All weights' loads are in flight at once, and positions' where registers hold them (32 key heads of
+  // 32768 slots: 42 us, eight at a time 52).
+  constexpr bool kPlaces = E > 0 && E <= 16;
+  int places[kPlaces ? E : 1];
+  each_run([&](int i, int slot) __attribute__((always_inline)) {
+    const int s = min(slot, n - 1);  // (past the run: the last slot's)
+    keys[i] = __builtin_bit_cast(uint32_t, w[s]);
+    if constexpr (kPlaces) places[i] = place != nullptr ? place[s] : s;
+  });
   if (place != nullptr) {
     int top = INT32_MIN;
-    if constexpr (E > 0 && E <= kOnce) {
-      each_run([&](int i, int slot) __attribute__((always_inline)) {
-        places[i] = place[min(slot, n - 1)];  // (past the run: the last slot's)
-        keys[i] = __builtin_bit_cast(uint32_t, w[min(slot, n - 1)]);
-      });
+    if constexpr (kPlaces) {
       each_run([&](int i, int) __attribute__((always_inline)) { top = max(top, places[i]); });
     } else {
 #pragma unroll 8
@@ -205,10 +209,8 @@ __global__ void __launch_bounds__(kThreads) evict_select(EvictArgs a) {
   };
   each_run([&](int i, int slot) __attribute__((always_inline)) {
     const int s = min(slot, n - 1);
-    if (E <= kOnce && place != nullptr)
-      keys[i] = key(__builtin_bit_cast(float, keys[i]), places[E <= kOnce ? i : 0]);
-    else
-      keys[i] = key(w[s], place != nullptr ? place[s] : s);
+    const int t = kPlaces ? places[kPlaces ? i : 0] : place != nullptr ? place[s] : s;
+    keys[i] = key(__builtin_bit_cast(float, keys[i]), t);
   });
   auto each_slot = [&](auto f) __attribute__((always_inline)) {  // (slot, there is one, its key)
     if constexpr (E > 0) {
@@ -415,7 +417,7 @@ hipError_t launch_cache_evict(const arthip_cache_evict_args& c, hipStream_t s) {
   const int most = std::min(c.keep, std::max(0, c.slots - c.keep));  // moves of a key head
   const bool here = most <= kMovesHere;
   const int each = (c.slots + kThreads - 1) / kThreads;
-  // (32768 slots of 32 key heads, keys in registers and read anew: 57 and 68 us.)
+  // (32768 slots of 32 key heads, keys in registers and read anew: 42 and 68 us.)
   const auto fn = each <= 4    ? select_of<4>(here)
                   : each <= 16 ? select_of<16>(here)
                   : each <= 40 ? select_of<40>(here)
