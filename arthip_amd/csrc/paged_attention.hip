@@ -13,6 +13,12 @@
 // in a row, are cut into equal ranges, one a workgroup; a range may end inside a row tile, whose
 // parts a second kernel joins in a fixed order. Every wave finds its range's beginning from the
 // lengths, a lane (or some) a sequence.
+//
+// Single tokens over long caches are bound by HBM: 16 over up to 16384 keys of 8 heads, 541 MB, 112 us
+// of which the tiles take 104 to 108 (5.0 TB/s). Large calls are bound by products and exponentials, which
+// share a SIMD's two or three waves: a prompt of 8192 with a window of 4096, 32 heads of 128, 444 us
+// (930 TFLOP/s; matrix unit 47%, vector unit 43% busy), a frame of 8160 tokens over 40800, 12 heads of 64,
+// 1199 us (850 TFLOP/s; 45% and 76%).
 
 #include <hip/hip_runtime.h>
 
