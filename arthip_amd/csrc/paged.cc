@@ -199,11 +199,11 @@ std::string check_cache_evict(const arthip_cache_evict_args& a) {
   if (a.keep < 1 || a.keep > kMaxTokens) return at + "keep must be positive";
   if (a.recent < 0 || a.first < 0 || static_cast<int64_t>(a.recent) + a.first > a.keep)
     return at + "recent and first must be positive and add up to keep at most";
-  if (p.batch == 0 || a.slots == 0) return "";
+  if (p.batch == 0) return "";
   if (static_cast<int64_t>(p.batch) * p.k_heads > int64_t{1} << 21) return at + "batch times heads too large";
-  if (a.weights == nullptr) return at + "null weights";
+  if (a.weights == nullptr && a.slots > 0) return at + "null weights";
   if (a.kept == nullptr) return at + "null kept";
-  if (a.positions_out != nullptr && a.positions == nullptr) return at + "positions_out without positions";
+  if (a.positions_out != nullptr && a.positions == nullptr && a.slots > 0) return at + "positions_out without positions";
   for (const void* x : {static_cast<const void*>(a.weights), static_cast<const void*>(a.positions),
                         static_cast<const void*>(a.new_len), static_cast<const void*>(a.weights_out),
                         static_cast<const void*>(a.positions_out), static_cast<const void*>(a.kept)})

@@ -171,6 +171,15 @@ def test_nothing_to_do():
     assert lib.arthip_key_weights(ctypes.byref(_weights(slots=0, out=None, weights=None)), None) == 0
 
 
+def test_evict_without_slots_still_writes():
+    """new_len and kept are written whatever the slots: their buffers have to be there."""
+    call = _lib.lib().arthip_cache_evict
+    _refused(call, _evict(slots=0, weights=None, kept=None), "null kept")
+    _refused(call, _evict(slots=0, kept=BUF + 2), "misaligned")
+    _refused(call, _evict(slots=0, new_len=BUF * 2), "overlap")
+    _refused(call, _evict(slots=0, batch=65536, k_heads=1024), "too large")
+
+
 def test_workspaces():
     """Of sizes alone; none for calls that are refused."""
     lib = _lib.lib()

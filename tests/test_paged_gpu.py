@@ -174,6 +174,37 @@ def test_attention(dtype, hq, hk, d, page, seqs, kw):
     _attend(c, c.normal(sum(c.n), hq, d), **kw)
 
 
+@pytest.mark.parametrize("dtype,hq,hk,d,page,seqs,kw", [
+    (F16, 12, 4, 72, 16, [(2001, 2500)], {}),                                  # rows and quads of no eight
+    (BF16, 4, 2, 96, 32, [(1500, 1500), (33, 700)], {}),                       # of eight, and not, in one call
+    (BF16, 8, 1, 128, 64, [(700, 6000)], {"cap": 20.0}),
+    (F16, 3, 3, 40, 16, [(900, 1900), (1, 5000)], {"causal": False}),
+    (F16, 2, 2, 256, 16, [(800, 1700)], {"left": 600}),
+])
+def test_attention_of_row_tiles_that_many_ranges_share(dtype, hq, hk, d, page, seqs, kw):
+    c = Cache(seqs, hk, d, dtype, page)
+    _attend(c, c.normal(sum(c.n), hq, d), **kw)
+
+
+def test_attention_counts_alike_for_long_page_tables():
+    """Sequences of few pages in a table of 2^20 slots, whose counts are of 64 bits: the same bits."""
+    c = Cache([(40, 900), (1, 300), (17, 17), (0, 50)], 16, 64, F16)
+    q = c.normal(sum(c.n), 64, 64).cuda()
+    k, v, pages, kv_len, offsets = c.cuda()
+    table = torch.full((4, 65536), -1, dtype=torch.int32, device="cuda")
+    table[:, :pages.shape[1]] = pages
+    want = paged.paged_attention(q, k, v, pages, kv_len, offsets, return_lse=True)
+    got = paged.paged_attention(q, k, v, table, kv_len, offsets, return_lse=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_evict_without_slots():
+    c = Cache([(1, 20), (0, 0)], 2, 64, F16)
+    k, v, pages, kv_len, _ = c.cuda()
+    new_len, weights, kept, _ = paged.cache_evict(k, v, pages, kv_len, torch.empty(2, 2, 0).cuda(), 5)
+    assert (new_len == 0).all() and weights.shape == (2, 2, 0) and (kept == -1).all()
+
+
 def test_attention_without_offsets_and_heads_first():
     c = Cache([(1, 70), (1, 4), (1, 300)], 2, 64, F16, heads_first=True)
     q = c.normal(3, 6, 64)
