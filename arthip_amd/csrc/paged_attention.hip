@@ -332,6 +332,9 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   // A wave at its exponentials goes before one at its products where the vector unit has more to do
   // (heads of 64, 8160 over 40800: 1265 -> 1203 us; capped heads of 128 110 -> 106; plain ones 454 -> 472).
   constexpr bool kFirst = DP <= 64 || SHAPE != kPlain;
+  // Two tiles a round of the walk: the next tile's scores need no copies (that frame 1212 -> 1169 us, prompts
+  // beside single tokens 450 -> 438, in bf16 428 -> 414; one prompt 454 -> 452).
+  constexpr int kRound = NW == 4 && DP <= 128 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   constexpr int v_at = 2 * L::kTile;  // V's buffers
@@ -525,7 +528,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     };
 
     // -- the products --------------------------------------------------------------------
-    f16v s[KB];  // scores of a tile, key block by key block
+    f16v s[kRound][KB];  // scores of a tile (and of the next), key block by key block
+    int u = 0;           // which
     auto scores = [&](int buf, f16v (&x)[KB]) __attribute__((always_inline)) {
       lds_byte* const from = lds0 + buf * L::kTile;
 #pragma unroll
@@ -561,7 +565,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[kb][r]));
+            for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(s[u][kb][r]));
         }
         if (SHAPE == kCap && !__any(!(far <= a.cap.reach))) {
           // Small scores: six plain operations where the exponential and the reciprocal take a
@@ -569,7 +573,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][r] = cap_near(a.cap, s[kb][r]);
+            for (int r = 0; r < 16; ++r) s[u][kb][r] = cap_near(a.cap, s[u][kb][r]);
         } else {
           // Off by some 2^-22 of the cap; large caps choose score by score.
           const float in = a.cap.in, out = a.cap.out;
@@ -577,10 +581,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const float x = s[kb][r];
+              const float x = s[u][kb][r];
               const float e = __builtin_amdgcn_exp2f(x * in);
               const float y = __builtin_fmaf(-2.0f * out, __builtin_amdgcn_rcpf(e + 1.0f), out);
-              s[kb][r] = SHAPE == kAny && fabsf(x) <= a.cap.reach ? cap_near(a.cap, x) : y;
+              s[u][kb][r] = SHAPE == kAny && fabsf(x) <= a.cap.reach ? cap_near(a.cap, x) : y;
             }
         }
       } else if constexpr (SHAPE == kAny) {
@@ -588,7 +592,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] *= unit;
+          for (int r = 0; r < 16; ++r) s[u][kb][r] *= unit;
       }
       if (partial) {
 #pragma unroll
@@ -596,16 +600,16 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int key = key0 + 32 * kb + 8 * (r / 4) + r % 4;
-            s[kb][r] = key >= lo && key < hi ? s[kb][r] : -__builtin_inff();
+            s[u][kb][r] = key >= lo && key < hi ? s[u][kb][r] : -__builtin_inff();
           }
       }
     };
     auto largest = [&]() __attribute__((always_inline)) {
-      float top = s[0][0];
+      float top = s[u][0][0];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][kb][r]);
       return halves_max(top);
     };
     // A row's base is a score near its largest so far; this makes it the largest. Where that has not
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     };
     // The weights of the scores against a row's base, packed; their sum.
     auto weight = [&](int e, float base, float& sum, float (&w)[8], frag (&p)[KT / 16]) __attribute__((always_inline)) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 16][e % 16], mul, -base));
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e / 16][e % 16], mul, -base));
       sum += x;
       w[e % 8] = x;
       if (e % 8 == 7) {
@@ -655,65 +659,69 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
       vm_wait();
       settle(then, begin + 2);
       lds_sync();
-      if (w_real) scores(0, s);
+      if (w_real) scores(0, s[0]);
       lds_sync();  // K's first buffer has been used
-      for (int t = begin; t < end; ++t) {
-        const int buf = (t - begin) & 1, k0 = t * KT;
-        if (t + 2 < end) stage_k(buf, t + 2, then);
-        if (t + 1 < end) stage_v(buf ^ 1, t + 1, next);
-        next = then;
-        ask(then, min(t + 3, end - 1));
-        if (w_real) {
-          ready(k0, !(k0 >= w_lo_max && k0 + KT <= w_hi_min));
-          if constexpr (!kLazy) {
-            if (__any((largest() - m) * mul > 8.0f)) follow();
-          }
-          // fp16's weights are raised to the top of its range, so that small ones, of which a long
-          // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
-          float base = (!kLazy && m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
-          f16v following[KB];
-          frag p[KT / 16];
-          float w[8], sum = 0.0f;
-          if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
-          {
-            // A product, the operand of the fourth after it, and its share of the exponentials.
-            constexpr int N = KS * KB, A = N < 4 ? N : 4;
-            lds_byte* const from = lds0 + (buf ^ 1) * L::kTile;
-            frag k[N];
-            auto read = [&](int i) __attribute__((always_inline)) {
-              k[i] = *(lds_frag*)(from + (k_lane ^ (i / KB * 32)) + i % KB * 32 * RB);
-            };
+      for (int t0 = begin; t0 < end; t0 += kRound) {
 #pragma unroll
-            for (int i = 0; i < A; ++i) read(i);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              following[i % KB] = E::mma(k[i], q[i / KB], i < KB ? f16v{} : following[i % KB]);
-              if (i + A < N) read(i + A);
-#pragma unroll
-              for (int e = i * 16 * KB / N; e < (i + 1) * 16 * KB / N; ++e) weight(e, base, sum, w, p);
-              __builtin_amdgcn_sched_barrier(0);
+        for (u = 0; u < kRound; ++u) {
+          const int t = t0 + u, buf = kRound > 1 ? u : (t - begin) & 1, k0 = t * KT;
+          if (u > 0 && t >= end) break;
+          if (t + 2 < end) stage_k(buf, t + 2, then);
+          if (t + 1 < end) stage_v(buf ^ 1, t + 1, next);
+          next = then;
+          ask(then, min(t + 3, end - 1));
+          if (w_real) {
+            ready(k0, !(k0 >= w_lo_max && k0 + KT <= w_hi_min));
+            if constexpr (!kLazy) {
+              if (__any((largest() - m) * mul > 8.0f)) follow();
             }
-          }
-          if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
-          if (kLazy && __any(!(sum <= E::kMost))) {
-            follow();
-            base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
-            sum = 0.0f;
+            // fp16's weights are raised to the top of its range, so that small ones, of which a long
+            // walk adds up many, keep their digits down to 2^-21 of a row's largest and are 0 below 2^-32.
+            float base = (!kLazy && m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+            f16v following[KB];
+            frag p[KT / 16];
+            float w[8], sum = 0.0f;
+            if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
+            {
+              // A product, the operand of the fourth after it, and its share of the exponentials.
+              constexpr int N = KS * KB, A = N < 4 ? N : 4;
+              lds_byte* const from = lds0 + (buf ^ 1) * L::kTile;
+              frag k[N];
+              auto read = [&](int i) __attribute__((always_inline)) {
+                k[i] = *(lds_frag*)(from + (k_lane ^ (i / KB * 32)) + i % KB * 32 * RB);
+              };
 #pragma unroll
-            for (int e = 0; e < 16 * KB; ++e) {
-              weight(e, base, sum, w, p);
-              if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // or registers run out
+              for (int i = 0; i < A; ++i) read(i);
+#pragma unroll
+              for (int i = 0; i < N; ++i) {
+                following[i % KB] = E::mma(k[i], q[i / KB], i < KB ? f16v{} : following[i % KB]);
+                if (i + A < N) read(i + A);
+#pragma unroll
+                for (int e = i * 16 * KB / N; e < (i + 1) * 16 * KB / N; ++e) weight(e, base, sum, w, p);
+                __builtin_amdgcn_sched_barrier(0);
+              }
             }
-          }
-          l += sum;  // this half's keys; the halves are added at the end
-          values(buf, p);
-          ahead<KT / 16 * DB, 2>();
+            if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
+            if (kLazy && __any(!(sum <= E::kMost))) {
+              follow();
+              base = (m == -__builtin_inff() ? 0.0f : m * mul) - E::kRaise;
+              sum = 0.0f;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) s[kb] = following[kb];
+              for (int e = 0; e < 16 * KB; ++e) {
+                weight(e, base, sum, w, p);
+                if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // or registers run out
+              }
+            }
+            l += sum;  // this half's keys; the halves are added at the end
+            values(buf, p);
+            ahead<KT / 16 * DB, 2>();
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kRound - 1 - u][kb] = following[kb];
+          }
+          vm_wait();
+          settle(then, t + 3);
+          lds_sync();
         }
-        vm_wait();
-        settle(then, t + 3);
-        lds_sync();
       }
     }
 
