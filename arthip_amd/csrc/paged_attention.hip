@@ -14,11 +14,11 @@
 // parts a second kernel joins in a fixed order. Every wave finds its range's beginning from the
 // lengths, a lane (or some) a sequence.
 //
-// Single tokens over long caches are bound by HBM: 16 over up to 16384 keys of 8 heads, 541 MB, 112 us
-// of which the tiles take 104 to 108 (5.0 TB/s). Large calls are bound by products and exponentials, which
-// share a SIMD's two or three waves: a prompt of 8192 with a window of 4096, 32 heads of 128, 444 us
-// (930 TFLOP/s; matrix unit 47%, vector unit 43% busy), a frame of 8160 tokens over 40800, 12 heads of 64,
-// 1199 us (850 TFLOP/s; 45% and 76%).
+// Single tokens over long caches are bound by HBM: 16 over up to 16384 keys of 8 heads, 541 MB, 109 to 112
+// us, of which the tiles take 102 to 108 (5.2 TB/s). Large calls are bound by products and exponentials, which
+// share a SIMD's two or three waves: a prompt of 8192 with a window of 4096, 32 heads of 128, 449 us
+// (918 TFLOP/s; matrix unit 48%, vector unit 40% busy), a frame of 8160 tokens over 40800, 12 heads of 64,
+// 1179 us (867 TFLOP/s; 48% and 75%).
 
 #include <hip/hip_runtime.h>
 
@@ -528,8 +528,8 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
     };
 
     // -- the products --------------------------------------------------------------------
-    f16v s[kRound][KB];  // scores of a tile (and of the next), key block by key block
-    int u = 0;           // which
+    f16v s[kRound][KB];  // scores of a tile, and of the next, key block by key block
+    int u = 0;           // the tile's
     auto scores = [&](int buf, f16v (&x)[KB]) __attribute__((always_inline)) {
       lds_byte* const from = lds0 + buf * L::kTile;
 #pragma unroll
