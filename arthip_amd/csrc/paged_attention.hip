@@ -333,8 +333,10 @@ __global__ void __launch_bounds__(NW * 64, DP > 128 ? 1 : DP > 64 || (DP > 32 &&
   // (heads of 64, 8160 over 40800: 1265 -> 1203 us; capped heads of 128 110 -> 106; plain ones 454 -> 472).
   constexpr bool kFirst = DP <= 64 || SHAPE != kPlain;
   // Two tiles a round of the walk: the next tile's scores need no copies (that frame 1212 -> 1169 us, prompts
-  // beside single tokens 450 -> 438, in bf16 428 -> 414; one prompt 454 -> 452).
-  constexpr int kRound = NW == 4 && DP <= 128 ? 2 : 1;
+  // beside single tokens 450 -> 438, in bf16 428 -> 414; one prompt 454 -> 452). Capped heads of 33 to 64 have
+  // no registers for it: spilled ones in the walk cost more (4096 tokens, 16 heads of 64: two tiles 101 us,
+  // one 90; 256 over 32765 keys 89 and 77; 8160 over 16320 without a mask 763 and 671).
+  constexpr int kRound = NW == 4 && DP <= 128 && !(SHAPE == kCap && DP == 64) ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   constexpr int v_at = 2 * L::kTile;  // V's buffers
