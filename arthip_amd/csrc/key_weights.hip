@@ -48,7 +48,7 @@ struct KeyArgs {
 };
 
 constexpr int kRows = 64;  // of a tile
-constexpr int kStarts = 4 * kRows * 4;  // bytes of their exponents' starts in LDS
+constexpr int kStarts = 4 * (kRows + 32) * 4;  // bytes of their exponents' starts in LDS
 constexpr int kItems = 2048;    // workgroups that many rows are divided into (1024: 284 us for 268 below)
 constexpr int kStreams = 5120;  // and waves that few rows are (2560, 10240: 78 and 76 us for 73.5)
 
@@ -114,6 +114,53 @@ __device__ __forceinline__ float start_of(const KeyArgs& a, const Sequence& s, i
   return lse == -__builtin_inff() ? lse : -lse * kLog2e;
 }
 
+// The sum of a lane's slot over the rows [from, to), by a wave from memory. A row whose start is -inf adds
+// nothing, whatever it and the key hold, but a score that is not finite takes its weight to NaN: the
+// kernels below find sums that became NaN once more by this, which leaves such rows out. (Asked
+// of every block of rows there, it took the 2000-token pieces from 307 to 324 us.)
+__device__ __forceinline__ void lds_wave() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <class T, int DP, Shape SHAPE>
+__device__ __forceinline__ float apart(const KeyArgs& a, const Sequence& seq, int b, int head, int slot, int k1, int from,
+                                       int to, float mul, float* starts) {
+  using E = Elem<T>;
+  using frag = typename E::frag;
+  constexpr int KS = DP / 16;
+  const arthip_pages& pg = a.c.p;
+  const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+  Rows mine = rows_of(a, seq, slot);
+  if (slot >= k1) mine.hi = 0;
+  const int64_t at = slot < k1 ? row_of(pg, a.by_page, pg.pages + b * pg.pages_stride, slot, a.c.k_cache_stride) : -1;
+  const T* const key = static_cast<const T*>(a.c.k_cache) + at + head * a.c.k_cache_stride[2];
+  float sum = 0.0f;
+  for (int row0 = from; row0 < to; row0 += 32) {
+    const int row = min(row0 + n, to - 1);
+    const int token = (int)fdiv((uint32_t)row, a.by_group), g = row - token * a.group;
+    const T* const query = static_cast<const T*>(a.c.q) + (int64_t)(seq.first + token) * a.c.q_stride[0] +
+                           (int64_t)(head * a.group + g) * a.c.q_stride[1];
+    f16v s[1] = {f16v{}};
+#pragma unroll 1
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + half * 8;
+      const bool in = d < pg.head_dim;
+      s[0] = E::mma(in ? *reinterpret_cast<const frag*>(query + d) : frag{},
+                    in && at != -1 ? *reinterpret_cast<const frag*>(key + d) : frag{}, s[0]);
+    }
+    transform<SHAPE>(a, s);
+    const float start = start_of(a, seq, head, row0 + n, to);
+    lds_wave();  // the last rows' have been read
+    if (half == 0) starts[n] = start;
+    lds_wave();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int of = 8 * (r / 4) + 4 * half + r % 4;
+      const float base = starts[of], w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], mul, base));
+      sum += row0 + of >= mine.lo && row0 + of < mine.hi && base != -__builtin_inff() ? w : 0.0f;
+    }
+  }
+  return halves_sum(sum);
+}
+
 template <class T, int DP, int KB, Shape SHAPE>  // KB: blocks of 32 keys a wave
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) key_tile(KeyArgs a) {
   using L = TileL<DP, kRows>;
@@ -125,6 +172,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) key_tile(KeyArgs a) {
   constexpr uint32_t kOob = 0x80000000u;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ __attribute__((aligned(16))) float starts[4][kRows];
+  __shared__ float apart_starts[4][32];
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   const arthip_pages& pg = a.c.p;
@@ -314,9 +362,23 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) key_tile(KeyArgs a) {
   }
 
   // -- results -------------------------------------------------------------------------------
+  bool odd_sum = false;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    const float x = halves_sum(sum[kb]);
+    sum[kb] = halves_sum(sum[kb]);
+    odd_sum = odd_sum || sum[kb] != sum[kb];
+  }
+  if (__builtin_expect(__any(odd_sum), 0)) {
+    for (int kb = 0; kb < KB; ++kb) {
+      const float x = apart<T, DP, SHAPE>(a, seq, b, head, w0 + 32 * kb + n, k1, row0 + first * kRows,
+                                          min(row0 + last * kRows, row_end), mul, apart_starts[wave]);
+#pragma unroll
+      for (int i = 0; i < KB; ++i) sum[i] = i == kb ? x : sum[i];
+    }
+  }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const float x = sum[kb];
     const int slot = w0 + 32 * kb + n;
     if (half != 0 || slot >= a.c.slots) continue;
     if (a.splits > 1) {
@@ -405,6 +467,7 @@ __global__ void __launch_bounds__(64) key_stream(KeyArgs a) {
     const uint32_t k_lane = n * RB + (half ^ L::k_swizzle(n)) * 16;
     const float mul = SHAPE != kPlain ? 1.0f : a.c.scale * kLog2e;
 
+    uint64_t odd_sums = 0;
     for (int from = row0; from < row_end; from += 32) {
       // The rows: as the left operand in registers, what their exponents start from by way of LDS.
       frag q[KS];
@@ -456,10 +519,18 @@ __global__ void __launch_bounds__(64) key_stream(KeyArgs a) {
           x += i >= seen.lo && i < seen.hi ? w : 0.0f;
         }
         x = halves_sum(x);
+        odd_sums |= __ballot(x != x);
         if (half == 0) sums[t * 32 + n] = from == row0 ? x : sums[t * 32 + n] + x;
       }
     }
     lds_sync();
+    if (__builtin_expect(odd_sums != 0, 0)) {
+      for (int t = 0; t < tiles; ++t) {
+        const float x = apart<T, DP, SHAPE>(a, seq, b, head, k0 + t * 32 + n, k1, row0, row_end, mul, starts);
+        if (half == 0) sums[t * 32 + n] = x;
+      }
+      lds_sync();
+    }
   }
   float* const out = a.c.out + b * a.c.out_stride[0] + head * a.c.out_stride[1];
   for (int slot = k0 + lane; slot < k_end; slot += 64)

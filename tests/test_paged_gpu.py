@@ -410,6 +410,30 @@ def test_weights_of_tokens_that_saw_nothing():
     assert abs(float(got.sum()) - 8) < 1e-5 and (got[0, 0, 4:] == 0).all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype,hq,d,n,lk,cap", [
+    (F16, 2, 64, 300, 500, 0.0), (BF16, 4, 128, 300, 500, 0.0), (BF16, 1, 256, 300, 300, 30.0), (F16, 3, 40, 200, 333, 100.0),
+    (F16, 2, 64, 3, 500, 0.0), (BF16, 4, 128, 7, 500, 30.0), (F16, 8, 256, 4, 90, 0.0),
+])
+def test_weights_of_tokens_without_a_sum_are_nothing_whatever_they_hold(dtype, hq, d, n, lk, cap, bad):
+    """A lse of -inf leaves a token's query out, also one that is not finite, in the middle of others and
+    at their end, and keys that are not finite which no one else sees."""
+    c = Cache([(n, lk)], 1, d, dtype)
+    q = c.normal(n, hq, d)
+    lse = pref.attention(c, q, cap=cap)[1][0].float()
+    out = [0, n // 2, n - 1] if n > 3 else [1, n - 1]
+    lse[out] = -math.inf
+    q[out] = 0
+    old = torch.rand(1, 1, lk + 9, generator=c.g)
+    c.k[int(c.table[0, (lk - 1) // 16]), (lk - 1) % 16] = 0  # seen by the last token alone
+    want = pref.weights(c, q, lse, old, cap=cap)
+    q[out] = bad
+    c.k[int(c.table[0, (lk - 1) // 16]), (lk - 1) % 16] = bad
+    k, _, pages, kv_len, offsets = c.cuda()
+    got = paged.key_weights(q.cuda(), k, pages, kv_len, offsets, lse.cuda(), old.cuda(), cap=cap)
+    ref.check(got, want, "weights")
+
+
 # -- eviction --------------------------------------------------------------------------------
 
 EVICT = [
