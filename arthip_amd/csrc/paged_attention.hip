@@ -959,9 +959,10 @@ __device__ void join_one(const PagedArgs& a, int job, int index, int wide, f4* s
         const float f = __builtin_amdgcn_exp2f(top[c] - base), w = __builtin_amdgcn_exp2f(st.x - base);
         top[c] = next;
         l[c] = l[c] * f + st.y * w;
-        // (A part that weighs nothing beside another is left out, whatever it holds.)
+        // (A part that weighs nothing beside another has a factor of 0, which infinities and NaN survive, as they
+        // do in the walk: its rows see them. Parts that hold some of what a row does not see are not joined.)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[c][e] = (f != 0.0f ? o[c][e] * f : 0.0f) + (w != 0.0f ? x[e] * w : 0.0f);
+        for (int e = 0; e < 4; ++e) o[c][e] = o[c][e] * f + x[e] * w;
       };
       if (step < steps) {
         for (int s0 = step; s0 < parts; s0 += ONCE * steps) {

@@ -290,6 +290,26 @@ def test_attention_means_of_the_largest_numbers(dtype):
     assert (out.float() / top - 1).abs().max() <= 2 * ref.UNIT[dtype]
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("depth", [20.0, 200.0])
+@pytest.mark.parametrize("dtype,d,n,lk", [(F16, 64, 1, 5000), (BF16, 128, 1, 5000), (BF16, 64, 100, 6000),
+                                          (F16, 128, 100, 6000)])
+def test_attention_seen_values_of_small_weight(dtype, d, n, lk, depth, bad):
+    """A value that is not finite reaches the rows that see it also where its weight rounds to 0 beside
+    the others', in its own range of keys or when the ranges are joined."""
+    for first, last in ((70, 70), (0, 3000)):  # keys that weigh e^-depth of the others
+        c = Cache([(n, lk)], 1, d, dtype)
+        q = c.normal(n, 4, d)
+        q[..., 0] = 1
+        for slot in range(lk):
+            c.k[int(c.table[0, slot // 16]), slot % 16, 0, 0] = -depth if first <= slot <= last else 0.0
+        c.v[int(c.table[0, 4]), 6, 0, 5] = bad  # slot 70
+        k, v, pages, kv_len, offsets = c.cuda()
+        out = paged.paged_attention(q.cuda(), k, v, pages, kv_len, offsets, scale=1.0)
+        assert not torch.isfinite(out[..., 5]).any(), last
+        assert torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 6:]).all(), last
+
+
 def test_attention_sequences_that_share_pages():
     """A common beginning lies in the cache once."""
     c = Cache([(3, 70), (1, 66)], 2, 64, F16)
