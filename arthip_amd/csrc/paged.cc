@@ -172,8 +172,9 @@ std::string check_key_weights(const arthip_key_weights_args& a) {
     if (!aligned(a.q, 16)) return at + "q must be aligned to 16 bytes";
     if (!multiples(a.q_stride, 2)) return at + "strides must be multiples of 8 elements";
     for (int i = 0; i < 2; ++i)
-      if (a.q_stride[i] < 0 || a.q_stride[i] > kMaxSlotStride) return at + "strides of q must be from 0 to 2^24";
-    // A tile's queries lie within 31 bits of its first.
+      if (a.q_stride[i] < 0 || a.q_stride[i] > kMaxTokens) return at + "strides of q must be from 0 to 2^30";
+    // A tile's queries, 64 rows of (token, head), lie within 31 bits of bytes of its first; one stride of
+    // each kind is room for a buffer's beginning before the rows.
     const int64_t group = a.q_heads / p.k_heads;
     if ((64 / group + 2) * a.q_stride[0] + group * a.q_stride[1] >= int64_t{1} << 30)
       return at + "queries too far apart";

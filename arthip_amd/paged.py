@@ -195,8 +195,9 @@ def key_weights(q, k_cache, pages, kv_len, q_offsets, lse, weights, *, decay: fl
                 cap: float = 0.0, causal: bool = True, left: int | None = None, out=None, workspace=None, stream=None):
     """decay * weights + the attention weight that the new tokens give each cached key,
     summed over the query heads of its key head, fp32 [B, Hk, slots]; see
-    arthip_key_weights. ``lse`` is paged_attention's, of the same queries and options.
-    out=weights adds in place."""
+    arthip_key_weights. ``lse`` is paged_attention's, of the same queries and options; queries
+    whose strides reach past 2^30 values in 64 rows (token, head) are refused. out=weights
+    adds in place."""
     scores = _scores("key_weights", scale, cap, causal, left)
     decay = _float("key_weights: decay", decay)
     key = ("weights", _sig(q), _sig(k_cache), _sig(pages), _sig(kv_len), _sig(q_offsets), _sig(lse), _sig(weights),

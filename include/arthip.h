@@ -664,7 +664,8 @@ typedef struct arthip_key_weights_args {
   float* out;               /* may be weights with its strides (in place) */
   void* workspace;          /* arthip_key_weights_workspace bytes */
   uint64_t workspace_bytes;
-  int64_t q_stride[2];      /* token, head: from 0 to 2^24 */
+  int64_t q_stride[2];      /* token, head: from 0 on; with g = q_heads / k_heads,
+                             * (64 / g + 2) token + g head is below 2^30 */
   int64_t k_cache_stride[3];
   int64_t weights_stride[2];  /* sequence, head; slots are contiguous */
   int64_t out_stride[2];

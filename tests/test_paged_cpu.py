@@ -237,3 +237,13 @@ def test_structs_have_the_headers_sizes(tmp_path):
         t = getattr(_lib, py)
         want = [getattr(t, f).offset for f, *_ in t._fields_] + [ctypes.sizeof(t)]
         assert [int(x) for x in line.split()] == want, py
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(q_stride=(256, -64)), "strides of q"), (dict(q_stride=(2 ** 30 + 8, 64)), "strides of q"),
+    (dict(q_stride=(256, 2 ** 62)), "strides of q"), (dict(q_stride=(64, 2 ** 29)), "too far apart"),
+    (dict(q_stride=(2 ** 25, 64)), "too far apart"),
+])
+def test_weights_refuse_queries_past_32_bits(change, text):
+    """34 tokens and two heads apart at most, as two query heads share a key head."""
+    _refused(_lib.lib().arthip_key_weights, _weights(**change), text)

@@ -454,6 +454,48 @@ def test_weights_of_tokens_without_a_sum_are_nothing_whatever_they_hold(dtype, h
     ref.check(got, want, "weights")
 
 
+@pytest.mark.parametrize("group,n", [(1, 40), (4, 70), (8, 3)])
+def test_weights_of_queries_that_lie_far_apart(group, n):
+    """Queries kept heads first, a head 2^24 values and more after the one before, and tokens as far
+    apart: what paged_attention takes."""
+    c = Cache([(n, 200)], 1, 64, F16)
+    q = c.normal(n, group, 64)
+    want = _weigh(c, group, 210, q=q)
+    k, v, pages, kv_len, offsets = c.cuda()
+    far = 2 ** 24 + 64
+    heads = torch.zeros(group * far, dtype=F16, device="cuda").as_strided((n, group, 64), (64, far, 1))
+    tokens = torch.zeros(min(n, 5) * far, dtype=F16, device="cuda").as_strided((min(n, 5), group, 64), (far, 64, 1))
+    g = torch.Generator().manual_seed(0)
+    old = torch.rand(1, 1, 210, generator=g).cuda()
+    lse = paged.paged_attention(q.cuda(), k, v, pages, kv_len, offsets, return_lse=True)[1]
+    heads.copy_(q)
+    a = paged.key_weights(heads, k, pages, kv_len, offsets, lse, old)
+    assert torch.equal(a, paged.key_weights(q.cuda(), k, pages, kv_len, offsets, lse, old))
+    assert torch.equal(paged.paged_attention(heads, k, v, pages, kv_len, offsets),
+                       paged.paged_attention(q.cuda(), k, v, pages, kv_len, offsets))
+    if group >= 4:
+        few = torch.tensor([0, len(tokens)], dtype=torch.int32).cuda()
+        tokens.copy_(q[:len(tokens)])
+        b = paged.key_weights(tokens, k, pages, kv_len, few, lse[:len(tokens)], old)
+        assert torch.equal(b, paged.key_weights(q[:len(tokens)].cuda(), k, pages, kv_len, few, lse[:len(tokens)], old))
+
+
+@pytest.mark.parametrize("group,token,head", [(2, 64, 2 ** 29 - 2176), (8, 107374080, 64), (3, 192, 2 ** 28 - 24 * 192)])
+def test_weights_of_queries_as_far_apart_as_they_may_be(group, token, head):
+    """Strides just below the limit, from memory of up to 2 GiB: (64 / group + 2) token + group head < 2^30."""
+    n = 10 if token > 2 ** 20 else 70
+    c = Cache([(n, 100)], 1, 64, BF16)
+    q = c.normal(n, group, 64).cuda()
+    k, v, pages, kv_len, offsets = c.cuda()
+    far = torch.empty((n - 1) * token + (group - 1) * head + 64, dtype=BF16, device="cuda")
+    far = far.as_strided((n, group, 64), (token, head, 1))
+    far.copy_(q)
+    lse = paged.paged_attention(q, k, v, pages, kv_len, offsets, return_lse=True)[1]
+    old = torch.zeros(1, 1, 100).cuda()
+    assert torch.equal(paged.key_weights(far, k, pages, kv_len, offsets, lse, old),
+                       paged.key_weights(q, k, pages, kv_len, offsets, lse, old))
+
+
 # -- eviction --------------------------------------------------------------------------------
 
 EVICT = [
