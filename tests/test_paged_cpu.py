@@ -247,3 +247,22 @@ def test_structs_have_the_headers_sizes(tmp_path):
 def test_weights_refuse_queries_past_32_bits(change, text):
     """34 tokens and two heads apart at most, as two query heads share a key head."""
     _refused(_lib.lib().arthip_key_weights, _weights(**change), text)
+
+
+def test_the_key_weights_plan(tmp_path):
+    """key_weights_plan, host code of the built library (tests/key_weights_plan.cc)."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    gxx = shutil.which("g++")
+    if gxx is None or not Path("/opt/rocm/include/hip/hip_runtime.h").exists():
+        pytest.skip("g++ or the HIP headers are not available")
+    _lib.lib()
+    here = Path(__file__).resolve().parent
+    exe = tmp_path / "key_weights_plan"
+    subprocess.run([gxx, "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I",
+                    str(here.parent / "arthip_amd" / "csrc"), str(here / "key_weights_plan.cc"), str(_lib.LIB_PATH),
+                    f"-Wl,-rpath,{_lib.LIB_PATH.parent}", "-L/opt/rocm/lib", "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)],
+                   check=True, capture_output=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr

@@ -566,6 +566,66 @@ def test_evict_positions_at_the_ends_of_their_type():
            recent=5)
 
 
+# Caches longer than the registers of the selecting workgroup hold (40960 slots: all of EVICT's are
+# shorter), whose weights are read anew in every pass; more than the 8192 moves that are listed at once; rows moved by the
+# selecting workgroup itself or by a kernel of their own.
+EVICT_LONG = [
+    (1, 8, 64, [41500, 70], 41500, 11700, 100, 3, True),   # read anew, two lists of moves
+    (1, 8, 128, [50001], 50001, 3000, 0, 0, False),        # the same without positions, one list
+    (2, 8, 64, [41100, 41050], 41100, 200, 10, 0, True),   # read anew, few moves
+    (1, 8, 64, [40960, 399], 40960, 11700, 0, 5, False),   # in registers, two lists
+    (1, 16, 64, [20000], 20100, 250, 50, 0, True),         # in registers, few moves
+    (2, 8, 16, [3000, 4000], 4096, 1500, 9, 2, True),      # four slots a lane, a kernel of their own
+]
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("hk,d,page,lens,slots,keep,recent,first,placed", EVICT_LONG)
+def test_evict_long_caches(hk, d, page, lens, slots, keep, recent, first, placed, ties):
+    c = Cache([(0, n) for n in lens], hk, d, F16, page)
+    weights = torch.rand(len(lens), hk, slots, generator=c.g)
+    if ties:
+        weights = (weights * 4).floor() - 1
+    positions = None
+    if placed:
+        positions = torch.stack([torch.randperm(3 * slots, generator=c.g)[:slots] for _ in range(len(lens) * hk)])
+        positions = positions.reshape(len(lens), hk, slots).to(torch.int32)
+    _evict(c, weights, keep, positions, recent=recent, first=first)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d,kw", [(32, {}), (64, {"cap": 30.0}), (96, {}), (128, {"left": 300}), (256, {}),
+                                  (72, {"cap": 100.0}), (128, {"causal": False})])
+def test_weights_of_few_rows_over_a_ring_of_tiles(dtype, d, kw):
+    """Workgroups of six tiles of 32 keys each (more than the ring has): lengths that end in the middle
+    of one, a page outside the pool, a sequence with more than 32 rows beside short ones."""
+    seqs = [(1, 5120), (40, 900), (1, 3777), (0, 700), (1, 1), (3, 2500)]
+    c = Cache(seqs, 32, d, dtype)
+    c.table[1, 5], c.table[2, 100] = -1, 2 ** 30
+    _weigh(c, 64 if d < 128 else 32, 5120, 0.9, **kw)
+
+
+MANY = [
+    # More sequences than the kernel that counts their tiles takes at once, none of which has new
+    # tokens where it goes on to the next.
+    (F16, 2, 1, 8, [(0 if 1000 <= i < 1060 else i % 3, 5 + i % 4) for i in range(1300)], {}),
+    (BF16, 4, 2, 16, [(1, 1 + i % 20) for i in range(1025)], {"cap": 30.0}),
+    # So many that they are looked for in three steps.
+    (F16, 1, 1, 8, [(1 if i % 5 else 0, 1 + i % 3) for i in range(4100)], {}),
+    # One with more row tiles than lanes: of a wave's rows, and of four waves'.
+    (F16, 32, 1, 32, [(1, 9 + i) for i in range(30)] + [(0, 3)] * 69 + [(70, 200)] + [(1, 20)] * 30, {}),
+    (BF16, 32, 1, 64, [(0, 3)] * 30 + [(300, 333)] + [(3, 20)] * 40, {"left": 60}),
+]
+
+
+@pytest.mark.parametrize("dtype,hq,hk,d,seqs,kw", MANY)
+def test_attention_and_weights_of_many_sequences(dtype, hq, hk, d, seqs, kw):
+    c = Cache(seqs, hk, d, dtype, spare=1, room=0)
+    q = c.normal(sum(c.n), hq, d)
+    _attend(c, q, **kw)
+    _weigh(c, hq, max(c.len), q=q, **kw)
+
+
 # -- together --------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,cap", [(F16, 0.0), (BF16, 30.0)])
