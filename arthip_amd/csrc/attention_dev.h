@@ -71,7 +71,10 @@ template <>
 struct Elem<_Float16> {
   typedef h8 frag;
   static constexpr float kZero = 0x1p-25f;  // numbers of 0 and more up to here round to 0
-  static constexpr float kRaise = 7.0f;     // weights are up to 2^(8 + 7), see weights()
+  // The power of 2 that weights are raised by, so that small ones, of which a long walk adds up many, keep
+  // their digits: those of a row's base are 2^7, and as a base is kept up to 2^8 below the row's largest
+  // score, weights are up to 2^15.
+  static constexpr float kRaise = 7.0f;
   static constexpr float kMost = 0x1p+15f;  // sum of weights that each are numbers of the type
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

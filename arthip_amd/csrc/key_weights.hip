@@ -40,7 +40,6 @@ struct KeyArgs {
   int group;   // query heads of a key head
   int tiles;   // workgroups along the slots
   int splits;  // and along the rows
-  int items;   // all workgroups
   int stream;  // slots of a workgroup with few rows
   FastDiv by_group, by_page, by_heads, by_tiles, by_splits;
   CapFit cap;
@@ -49,8 +48,11 @@ struct KeyArgs {
 
 constexpr int kRows = 64;  // of a tile
 constexpr int kStarts = 4 * (kRows + 32) * 4;  // bytes of their exponents' starts in LDS
-constexpr int kItems = 2048;    // workgroups that many rows are divided into (1024: 284 us for 268 below)
-constexpr int kStreams = 5120;  // and waves that few rows are (2560, 10240: 78 and 76 us for 73.5)
+// Workgroups that many rows are divided into. (2 x 2000 tokens over up to 8192 keys: 32 heads of 128 with 1024,
+// 2048, 4096: 272, 283, 282 us; 16 of 64 112, 98, 98.)
+constexpr int kItems = 2048;
+// And waves that few rows are. (16 tokens over up to 16384 keys with 2560, 5120, 10240: 87, 88, 90 us.)
+constexpr int kStreams = 5120;
 
 __device__ __forceinline__ float started(const KeyArgs& a, const Sequence& s, int b, int head, int slot) {
   if (slot >= s.start() || a.c.decay == 0.0f) return 0.0f;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) key_tile(KeyArgs a) {
   const arthip_pages& pg = a.c.p;
   auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   // Items go round the eight XCDs as they come: sequences differ in length. (Each XCD an eighth of them
-  // in a row, which then share the queries: two sequences of 2000 tokens 298 us, 268 so.)
+  // in a row, which then share the queries: the calls above 277 for 283 us, 100 for 98.)
   const int item = (int)blockIdx.x;
   const int rest = (int)fdiv((uint32_t)item, a.by_splits), split = item - rest * a.splits;
   const int bh = (int)fdiv((uint32_t)rest, a.by_tiles), tile = rest - bh * a.tiles;
@@ -552,20 +554,19 @@ __global__ void __launch_bounds__(256) key_join(KeyArgs a, int64_t first_block, 
   a.c.out[b * a.c.out_stride[0] + head * a.c.out_stride[1] + slot] = sum;
 }
 
-// blocks: of 32 keys a wave, or 0 for few rows.
 template <class T, int DP>
-void (*pick(int blocks, Shape shape))(KeyArgs) {
-  if (blocks == 0)
+void (*pick(bool stream, Shape shape))(KeyArgs) {
+  if (stream)
     return shape == kPlain ? key_stream<T, DP, kPlain> : shape == kCap ? key_stream<T, DP, kCap> : key_stream<T, DP, kAny>;
   return shape == kPlain ? key_tile<T, DP, 2, kPlain> : shape == kCap ? key_tile<T, DP, 2, kCap> : key_tile<T, DP, 2, kAny>;
 }
 template <class T>
-void (*pick(int d, int blocks, Shape shape))(KeyArgs) {
-  if (d <= 32) return pick<T, 32>(blocks, shape);
-  if (d <= 64) return pick<T, 64>(blocks, shape);
-  if (d <= 96) return pick<T, 96>(blocks, shape);
-  if (d <= 128) return pick<T, 128>(blocks, shape);
-  return pick<T, 256>(blocks, shape);
+void (*pick(int d, bool stream, Shape shape))(KeyArgs) {
+  if (d <= 32) return pick<T, 32>(stream, shape);
+  if (d <= 64) return pick<T, 64>(stream, shape);
+  if (d <= 96) return pick<T, 96>(stream, shape);
+  if (d <= 128) return pick<T, 128>(stream, shape);
+  return pick<T, 256>(stream, shape);
 }
 int tile_bytes(int d) {
   return kRows * (d <= 32 ? 64 : d <= 64 ? 128 : d <= 128 ? 256 : 512);
@@ -603,7 +604,7 @@ hipError_t launch_key_weights(const arthip_key_weights_args& c, hipStream_t s) {
   a.stream = plan.stream;
   a.splits = plan.splits;
   const int64_t heads = (int64_t)c.p.batch * c.p.k_heads;
-  a.items = (int)(heads * a.tiles * a.splits);
+  const unsigned items = (unsigned)(heads * a.tiles * a.splits);
   a.by_group = make_fastdiv((uint32_t)a.group);
   a.by_page = make_fastdiv((uint32_t)c.p.page_size);
   a.by_heads = make_fastdiv((uint32_t)c.p.k_heads);
@@ -612,10 +613,10 @@ hipError_t launch_key_weights(const arthip_key_weights_args& c, hipStream_t s) {
   if (c.cap > 0) a.cap = make_cap(c.cap, c.scale);
   a.part = static_cast<float*>(c.workspace);
   const Shape shape = c.cap > kCapSmall || !(c.scale > 0) ? kAny : c.cap > 0 ? kCap : kPlain;
-  const auto fn = c.p.dtype == ARTHIP_TYPE_F16 ? pick<_Float16>(c.p.head_dim, plan.stream > 0 ? 0 : 2, shape)
-                                               : pick<__bf16>(c.p.head_dim, plan.stream > 0 ? 0 : 2, shape);
+  const auto fn = c.p.dtype == ARTHIP_TYPE_F16 ? pick<_Float16>(c.p.head_dim, plan.stream > 0, shape)
+                                               : pick<__bf16>(c.p.head_dim, plan.stream > 0, shape);
   if (plan.stream > 0) {
-    hipLaunchKernelGGL(fn, dim3((unsigned)a.items), dim3(64), 0, s, a);
+    hipLaunchKernelGGL(fn, dim3(items), dim3(64), 0, s, a);
     return hipGetLastError();
   }
   const int bytes = 2 * tile_bytes(c.p.head_dim);
@@ -623,7 +624,7 @@ hipError_t launch_key_weights(const arthip_key_weights_args& c, hipStream_t s) {
   if (bytes + kStarts > 65536)  // what a kernel may have without asking
     e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(fn, dim3((unsigned)a.items), dim3(256), bytes, s, a);
+  hipLaunchKernelGGL(fn, dim3(items), dim3(256), bytes, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t total = heads * c.slots;

@@ -143,7 +143,8 @@ std::string check_key_weights_shape(const arthip_key_weights_args& a) {
   if (!wrong.empty()) return wrong;
   if (a.q_heads == 0) return at + "no query heads";
   if (a.slots < 0 || a.slots > kMaxTokens) return at + "slots out of range";
-  // A launch takes fewer than 2^32 threads, of 256 for every 128 slots of a head.
+  // A workgroup of 256 threads takes 256 slots of a head, and splits come only to few workgroups: 2^23 times
+  // 128 slots keep a launch's threads, and the workspace's entries of a split, below 2^31.
   const int64_t items = (static_cast<int64_t>(a.slots) + 127) / 128;
   if (items > 0 && static_cast<int64_t>(a.p.batch) * a.p.k_heads > (int64_t{1} << 23) / items)
     return at + "batch times heads times slots too large";
