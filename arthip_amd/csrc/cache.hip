@@ -2,7 +2,7 @@
 // eviction of the slots with little weight (arthip_cache_evict).
 //
 // Writing is bound by HBM: 65280 tokens of 16 heads of 64, 535 MB in 107 us (5.0 TB/s). Eviction of 4
-// caches of up to 32768 slots to 8192, 8 heads of 128, takes 89 us: 41 for the selection, by one
+// caches of up to 32768 slots to 8192, 8 heads of 128, takes 87 us: 41 for the selection, by one
 // workgroup a key head, whose passes over the keys wait for one another, and 46 for moving 180 MB.
 
 #include <hip/hip_runtime.h>

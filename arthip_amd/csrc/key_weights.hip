@@ -12,8 +12,8 @@
 // itself streams the keys through a ring of tiles in LDS.
 //
 // Many rows are bound by their products and exponentials: 2 x 2000 tokens over up to 8192 keys, 32 heads
-// of 128, 247 us (735 TFLOP/s; vector unit 46%, matrix unit 32% busy). Few rows by HBM: 16 tokens over up
-// to 16384 keys of 8 heads, 279 MB in 74 us (3.8 TB/s).
+// of 128, 261 us (695 TFLOP/s; vector unit 45%, matrix unit 32% busy; cards differ, 244 to 261). Few rows by
+// HBM: 16 tokens over up to 16384 keys of 8 heads, 279 MB in 74 us (3.7 TB/s).
 
 #include <hip/hip_runtime.h>
 

@@ -16,9 +16,9 @@
 //
 // Single tokens over long caches are bound by HBM: 16 over up to 16384 keys of 8 heads, 541 MB, 109 to 112
 // us, of which the tiles take 102 to 108 (5.2 TB/s). Large calls are bound by products and exponentials, which
-// share a SIMD's two or three waves: a prompt of 8192 with a window of 4096, 32 heads of 128, 449 us
-// (918 TFLOP/s; matrix unit 48%, vector unit 40% busy), a frame of 8160 tokens over 40800, 12 heads of 64,
-// 1179 us (867 TFLOP/s; 48% and 75%).
+// share a SIMD's two or three waves: a prompt of 8192 with a window of 4096, 32 heads of 128, 467 us
+// (884 TFLOP/s; matrix unit 48%, vector unit 40% busy), a frame of 8160 tokens over 40800, 12 heads of 64,
+// 1230 us (832 TFLOP/s; 48% and 75%). (Cards differ: 444 to 482 us, 1123 to 1230.)
 
 #include <hip/hip_runtime.h>
 

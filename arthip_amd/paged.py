@@ -152,8 +152,8 @@ def paged_attention(q, k_cache, v_cache, pages, kv_len, q_offsets=None, *, scale
                     cap: float = 0.0, causal: bool = True, left: int | None = None, out=None,
                     return_lse: bool = False, workspace=None, stream=None):
     """softmax(score) V of the new tokens' queries [T, Hq, D] over their sequences' slots;
-    see arthip_paged_attention. ``left`` counts the keys before a token's own that it sees
-    (None: all). Returns out, or (out, lse) with lse fp32 [T, Hq]; rows behind the last
+    see arthip_paged_attention. ``left`` counts the slots before a token's own that it sees
+    (None: all); after cache_evict these are not the tokens last written. Returns out, or (out, lse) with lse fp32 [T, Hq]; rows behind the last
     sequence are not written. Without ``workspace`` (uint8) a call makes it."""
     scores = _scores("paged_attention", scale, cap, causal, left)
     key = ("paged", _sig(q), _sig(k_cache), _sig(v_cache), _sig(pages), _sig(kv_len), _sig(q_offsets), scores, _sig(out))

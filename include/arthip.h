@@ -624,7 +624,10 @@ int arthip_cache_write(const arthip_cache_write_args* args, void* stream);
  * scale * q_i . k_j, then cap * tanh(score / cap) if cap > 0. Token i of n new ones has the
  * position p = kv_len - n + i and sees slots j < kv_len with p - left <= j and, if causal,
  * j <= p. A token that sees nothing gives zeros, and -inf as its log-sum. Slots that a token does
- * not see add nothing to it, whatever they hold. */
+ * not see add nothing to it, whatever they hold; a value that is not finite reaches the tokens
+ * that see it, as infinity or NaN, whatever its weight. bf16 sums stay finite where the largest
+ * value times the number of keys is below 2^117. `left` counts slots, which arthip_cache_evict
+ * leaves in no order of time: a window after it sees other tokens than the last ones. */
 typedef struct arthip_paged_attention_args {
   arthip_pages p;
   const void* q;
@@ -645,7 +648,7 @@ typedef struct arthip_paged_attention_args {
   int32_t pad;
 } arthip_paged_attention_args;
 
-/* Bytes of workspace for these sizes, whatever the lengths; 0 where the call refuses them. */
+/* Bytes of workspace for these sizes, whatever the lengths (9 to 69 MB); 0 where the call refuses them. */
 size_t arthip_paged_attention_workspace(const arthip_paged_attention_args* args);
 int arthip_paged_attention(const arthip_paged_attention_args* args, void* stream);
 
@@ -654,7 +657,7 @@ int arthip_paged_attention(const arthip_paged_attention_args* args, void* stream
  * over the new tokens i that see slot j and the query heads that share key head h, with the
  * scores of arthip_paged_attention and its lse. The new tokens' own slots start from 0 instead of
  * the old weight, as do all with a decay of 0 (then weights may be NULL); slots from kv_len on
- * get 0. A token whose lse is -inf adds nothing. */
+ * get 0. A token whose lse is -inf adds nothing, whatever it and the keys hold. */
 typedef struct arthip_key_weights_args {
   arthip_pages p;
   const void* q;            /* [tokens][q_heads][D] */
@@ -687,7 +690,8 @@ int arthip_key_weights(const arthip_key_weights_args* args, void* stream);
  * positions[b][h][slot]. Staying slots from `keep` on move, in order, into the others below `keep`,
  * in order; the rest stay where they are, as does what lies behind. Sequences of up to `keep`
  * slots stay whole. A move from or to a page outside the pool is left out. Results of slots past
- * the new length: weight 0, kept -1, position -1. */
+ * the new length: weight 0, kept -1, position -1. All of `slots` is gone over, whatever the
+ * lengths: weights with room for many more slots than are in use cost time. */
 typedef struct arthip_cache_evict_args {
   arthip_pages p;           /* tokens and q_offsets are not used */
   void* k_cache;
