@@ -116,12 +116,13 @@ __device__ __forceinline__ float start_of(const KeyArgs& a, const Sequence& s, i
   return lse == -__builtin_inff() ? lse : -lse * kLog2e;
 }
 
+// A wave's own reads and writes of LDS so far are done.
+__device__ __forceinline__ void lds_wave() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // The sum of a lane's slot over the rows [from, to), by a wave from memory. A row whose start is -inf adds
 // nothing, whatever it and the key hold, but a score that is not finite takes its weight to NaN: the
 // kernels below find sums that became NaN once more by this, which leaves such rows out. (Asked
 // of every block of rows there, it took the 2000-token pieces from 307 to 324 us.)
-__device__ __forceinline__ void lds_wave() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
 template <class T, int DP, Shape SHAPE>
 __device__ __forceinline__ float apart(const KeyArgs& a, const Sequence& seq, int b, int head, int slot, int k1, int from,
                                        int to, float mul, float* starts) {
